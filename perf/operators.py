@@ -301,7 +301,8 @@ def run(state):
     if case["kind"] == "attention":
         if not own:
             return _attention_plain(state, case)
-        return state["cache"].attention(state["q"], state["positions"], slots=state["slots"], window=case["window"], max_len=case["keys"], dtype=TYPES[case["out"]])
+        return state["cache"].attention(state["q"], state["positions"], slots=state["slots"], window=case["window"], max_len=case["keys"], chunk=case["queries"],
+                                        dtype=TYPES[case["out"]])
     if not own:
         return _log_probs_plain(state, case)
     logprobs, entropy, ids, values = _package().log_probs(state["logits"], state["targets"], top=case["top"])
