@@ -9,7 +9,7 @@ Kinds
 A cache holds groups of 32 neighbouring entries of a head: a scale d in 16 bits and codes c of 4 bits, value d * (c - 8).
 
 ``draw`` gives cases of the same ranges: heads of 32 to 256 with 1 to 16 query heads on a key head, 1 to 64 sequences, up to 131072 keys,
-chunks of 2 to 512 tokens, vocabularies of 1000 to 262144, FP32, FP16 and BF16 rows.
+chunks of 2 to 512 tokens, vocabularies of 1000 to 151936, FP32, FP16 and BF16 rows.
 """
 import functools
 import importlib.util
@@ -66,9 +66,9 @@ def listed():
         # a step of a batch of conversations of very different lengths, one of them without a key
         _attention("step_batch", 32, 8, 64, 48, 1, 4099, "f32", empty=True),
         # a chunk of a long prompt
-        _attention("chunk_long", 32, 8, 128, 1, 512, 8192, "f16"),
+        _attention("chunk_long", 32, 8, 128, 1, 512, 8192, "bf16"),
         # ragged chunks of several prompts through a sliding window
-        _attention("chunk_window", 24, 8, 96, 3, 111, 1999, "f16", window=500),
+        _attention("chunk_window", 24, 8, 96, 3, 111, 1999, "bf16", window=500),
         # log probability of the token that a decode step chose
         _log_probs("logprob_step", 1, 128256, 5, "f32"),
         # a prompt chunk is scored: every row of it, with the usual most alternatives
@@ -100,12 +100,12 @@ def draw(rng):
         elif rng.random() < 0.6:
             seqs = rng.choice((1, _spread(rng, 1, 64)))
             keys = _spread(rng, 1, 131072 // seqs if seqs > 1 else 131072)
-            case = _attention("", heads, kv_heads, head, seqs, 1, keys, rng.choice(("f32", "f16")), rng.choice((0, 0, 300)), seqs > 1 and rng.random() < 0.5)
+            case = _attention("", heads, kv_heads, head, seqs, 1, keys, rng.choice(("f32", "bf16")), rng.choice((0, 0, 300)), seqs > 1 and rng.random() < 0.5)
         else:
             seqs = rng.choice((1, 1, 2, 5))
             queries = max(2, _spread(rng, 2, 512) // seqs)
             keys = max(queries, _spread(rng, queries, 8192) // seqs)
-            case = _attention("", heads, kv_heads, head, seqs, queries, keys, "f16" if queries * seqs > 32 else rng.choice(("f32", "f16")), rng.choice((0, 0, 300)),
+            case = _attention("", heads, kv_heads, head, seqs, queries, keys, "bf16" if queries * seqs > 32 else rng.choice(("f32", "bf16")), rng.choice((0, 0, 300)),
                               seqs > 1 and rng.random() < 0.5)
     del case["name"]
     return case
