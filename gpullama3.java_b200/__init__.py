@@ -6,3 +6,12 @@ Llama/Qwen3 GGUF models (Q8_0 / FP16) as hand-written sm_100a CUDA behind a C AB
 from . import chat_format, engine, gguf, llama_bench, loader, native, plan, safetensors, sampler, synth, tokenizer  # noqa: F401
 from .loader import load_model  # noqa: F401
 from .plan import B200MasterPlan  # noqa: F401
+
+
+def __getattr__(name):  # the operators work on torch tensors: torch is imported when they are asked for
+    if name in ("operators", "KV4Cache", "log_probs"):
+        import importlib
+
+        operators = importlib.import_module(".operators", __name__)
+        return operators if name == "operators" else getattr(operators, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -9,11 +9,21 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libb200llama.so")
-SOURCES = ["plan.cu"]
+SOURCES = ["plan.cu", "operators.cu"]
 
 
-def _deps():
-    d = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh", ".h"))]
+# Headers that only operators.cu reads: the other objects are not rebuilt for them.
+OPERATOR_HEADERS = ("kv4.cuh", "logprobs.cuh")
+
+
+def _deps(source: str | None = None):
+    """What the library, or the object of one of its sources, is made from."""
+    d = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
+    if source == "operators.cu":
+        d = [f for f in d if os.path.basename(f) in (*OPERATOR_HEADERS, "common.cuh", "operators.h")]
+    elif source is not None:
+        d = [f for f in d if os.path.basename(f) not in OPERATOR_HEADERS]
+    d += [os.path.join(CSRC, f) for f in SOURCES if source in (None, f)]
     exp = os.path.join(CSRC, "experimental")
     if os.path.isdir(exp):
         d += [os.path.join(exp, f) for f in os.listdir(exp) if f.endswith((".cuh", ".h"))]
@@ -25,7 +35,7 @@ NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     # Java never contracts a*b+c; the kernels reproduce the CPU path's float order exactly.
     "-fmad=false", "-prec-div=true", "-prec-sqrt=true", "-ftz=false",
-    "-Xcompiler", "-fPIC", "-Xcompiler", "-pthread", "-shared", "-Xptxas", "-v",
+    "-Xcompiler", "-fPIC", "-Xcompiler", "-pthread", "-Xptxas", "-v",
 ]
 
 
@@ -51,14 +61,34 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not needs_build():
         return LIB
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    cmd = [nvcc, *NVCC_FLAGS, *[f"-D{d}" for d in _defines()], "-o", LIB, *[os.path.join(CSRC, s) for s in SOURCES], "-lcudart"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or r.returncode != 0:
-        sys.stderr.write(r.stdout + r.stderr)
-    if r.returncode != 0:
-        raise RuntimeError("nvcc failed building libb200llama.so")
+    built_with = open(STAMP).read().split() if os.path.exists(STAMP) else []
+    running, objects, log = [], [], ""
+    for s in SOURCES:  # one compiler per source, at the same time
+        obj = os.path.join(CSRC, os.path.splitext(s)[0] + ".o")
+        objects.append(obj)
+        stale = force or built_with != _defines() or not os.path.exists(obj) or any(os.path.getmtime(d) > os.path.getmtime(obj) for d in [*_deps(s), __file__])
+        if stale:
+            cmd = [nvcc, *NVCC_FLAGS, *[f"-D{d}" for d in _defines()], "-c", "-o", obj, os.path.join(CSRC, s)]
+            running.append((s, obj, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    failed = []
+    for s, obj, p in running:
+        out = p.communicate()[0]
+        log += out
+        if p.returncode != 0:
+            failed.append(s)
+            if os.path.exists(obj):
+                os.remove(obj)
+        if verbose or p.returncode != 0:
+            sys.stderr.write(out)
+    if not failed:
+        r = subprocess.run([nvcc, *NVCC_FLAGS[:2], "-Xcompiler", "-fPIC", "-Xcompiler", "-pthread", "-shared", "-o", LIB, *objects, "-lcudart"], capture_output=True, text=True)
+        if r.returncode != 0:
+            sys.stderr.write(r.stdout + r.stderr)
+            failed.append("libb200llama.so")
+    if failed:
+        raise RuntimeError(f"nvcc failed building {', '.join(failed)}")
     with open(os.path.join(CSRC, "ptxas.log"), "w") as f:
-        f.write(r.stderr)
+        f.write(log)
     with open(STAMP, "w") as f:
         f.write(" ".join(_defines()))
     return LIB

@@ -58,7 +58,7 @@ __device__ __forceinline__ unsigned long long gtime_ns() {
     return t;
 }
 // one thread; bounded: a rank that errored out or died must not leave the others spinning inside a captured graph
-__device__ __noinline__ void tp_wait(const TpCtx &t, int slot, unsigned seq) {
+static __device__ __noinline__ void tp_wait(const TpCtx &t, int slot, unsigned seq) {
     const unsigned *f = reinterpret_cast<const unsigned *>(t.peer[t.rank] + t.off_flags) + slot * TP_MAX;
     unsigned it = 0;
     unsigned long long t0 = 0;

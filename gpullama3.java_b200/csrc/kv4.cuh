@@ -1,0 +1,543 @@
+// kv4.cuh -- a key/value cache of 4-bit codes: append (head norms, rotation and quantisation in one pass), read-back, and the attention of single query rows over it.
+//
+// A group is 32 neighbouring entries of a head: a scale d (FP16) and codes c of 4 bits, value d * (c - 8).  m = the group's entry of largest magnitude (the first of equal ones),
+// d = f16(m / -8), c = clamp(rint(x / d) + 8, 0, 15): m itself lands on an end of the range whatever its sign.  A group with an infinity or a NaN is stored with a NaN scale.
+//
+// Memory: [slot][key/value head][block of 16 positions] records of 18 * HS bytes, so that any run of positions of a head is ONE contiguous stretch:
+//   key codes    [half: positions 0-7, 8-15][words of a lane / VW][lane = 4 g + t][VW words]: lane (g, t) holds position 8 * half + g, entries 32 grp + 8 t .. + 7 in word grp
+//   value codes  the same order; lane (g, t) holds positions 8 * half + 2 t, + 1 (low and high half of a word) and entries 32 grp + 4 g .. + 3
+//   key scales   [g][grp] words of two halves: positions g and g + 8; value scales likewise
+// These are the operands of mma.m16n8k16 as its lanes want them: a lane reads its words in one vector load without bank conflicts and a mask turns a word into register pairs.
+#pragma once
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math_constants.h>
+
+#include "common.cuh"
+
+namespace kv4 {
+
+namespace cg = cooperative_groups;
+using bf16 = __nv_bfloat16;
+
+constexpr int GROUP = 32, BLOCK = 16; // entries of a group, positions of a record
+__host__ __device__ constexpr int groups(int hs) { return hs / GROUP; }
+__host__ __device__ constexpr int vec_words(int hs) { return groups(hs) > 4 ? 4 : groups(hs); } // words that a lane loads at a time
+__host__ __device__ constexpr int record_bytes(int hs) { return 18 * hs; }
+
+struct View {
+    unsigned char *base;
+    int slots, context, blocks, kv_heads; // blocks of a head and slot
+};
+struct Rows { // row r stands at position `positions ? positions[r] : start + r` of slot `slots ? slots[r] : slot`
+    const int *positions, *slots;
+    int n, start, slot;
+    __device__ __forceinline__ int position(int r) const { return positions ? positions[r] : start + r; }
+    __device__ __forceinline__ int slot_of(int r) const { return slots ? slots[r] : slot; }
+};
+
+template <int HS> __device__ __forceinline__ unsigned char *record(const View &kv, int slot, int head, int block) {
+    return kv.base + (((size_t)slot * kv.kv_heads + head) * kv.blocks + block) * record_bytes(HS);
+}
+// Index of a lane's word `grp` in the codes of a record's half.
+template <int HS> __device__ __forceinline__ int word_of(int half, int lane, int grp) {
+    constexpr int NG = groups(HS), VW = vec_words(HS);
+    return half * 32 * NG + (grp / VW) * 32 * VW + lane * VW + grp % VW;
+}
+
+__device__ __forceinline__ float load_f32(const float *p) { return *p; }
+__device__ __forceinline__ void load8(const float *p, float (&x)[8], bool vec) {
+    if (vec) {
+        const float4 a = *reinterpret_cast<const float4 *>(p), b = *reinterpret_cast<const float4 *>(p + 4);
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = p[i];
+}
+__device__ __forceinline__ float2 to_f32x2(uint32_t w, const __half *) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ float2 to_f32x2(uint32_t w, const bf16 *) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(bf16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ void load8(const T *p, float (&x)[8], bool vec) {
+    if (vec) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = to_f32x2(v[i], p);
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        }
+    } else
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = to_f32(p[i]);
+}
+
+// ---- append ---------------------------------------------------------------------------------------------------------------------------------------------------
+struct Append {
+    View kv;
+    Rows rows;
+    const void *q, *k, *v;
+    long long ldq, ldk, ldv, ldo; // entries between rows
+    int heads;                    // query heads; 0: none
+    int interleaved, vec;         // vec: every row starts on a 16-byte boundary
+    const float *q_norm, *k_norm, *cos, *sin; // norms and tables: null where there is none
+    float eps;
+    float *q_out;
+};
+
+// 4-bit codes of a lane's 8 entries; the four lanes of a group hold its 32.
+__device__ __forceinline__ void quantize8(const float (&x)[8], unsigned lanes, __half &scale, int (&c)[8]) {
+    float top = x[0];
+    bool bad = !(fabsf(x[0]) < CUDART_INF_F);
+#pragma unroll
+    for (int i = 1; i < 8; i++) {
+        if (fabsf(x[i]) > fabsf(top)) top = x[i];
+        bad |= !(fabsf(x[i]) < CUDART_INF_F);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        const float other = __shfl_xor_sync(lanes, top, o);
+        const bool lower = (threadIdx.x & o) != 0; // the other lane's entries stand in front of this one's
+        if (fabsf(other) > fabsf(top) || (fabsf(other) == fabsf(top) && lower)) top = other;
+        bad |= (bool)__shfl_xor_sync(lanes, (int)bad, o);
+    }
+    scale = bad ? __ushort_as_half(0x7fff) : __float2half_rn(fminf(fmaxf(top * -0.125f, -65504.0f), 65504.0f));
+    const float d = __half2float(scale);
+#pragma unroll
+    for (int i = 0; i < 8; i++) c[i] = bad || d == 0.0f ? 8 : (int)fminf(fmaxf(rintf(__fdiv_rn(x[i], d)), -8.0f), 7.0f) + 8;
+}
+
+// Lanes of a head: 8 entries each, so that pairs of neighbours lie in a lane, pairs half a head apart in lanes half the head's lanes apart, and a group in four lanes.
+// A segment of WIDTH lanes (a power of two) serves one head, 32 / WIDTH heads a warp.  Bytes bound it: 512 rows of (32 + 2 * 8) heads of 128 read 12.6 MB and write 9.0.
+template <int HS, typename T> __global__ void __launch_bounds__(256) k_append(const Append a) {
+    constexpr int L = HS / 8, WIDTH = L == 4 ? 4 : L == 8 ? 8 : L <= 16 ? 16 : 32, PER_WARP = 32 / WIDTH;
+    pdl_wait();
+    const int lane = threadIdx.x & 31, li = lane & (WIDTH - 1), G = a.kv.kv_heads, total = a.heads + 2 * G;
+    const long long item = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / WIDTH;
+    const int row = (int)(item / total), which = (int)(item % total);
+    int pos = 0, slot = -1;
+    if (row < a.rows.n) { pos = a.rows.position(row); slot = a.rows.slot_of(row); }
+    const bool on = row < a.rows.n && pos >= 0 && pos < a.kv.context && slot >= 0 && slot < a.kv.slots, mine = on && li < L;
+    if (!__any_sync(0xffffffffu, on)) return; // (a whole warp: the shuffles below take every lane)
+    const bool is_q = which < a.heads, is_v = which >= a.heads + G;
+    const int head = is_q ? which : is_v ? which - a.heads - G : which - a.heads;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = 0.0f;
+    if (mine) {
+        const T *src = is_q ? (const T *)a.q + row * a.ldq : is_v ? (const T *)a.v + row * a.ldv : (const T *)a.k + row * a.ldk;
+        load8(src + head * HS + li * 8, x, a.vec);
+    }
+    const float *norm = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+    { // mean of squares in 64 bits: one rounding to FP32, whatever the order of the sum
+        double ss = 0.0;
+        if (a.q_norm || a.k_norm) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss += (double)x[i] * (double)x[i];
+#pragma unroll
+            for (int o = WIDTH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        }
+        if (norm && mine) {
+            const float s = (float)(1.0 / sqrt(ss / HS + (double)a.eps));
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = norm[li * 8 + i] * (s * x[i]);
+        }
+    }
+    if (a.cos) {
+        const float *cs = a.cos + (size_t)pos * (HS / 2), *sn = a.sin + (size_t)pos * (HS / 2);
+        if (a.interleaved) {
+            if (mine && !is_v)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float c = cs[li * 4 + i], s = sn[li * 4 + i], u = x[2 * i], w = x[2 * i + 1];
+                    x[2 * i] = u * c - w * s;
+                    x[2 * i + 1] = u * s + w * c;
+                }
+        } else {
+            const bool low = li < L / 2;
+            const int partner = lane - li + (low ? li + L / 2 : li < L ? li - L / 2 : li);
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], partner);
+            if (mine && !is_v)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int at = (low ? li : li - L / 2) * 8 + i;
+                    const float c = cs[at], s = sn[at];
+                    x[i] = low ? x[i] * c - y[i] * s : y[i] * s + x[i] * c;
+                }
+        }
+    }
+    if (is_q) {
+        if (mine) {
+            float *o = a.q_out + row * a.ldo + head * HS + li * 8;
+            if (a.vec) {
+                *reinterpret_cast<float4 *>(o) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4 *>(o + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            } else
+#pragma unroll
+                for (int i = 0; i < 8; i++) o[i] = x[i];
+        }
+    }
+    __half scale;
+    int c[8];
+    quantize8(x, 0xffffffffu, scale, c);
+    if (!mine || is_q) return;
+    unsigned char *rec = record<HS>(a.kv, slot, head, pos / BLOCK);
+    const int in = pos % BLOCK, half = in >> 3, grp = li >> 2, t = li & 3;
+    if (!is_v) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w |= (uint32_t)c[i] << (4 * (i >> 1) + 16 * (i & 1));
+        reinterpret_cast<uint32_t *>(rec)[word_of<HS>(half, 4 * (in & 7) + t, grp)] = w;
+    } else {
+        uint16_t *codes = reinterpret_cast<uint16_t *>(rec + 8 * HS);
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const uint32_t w = c[4 * u] | c[4 * u + 1] << 4 | c[4 * u + 2] << 8 | c[4 * u + 3] << 12;
+            codes[2 * word_of<HS>(half, 4 * (2 * t + u) + ((in & 7) >> 1), grp) + (in & 1)] = (uint16_t)w;
+        }
+    }
+    if (t == 0) reinterpret_cast<__half *>(rec + 16 * HS + (is_v ? HS : 0))[2 * ((in & 7) * groups(HS) + grp) + half] = scale;
+}
+
+// ---- read-back: the values that the codes of some rows stand for -----------------------------------------------------------------------------------------------
+__device__ __forceinline__ void put(float *p, float v) { *p = v; }
+__device__ __forceinline__ void put(__half *p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void put(bf16 *p, float v) { *p = __float2bfloat16_rn(v); }
+
+template <int HS, typename T> __global__ void __launch_bounds__(256) k_read(View kv, Rows rows, T *__restrict__ k, T *__restrict__ v) {
+    constexpr int L = HS / 8;
+    pdl_wait();
+    const long long item = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int li = (int)(item % L), G = kv.kv_heads, which = (int)(item / L % (2 * G));
+    const long long row = item / L / (2 * G);
+    if (row >= rows.n) return;
+    const int pos = rows.position((int)row), slot = rows.slot_of((int)row);
+    if (pos < 0 || pos >= kv.context || slot < 0 || slot >= kv.slots) return;
+    const bool is_v = which >= G;
+    const int head = is_v ? which - G : which, in = pos % BLOCK, half = in >> 3, grp = li >> 2, t = li & 3;
+    const unsigned char *rec = record<HS>(kv, slot, head, pos / BLOCK);
+    const float d = __half2float(reinterpret_cast<const __half *>(rec + 16 * HS + (is_v ? HS : 0))[2 * ((in & 7) * groups(HS) + grp) + half]);
+    T *out = (is_v ? v : k) + (row * G + head) * HS + li * 8;
+    int c[8];
+    if (!is_v) {
+        const uint32_t w = reinterpret_cast<const uint32_t *>(rec)[word_of<HS>(half, 4 * (in & 7) + t, grp)];
+#pragma unroll
+        for (int i = 0; i < 8; i++) c[i] = w >> (4 * (i >> 1) + 16 * (i & 1)) & 15;
+    } else {
+        const uint16_t *codes = reinterpret_cast<const uint16_t *>(rec + 8 * HS);
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const uint32_t w = codes[2 * word_of<HS>(half, 4 * (2 * t + u) + ((in & 7) >> 1), grp) + (in & 1)];
+#pragma unroll
+            for (int i = 0; i < 4; i++) c[4 * u + i] = w >> (4 * i) & 15;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) put(out + i, d * (float)(c[i] - 8));
+}
+
+// ---- attention of single rows ----------------------------------------------------------------------------------------------------------------------------------
+struct Step {
+    View kv;
+    Rows rows;
+    const float *q;
+    long long ldq, ldo; // entries between rows
+    int heads, window, vec, out_type;
+    float scale;
+    void *out;
+    int8_t *quants; // out_type KV4_OUT_Q8: blocks of 32
+    float *scales;
+};
+
+__device__ __forceinline__ float ex2(float x) { // 2^x
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+template <int VW> __device__ __forceinline__ void lds_words(const uint32_t *p, uint32_t (&w)[VW]) {
+    if constexpr (VW == 4) { const uint4 v = *reinterpret_cast<const uint4 *>(p); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+    else if constexpr (VW == 2) { const uint2 v = *reinterpret_cast<const uint2 *>(p); w[0] = v.x; w[1] = v.y; }
+    else
+#pragma unroll
+        for (int i = 0; i < VW; i++) w[i] = p[i];
+}
+
+// Two BF16 codes (c - 8, exact) of nibble I (0 .. 3) of the word's low and high half: 128 + c by the bits alone, then -136.
+template <int I> __device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
+    const uint32_t u = (w >> (4 * I) & 0x000f000fu) | 0x43004300u;
+    uint32_t r;
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x43084308u));
+    return r;
+}
+
+constexpr int STEP_WARPS = 8, STEP_MAX_CLUSTER = 16;
+__host__ __device__ constexpr int step_stages(int hs) { return hs >= 256 ? 3 : 4; }
+__host__ __device__ constexpr size_t step_ring_bytes(int hs) { return (size_t)STEP_WARPS * step_stages(hs) * record_bytes(hs); }
+__host__ __device__ constexpr size_t step_merge_bytes(int hs, int heads) { return (size_t)(STEP_WARPS + 1) * heads * (hs + 2) * 4; } // the warps' parts and the CTA's
+__host__ __device__ constexpr size_t step_smem_bytes(int hs, int heads) { return step_ring_bytes(hs) > step_merge_bytes(hs, heads) ? step_ring_bytes(hs) : step_merge_bytes(hs, heads); }
+
+// One query row and up to 4 NT query heads of a key/value head: the row's visible positions are split over the warps of a cluster of CTAs, each warp runs through its records
+// (cp.async ring of its own, no barrier in the loop) with its own running maximum, and the parts are joined in shared memory, then over the cluster: one launch, no workspace,
+// nothing that depends on an order of arrival.
+//   scores  C[16 positions x 8] = codes (FP16: a masked code IS a subnormal, c 2^-24, exact) x queries; the eight columns are four heads, each as a high and a low FP16 part, so that
+//           a query keeps 22 bits; accumulators start at -8 sum q (the codes' offset) and are scaled group by group in FP32
+//   values  C[16 entries x 8] = codes - 8 (BF16, exact) x (p d), again as a high and a low part (16 bits, FP32's range: no scale of the values under- or overflows)
+// A lane keeps the running sums of ONE head (t); what crosses lanes in the loop is the transposition of the probabilities and, where a maximum grows by more than 2^8, its update.
+template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_step(const Step a, const int units_per_head) {
+    constexpr int NG = groups(HS), VW = vec_words(HS), R = record_bytes(HS), S = step_stages(HS), H = 4 * NT, CHUNKS = R / 16;
+    extern __shared__ __align__(16) unsigned char smem[];
+    pdl_wait();
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int G = a.kv.kv_heads, mul = a.heads / G;
+    const int unit = blockIdx.x / ranks, row = unit / (G * units_per_head), kvh = unit / units_per_head % G, first = unit % units_per_head * H; // first head within the group
+    const int pos = a.rows.position(row), slot = a.rows.slot_of(row);
+    if (slot < 0 || slot >= a.kv.slots || pos >= a.kv.context) return; // a padding row (the whole cluster leaves)
+    const int lo = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0, hi = pos + 1;
+    const int b0 = lo / BLOCK, nb = hi > lo ? (hi + BLOCK - 1) / BLOCK - b0 : 0, per = (nb + ranks * STEP_WARPS - 1) / (ranks * STEP_WARPS);
+    const int begin = b0 + min(nb, (rank * STEP_WARPS + warp) * per), end = b0 + min(nb, (rank * STEP_WARPS + warp + 1) * per);
+
+    unsigned char *ring = smem + (size_t)warp * S * R;
+    const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
+    const unsigned char *src = record<HS>(a.kv, slot, kvh, 0);
+    auto fetch = [&](int block, int stage) {
+        if (block < end) {
+            const unsigned char *s = src + (size_t)block * R + lane * 16;
+            const uint32_t d = ring_addr + stage * R + lane * 16;
+#pragma unroll
+            for (int i = 0; i < CHUNKS / 32; i++) cp16(d + i * 512, s + i * 512);
+            if (CHUNKS % 32 && lane < CHUNKS % 32) cp16(d + CHUNKS / 32 * 512, s + CHUNKS / 32 * 512);
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) fetch(begin + i, i);
+
+    // queries: lane (g, t) holds column g = head g >> 1, part g & 1, of entries 32 grp + 8 t .. + 7
+    uint32_t qf[NT][NG][4];
+    float off[NT][NG], sc[NT]; // of head t: -8 sum q of every group, and what turns a sum into a score in units of log2
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        const int h = first + 4 * n + (g >> 1);
+        float x[NG][8], top = 0.0f;
+#pragma unroll
+        for (int grp = 0; grp < NG; grp++) {
+            if (h < mul) load8(a.q + row * a.ldq + (size_t)(kvh * mul + h) * HS + grp * 32 + t * 8, x[grp], a.vec);
+            else
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[grp][i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) top = fmaxf(top, fabsf(x[grp][i]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = min(max((int)(__float_as_uint(top) >> 23), 12), 230); // q times a power of two: below 1024, whatever its size
+        const float up = __uint_as_float((unsigned)(263 - e) << 23), down = __uint_as_float((unsigned)(e - 9) << 23);
+#pragma unroll
+        for (int grp = 0; grp < NG; grp++) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                x[grp][i] *= up;
+                sum += x[grp][i];
+                if (i & 2) x[grp][i] *= 0.0625f; // these meet codes in bits 4 - 7: 16 c
+                const float high = __half2float(__float2half_rn(x[grp][i]));
+                x[grp][i] = g & 1 ? x[grp][i] - high : high;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) qf[n][grp][i] = pack_f16(x[grp][2 * i], x[grp][2 * i + 1]);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            off[n][grp] = __shfl_sync(0xffffffffu, sum, 8 * t) * (-8.0f * 5.9604644775390625e-8f);
+        }
+        sc[n] = __shfl_sync(0xffffffffu, down, 8 * t) * 16777216.0f * (a.scale * 1.4426950408889634f);
+    }
+
+    float m[NT], l[NT], o[NT][2 * NG][4];
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+        m[n] = -CUDART_INF_F; l[n] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * NG; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+    }
+    int stage = 0;
+    for (int block = begin; block < end; block++) {
+        cp_wait<S - 2>();
+        __syncwarp(); // and every lane has read the stage that the next copy overwrites
+        fetch(block + S - 1, stage == 0 ? S - 1 : stage - 1);
+        const uint32_t *words = reinterpret_cast<const uint32_t *>(ring + stage * R);
+        const uint32_t *ks = words + 4 * HS + g * NG, *vs = ks + 8 * NG; // scales of positions g and g + 8
+        const int p0 = block * BLOCK + g;
+        const bool see0 = p0 >= lo && p0 < hi, see1 = p0 + 8 >= lo && p0 + 8 < hi;
+        float s[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NG / VW; v++) {
+            uint32_t wa[VW], wb[VW], d[VW];
+            lds_words<VW>(words + word_of<HS>(0, lane, v * VW), wa);
+            lds_words<VW>(words + word_of<HS>(1, lane, v * VW), wb);
+            lds_words<VW>(ks + v * VW, d);
+#pragma unroll
+            for (int i = 0; i < VW; i++) {
+                const int grp = v * VW + i;
+                const uint32_t c0[4] = {wa[i] & 0x000f000fu, wb[i] & 0x000f000fu, wa[i] & 0x00f000f0u, wb[i] & 0x00f000f0u};
+                const uint32_t ha = wa[i] >> 8, hb = wb[i] >> 8;
+                const uint32_t c1[4] = {ha & 0x000f000fu, hb & 0x000f000fu, ha & 0x00f000f0u, hb & 0x00f000f0u};
+                const float2 dk = __half22float2(*reinterpret_cast<const __half2 *>(&d[i]));
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float acc[4] = {off[n][grp], 0.0f, off[n][grp], 0.0f};
+                    mma_f16(acc, c0, qf[n][grp][0], qf[n][grp][1]);
+                    mma_f16(acc, c1, qf[n][grp][2], qf[n][grp][3]);
+                    s[n][0] = fmaf(dk.x, acc[0] + acc[1], s[n][0]);
+                    s[n][1] = fmaf(dk.y, acc[2] + acc[3], s[n][1]);
+                }
+            }
+        }
+        float p[NT][2];
+        bool grow = false;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            s[n][0] = see0 ? s[n][0] * sc[n] : -CUDART_INF_F;
+            s[n][1] = see1 ? s[n][1] * sc[n] : -CUDART_INF_F;
+            grow |= fmaxf(s[n][0], s[n][1]) > m[n] + 8.0f;
+        }
+        if (__any_sync(0xffffffffu, grow))
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float mx = fmaxf(s[n][0], s[n][1]);
+#pragma unroll
+                for (int i = 4; i < 32; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
+                mx = fmaxf(mx, m[n]);
+                const float alpha = m[n] == mx ? 1.0f : ex2(m[n] - mx);
+                m[n] = mx;
+                l[n] *= alpha;
+#pragma unroll
+                for (int i = 0; i < 2 * NG; i++) { o[n][i][0] *= alpha; o[n][i][1] *= alpha; o[n][i][2] *= alpha; o[n][i][3] *= alpha; }
+            }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const float ref = m[n] == -CUDART_INF_F ? 0.0f : m[n]; // nothing seen yet: 2^(-inf) = 0
+            p[n][0] = ex2(s[n][0] - ref);
+            p[n][1] = ex2(s[n][1] - ref);
+            l[n] += p[n][0] + p[n][1];
+        }
+#pragma unroll
+        for (int v = 0; v < NG / VW; v++) {
+            uint32_t wa[VW], wb[VW], d[VW];
+            lds_words<VW>(words + 2 * HS + word_of<HS>(0, lane, v * VW), wa);
+            lds_words<VW>(words + 2 * HS + word_of<HS>(1, lane, v * VW), wb);
+            lds_words<VW>(vs + v * VW, d);
+#pragma unroll
+            for (int i = 0; i < VW; i++) {
+                const int grp = v * VW + i;
+                float2 dv = __half22float2(*reinterpret_cast<const __half2 *>(&d[i]));
+                if (!see0) dv.x = 0.0f; // whatever stands behind the mask
+                if (!see1) dv.y = 0.0f;
+                const uint32_t c0[4] = {codes_bf16<0>(wa[i]), codes_bf16<1>(wa[i]), codes_bf16<0>(wb[i]), codes_bf16<1>(wb[i])};
+                const uint32_t c1[4] = {codes_bf16<2>(wa[i]), codes_bf16<3>(wa[i]), codes_bf16<2>(wb[i]), codes_bf16<3>(wb[i])};
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    const float x0 = p[n][0] * dv.x, x1 = p[n][1] * dv.y;
+                    const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffff0000u), h1 = __uint_as_float(__float_as_uint(x1) & 0xffff0000u);
+                    const uint32_t f0 = transpose8x8(pack_bf16(h0, x0 - h0)), f1 = transpose8x8(pack_bf16(h1, x1 - h1));
+                    mma_bf16(o[n][2 * grp], c0, f0, f1);
+                    mma_bf16(o[n][2 * grp + 1], c1, f0, f1);
+                }
+            }
+        }
+        stage = stage + 1 == S ? 0 : stage + 1;
+    }
+    cp_wait<0>();
+    __syncthreads();
+
+    // ---- join: warps, then CTAs -------------------------------------------------------------------------------------------------------------------------------
+    float *part = reinterpret_cast<float *>(smem), *pm = part + (STEP_WARPS + 1) * H * HS, *pl = pm + (STEP_WARPS + 1) * H; // [warp, or the CTA's][head][entry]
+#pragma unroll
+    for (int n = 0; n < NT; n++) {
+#pragma unroll
+        for (int i = 4; i < 32; i <<= 1) l[n] += __shfl_xor_sync(0xffffffffu, l[n], i);
+        const int h = 4 * n + t;
+        if (g == 0) { pm[warp * H + h] = m[n]; pl[warp * H + h] = l[n]; }
+#pragma unroll
+        for (int grp = 0; grp < NG; grp++)
+            *reinterpret_cast<float4 *>(part + (warp * H + h) * HS + grp * 32 + g * 4) =
+                make_float4(o[n][2 * grp][0] + o[n][2 * grp][1], o[n][2 * grp][2] + o[n][2 * grp][3], o[n][2 * grp + 1][0] + o[n][2 * grp + 1][1], o[n][2 * grp + 1][2] + o[n][2 * grp + 1][3]);
+    }
+    __syncthreads();
+    const int mine = STEP_WARPS * H; // rows behind the warps': the CTA's
+    for (int i = threadIdx.x; i < H * HS; i += STEP_WARPS * 32) {
+        const int h = i / HS;
+        float M = -CUDART_INF_F, L = 0.0f, O = 0.0f;
+#pragma unroll
+        for (int w = 0; w < STEP_WARPS; w++) M = fmaxf(M, pm[w * H + h]);
+        const float ref = M == -CUDART_INF_F ? 0.0f : M;
+#pragma unroll
+        for (int w = 0; w < STEP_WARPS; w++) {
+            const float f = ex2(pm[w * H + h] - ref);
+            L = fmaf(f, pl[w * H + h], L);
+            O = fmaf(f, part[(w * H) * HS + i], O);
+        }
+        part[mine * HS + i] = O;
+        if (i % HS == 0) { pm[mine + h] = M; pl[mine + h] = L; }
+    }
+    if (ranks > 1) cluster.sync(); else __syncthreads();
+    const int slice = H * HS / ranks;
+    for (int j = threadIdx.x; j < slice; j += STEP_WARPS * 32) { // (whole warps: slice is a multiple of 32 where the blocks of 32 below need it)
+        const int i = rank * slice + j, h = i / HS;
+        float M = -CUDART_INF_F, L = 0.0f, O = 0.0f;
+        for (int r = 0; r < ranks; r++) M = fmaxf(M, *cluster.map_shared_rank(pm + mine + h, r));
+        const float ref = M == -CUDART_INF_F ? 0.0f : M;
+        for (int r = 0; r < ranks; r++) {
+            const float f = ex2(*cluster.map_shared_rank(pm + mine + h, r) - ref);
+            L = fmaf(f, *cluster.map_shared_rank(pl + mine + h, r), L);
+            O = fmaf(f, *cluster.map_shared_rank(part + mine * HS + i, r), O);
+        }
+        const float v = hi <= lo ? 0.0f : O / L; // a row that sees nothing: zeros
+        const bool on = first + h < mul;
+        const size_t at = (size_t)(kvh * mul + first + h) * HS + i % HS;
+        if (a.out_type == KV4_OUT_Q8) {
+            float as;
+            const int qv = quant_block_lane(v, as);
+            if (on) {
+                a.quants[row * a.ldo + at] = (int8_t)qv;
+                if (lane == 0) a.scales[(row * a.ldo + at) / 32] = as;
+            }
+        } else if (!on) continue;
+        else if (a.out_type == B200_GGML_F32) ((float *)a.out)[row * a.ldo + at] = v;
+        else if (a.out_type == B200_GGML_F16) put((__half *)a.out + row * a.ldo + at, v);
+        else put((bf16 *)a.out + row * a.ldo + at, v);
+    }
+    if (ranks > 1) cluster.sync(); // no CTA leaves while another reads its part
+}
+
+} // namespace kv4

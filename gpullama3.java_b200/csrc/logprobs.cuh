@@ -1,0 +1,267 @@
+// logprobs.cuh -- log probabilities of given tokens, entropy and the most likely alternatives of logits rows, in one pass over the row.
+//
+// With M the largest logit and Z' = sum of exp(x - M) over every entry but ONE of the largest: log p(t) = x_t - M - log1p(Z'), H = log1p(Z') - S / (1 + Z') with
+// S = sum (x - M) exp(x - M).  Leaving the largest entry out of the sum keeps the small ones that a sum starting at 1 would round away: a sure model's log p(t) = -log1p(Z').
+// Sums of parts (m, z, s) join as z1 + (1 + z2) e^d, s1 + e^d (s2 + d (1 + z2)) with d = m2 - m1 <= 0.
+// Alternatives go by value, equal ones by index: 64-bit keys (the value's bits, ordered as integers | ~index), no two alike.  A NaN is no alternative.
+#pragma once
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <math_constants.h>
+
+#include "common.cuh"
+
+namespace lp {
+
+namespace cg = cooperative_groups;
+using bf16 = __nv_bfloat16;
+typedef unsigned long long u64;
+
+constexpr int THREADS = 512, PER_THREAD = 16, BATCH = THREADS * PER_THREAD, MAX_TOP = 32, MAX_CLUSTER = 16;
+constexpr int PUSHERS = 64;                                // threads that may add candidates in a batch: more of them raise the threshold first
+constexpr int BUFFER = MAX_TOP + 2 * PUSHERS * PER_THREAD; // what is left of the last selection, and two batches' worth
+
+struct Args {
+    const void *logits;
+    long long ld; // entries between rows
+    int rows, vocab, top;
+    const int *targets;
+    float *logprobs, *entropy, *top_logprobs;
+    int *top_ids;
+};
+
+__device__ __forceinline__ u64 key_of(float x, unsigned index) {
+    const unsigned b = __float_as_uint(x + 0.0f); // (-0 and 0 are equal)
+    return (u64)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | ~index;
+}
+__device__ __forceinline__ float value_of(u64 key) {
+    const unsigned b = (unsigned)(key >> 32);
+    return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ unsigned index_of(u64 key) { return ~(unsigned)key; }
+
+struct Sum { // of a set of entries: its largest, and what the others add
+    float m, z, s;
+};
+__device__ __forceinline__ Sum join(const Sum &p, const Sum &q) {
+    const bool first = p.m >= q.m;
+    const Sum &a = first ? p : q, &b = first ? q : p;
+    const float d = b.m - a.m; // (-inf where a set is empty; NaN where both are)
+    Sum r = a;
+    if (d > -CUDART_INF_F) {
+        const float e = __expf(d);
+        r.z = fmaf(1.0f + b.z, e, a.z);
+        r.s = fmaf(fmaf(d, 1.0f + b.z, b.s), e, a.s);
+    }
+    r.z += b.z - b.z; // a NaN stays one, wherever it was
+    return r;
+}
+
+template <typename T> struct Load;
+template <> struct Load<float> {
+    static constexpr int VEC = 4;
+    static __device__ __forceinline__ void vec(const float *p, float *x) {
+        const float4 v = __ldcs(reinterpret_cast<const float4 *>(p));
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+    }
+    static __device__ __forceinline__ float one(const float *p) { return *p; }
+};
+template <> struct Load<__half> {
+    static constexpr int VEC = 8;
+    static __device__ __forceinline__ void vec(const __half *p, float *x) {
+        const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(p));
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[i]));
+            x[2 * i] = f.x; x[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ float one(const __half *p) { return __half2float(*p); }
+};
+template <> struct Load<bf16> {
+    static constexpr int VEC = 8;
+    static __device__ __forceinline__ void vec(const bf16 *p, float *x) {
+        const uint4 w = __ldcs(reinterpret_cast<const uint4 *>(p));
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { x[2 * i] = __uint_as_float(u[i] << 16); x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u); }
+    }
+    static __device__ __forceinline__ float one(const bf16 *p) { return __bfloat162float(*p); }
+};
+
+struct Smem {
+    u64 buffer[BUFFER], best[MAX_TOP]; // candidates; the CTA's alternatives in order
+    Sum warps[THREADS / 32], cta;
+    u64 merged[MAX_TOP];
+    int pushed, n_best;
+};
+
+// The `n` largest keys of buffer[0 .. total), in order, into best: a key's place is the number of larger ones.
+__device__ __forceinline__ void select(Smem &sm, int total, int n) {
+    for (int i = threadIdx.x; i < total; i += THREADS) {
+        const u64 k = sm.buffer[i];
+        int place = 0;
+        for (int j = 0; j < total; j++) place += sm.buffer[j] > k;
+        if (place < n) sm.best[place] = k;
+    }
+    __syncthreads();
+    const int kept = min(total, n);
+    if (threadIdx.x < kept) sm.buffer[threadIdx.x] = sm.best[threadIdx.x];
+    if (threadIdx.x == 0) sm.pushed = sm.n_best = kept;
+    __syncthreads();
+}
+
+// A cluster of CTAs reads a row, each a stretch of it in batches of 16 entries a thread.  A thread keeps the sum of its own entries; candidates for the alternatives are the entries
+// above a threshold that at least `top` known ones reach, so that after the first batch hardly any is looked at twice.
+template <typename T> __global__ void __launch_bounds__(THREADS) k_log_probs(const Args a) {
+    constexpr int VEC = Load<T>::VEC;
+    __shared__ Smem sm;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ranks, tid = threadIdx.x;
+    const T *x = (const T *)a.logits + row * a.ld;
+    const int skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)); // entries between the 16-byte boundary in front of the row and its start
+    const long long span = (long long)skew + a.vocab;
+    // stretches of whole vectors, as even as that allows
+    const long long vecs = (span + VEC - 1) / VEC, begin = vecs * rank / ranks * VEC, end = vecs * (rank + 1) / ranks * VEC;
+    if (tid == 0) { sm.pushed = 0; sm.n_best = 0; }
+    Sum mine = {-CUDART_INF_F, 0.0f, 0.0f};
+    u64 bar = 0; // keys that are not larger are no candidates
+    float bar_value = -CUDART_INF_F;
+    __syncthreads();
+    for (long long base = begin; base < end; base += BATCH) {
+        float v[PER_THREAD];
+#pragma unroll
+        for (int i = 0; i < PER_THREAD / VEC; i++) {
+            const long long at = base + ((long long)i * THREADS + tid) * VEC - skew; // index in the row
+            if (at >= 0 && at + VEC <= a.vocab && at + skew < end) Load<T>::vec(x + at, v + i * VEC);
+            else
+#pragma unroll
+                for (int j = 0; j < VEC; j++) v[i * VEC + j] = at + j >= 0 && at + j < a.vocab && at + skew < end ? Load<T>::one(x + at + j) : -CUDART_INF_F;
+        }
+        float top = v[0];
+#pragma unroll
+        for (int i = 1; i < PER_THREAD; i++) top = fmaxf(top, v[i]);
+        if (top > mine.m) { // a new largest entry: the sum goes on without its first one
+            Sum add = {top, 0.0f, 0.0f};
+            bool out = false;
+#pragma unroll
+            for (int i = 0; i < PER_THREAD; i++) {
+                const float y = v[i] - top;
+                const float e = !out && v[i] == top ? 0.0f : __expf(y);
+                out |= v[i] == top;
+                add.z += e;
+                add.s = fmaf(fmaxf(y, -1000.0f), e, add.s);
+            }
+            mine = join(add, mine);
+        } else {
+            const float ref = mine.m == -CUDART_INF_F ? 0.0f : mine.m;
+#pragma unroll
+            for (int i = 0; i < PER_THREAD; i++) {
+                const float y = v[i] - ref, e = __expf(y);
+                mine.z += e;
+                mine.s = fmaf(fmaxf(y, -1000.0f), e, mine.s);
+            }
+        }
+        if (a.top == 0) continue;
+        u64 largest = 0;
+        if (top >= bar_value)
+#pragma unroll
+            for (int i = 0; i < PER_THREAD; i++) {
+                const long long at = base + ((long long)(i / VEC) * THREADS + tid) * VEC + i % VEC;
+                const u64 k = key_of(v[i], (unsigned)(at - skew));
+                if (at >= skew && at < span && at < end && v[i] == v[i] && k > largest) largest = k;
+            }
+        const bool over = largest > bar;
+        const int n = __syncthreads_count(over);
+        if (n == 0) continue;
+        u64 least = bar + 1;
+        if (n > PUSHERS) { // at least `top` and at most PUSHERS threads hold a key from here on: half the interval at a time (the keys are no two alike, so such a bar exists)
+            u64 low = bar, high = ~0ull;
+            for (;;) {
+                least = low + (high - low) / 2;
+                const int above = __syncthreads_count(over && largest >= least);
+                if (above > PUSHERS) low = least;
+                else if (above < a.top) high = least;
+                else break;
+            }
+        }
+        if (sm.pushed + PUSHERS * PER_THREAD > BUFFER) { // (the same for every thread: the barrier above follows the last push)
+            __syncthreads();
+            select(sm, sm.pushed, a.top);
+            if (sm.n_best == a.top && sm.buffer[a.top - 1] > bar) { bar = sm.buffer[a.top - 1]; bar_value = value_of(bar); }
+        }
+        __syncthreads();
+        if (over && largest >= least)
+#pragma unroll
+            for (int i = 0; i < PER_THREAD; i++) {
+                const long long at = base + ((long long)(i / VEC) * THREADS + tid) * VEC + i % VEC;
+                const u64 k = key_of(v[i], (unsigned)(at - skew));
+                if (at >= skew && at < span && at < end && v[i] == v[i] && k >= least) sm.buffer[atomicAdd(&sm.pushed, 1)] = k;
+            }
+        if (n > PUSHERS && least > bar) { // `top` candidates reach it
+            bar = least - 1;
+            bar_value = value_of(least);
+        }
+    }
+    // ---- join: threads, then CTAs -------------------------------------------------------------------------------------------------------------------------------
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const Sum other = {__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.z, o), __shfl_xor_sync(0xffffffffu, mine.s, o)};
+        mine = join(mine, other);
+    }
+    if ((tid & 31) == 0) sm.warps[tid >> 5] = mine;
+    __syncthreads();
+    if (a.top) select(sm, sm.pushed, a.top);
+    if (tid == 0) {
+        Sum all = sm.warps[0];
+        for (int w = 1; w < THREADS / 32; w++) all = join(all, sm.warps[w]);
+        sm.cta = all;
+    }
+    if (ranks > 1) cluster.sync(); else __syncthreads();
+    if (rank == 0) {
+        Sum all = sm.cta;
+        for (int r = 1; r < ranks; r++) all = join(all, *cluster.map_shared_rank(&sm.cta, r));
+        const float log_z = all.m < CUDART_INF_F ? log1pf(all.z) : CUDART_NAN_F; // (an infinite logit, or none that is not -inf)
+        const float inv = 1.0f / (1.0f + all.z);
+        const bool none = !(all.m > -CUDART_INF_F);
+        if (tid == 0) {
+            if (a.logprobs) {
+                const int t = a.targets ? a.targets[row] : -1;
+                a.logprobs[row] = t < 0 || t >= a.vocab ? 0.0f : none ? CUDART_NAN_F : Load<T>::one(x + t) - all.m - log_z;
+            }
+            if (a.entropy) a.entropy[row] = none ? CUDART_NAN_F : log_z - all.s * inv;
+        }
+        if (a.top) {
+            for (int i = tid; i < ranks * MAX_TOP; i += THREADS) {
+                const int r = i / MAX_TOP, j = i % MAX_TOP;
+                if (j >= *cluster.map_shared_rank(&sm.n_best, r)) continue;
+                const u64 k = *cluster.map_shared_rank(&sm.best[j], r);
+                int place = 0;
+                for (int q = 0; q < ranks; q++) { // every CTA's keys are in order: half of them at a time
+                    const u64 *best = cluster.map_shared_rank(sm.best, q);
+                    int low = 0, high = *cluster.map_shared_rank(&sm.n_best, q);
+                    while (low < high) {
+                        const int mid = (low + high) / 2;
+                        if (best[mid] > k) low = mid + 1; else high = mid;
+                    }
+                    place += low;
+                }
+                if (place < a.top) sm.merged[place] = k;
+            }
+            int have = 0;
+            for (int r = 0; r < ranks; r++) have += *cluster.map_shared_rank(&sm.n_best, r);
+            __syncthreads();
+            if (tid < a.top) { // fewer than `top` numbers in the row: -1
+                const bool is = tid < have;
+                const u64 k = is ? sm.merged[tid] : 0;
+                if (a.top_ids) a.top_ids[(size_t)row * a.top + tid] = is ? (int)index_of(k) : -1;
+                if (a.top_logprobs) a.top_logprobs[(size_t)row * a.top + tid] = none || !is ? CUDART_NAN_F : value_of(k) - all.m - log_z;
+            }
+        }
+    }
+    if (ranks > 1) cluster.sync(); // no CTA leaves while the first one reads its part
+}
+
+} // namespace lp

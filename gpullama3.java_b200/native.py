@@ -71,7 +71,28 @@ class Tensor(C.Structure):
                 ("dims", C.c_int64 * 4)]
 
 
-EXPORTS = ["b200_plan_create_layered", "b200_forward_batch_logits", "b200_layered_info", "b200_plan_create", "b200_forward_decode", "b200_forward_prefill", "b200_forward_batch_prefill", "b200_set_prefill_mode", "b200_prefill_info", "b200_exact_prefill_info",
+class KV4Append(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n", "heads", "type", "rope_layout")] + [(n, C.c_void_p) for n in ("q", "k", "v")] + \
+               [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + [("positions", C.c_void_p), ("slots", C.c_void_p)] + \
+               [("start", C.c_int32), ("slot", C.c_int32)] + [(n, C.c_void_p) for n in ("q_norm", "k_norm", "cos", "sin")] + [("eps", C.c_float), ("q_out", C.c_void_p)]
+
+
+class KV4Attention(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n", "heads", "window", "max_len", "chunk", "out_type")] + [("q", C.c_void_p), ("out", C.c_void_p)] + \
+               [("q_stride", C.c_int64), ("out_stride", C.c_int64), ("positions", C.c_void_p), ("slots", C.c_void_p), ("start", C.c_int32), ("slot", C.c_int32), ("scale", C.c_float)]
+
+
+class KV4Read(C.Structure):
+    _fields_ = [("n", C.c_int32), ("type", C.c_int32)] + [(n, C.c_void_p) for n in ("k", "v", "positions", "slots")] + [("start", C.c_int32), ("slot", C.c_int32)]
+
+
+class LogProbs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_int64)] + [(n, C.c_int32) for n in ("rows", "vocab", "type", "top", "device")] + \
+               [(n, C.c_void_p) for n in ("targets", "logprobs", "entropy", "top_ids", "top_logprobs")]
+
+
+EXPORTS = ["b200_kv4_create", "b200_kv4_free", "b200_kv4_reset", "b200_kv4_device_bytes", "b200_kv4_last_error", "b200_kv4_append", "b200_kv4_attention", "b200_kv4_read", "b200_log_probs",
+           "b200_plan_create_layered", "b200_forward_batch_logits", "b200_layered_info", "b200_plan_create", "b200_forward_decode", "b200_forward_prefill", "b200_forward_batch_prefill", "b200_set_prefill_mode", "b200_prefill_info", "b200_exact_prefill_info",
            "b200_set_decode_mode", "b200_decode_info", "b200_trace_persistent", "b200_test_seqsum2", "b200_test_exact_prefill_wait", "b200_test_exact_prefill_wait_form", "b200_forward_decode_sample", "b200_upload_info", "b200_requant_kquant",
            "b200_decode_sequence", "b200_time_kernel", "b200_tp_handle", "b200_tp_attach", "b200_trace_decode", "b200_profile_norm", "b200_test_seqsum", "b200_gemm_f16", "b200_kv_reset", "b200_read_buffer", "b200_launches_per_decode",
            "b200_device_bytes", "b200_plan_free", "b200_last_error", "b200_version"]
@@ -124,6 +145,15 @@ def lib() -> C.CDLL:
     L.b200_last_error.argtypes = [vp]
     L.b200_last_error.restype = C.c_char_p
     L.b200_version.restype = C.c_char_p
+    L.b200_kv4_create.argtypes = [i32, i32, i32, i32, i32, C.POINTER(vp), C.c_char_p, C.c_size_t]
+    L.b200_kv4_free.argtypes, L.b200_kv4_free.restype = [vp], None
+    L.b200_kv4_reset.argtypes = [vp, vp]
+    L.b200_kv4_device_bytes.argtypes, L.b200_kv4_device_bytes.restype = [vp], C.c_int64
+    L.b200_kv4_last_error.argtypes, L.b200_kv4_last_error.restype = [vp], C.c_char_p
+    L.b200_kv4_append.argtypes = [vp, vp, vp]
+    L.b200_kv4_attention.argtypes = [vp, vp, vp]
+    L.b200_kv4_read.argtypes = [vp, vp, vp]
+    L.b200_log_probs.argtypes = [vp, vp, C.c_char_p, C.c_size_t]
     _lib = L
     return L
 

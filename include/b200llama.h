@@ -483,6 +483,80 @@ int b200_gemm_f16(const uint16_t *a, const uint16_t *b, float *c, int32_t m, int
  * stream -> double-buffered device staging -> repack kernel on the plan's stream; B200_UPLOAD_SYNC=1 selects blocking copies. */
 int b200_upload_info(b200_plan *plan, double *seconds, double *host_copy_seconds, int64_t *h2d_bytes);
 
+/* ---- operators on device memory ------------------------------------------------------------------------------------------------------
+ * These take DEVICE pointers and a stream (a cudaStream_t; NULL: the legacy default stream) of the device that they name, launch on it and return without a wait: what goes wrong
+ * on the device shows at the caller's next synchronisation.  They allocate nothing, use no workspace, keep nothing between calls and can be captured into CUDA graphs; the calling
+ * thread's current device is left as it was.  Nothing of this exists in the reference. */
+
+/* A key/value cache that holds a head's entries in 4 bits: groups of 32 neighbouring entries with one FP16 scale d, codes c of 0 .. 15, value d * (c - 8).  m = the entry of largest
+ * magnitude (the first of equal ones), d = f16(m / -8) (saturating), c = clamp(rint(x / d) + 8, 0, 15), 8 where d = 0; a group with an infinity or NaN reads as NaN.  4.5 bits an
+ * entry.  `slots` independent sequences (or layers) of `context` positions; head sizes 32, 64, 96, 128, 256.  Created empty: every position reads as zeros.
+ * Calls on one cache that append to and read the same positions are ordered by the caller (one stream, or events); otherwise several streams may use a cache at once.  The error
+ * message belongs to the cache: one thread at a time calls into it. */
+typedef struct b200_kv4 b200_kv4;
+int b200_kv4_create(int32_t slots, int32_t context, int32_t kv_heads, int32_t head_size, int32_t device, b200_kv4 **out, char *err, size_t err_len);
+void b200_kv4_free(b200_kv4 *kv); /* waits for the device's work */
+int b200_kv4_reset(b200_kv4 *kv, void *stream); /* every position of every slot reads as zeros again */
+int64_t b200_kv4_device_bytes(const b200_kv4 *kv);
+const char *b200_kv4_last_error(const b200_kv4 *kv);
+
+/* The rows of a call: row r belongs to position `positions ? positions[r] : start + r` of slot `slots ? slots[r] : slot` (device arrays of n).  A row whose slot lies outside
+ * [0, slots) or whose position lies behind the cache is padding: nothing is read, stored or written for it.  A negative position is a row without keys. */
+
+/* Rows of a QKV product -> cache.  k, v: n rows of kv_heads heads, q (heads > 0): of `heads` heads; `type` (B200_GGML_F32, _F16, _BF16) and the strides between rows, in entries, are
+ * free (parts of one wider row).  q_norm / k_norm (FP32 [head_size], nullable): every head of q / k is RMS-normed, w * (x * s) with s = 1 / sqrt(mean(x^2) + eps) computed in 64 bits;
+ * cos / sin (FP32 [context][head_size / 2], nullable): then rotated, pairs by rope_layout.  v is stored as it is.  q_out receives the queries in FP32 (it may not overlap q).
+ * A row of a negative position is not stored and its q_out not written.  Two rows of a call must not name the same place. */
+typedef struct b200_kv4_append_args {
+    int32_t n, heads, type, rope_layout; /* B200_ROPE_* */
+    const void *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const int32_t *positions, *slots;
+    int32_t start, slot;
+    const float *q_norm, *k_norm, *cos, *sin;
+    float eps;
+    float *q_out;
+} b200_kv4_append_args;
+int b200_kv4_append(b200_kv4 *kv, const b200_kv4_append_args *args, void *stream);
+
+/* Causal attention of n query rows over the cache: row r at position p sees the positions j <= p of its slot, the last `window` of them where window > 0; query head h reads key/value
+ * head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type.  A row that sees nothing is zeros.  max_len (0: unknown) is the largest position + 1 as far as the host
+ * knows, chunk (0 or 1: single steps) how many neighbouring rows are successive tokens of one sequence: both only choose how the work is split. */
+typedef struct b200_kv4_attention_args {
+    int32_t n, heads, window, max_len, chunk, out_type;
+    const float *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    const int32_t *positions, *slots;
+    int32_t start, slot;
+    float scale;
+} b200_kv4_attention_args;
+int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *args, void *stream);
+
+/* The values that the cache holds at n rows: k and v [n][kv_heads][head_size] in `type`.  A row of a negative position is left as it was. */
+typedef struct b200_kv4_read_args {
+    int32_t n, type;
+    void *k, *v;
+    const int32_t *positions, *slots;
+    int32_t start, slot;
+} b200_kv4_read_args;
+int b200_kv4_read(b200_kv4 *kv, const b200_kv4_read_args *args, void *stream);
+
+/* Of every row of logits ([rows][vocab], `type` B200_GGML_F32, _F16 or _BF16, row_stride entries apart): the log probability of token targets[row] (logprobs; 0 where the target lies
+ * outside the vocabulary, as for "no target", or where targets is NULL), the entropy of the distribution in nats, and the `top` (0 .. 32, at most vocab) most likely tokens with their
+ * log probabilities, in order, equal ones by index (top_ids, top_logprobs [rows][top]).  Every output may be NULL.  A row with a NaN, with an infinite logit or with none above -inf has
+ * NaN for its numbers; NaN entries are no alternatives (id -1 where fewer than `top` are left). */
+typedef struct b200_log_probs_args {
+    const void *logits;
+    int64_t row_stride;
+    int32_t rows, vocab, type, top, device;
+    const int32_t *targets;
+    float *logprobs, *entropy;
+    int32_t *top_ids;
+    float *top_logprobs;
+} b200_log_probs_args;
+int b200_log_probs(const b200_log_probs_args *args, void *stream, char *err, size_t err_len);
+
 /* Number of kernels one decode step launches (bench.py's gpu_launches). */
 int b200_launches_per_decode(b200_plan *plan);
 

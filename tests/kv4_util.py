@@ -1,0 +1,90 @@
+"""Plain 64-bit forms of the 4-bit cache's operators (numpy / torch on the CPU), and the bounds that their kernels are held to."""
+import math
+
+import numpy as np
+import torch
+
+
+def quantize(x: torch.Tensor):
+    """Rows [..., hs] in FP32 -> (values in float64, scales in float64 [..., hs / 32]), by the definition: d = f16(m / -8), c = clamp(rint(x / d) + 8, 0, 15)."""
+    x = x.float().cpu().numpy()
+    g = x.reshape(*x.shape[:-1], -1, 32)
+    with np.errstate(all="ignore"):
+        m = np.take_along_axis(g, np.argmax(np.abs(np.nan_to_num(g, nan=0.0, posinf=np.inf, neginf=-np.inf)), -1)[..., None], -1)
+        d = np.clip(m * np.float32(-0.125), -65504, 65504).astype(np.float16).astype(np.float32)
+        c = np.where(d == 0, 0, np.clip(np.rint(g / np.where(d == 0, 1, d)), -8, 7))
+    bad = ~np.isfinite(g).all(-1, keepdims=True)
+    d = np.where(bad, np.nan, d)
+    v = c.astype(np.float64) * d.astype(np.float64)
+    return torch.from_numpy(np.where(bad, np.nan, v).reshape(x.shape)), torch.from_numpy(d[..., 0].astype(np.float64))
+
+
+def turn(x, weight, eps, cos, sin, positions, layout):
+    """Norm and rotation of rows [n, heads, hs] in float64."""
+    x = x.double().cpu()
+    if weight is not None:
+        x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * weight.double().cpu()
+    if cos is None:
+        return x
+    c, s = cos.double().cpu()[positions.long().cpu()][:, None], sin.double().cpu()[positions.long().cpu()][:, None]
+    h = x.shape[-1] // 2
+    y = torch.empty_like(x)
+    if layout == "half":
+        a, b = x[..., :h], x[..., h:]
+        y[..., :h], y[..., h:] = a * c - b * s, a * s + b * c
+    else:
+        a, b = x[..., 0::2], x[..., 1::2]
+        y[..., 0::2], y[..., 1::2] = a * c - b * s, a * s + b * c
+    return y
+
+
+def attention(q, k, v, d, positions, slots, scale, window):
+    """q [n, H, hs]; k, v [slots, context, G, hs] and key scales d [slots, context, G, hs / 32], all float64 on the CPU -> (out, bound) where bound is how far a kernel may be off
+    in FP32.
+
+    The bound: a query keeps 22 bits of its largest entry's magnitude and meets codes of at most 16 steps, so that a score's error is at most 2^-21 + hs 2^-24 (products and
+    sums in FP32) of A = scale * max|q| * sum over groups of 32 * 16 |d|; a probability's relative error is twice that error (numerator and sum), plus 2^-20 for its exponential;
+    its product with a value keeps 16 bits (2^-16), and sums of n products in FP32 add n 2^-24 at most.  All relative to sum p |v|."""
+    n, H, hs = q.shape
+    G = k.shape[2]
+    out, bound = torch.zeros_like(q), torch.zeros_like(q)
+    for r in range(n):
+        p, s = int(positions[r]), int(slots[r])
+        lo = max(0, p - window + 1) if window else 0
+        if p < 0:
+            continue
+        for h in range(H):
+            g = h // (H // G)
+            kk, vv = k[s, lo:p + 1, g], v[s, lo:p + 1, g]
+            x = kk @ q[r, h] * scale
+            w = torch.softmax(x, 0)
+            A = scale * q[r, h].abs().max() * d[s, lo:p + 1, g].abs().sum(-1).max() * 32 * 16
+            out[r, h] = w @ vv
+            bound[r, h] = (w @ vv.abs()) * (2 * A * (2.0 ** -21 + hs * 2.0 ** -24) + 2.0 ** -16 + 2.0 ** -20 + (p + 1 - lo) * 2.0 ** -24)
+    return out, bound
+
+
+def log_probs(x, targets, top):
+    """(logprobs, entropy, ids, values) in float64 of rows x."""
+    x = x.double().cpu()
+    lp = torch.log_softmax(x, -1)
+    p = lp.exp()
+    entropy = -(torch.where(p > 0, p * lp, torch.zeros_like(p))).sum(-1)
+    ids = torch.argsort(-x, dim=-1, stable=True)[:, :top]
+    t = targets.long().cpu()
+    ok = (t >= 0) & (t < x.shape[1])
+    chosen = torch.where(ok, lp.gather(1, t.clamp(0, x.shape[1] - 1)[:, None])[:, 0], torch.zeros(len(t), dtype=torch.float64))
+    return chosen, entropy, ids.int(), lp.gather(1, ids)
+
+
+def tables(context, hs, base=10000.0):
+    a = torch.arange(context, dtype=torch.float64)[:, None] * base ** (-torch.arange(0, hs, 2, dtype=torch.float64) / hs)
+    return a.cos().float(), a.sin().float()
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rsqrt(hs):
+    return 1.0 / math.sqrt(hs)
