@@ -94,6 +94,36 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+OPS_LIB = os.path.join(CSRC, "_b200ops.so")
+OPS_SRC = os.path.join(CSRC, "torch_ops.cpp")
+
+
+def _ops_command() -> list[str]:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    # torch's own libstdc++ (the shared one), also where the compiler would link a static copy into a shared object: two of them do not share their streams' tables
+    inc = [f"-I{d}" for d in [*cpp_extension.include_paths(), "/usr/local/cuda/include", sysconfig.get_paths()["include"]]]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *inc, "-o", OPS_LIB, OPS_SRC,
+            f"-L{CSRC}", "-l:libb200llama.so", f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-nostdlib++", "-l:libstdc++.so.6", "-lm", "-Wl,-rpath,$ORIGIN",
+            f"-Wl,-rpath,{lib}"]
+
+
+def build_operators(force: bool = False) -> str:
+    """_b200ops.so: the operators on torch tensors (csrc/torch_ops.cpp), linked against libb200llama.so next to it."""
+    hdr = os.path.join(HERE, "..", "include", "b200llama.h")
+    if not force and os.path.exists(OPS_LIB) and os.path.getmtime(OPS_LIB) >= max(os.path.getmtime(f) for f in (OPS_SRC, hdr, __file__)):
+        return OPS_LIB
+    r = subprocess.run(_ops_command(), capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError("g++ failed building _b200ops.so")
+    return OPS_LIB
+
+
 TOK_LIB = os.path.join(CSRC, "libb200tok.so")
 TOK_SRC = os.path.join(CSRC, "tokenizer.cpp")
 
@@ -113,4 +143,5 @@ def build_tokenizer(force: bool = False) -> str:
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True))
+    print(build_operators(force="--force" in sys.argv))
     print(build_tokenizer(force="--force" in sys.argv))

@@ -7,7 +7,7 @@
 //   key codes    [half: positions 0-7, 8-15][words of a lane / VW][lane = 4 g + t][VW words]: lane (g, t) holds position 8 * half + g, entries 32 grp + 8 t .. + 7 in word grp
 //   value codes  the same order; lane (g, t) holds positions 8 * half + 2 t, + 1 (low and high half of a word) and entries 32 grp + 4 g .. + 3
 //   key scales   [g][grp] words of two halves: positions g and g + 8; value scales likewise
-// These are the operands of mma.m16n8k16 as its lanes want them: a lane reads its words in one vector load without bank conflicts and a mask turns a word into register pairs.
+// These are the operands of mma.m16n8k16 as its lanes want them: a lane reads its words in one vector load without bank conflicts, and a word's eight codes are four register pairs.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -250,6 +250,7 @@ struct Step {
     void *out;
     int8_t *quants; // out_type KV4_OUT_Q8: blocks of 32
     float *scales;
+    float *work; // parts of units that several clusters share
 };
 
 __device__ __forceinline__ float ex2(float x) { // 2^x
@@ -261,18 +262,23 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { // d = a b
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+// The codes of a word as pairs of FP16 numbers c - 8: pair i holds nibbles i and i + 4.  The bits of 1024 + c (or 1024 + 16 c) come from a mask, the rest is one exact operation.  (A masked
+// code by itself is a number too, c 2^-24, but products of subnormals are added with as many bits less as they have leading zeros: 2^-17 in a score.)
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&c)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint32_t v = i ? w >> 8 : w, even = (v & 0x000f000fu) | 0x64006400u, odd = (v & 0x00f000f0u) | 0x64006400u;
+        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(c[2 * i]) : "r"(even), "r"(0x64086408u));                                    // - 1032
+        asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(c[2 * i + 1]) : "r"(odd), "r"(0x2c002c00u), "r"(0xd480d480u)); // / 16 - 72
+    }
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
@@ -290,60 +296,76 @@ template <int VW> __device__ __forceinline__ void lds_words(const uint32_t *p, u
         for (int i = 0; i < VW; i++) w[i] = p[i];
 }
 
-// Two BF16 codes (c - 8, exact) of nibble I (0 .. 3) of the word's low and high half: 128 + c by the bits alone, then -136.
-template <int I> __device__ __forceinline__ uint32_t codes_bf16(uint32_t w) {
-    const uint32_t u = (w >> (4 * I) & 0x000f000fu) | 0x43004300u;
-    uint32_t r;
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x43084308u));
-    return r;
-}
-
-constexpr int STEP_WARPS = 8, STEP_MAX_CLUSTER = 16;
+constexpr int STEP_WARPS = 8, STEP_MAX_CLUSTER = 8;
 __host__ __device__ constexpr int step_stages(int hs) { return hs >= 256 ? 3 : 4; }
 __host__ __device__ constexpr size_t step_ring_bytes(int hs) { return (size_t)STEP_WARPS * step_stages(hs) * record_bytes(hs); }
 __host__ __device__ constexpr size_t step_merge_bytes(int hs, int heads) { return (size_t)(STEP_WARPS + 1) * heads * (hs + 2) * 4; } // the warps' parts and the CTA's
 __host__ __device__ constexpr size_t step_smem_bytes(int hs, int heads) { return step_ring_bytes(hs) > step_merge_bytes(hs, heads) ? step_ring_bytes(hs) : step_merge_bytes(hs, heads); }
 
+// The bounds of what row r sees: positions [lo, hi); none: lo >= hi.
+__device__ __forceinline__ void visible(int pos, int window, int &lo, int &hi) {
+    lo = window > 0 && pos >= window ? pos - window + 1 : 0;
+    hi = pos + 1;
+}
+// One entry of a result row (whole warps, 32 neighbouring entries, where the blocks of 32 quants want them).
+__device__ __forceinline__ void put_result(const Step &a, int row, size_t at, float v, bool on) {
+    if (a.out_type == KV4_OUT_Q8) {
+        float as;
+        const int qv = quant_block_lane(v, as);
+        if (on) {
+            a.quants[row * a.ldo + at] = (int8_t)qv;
+            if ((threadIdx.x & 31) == 0) a.scales[(row * a.ldo + at) / 32] = as;
+        }
+    } else if (!on) return;
+    else if (a.out_type == B200_GGML_F32) ((float *)a.out)[row * a.ldo + at] = v;
+    else if (a.out_type == B200_GGML_F16) put((__half *)a.out + row * a.ldo + at, v);
+    else put((bf16 *)a.out + row * a.ldo + at, v);
+}
+
 // One query row and up to 4 NT query heads of a key/value head: the row's visible positions are split over the warps of a cluster of CTAs, each warp runs through its records
-// (cp.async ring of its own, no barrier in the loop) with its own running maximum, and the parts are joined in shared memory, then over the cluster: one launch, no workspace,
-// nothing that depends on an order of arrival.
-//   scores  C[16 positions x 8] = codes (FP16: a masked code IS a subnormal, c 2^-24, exact) x queries; the eight columns are four heads, each as a high and a low FP16 part, so that
-//           a query keeps 22 bits; accumulators start at -8 sum q (the codes' offset) and are scaled group by group in FP32
-//   values  C[16 entries x 8] = codes - 8 (BF16, exact) x (p d), again as a high and a low part (16 bits, FP32's range: no scale of the values under- or overflows)
+// (cp.async ring of its own, no barrier in the loop) with its own running maximum, and the parts are joined in shared memory, then over the cluster.  Where 8 CTAs a unit leave SMs
+// idle, `splits` clusters share a unit: their parts go to the workspace, and k_step_join joins them.  Nothing depends on an order of arrival.
+//   scores  C[16 positions x 8] = codes x queries in FP16; the eight columns are four heads, each as a high and a low part, so that a query keeps 22 bits; scaled group by group in FP32
+//   values  C[16 entries x 8] = codes x (p d), again as a high and a low part.  p d is kept in FP16's range by a power of two that follows the largest value scale seen so far
 // A lane keeps the running sums of ONE head (t); what crosses lanes in the loop is the transposition of the probabilities and, where a maximum grows by more than 2^8, its update.
-template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_step(const Step a, const int units_per_head) {
+template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_step(const Step a, const int units_per_head, const int splits) {
     constexpr int NG = groups(HS), VW = vec_words(HS), R = record_bytes(HS), S = step_stages(HS), H = 4 * NT, CHUNKS = R / 16;
     extern __shared__ __align__(16) unsigned char smem[];
     pdl_wait();
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int G = a.kv.kv_heads, mul = a.heads / G;
-    const int unit = blockIdx.x / ranks, row = unit / (G * units_per_head), kvh = unit / units_per_head % G, first = unit % units_per_head * H; // first head within the group
+    const int split = blockIdx.x / ranks % splits, unit = blockIdx.x / ranks / splits, row = unit / (G * units_per_head), kvh = unit / units_per_head % G;
+    const int first = unit % units_per_head * H; // first head within the group
     const int pos = a.rows.position(row), slot = a.rows.slot_of(row);
     if (slot < 0 || slot >= a.kv.slots || pos >= a.kv.context) return; // a padding row (the whole cluster leaves)
-    const int lo = a.window > 0 && pos >= a.window ? pos - a.window + 1 : 0, hi = pos + 1;
-    const int b0 = lo / BLOCK, nb = hi > lo ? (hi + BLOCK - 1) / BLOCK - b0 : 0, per = (nb + ranks * STEP_WARPS - 1) / (ranks * STEP_WARPS);
-    const int begin = b0 + min(nb, (rank * STEP_WARPS + warp) * per), end = b0 + min(nb, (rank * STEP_WARPS + warp + 1) * per);
+    int lo, hi;
+    visible(pos, a.window, lo, hi);
+    const int workers = splits * ranks * STEP_WARPS, worker = (split * ranks + rank) * STEP_WARPS + warp;
+    const int b0 = lo / BLOCK, nb = hi > lo ? (hi + BLOCK - 1) / BLOCK - b0 : 0, per = (nb + workers - 1) / workers;
+    const int begin = b0 + min(nb, worker * per), end = b0 + min(nb, (worker + 1) * per);
 
     unsigned char *ring = smem + (size_t)warp * S * R;
-    const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
-    const unsigned char *src = record<HS>(a.kv, slot, kvh, 0);
-    auto fetch = [&](int block, int stage) {
-        if (block < end) {
-            const unsigned char *s = src + (size_t)block * R + lane * 16;
-            const uint32_t d = ring_addr + stage * R + lane * 16;
+    const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
+    const unsigned char *src = record<HS>(a.kv, slot, kvh, begin) + lane * 16;
+    int fetched = begin;
+    auto fetch = [&](int stage) {
+        if (fetched < end) {
+            const uint32_t d = ring_addr + stage * R;
 #pragma unroll
-            for (int i = 0; i < CHUNKS / 32; i++) cp16(d + i * 512, s + i * 512);
-            if (CHUNKS % 32 && lane < CHUNKS % 32) cp16(d + CHUNKS / 32 * 512, s + CHUNKS / 32 * 512);
+            for (int i = 0; i < CHUNKS / 32; i++) cp16(d + i * 512, src + i * 512);
+            if (CHUNKS % 32 && lane < CHUNKS % 32) cp16(d + CHUNKS / 32 * 512, src + CHUNKS / 32 * 512);
+            src += R;
+            fetched++;
         }
         cp_commit();
     };
 #pragma unroll
-    for (int i = 0; i < S - 1; i++) fetch(begin + i, i);
+    for (int i = 0; i < S - 1; i++) fetch(i);
 
     // queries: lane (g, t) holds column g = head g >> 1, part g & 1, of entries 32 grp + 8 t .. + 7
     uint32_t qf[NT][NG][4];
-    float off[NT][NG], sc[NT]; // of head t: -8 sum q of every group, and what turns a sum into a score in units of log2
+    float sc[NT]; // of head t: what turns a sum into a score in units of log2
 #pragma unroll
     for (int n = 0; n < NT; n++) {
         const int h = first + 4 * n + (g >> 1);
@@ -363,22 +385,16 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
         const float up = __uint_as_float((unsigned)(263 - e) << 23), down = __uint_as_float((unsigned)(e - 9) << 23);
 #pragma unroll
         for (int grp = 0; grp < NG; grp++) {
-            float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 x[grp][i] *= up;
-                sum += x[grp][i];
-                if (i & 2) x[grp][i] *= 0.0625f; // these meet codes in bits 4 - 7: 16 c
                 const float high = __half2float(__float2half_rn(x[grp][i]));
                 x[grp][i] = g & 1 ? x[grp][i] - high : high;
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) qf[n][grp][i] = pack_f16(x[grp][2 * i], x[grp][2 * i + 1]);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            off[n][grp] = __shfl_sync(0xffffffffu, sum, 8 * t) * (-8.0f * 5.9604644775390625e-8f);
         }
-        sc[n] = __shfl_sync(0xffffffffu, down, 8 * t) * 16777216.0f * (a.scale * 1.4426950408889634f);
+        sc[n] = __shfl_sync(0xffffffffu, down, 8 * t) * (a.scale * 1.4426950408889634f);
     }
 
     float m[NT], l[NT], o[NT][2 * NG][4];
@@ -388,90 +404,121 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
 #pragma unroll
         for (int i = 0; i < 2 * NG; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
     }
+    int lift = 0;            // p d is held times 2^lift
+    uint32_t most = 0u;      // scales up to here (their bits) have been seen: 2^lift * scale < 2^7
     int stage = 0;
+#pragma unroll 1
     for (int block = begin; block < end; block++) {
         cp_wait<S - 2>();
         __syncwarp(); // and every lane has read the stage that the next copy overwrites
-        fetch(block + S - 1, stage == 0 ? S - 1 : stage - 1);
+        fetch(stage == 0 ? S - 1 : stage - 1);
         const uint32_t *words = reinterpret_cast<const uint32_t *>(ring + stage * R);
         const uint32_t *ks = words + 4 * HS + g * NG, *vs = ks + 8 * NG; // scales of positions g and g + 8
-        const int p0 = block * BLOCK + g;
-        const bool see0 = p0 >= lo && p0 < hi, see1 = p0 + 8 >= lo && p0 + 8 < hi;
         float s[NT][2];
+        uint32_t dv[NG];
 #pragma unroll
         for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = 0.0f;
 #pragma unroll
         for (int v = 0; v < NG / VW; v++) {
-            uint32_t wa[VW], wb[VW], d[VW];
+            uint32_t wa[VW], wb[VW], d[VW], dw[VW];
             lds_words<VW>(words + word_of<HS>(0, lane, v * VW), wa);
             lds_words<VW>(words + word_of<HS>(1, lane, v * VW), wb);
             lds_words<VW>(ks + v * VW, d);
+            lds_words<VW>(vs + v * VW, dw);
 #pragma unroll
             for (int i = 0; i < VW; i++) {
                 const int grp = v * VW + i;
-                const uint32_t c0[4] = {wa[i] & 0x000f000fu, wb[i] & 0x000f000fu, wa[i] & 0x00f000f0u, wb[i] & 0x00f000f0u};
-                const uint32_t ha = wa[i] >> 8, hb = wb[i] >> 8;
-                const uint32_t c1[4] = {ha & 0x000f000fu, hb & 0x000f000fu, ha & 0x00f000f0u, hb & 0x00f000f0u};
+                dv[grp] = dw[i];
+                uint32_t ca[4], cb[4];
+                unpack(wa[i], ca);
+                unpack(wb[i], cb);
+                const uint32_t c0[4] = {ca[0], cb[0], ca[1], cb[1]}, c1[4] = {ca[2], cb[2], ca[3], cb[3]};
                 const float2 dk = __half22float2(*reinterpret_cast<const __half2 *>(&d[i]));
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    float acc[4] = {off[n][grp], 0.0f, off[n][grp], 0.0f};
-                    mma_f16(acc, c0, qf[n][grp][0], qf[n][grp][1]);
+                    float acc[4];
+                    mma_f16_first(acc, c0, qf[n][grp][0], qf[n][grp][1]);
                     mma_f16(acc, c1, qf[n][grp][2], qf[n][grp][3]);
                     s[n][0] = fmaf(dk.x, acc[0] + acc[1], s[n][0]);
                     s[n][1] = fmaf(dk.y, acc[2] + acc[3], s[n][1]);
                 }
             }
         }
-        float p[NT][2];
-        bool grow = false;
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            s[n][0] = see0 ? s[n][0] * sc[n] : -CUDART_INF_F;
-            s[n][1] = see1 ? s[n][1] * sc[n] : -CUDART_INF_F;
-            grow |= fmaxf(s[n][0], s[n][1]) > m[n] + 8.0f;
+        for (int n = 0; n < NT; n++) { s[n][0] *= sc[n]; s[n][1] *= sc[n]; }
+        if (block * BLOCK < lo || block * BLOCK + BLOCK > hi) { // an end of what the row sees: whatever stands behind it has no weight and no scale
+            const int p0 = block * BLOCK + g;
+            const bool see0 = p0 >= lo && p0 < hi, see1 = p0 + 8 >= lo && p0 + 8 < hi;
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                if (!see0) s[n][0] = -CUDART_INF_F;
+                if (!see1) s[n][1] = -CUDART_INF_F;
+            }
+#pragma unroll
+            for (int grp = 0; grp < NG; grp++) dv[grp] &= (see0 ? 0xffffu : 0u) | (see1 ? 0xffff0000u : 0u);
         }
-        if (__any_sync(0xffffffffu, grow))
+        uint32_t all = 0; // not below any of the scales: their bits together
+#pragma unroll
+        for (int grp = 0; grp < NG; grp++) all |= dv[grp];
+        bool rare = (all & 0x7fffu) > most || (all >> 16 & 0x7fffu) > most;
+#pragma unroll
+        for (int n = 0; n < NT; n++) rare |= fmaxf(s[n][0], s[n][1]) > m[n] + 8.0f;
+        if (__any_sync(0xffffffffu, rare)) {
+            uint32_t big = 0;
+#pragma unroll
+            for (int grp = 0; grp < NG; grp++) big = max(big, max(dv[grp] & 0x7fffu, dv[grp] >> 16 & 0x7fffu));
+            big = __reduce_max_sync(0xffffffffu, big);
+            float beta = 1.0f;
+            if (big > most && big <= 0x7c00u) { // (a NaN changes nothing)
+                const int was = lift;
+                lift = 21 - (int)(big >> 10); // the scale is below 2^(big >> 10 - 14)
+                if (most) beta = __uint_as_float((unsigned)(127 + lift - was) << 23); // (no sums before the first scale)
+                most = big | 0x3ffu;
+            }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 float mx = fmaxf(s[n][0], s[n][1]);
 #pragma unroll
                 for (int i = 4; i < 32; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
                 mx = fmaxf(mx, m[n]);
-                const float alpha = m[n] == mx ? 1.0f : ex2(m[n] - mx);
+                const float alpha = m[n] == mx ? 1.0f : ex2(m[n] - mx), gamma = alpha * beta;
                 m[n] = mx;
                 l[n] *= alpha;
 #pragma unroll
-                for (int i = 0; i < 2 * NG; i++) { o[n][i][0] *= alpha; o[n][i][1] *= alpha; o[n][i][2] *= alpha; o[n][i][3] *= alpha; }
+                for (int i = 0; i < 2 * NG; i++) { o[n][i][0] *= gamma; o[n][i][1] *= gamma; o[n][i][2] *= gamma; o[n][i][3] *= gamma; }
             }
+        }
+        float p[NT][2];
+        const float two_to_lift = __uint_as_float((unsigned)(127 + lift) << 23);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const float ref = m[n] == -CUDART_INF_F ? 0.0f : m[n]; // nothing seen yet: 2^(-inf) = 0
             p[n][0] = ex2(s[n][0] - ref);
             p[n][1] = ex2(s[n][1] - ref);
             l[n] += p[n][0] + p[n][1];
+            p[n][0] *= two_to_lift;
+            p[n][1] *= two_to_lift;
         }
 #pragma unroll
         for (int v = 0; v < NG / VW; v++) {
-            uint32_t wa[VW], wb[VW], d[VW];
+            uint32_t wa[VW], wb[VW];
             lds_words<VW>(words + 2 * HS + word_of<HS>(0, lane, v * VW), wa);
             lds_words<VW>(words + 2 * HS + word_of<HS>(1, lane, v * VW), wb);
-            lds_words<VW>(vs + v * VW, d);
 #pragma unroll
             for (int i = 0; i < VW; i++) {
                 const int grp = v * VW + i;
-                float2 dv = __half22float2(*reinterpret_cast<const __half2 *>(&d[i]));
-                if (!see0) dv.x = 0.0f; // whatever stands behind the mask
-                if (!see1) dv.y = 0.0f;
-                const uint32_t c0[4] = {codes_bf16<0>(wa[i]), codes_bf16<1>(wa[i]), codes_bf16<0>(wb[i]), codes_bf16<1>(wb[i])};
-                const uint32_t c1[4] = {codes_bf16<2>(wa[i]), codes_bf16<3>(wa[i]), codes_bf16<2>(wb[i]), codes_bf16<3>(wb[i])};
+                const float2 d = __half22float2(*reinterpret_cast<const __half2 *>(&dv[grp]));
+                uint32_t ca[4], cb[4];
+                unpack(wa[i], ca);
+                unpack(wb[i], cb);
+                const uint32_t c0[4] = {ca[0], ca[1], cb[0], cb[1]}, c1[4] = {ca[2], ca[3], cb[2], cb[3]};
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    const float x0 = p[n][0] * dv.x, x1 = p[n][1] * dv.y;
-                    const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffff0000u), h1 = __uint_as_float(__float_as_uint(x1) & 0xffff0000u);
-                    const uint32_t f0 = transpose8x8(pack_bf16(h0, x0 - h0)), f1 = transpose8x8(pack_bf16(h1, x1 - h1));
-                    mma_bf16(o[n][2 * grp], c0, f0, f1);
-                    mma_bf16(o[n][2 * grp + 1], c1, f0, f1);
+                    const float x0 = p[n][0] * d.x, x1 = p[n][1] * d.y; // the high part: the 11 bits that FP16 has, cut off
+                    const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(x1) & 0xffffe000u);
+                    const uint32_t f0 = transpose8x8(pack_f16(h0, x0 - h0)), f1 = transpose8x8(pack_f16(h1, x1 - h1));
+                    mma_f16(o[n][2 * grp], c0, f0, f1);
+                    mma_f16(o[n][2 * grp + 1], c1, f0, f1);
                 }
             }
         }
@@ -480,8 +527,9 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
     cp_wait<0>();
     __syncthreads();
 
-    // ---- join: warps, then CTAs -------------------------------------------------------------------------------------------------------------------------------
+    // ---- join: warps, then CTAs, then (through the workspace) clusters -------------------------------------------------------------------------------------------
     float *part = reinterpret_cast<float *>(smem), *pm = part + (STEP_WARPS + 1) * H * HS, *pl = pm + (STEP_WARPS + 1) * H; // [warp, or the CTA's][head][entry]
+    const float unit_of = __uint_as_float((unsigned)(127 - lift) << 23);
 #pragma unroll
     for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -491,7 +539,8 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
 #pragma unroll
         for (int grp = 0; grp < NG; grp++)
             *reinterpret_cast<float4 *>(part + (warp * H + h) * HS + grp * 32 + g * 4) =
-                make_float4(o[n][2 * grp][0] + o[n][2 * grp][1], o[n][2 * grp][2] + o[n][2 * grp][3], o[n][2 * grp + 1][0] + o[n][2 * grp + 1][1], o[n][2 * grp + 1][2] + o[n][2 * grp + 1][3]);
+                make_float4((o[n][2 * grp][0] + o[n][2 * grp][1]) * unit_of, (o[n][2 * grp][2] + o[n][2 * grp][3]) * unit_of, (o[n][2 * grp + 1][0] + o[n][2 * grp + 1][1]) * unit_of,
+                            (o[n][2 * grp + 1][2] + o[n][2 * grp + 1][3]) * unit_of);
     }
     __syncthreads();
     const int mine = STEP_WARPS * H; // rows behind the warps': the CTA's
@@ -512,7 +561,7 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
     }
     if (ranks > 1) cluster.sync(); else __syncthreads();
     const int slice = H * HS / ranks;
-    for (int j = threadIdx.x; j < slice; j += STEP_WARPS * 32) { // (whole warps: slice is a multiple of 32 where the blocks of 32 below need it)
+    for (int j = threadIdx.x; j < slice; j += STEP_WARPS * 32) { // (whole warps: slice is a multiple of 32 where blocks of 32 quants need it)
         const int i = rank * slice + j, h = i / HS;
         float M = -CUDART_INF_F, L = 0.0f, O = 0.0f;
         for (int r = 0; r < ranks; r++) M = fmaxf(M, *cluster.map_shared_rank(pm + mine + h, r));
@@ -522,22 +571,40 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
             L = fmaf(f, *cluster.map_shared_rank(pl + mine + h, r), L);
             O = fmaf(f, *cluster.map_shared_rank(part + mine * HS + i, r), O);
         }
-        const float v = hi <= lo ? 0.0f : O / L; // a row that sees nothing: zeros
-        const bool on = first + h < mul;
-        const size_t at = (size_t)(kvh * mul + first + h) * HS + i % HS;
-        if (a.out_type == KV4_OUT_Q8) {
-            float as;
-            const int qv = quant_block_lane(v, as);
-            if (on) {
-                a.quants[row * a.ldo + at] = (int8_t)qv;
-                if (lane == 0) a.scales[(row * a.ldo + at) / 32] = as;
+        if (splits > 1) { // [row][head][split]: maximum, sum, entries
+            if (first + h < mul) {
+                float *w = a.work + (((size_t)row * a.heads + kvh * mul + first + h) * splits + split) * (HS + 2);
+                w[2 + i % HS] = O;
+                if (i % HS == 0) { w[0] = M; w[1] = L; }
             }
-        } else if (!on) continue;
-        else if (a.out_type == B200_GGML_F32) ((float *)a.out)[row * a.ldo + at] = v;
-        else if (a.out_type == B200_GGML_F16) put((__half *)a.out + row * a.ldo + at, v);
-        else put((bf16 *)a.out + row * a.ldo + at, v);
+        } else put_result(a, row, (size_t)(kvh * mul + first + h) * HS + i % HS, hi <= lo ? 0.0f : O / L, first + h < mul); // a row that sees nothing: zeros
     }
     if (ranks > 1) cluster.sync(); // no CTA leaves while another reads its part
+}
+
+// Joins the splits of a unit: one thread an entry.
+template <int HS> __global__ void __launch_bounds__(HS < 64 ? 64 : HS) k_step_join(const Step a, const int splits) {
+    constexpr int HEADS = HS < 64 ? 64 / HS : 1; // heads of a CTA
+    pdl_wait();
+    const int h = blockIdx.x % ((a.heads + HEADS - 1) / HEADS) * HEADS + threadIdx.x / HS, row = blockIdx.x / ((a.heads + HEADS - 1) / HEADS), i = threadIdx.x % HS;
+    const int pos = a.rows.position(row), slot = a.rows.slot_of(row);
+    if (slot < 0 || slot >= a.kv.slots || pos >= a.kv.context) return;
+    const bool on = h < a.heads;
+    int lo, hi;
+    visible(pos, a.window, lo, hi);
+    float M = -CUDART_INF_F, L = 0.0f, O = 0.0f;
+    if (on && hi > lo) {
+        const float *w = a.work + ((size_t)row * a.heads + h) * splits * (HS + 2);
+        for (int s = 0; s < splits; s++) M = fmaxf(M, w[s * (HS + 2)]);
+        const float ref = M == -CUDART_INF_F ? 0.0f : M;
+#pragma unroll 4
+        for (int s = 0; s < splits; s++) {
+            const float f = ex2(w[s * (HS + 2)] - ref);
+            L = fmaf(f, w[s * (HS + 2) + 1], L);
+            O = fmaf(f, w[s * (HS + 2) + 2 + i], O);
+        }
+    }
+    put_result(a, row, (size_t)h * HS + i, hi <= lo ? 0.0f : O / L, on);
 }
 
 } // namespace kv4

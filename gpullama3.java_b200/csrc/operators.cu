@@ -11,7 +11,7 @@
 
 struct b200_kv4 {
     kv4::View view{};
-    int head_size = 0, device = 0;
+    int head_size = 0, device = 0, sms = 148;
     size_t bytes = 0;
     char err[256] = "";
 };
@@ -125,6 +125,31 @@ cudaError_t kv4_append_launch(const b200_kv4 *kv, const b200_kv4_append_args &a,
     });
 }
 
+// How the work of single rows is cut: heads of a unit, units of a row and key/value head, CTAs of a cluster, clusters of a unit.
+struct StepCut {
+    int heads, per_head, cluster, splits;
+};
+static StepCut step_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, bool quants) {
+    StepCut c;
+    const int G = kv->view.kv_heads, mul = a.heads / G, hs = kv->head_size, sms = kv->sms;
+    c.heads = mul > 4 && hs < 256 ? 8 : 4;
+    c.per_head = (mul + c.heads - 1) / c.heads;
+    const long long units = (long long)a.n * G * c.per_head;
+    const int len = a.max_len > 0 && a.max_len < kv->view.context ? a.max_len : kv->view.context, seen = a.window > 0 && a.window < len ? a.window : len;
+    int most = (seen + kv4::BLOCK * kv4::STEP_WARPS - 1) / (kv4::BLOCK * kv4::STEP_WARPS); // a record a warp
+    if (most > kv4::STEP_MAX_CLUSTER) most = kv4::STEP_MAX_CLUSTER;
+    if (quants && most > c.heads * hs / 32) most = c.heads * hs / 32; // whole blocks of 32 quants a CTA
+    c.cluster = cluster_for(units, 2 * sms, most);
+    long long splits = c.cluster == kv4::STEP_MAX_CLUSTER ? 2LL * sms / (units * c.cluster) : 1;
+    const long long worth = seen / (kv4::BLOCK * kv4::STEP_WARPS * kv4::STEP_MAX_CLUSTER * 4); // four records a warp
+    if (splits > worth) splits = worth;
+    c.splits = splits < 1 ? 1 : (int)splits;
+    return c;
+}
+static size_t step_work_bytes(const b200_kv4 *kv, const b200_kv4_attention_args &a, const StepCut &c) {
+    return c.splits > 1 ? (size_t)a.n * a.heads * c.splits * (kv->head_size + 2) * 4 : 0;
+}
+
 cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_args &a, int8_t *quants, float *scales, cudaStream_t stream, bool pdl) {
     kv4::Step k;
     k.kv = kv->view;
@@ -136,23 +161,21 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
     k.out_type = quants ? KV4_OUT_Q8 : a.out_type;
     k.scale = a.scale;
     k.out = a.out; k.quants = quants; k.scales = scales;
-    const int G = kv->view.kv_heads, mul = a.heads / G;
+    StepCut c = step_cut(kv, a, quants != nullptr);
+    if (step_work_bytes(kv, a, c) > a.workspace_bytes || !a.workspace) c.splits = 1;
+    k.work = a.workspace;
     return by_head_size(kv->head_size, [&](auto hs) {
         auto go = [&](auto nt) {
-            constexpr int H = 4 * nt;
-            constexpr size_t smem = kv4::step_smem_bytes(hs, H);
-            const int per_head = (mul + H - 1) / H;
-            const long long units = (long long)a.n * G * per_head;
-            const int len = a.max_len > 0 && a.max_len < kv->view.context ? a.max_len : kv->view.context, seen = a.window > 0 && a.window < len ? a.window : len;
-            int most = (seen + kv4::BLOCK * kv4::STEP_WARPS - 1) / (kv4::BLOCK * kv4::STEP_WARPS); // a record a warp
-            if (most > kv4::STEP_MAX_CLUSTER) most = kv4::STEP_MAX_CLUSTER;
-            if (quants && most > H * hs / 32) most = H * hs / 32; // whole blocks of 32 quants a CTA
-            const int cluster = cluster_for(units, 2 * sm_count(kv->device), most);
+            constexpr size_t smem = kv4::step_smem_bytes(hs, 4 * nt);
+            const unsigned grid = (unsigned)a.n * kv->view.kv_heads * c.per_head * c.splits * c.cluster;
             auto kern = kv4::k_step<hs, nt>;
-            cudaError_t e = prepare(kern, smem, cluster);
-            return e != cudaSuccess ? e : launch(kern, (unsigned)(units * cluster), kv4::STEP_WARPS * 32, smem, cluster, pdl, stream, k, per_head);
+            cudaError_t e = prepare(kern, smem, c.cluster);
+            if (e == cudaSuccess) e = launch(kern, grid, kv4::STEP_WARPS * 32, smem, c.cluster, pdl, stream, k, c.per_head, c.splits);
+            if (e != cudaSuccess || c.splits == 1) return e;
+            constexpr int per_cta = hs < 64 ? 64 / hs : 1;
+            return launch(kv4::k_step_join<hs>, (unsigned)a.n * ((a.heads + per_cta - 1) / per_cta), hs < 64 ? 64 : hs, 0, 1, true, stream, k, c.splits);
         };
-        if constexpr (hs < 256) if (mul > 4) return go(std::integral_constant<int, 2>());
+        if constexpr (hs < 256) if (c.heads == 8) return go(std::integral_constant<int, 2>());
         return go(std::integral_constant<int, 1>());
     });
 }
@@ -190,6 +213,7 @@ int b200_kv4_create(int32_t slots, int32_t context, int32_t kv_heads, int32_t he
     if (!kv) return say(err, err_len, B200_ERR_OOM, "no host memory");
     kv->head_size = head_size;
     kv->device = device;
+    kv->sms = sm_count(device);
     kv->view = {nullptr, slots, context, (context + kv4::BLOCK - 1) / kv4::BLOCK, kv_heads};
     const unsigned __int128 bytes = (unsigned __int128)slots * kv_heads * kv->view.blocks * kv4::record_bytes(head_size);
     OnDevice on(device);
@@ -263,6 +287,7 @@ int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *a, void *str
     if (rc) return rc;
     if (a->heads <= 0 || a->heads % kv->view.kv_heads) return fail(kv, B200_ERR_BAD_ARG, "%d query heads over %d key/value heads", a->heads, kv->view.kv_heads);
     if (!known_type(a->out_type)) return fail(kv, B200_ERR_UNSUPPORTED, "results of type %d (FP32, FP16 and BF16 are known)", a->out_type);
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 4) return fail(kv, B200_ERR_BAD_ARG, "the workspace is not aligned");
     if (a->window < 0 || a->max_len < 0 || a->chunk < 0) return fail(kv, B200_ERR_BAD_ARG, "a negative window, length or chunk");
     if (a->n == 0) return B200_OK;
     if (!a->q || !a->out) return fail(kv, B200_ERR_BAD_ARG, "null rows");
@@ -273,6 +298,11 @@ int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *a, void *str
     cudaError_t e = on.error;
     if (e == cudaSuccess) e = kv4_attention_launch(kv, *a, nullptr, nullptr, (cudaStream_t)stream, false);
     return e == cudaSuccess ? B200_OK : fail(kv, cuda_code(e), "%s", cudaGetErrorString(e));
+}
+
+size_t b200_kv4_attention_workspace(const b200_kv4 *kv, const b200_kv4_attention_args *a) {
+    if (!kv || !a || a->n <= 0 || a->heads <= 0 || a->heads % kv->view.kv_heads) return 0;
+    return step_work_bytes(kv, *a, step_cut(kv, *a, false));
 }
 
 int b200_kv4_read(b200_kv4 *kv, const b200_kv4_read_args *a, void *stream) {

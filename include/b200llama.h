@@ -485,7 +485,7 @@ int b200_upload_info(b200_plan *plan, double *seconds, double *host_copy_seconds
 
 /* ---- operators on device memory ------------------------------------------------------------------------------------------------------
  * These take DEVICE pointers and a stream (a cudaStream_t; NULL: the legacy default stream) of the device that they name, launch on it and return without a wait: what goes wrong
- * on the device shows at the caller's next synchronisation.  They allocate nothing, use no workspace, keep nothing between calls and can be captured into CUDA graphs; the calling
+ * on the device shows at the caller's next synchronisation.  They allocate nothing, keep nothing between calls and can be captured into CUDA graphs; the calling
  * thread's current device is left as it was.  Nothing of this exists in the reference. */
 
 /* A key/value cache that holds a head's entries in 4 bits: groups of 32 neighbouring entries with one FP16 scale d, codes c of 0 .. 15, value d * (c - 8).  m = the entry of largest
@@ -521,7 +521,9 @@ int b200_kv4_append(b200_kv4 *kv, const b200_kv4_append_args *args, void *stream
 
 /* Causal attention of n query rows over the cache: row r at position p sees the positions j <= p of its slot, the last `window` of them where window > 0; query head h reads key/value
  * head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type.  A row that sees nothing is zeros.  max_len (0: unknown) is the largest position + 1 as far as the host
- * knows, chunk (0 or 1: single steps) how many neighbouring rows are successive tokens of one sequence: both only choose how the work is split. */
+ * knows, chunk (0 or 1: single steps) how many neighbouring rows are successive tokens of one sequence: both only choose how the work is split.  So does a workspace: few rows over
+ * many positions fill the GPU where the call gets b200_kv4_attention_workspace(kv, args) bytes (0: it needs none) of device memory, whose content before and after does not matter
+ * and which no other call under way may use; NULL or fewer bytes: the call does without. */
 typedef struct b200_kv4_attention_args {
     int32_t n, heads, window, max_len, chunk, out_type;
     const float *q;
@@ -530,7 +532,10 @@ typedef struct b200_kv4_attention_args {
     const int32_t *positions, *slots;
     int32_t start, slot;
     float scale;
+    float *workspace;
+    size_t workspace_bytes;
 } b200_kv4_attention_args;
+size_t b200_kv4_attention_workspace(const b200_kv4 *kv, const b200_kv4_attention_args *args);
 int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *args, void *stream);
 
 /* The values that the cache holds at n rows: k and v [n][kv_heads][head_size] in `type`.  A row of a negative position is left as it was. */

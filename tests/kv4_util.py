@@ -39,12 +39,14 @@ def turn(x, weight, eps, cos, sin, positions, layout):
 
 
 def attention(q, k, v, d, positions, slots, scale, window):
-    """q [n, H, hs]; k, v [slots, context, G, hs] and key scales d [slots, context, G, hs / 32], all float64 on the CPU -> (out, bound) where bound is how far a kernel may be off
-    in FP32.
+    """q [n, H, hs]; k, v [slots, context, G, hs] and their scales d (two of [slots, context, G, hs / 32]), all float64 on the CPU -> (out, bound) where bound is how far a kernel may
+    be off in FP32.
 
     The bound: a query keeps 22 bits of its largest entry's magnitude and meets codes of at most 16 steps, so that a score's error is at most 2^-21 + hs 2^-24 (products and
     sums in FP32) of A = scale * max|q| * sum over groups of 32 * 16 |d|; a probability's relative error is twice that error (numerator and sum), plus 2^-20 for its exponential;
-    its product with a value keeps 16 bits (2^-16), and sums of n products in FP32 add n 2^-24 at most.  All relative to sum p |v|."""
+    its product with a value's scale keeps 16 bits (2^-16), and sums of n products in FP32 add n 2^-24 at most.  All relative to sum p |v|.  A value is (c - 8) d with c of up to 15,
+    and the sums of p d c and of -8 p d go through the same accumulators: what they round, n / 16 + 16 times 2^-22 at most, is relative to 16 sum p |d|."""
+    kd, vd = d
     n, H, hs = q.shape
     G = k.shape[2]
     out, bound = torch.zeros_like(q), torch.zeros_like(q)
@@ -58,9 +60,10 @@ def attention(q, k, v, d, positions, slots, scale, window):
             kk, vv = k[s, lo:p + 1, g], v[s, lo:p + 1, g]
             x = kk @ q[r, h] * scale
             w = torch.softmax(x, 0)
-            A = scale * q[r, h].abs().max() * d[s, lo:p + 1, g].abs().sum(-1).max() * 32 * 16
+            A = scale * q[r, h].abs().max() * kd[s, lo:p + 1, g].abs().sum(-1).max() * 32 * 16
             out[r, h] = w @ vv
             bound[r, h] = (w @ vv.abs()) * (2 * A * (2.0 ** -21 + hs * 2.0 ** -24) + 2.0 ** -16 + 2.0 ** -20 + (p + 1 - lo) * 2.0 ** -24)
+            bound[r, h] += (w @ vd[s, lo:p + 1, g].abs()).repeat_interleave(32) * 16 * ((p + 1 - lo) / 16 + 16) * 2.0 ** -22
     return out, bound
 
 

@@ -8,7 +8,7 @@ import kv4_util as U
 
 
 def test_argument_blocks_have_the_headers_layout(pkg):
-    assert [C.sizeof(t) for t in (pkg.native.KV4Append, pkg.native.KV4Attention, pkg.native.KV4Read, pkg.native.LogProbs)] == [144, 88, 48, 80]
+    assert [C.sizeof(t) for t in (pkg.native.KV4Append, pkg.native.KV4Attention, pkg.native.KV4Read, pkg.native.LogProbs)] == [144, 104, 48, 80]
 
 
 @pytest.mark.parametrize("slots,context,heads,hs,code,word", [(0, 16, 1, 64, -1, "positive"), (1, 0, 1, 64, -1, "positive"), (1, 16, 0, 64, -1, "positive"), (1, 16, 1, 80, -2, "80"),
