@@ -268,10 +268,18 @@ __device__ __forceinline__ void mma_f16_first(float (&d)[4], const uint32_t (&a)
 }
 // The codes of a word as pairs of FP16 numbers c - 8: pair i holds nibbles i and i + 4.  The bits of 1024 + c (or 1024 + 16 c) come from a mask, the rest is one exact operation.  (A masked
 // code by itself is a number too, c 2^-24, but products of subnormals are added with as many bits less as they have leading zeros: 2^-17 in a score.)
-__device__ __forceinline__ void unpack(uint32_t w, uint32_t (&c)[4]) {
+__device__ __forceinline__ uint32_t magic() { // 1024 in both halves, in a register: a mask and an or with two literals would be two instructions
+    uint32_t m;
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(m));
+    return m;
+}
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t one, uint32_t (&c)[4]) {
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        const uint32_t v = i ? w >> 8 : w, even = (v & 0x000f000fu) | 0x64006400u, odd = (v & 0x00f000f0u) | 0x64006400u;
+        const uint32_t v = i ? w >> 8 : w;
+        uint32_t even, odd;
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(even) : "r"(v), "n"(0x000f000f), "r"(one)); // (v & mask) | one
+        asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(odd) : "r"(v), "n"(0x00f000f0), "r"(one));
         asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(c[2 * i]) : "r"(even), "r"(0x64086408u));                                    // - 1032
         asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(c[2 * i + 1]) : "r"(odd), "r"(0x2c002c00u), "r"(0xd480d480u)); // / 16 - 72
     }
@@ -286,6 +294,9 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     return r;
 }
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void cp16_if(bool on, uint32_t dst, const void *src) { // predicated, not branched around
+    asm volatile("{.reg .pred p; setp.ne.b32 p, %2, 0; @p cp.async.cg.shared.global [%0], [%1], 16;}" ::"r"(dst), "l"(src), "r"((int)on) : "memory");
+}
 __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 template <int VW> __device__ __forceinline__ void lds_words(const uint32_t *p, uint32_t (&w)[VW]) {
@@ -297,8 +308,9 @@ template <int VW> __device__ __forceinline__ void lds_words(const uint32_t *p, u
 }
 
 constexpr int STEP_WARPS = 8, STEP_MAX_CLUSTER = 8;
-__host__ __device__ constexpr int step_stages(int hs) { return hs >= 256 ? 3 : 4; }
-__host__ __device__ constexpr size_t step_ring_bytes(int hs) { return (size_t)STEP_WARPS * step_stages(hs) * record_bytes(hs); }
+__host__ __device__ constexpr int step_records(int hs) { return hs >= 256 ? 1 : 2; }          // records that a warp takes at a time
+__host__ __device__ constexpr int step_stages(int hs) { return hs >= 128 ? 3 : hs >= 64 ? 4 : 5; } // ... and has room for, with those under way
+__host__ __device__ constexpr size_t step_ring_bytes(int hs) { return (size_t)STEP_WARPS * step_stages(hs) * step_records(hs) * record_bytes(hs); }
 __host__ __device__ constexpr size_t step_merge_bytes(int hs, int heads) { return (size_t)(STEP_WARPS + 1) * heads * (hs + 2) * 4; } // the warps' parts and the CTA's
 __host__ __device__ constexpr size_t step_smem_bytes(int hs, int heads) { return step_ring_bytes(hs) > step_merge_bytes(hs, heads) ? step_ring_bytes(hs) : step_merge_bytes(hs, heads); }
 
@@ -329,7 +341,7 @@ __device__ __forceinline__ void put_result(const Step &a, int row, size_t at, fl
 //   values  C[16 entries x 8] = codes x (p d), again as a high and a low part.  p d is kept in FP16's range by a power of two that follows the largest value scale seen so far
 // A lane keeps the running sums of ONE head (t); what crosses lanes in the loop is the transposition of the probabilities and, where a maximum grows by more than 2^8, its update.
 template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_step(const Step a, const int units_per_head, const int splits) {
-    constexpr int NG = groups(HS), VW = vec_words(HS), R = record_bytes(HS), S = step_stages(HS), H = 4 * NT, CHUNKS = R / 16;
+    constexpr int NG = groups(HS), VW = vec_words(HS), R = record_bytes(HS), KB = step_records(HS), S = step_stages(HS), H = 4 * NT, CHUNKS = R / 16;
     extern __shared__ __align__(16) unsigned char smem[];
     pdl_wait();
     cg::cluster_group cluster = cg::this_cluster();
@@ -342,22 +354,19 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
     int lo, hi;
     visible(pos, a.window, lo, hi);
     const int workers = splits * ranks * STEP_WARPS, worker = (split * ranks + rank) * STEP_WARPS + warp;
-    const int b0 = lo / BLOCK, nb = hi > lo ? (hi + BLOCK - 1) / BLOCK - b0 : 0, per = (nb + workers - 1) / workers;
-    const int begin = b0 + min(nb, worker * per), end = b0 + min(nb, (worker + 1) * per);
+    const int b0 = lo / BLOCK, nb = hi > lo ? (hi + BLOCK - 1) / BLOCK - b0 : 0, per = (nb + workers * KB - 1) / (workers * KB) * KB;
+    const int begin = b0 + min(nb, worker * per), end = b0 + min(nb, (worker + 1) * per), stop = min(hi, end * BLOCK); // positions from `stop` on are none of this warp's
 
-    unsigned char *ring = smem + (size_t)warp * S * R;
+    unsigned char *ring = smem + (size_t)warp * S * KB * R;
     const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring) + lane * 16;
     const unsigned char *src = record<HS>(a.kv, slot, kvh, begin) + lane * 16;
-    int fetched = begin;
+    int left = (end - begin) * CHUNKS - lane; // copies of 16 bytes, from this lane's first on
     auto fetch = [&](int stage) {
-        if (fetched < end) {
-            const uint32_t d = ring_addr + stage * R;
+        const uint32_t d = ring_addr + stage * KB * R;
 #pragma unroll
-            for (int i = 0; i < CHUNKS / 32; i++) cp16(d + i * 512, src + i * 512);
-            if (CHUNKS % 32 && lane < CHUNKS % 32) cp16(d + CHUNKS / 32 * 512, src + CHUNKS / 32 * 512);
-            src += R;
-            fetched++;
-        }
+        for (int i = 0; i < (KB * CHUNKS + 31) / 32; i++) cp16_if(left > 32 * i && (32 * i + 31 < KB * CHUNKS || lane + 32 * i < KB * CHUNKS), d + i * 512, src + i * 512);
+        src += KB * R;
+        left -= KB * CHUNKS;
         cp_commit();
     };
 #pragma unroll
@@ -406,68 +415,81 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
     }
     int lift = 0;            // p d is held times 2^lift
     uint32_t most = 0u;      // scales up to here (their bits) have been seen: 2^lift * scale < 2^7
+    const uint32_t one = magic();
     int stage = 0;
 #pragma unroll 1
-    for (int block = begin; block < end; block++) {
+    for (int block = begin; block < end; block += KB) {
         cp_wait<S - 2>();
         __syncwarp(); // and every lane has read the stage that the next copy overwrites
         fetch(stage == 0 ? S - 1 : stage - 1);
-        const uint32_t *words = reinterpret_cast<const uint32_t *>(ring + stage * R);
-        const uint32_t *ks = words + 4 * HS + g * NG, *vs = ks + 8 * NG; // scales of positions g and g + 8
-        float s[NT][2];
-        uint32_t dv[NG];
+        const uint32_t *words = reinterpret_cast<const uint32_t *>(ring + stage * KB * R);
+        float s[KB][NT][2];
+        uint32_t dv[KB][NG]; // value scales of positions g and g + 8
 #pragma unroll
-        for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = 0.0f;
+        for (int b = 0; b < KB; b++) {
+            const uint32_t *codes = words + b * (R / 4), *ks = codes + 4 * HS + g * NG;
 #pragma unroll
-        for (int v = 0; v < NG / VW; v++) {
-            uint32_t wa[VW], wb[VW], d[VW], dw[VW];
-            lds_words<VW>(words + word_of<HS>(0, lane, v * VW), wa);
-            lds_words<VW>(words + word_of<HS>(1, lane, v * VW), wb);
-            lds_words<VW>(ks + v * VW, d);
-            lds_words<VW>(vs + v * VW, dw);
+            for (int n = 0; n < NT; n++) s[b][n][0] = s[b][n][1] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < VW; i++) {
-                const int grp = v * VW + i;
-                dv[grp] = dw[i];
-                uint32_t ca[4], cb[4];
-                unpack(wa[i], ca);
-                unpack(wb[i], cb);
-                const uint32_t c0[4] = {ca[0], cb[0], ca[1], cb[1]}, c1[4] = {ca[2], cb[2], ca[3], cb[3]};
-                const float2 dk = __half22float2(*reinterpret_cast<const __half2 *>(&d[i]));
+            for (int v = 0; v < NG / VW; v++) {
+                uint32_t wa[VW], wb[VW], d[VW], dw[VW];
+                lds_words<VW>(codes + word_of<HS>(0, lane, v * VW), wa);
+                lds_words<VW>(codes + word_of<HS>(1, lane, v * VW), wb);
+                lds_words<VW>(ks + v * VW, d);
+                lds_words<VW>(ks + 8 * NG + v * VW, dw);
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    float acc[4];
-                    mma_f16_first(acc, c0, qf[n][grp][0], qf[n][grp][1]);
-                    mma_f16(acc, c1, qf[n][grp][2], qf[n][grp][3]);
-                    s[n][0] = fmaf(dk.x, acc[0] + acc[1], s[n][0]);
-                    s[n][1] = fmaf(dk.y, acc[2] + acc[3], s[n][1]);
+                for (int i = 0; i < VW; i++) {
+                    const int grp = v * VW + i;
+                    dv[b][grp] = dw[i];
+                    uint32_t ca[4], cb[4];
+                    unpack(wa[i], one, ca);
+                    unpack(wb[i], one, cb);
+                    const uint32_t c0[4] = {ca[0], cb[0], ca[1], cb[1]}, c1[4] = {ca[2], cb[2], ca[3], cb[3]};
+                    const float2 dk = __half22float2(*reinterpret_cast<const __half2 *>(&d[i]));
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        float acc[4];
+                        mma_f16_first(acc, c0, qf[n][grp][0], qf[n][grp][1]);
+                        mma_f16(acc, c1, qf[n][grp][2], qf[n][grp][3]);
+                        s[b][n][0] = fmaf(dk.x, acc[0] + acc[1], s[b][n][0]);
+                        s[b][n][1] = fmaf(dk.y, acc[2] + acc[3], s[b][n][1]);
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int n = 0; n < NT; n++) { s[n][0] *= sc[n]; s[n][1] *= sc[n]; }
-        if (block * BLOCK < lo || block * BLOCK + BLOCK > hi) { // an end of what the row sees: whatever stands behind it has no weight and no scale
-            const int p0 = block * BLOCK + g;
-            const bool see0 = p0 >= lo && p0 < hi, see1 = p0 + 8 >= lo && p0 + 8 < hi;
+        for (int b = 0; b < KB; b++)
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-                if (!see0) s[n][0] = -CUDART_INF_F;
-                if (!see1) s[n][1] = -CUDART_INF_F;
+            for (int n = 0; n < NT; n++) { s[b][n][0] *= sc[n]; s[b][n][1] *= sc[n]; }
+        if (block * BLOCK < lo || (block + KB) * BLOCK > stop) { // an end of what the warp takes: whatever stands behind it has no weight and no scale
+#pragma unroll
+            for (int b = 0; b < KB; b++) {
+                const int p0 = (block + b) * BLOCK + g;
+                const bool see0 = p0 >= lo && p0 < stop, see1 = p0 + 8 >= lo && p0 + 8 < stop;
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    if (!see0) s[b][n][0] = -CUDART_INF_F;
+                    if (!see1) s[b][n][1] = -CUDART_INF_F;
+                }
+#pragma unroll
+                for (int grp = 0; grp < NG; grp++) dv[b][grp] &= (see0 ? 0xffffu : 0u) | (see1 ? 0xffff0000u : 0u);
             }
-#pragma unroll
-            for (int grp = 0; grp < NG; grp++) dv[grp] &= (see0 ? 0xffffu : 0u) | (see1 ? 0xffff0000u : 0u);
         }
-        uint32_t all = 0; // not below any of the scales: their bits together
+        __half2 widest = __habs2(*reinterpret_cast<const __half2 *>(&dv[0][0])); // (NaN loses against a number)
 #pragma unroll
-        for (int grp = 0; grp < NG; grp++) all |= dv[grp];
-        bool rare = (all & 0x7fffu) > most || (all >> 16 & 0x7fffu) > most;
+        for (int grp = 1; grp < KB * NG; grp++) widest = __hmax2(widest, __habs2(*reinterpret_cast<const __half2 *>(&dv[grp / NG][grp % NG])));
+        const uint32_t wide = *reinterpret_cast<const uint32_t *>(&widest);
+        bool rare = ((0x80008000u + most * 0x10001u) - wide & 0x80008000u) != 0x80008000u; // a half of it above `most`
+        float mx[NT];
 #pragma unroll
-        for (int n = 0; n < NT; n++) rare |= fmaxf(s[n][0], s[n][1]) > m[n] + 8.0f;
+        for (int n = 0; n < NT; n++) {
+            mx[n] = fmaxf(s[0][n][0], s[0][n][1]);
+#pragma unroll
+            for (int b = 1; b < KB; b++) mx[n] = fmaxf(mx[n], fmaxf(s[b][n][0], s[b][n][1]));
+            rare |= mx[n] > m[n] + 8.0f;
+        }
         if (__any_sync(0xffffffffu, rare)) {
-            uint32_t big = 0;
-#pragma unroll
-            for (int grp = 0; grp < NG; grp++) big = max(big, max(dv[grp] & 0x7fffu, dv[grp] >> 16 & 0x7fffu));
-            big = __reduce_max_sync(0xffffffffu, big);
+            const uint32_t big = __reduce_max_sync(0xffffffffu, max(wide & 0xffffu, wide >> 16));
             float beta = 1.0f;
             if (big > most && big <= 0x7c00u) { // (a NaN changes nothing)
                 const int was = lift;
@@ -477,48 +499,53 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                float mx = fmaxf(s[n][0], s[n][1]);
 #pragma unroll
-                for (int i = 4; i < 32; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
-                mx = fmaxf(mx, m[n]);
-                const float alpha = m[n] == mx ? 1.0f : ex2(m[n] - mx), gamma = alpha * beta;
-                m[n] = mx;
+                for (int i = 4; i < 32; i <<= 1) mx[n] = fmaxf(mx[n], __shfl_xor_sync(0xffffffffu, mx[n], i));
+                mx[n] = fmaxf(mx[n], m[n]);
+                const float alpha = m[n] == mx[n] ? 1.0f : ex2(m[n] - mx[n]), gamma = alpha * beta;
+                m[n] = mx[n];
                 l[n] *= alpha;
 #pragma unroll
                 for (int i = 0; i < 2 * NG; i++) { o[n][i][0] *= gamma; o[n][i][1] *= gamma; o[n][i][2] *= gamma; o[n][i][3] *= gamma; }
             }
         }
-        float p[NT][2];
         const float two_to_lift = __uint_as_float((unsigned)(127 + lift) << 23);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
             const float ref = m[n] == -CUDART_INF_F ? 0.0f : m[n]; // nothing seen yet: 2^(-inf) = 0
-            p[n][0] = ex2(s[n][0] - ref);
-            p[n][1] = ex2(s[n][1] - ref);
-            l[n] += p[n][0] + p[n][1];
-            p[n][0] *= two_to_lift;
-            p[n][1] *= two_to_lift;
+#pragma unroll
+            for (int b = 0; b < KB; b++) {
+                s[b][n][0] = ex2(s[b][n][0] - ref);
+                s[b][n][1] = ex2(s[b][n][1] - ref);
+                l[n] += s[b][n][0] + s[b][n][1];
+                s[b][n][0] *= two_to_lift;
+                s[b][n][1] *= two_to_lift;
+            }
         }
 #pragma unroll
-        for (int v = 0; v < NG / VW; v++) {
-            uint32_t wa[VW], wb[VW];
-            lds_words<VW>(words + 2 * HS + word_of<HS>(0, lane, v * VW), wa);
-            lds_words<VW>(words + 2 * HS + word_of<HS>(1, lane, v * VW), wb);
+        for (int b = 0; b < KB; b++) {
+            const uint32_t *codes = words + b * (R / 4) + 2 * HS;
 #pragma unroll
-            for (int i = 0; i < VW; i++) {
-                const int grp = v * VW + i;
-                const float2 d = __half22float2(*reinterpret_cast<const __half2 *>(&dv[grp]));
-                uint32_t ca[4], cb[4];
-                unpack(wa[i], ca);
-                unpack(wb[i], cb);
-                const uint32_t c0[4] = {ca[0], ca[1], cb[0], cb[1]}, c1[4] = {ca[2], ca[3], cb[2], cb[3]};
+            for (int v = 0; v < NG / VW; v++) {
+                uint32_t wa[VW], wb[VW];
+                lds_words<VW>(codes + word_of<HS>(0, lane, v * VW), wa);
+                lds_words<VW>(codes + word_of<HS>(1, lane, v * VW), wb);
 #pragma unroll
-                for (int n = 0; n < NT; n++) {
-                    const float x0 = p[n][0] * d.x, x1 = p[n][1] * d.y; // the high part: the 11 bits that FP16 has, cut off
-                    const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(x1) & 0xffffe000u);
-                    const uint32_t f0 = transpose8x8(pack_f16(h0, x0 - h0)), f1 = transpose8x8(pack_f16(h1, x1 - h1));
-                    mma_f16(o[n][2 * grp], c0, f0, f1);
-                    mma_f16(o[n][2 * grp + 1], c1, f0, f1);
+                for (int i = 0; i < VW; i++) {
+                    const int grp = v * VW + i;
+                    const float2 d = __half22float2(*reinterpret_cast<const __half2 *>(&dv[b][grp]));
+                    uint32_t ca[4], cb[4];
+                    unpack(wa[i], one, ca);
+                    unpack(wb[i], one, cb);
+                    const uint32_t c0[4] = {ca[0], ca[1], cb[0], cb[1]}, c1[4] = {ca[2], ca[3], cb[2], cb[3]};
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        const float x0 = s[b][n][0] * d.x, x1 = s[b][n][1] * d.y; // the high part: the 11 bits that FP16 has, cut off
+                        const float h0 = __uint_as_float(__float_as_uint(x0) & 0xffffe000u), h1 = __uint_as_float(__float_as_uint(x1) & 0xffffe000u);
+                        const uint32_t f0 = transpose8x8(pack_f16(h0, x0 - h0)), f1 = transpose8x8(pack_f16(h1, x1 - h1));
+                        mma_f16(o[n][2 * grp], c0, f0, f1);
+                        mma_f16(o[n][2 * grp + 1], c1, f0, f1);
+                    }
                 }
             }
         }
@@ -582,27 +609,31 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
     if (ranks > 1) cluster.sync(); // no CTA leaves while another reads its part
 }
 
-// Joins the splits of a unit: one thread an entry.
+// Joins the parts of a row's head: the weights of the splits once, then an entry a thread.  At most STEP_MAX_SPLITS parts.
+constexpr int STEP_MAX_SPLITS = 296;
 template <int HS> __global__ void __launch_bounds__(HS < 64 ? 64 : HS) k_step_join(const Step a, const int splits) {
-    constexpr int HEADS = HS < 64 ? 64 / HS : 1; // heads of a CTA
+    constexpr int HEADS = HS < 64 ? 64 / HS : 1, LD = HS + 2; // heads of a CTA
+    __shared__ float weight[HEADS][STEP_MAX_SPLITS], sum[HEADS][STEP_MAX_SPLITS];
     pdl_wait();
-    const int h = blockIdx.x % ((a.heads + HEADS - 1) / HEADS) * HEADS + threadIdx.x / HS, row = blockIdx.x / ((a.heads + HEADS - 1) / HEADS), i = threadIdx.x % HS;
+    const int at = threadIdx.x / HS, h = blockIdx.x % ((a.heads + HEADS - 1) / HEADS) * HEADS + at, row = blockIdx.x / ((a.heads + HEADS - 1) / HEADS), i = threadIdx.x % HS;
     const int pos = a.rows.position(row), slot = a.rows.slot_of(row);
     if (slot < 0 || slot >= a.kv.slots || pos >= a.kv.context) return;
     const bool on = h < a.heads;
     int lo, hi;
     visible(pos, a.window, lo, hi);
+    const float *w = a.work + ((size_t)row * a.heads + (on ? h : 0)) * splits * LD;
+    for (int s = i; s < splits; s += HS) { weight[at][s] = w[s * LD]; sum[at][s] = w[s * LD + 1]; }
+    __syncthreads();
     float M = -CUDART_INF_F, L = 0.0f, O = 0.0f;
-    if (on && hi > lo) {
-        const float *w = a.work + ((size_t)row * a.heads + h) * splits * (HS + 2);
-        for (int s = 0; s < splits; s++) M = fmaxf(M, w[s * (HS + 2)]);
-        const float ref = M == -CUDART_INF_F ? 0.0f : M;
-#pragma unroll 4
-        for (int s = 0; s < splits; s++) {
-            const float f = ex2(w[s * (HS + 2)] - ref);
-            L = fmaf(f, w[s * (HS + 2) + 1], L);
-            O = fmaf(f, w[s * (HS + 2) + 2 + i], O);
-        }
+    for (int s = 0; s < splits; s++) M = fmaxf(M, weight[at][s]);
+    const float ref = M == -CUDART_INF_F ? 0.0f : M;
+    __syncthreads();
+    for (int s = i; s < splits; s += HS) weight[at][s] = ex2(weight[at][s] - ref);
+    __syncthreads();
+#pragma unroll 8
+    for (int s = 0; s < splits; s++) {
+        L = fmaf(weight[at][s], sum[at][s], L);
+        O = fmaf(weight[at][s], w[s * LD + 2 + i], O);
     }
     put_result(a, row, (size_t)h * HS + i, hi <= lo ? 0.0f : O / L, on);
 }

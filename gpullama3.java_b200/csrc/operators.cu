@@ -5,6 +5,7 @@
 
 #include <stdarg.h>
 #include <stdio.h>
+#include <stdlib.h>
 #include <string.h>
 
 #include <new>
@@ -131,19 +132,22 @@ struct StepCut {
 };
 static StepCut step_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, bool quants) {
     StepCut c;
-    const int G = kv->view.kv_heads, mul = a.heads / G, hs = kv->head_size, sms = kv->sms;
+    const int G = kv->view.kv_heads, mul = a.heads / G, hs = kv->head_size;
     c.heads = mul > 4 && hs < 256 ? 8 : 4;
     c.per_head = (mul + c.heads - 1) / c.heads;
     const long long units = (long long)a.n * G * c.per_head;
     const int len = a.max_len > 0 && a.max_len < kv->view.context ? a.max_len : kv->view.context, seen = a.window > 0 && a.window < len ? a.window : len;
-    int most = (seen + kv4::BLOCK * kv4::STEP_WARPS - 1) / (kv4::BLOCK * kv4::STEP_WARPS); // a record a warp
+    const int group = kv4::BLOCK * kv4::step_records(hs) * kv4::STEP_WARPS; // positions that a CTA takes at a time
+    // Few units over many positions: two CTAs for every SM, evenly, through the workspace (clusters of 8 leave SMs with one CTA beside SMs with two: the kernel took 42 us for 131071
+    // positions of 8 heads, cut evenly 36.6).
+    c.splits = units * kv4::STEP_MAX_CLUSTER < 2 * kv->sms && seen >= 4 * group * kv4::STEP_MAX_CLUSTER ? (int)(2 * kv->sms / units) : 1;
+    if (c.splits > seen / (4 * group)) c.splits = seen / (4 * group); // at least four rounds a warp
+    if (c.splits < 1) c.splits = 1;
+    if (c.splits > kv4::STEP_MAX_SPLITS) c.splits = kv4::STEP_MAX_SPLITS;
+    int most = (seen + group - 1) / group;
     if (most > kv4::STEP_MAX_CLUSTER) most = kv4::STEP_MAX_CLUSTER;
     if (quants && most > c.heads * hs / 32) most = c.heads * hs / 32; // whole blocks of 32 quants a CTA
-    c.cluster = cluster_for(units, 2 * sms, most);
-    long long splits = c.cluster == kv4::STEP_MAX_CLUSTER ? 2LL * sms / (units * c.cluster) : 1;
-    const long long worth = seen / (kv4::BLOCK * kv4::STEP_WARPS * kv4::STEP_MAX_CLUSTER * 4); // four records a warp
-    if (splits > worth) splits = worth;
-    c.splits = splits < 1 ? 1 : (int)splits;
+    c.cluster = cluster_for(units, 8 * kv->sms, most);
     return c;
 }
 static size_t step_work_bytes(const b200_kv4 *kv, const b200_kv4_attention_args &a, const StepCut &c) {
@@ -162,7 +166,8 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
     k.scale = a.scale;
     k.out = a.out; k.quants = quants; k.scales = scales;
     StepCut c = step_cut(kv, a, quants != nullptr);
-    if (step_work_bytes(kv, a, c) > a.workspace_bytes || !a.workspace) c.splits = 1;
+    if (c.splits > 1 && a.workspace && step_work_bytes(kv, a, c) <= a.workspace_bytes) c.cluster = 1;
+    else c.splits = 1;
     k.work = a.workspace;
     return by_head_size(kv->head_size, [&](auto hs) {
         auto go = [&](auto nt) {
