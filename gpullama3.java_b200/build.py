@@ -13,7 +13,7 @@ SOURCES = ["plan.cu", "operators.cu"]
 
 
 # Headers that only operators.cu reads: the other objects are not rebuilt for them.
-OPERATOR_HEADERS = ("kv4.cuh", "logprobs.cuh")
+OPERATOR_HEADERS = ("kv4.cuh", "kv4_chunk.cuh", "logprobs.cuh")
 
 
 def _deps(source: str | None = None):

@@ -1,6 +1,6 @@
 // operators.cu -- libb200llama.so: operators that work on a caller's device memory and stream (b200_kv4_*, b200_log_probs) and that plans call on theirs.
 #include "operators.h"
-#include "kv4.cuh"
+#include "kv4_chunk.cuh"
 #include "logprobs.cuh"
 
 #include <stdarg.h>
@@ -14,6 +14,7 @@ struct b200_kv4 {
     kv4::View view{};
     int head_size = 0, device = 0, sms = 148;
     size_t bytes = 0;
+    unsigned *host_error = nullptr, *device_error = nullptr; // a mapped word: what a wait that gave up leaves (kv4_chunk.cuh); null where the host had no memory for it
     char err[256] = "";
 };
 
@@ -150,8 +151,29 @@ static StepCut step_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, bo
     c.cluster = cluster_for(units, 8 * kv->sms, most);
     return c;
 }
-static size_t step_work_bytes(const b200_kv4 *kv, const b200_kv4_attention_args &a, const StepCut &c) {
-    return c.splits > 1 ? (size_t)a.n * a.heads * c.splits * (kv->head_size + 2) * 4 : 0;
+static size_t parts_bytes(const b200_kv4 *kv, const b200_kv4_attention_args &a, int splits) { return splits > 1 ? (size_t)a.n * a.heads * splits * (kv->head_size + 2) * 4 : 0; }
+
+// Chunks on the tensor cores: 16-bit results, heads of 64, 96 or 128.  A tile takes 128 rows whether they are used or not, single rows read the cache once each: 16 tokens of 4 heads
+// over 8192 positions 38 us there and 47 here, 32 tokens 70 and 49 (heads of 128, 8 key/value heads).
+const int CHUNK_MIN_ROWS = 2;
+struct ChunkCut {
+    int tokens, splits;
+    bool use;
+};
+static ChunkCut chunk_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, bool quants) {
+    ChunkCut c = {};
+    const int G = kv->view.kv_heads, mul = a.heads / G, hs = kv->head_size;
+    const int chunk = a.chunk < a.n ? a.chunk : a.n;
+    c.use = !quants && a.out_type != B200_GGML_F32 && (hs == 64 || hs == 96 || hs == 128) && mul <= kv4::CHUNK_ROWS && chunk > 1 && (long long)chunk * mul >= CHUNK_MIN_ROWS;
+    if (!c.use) return c;
+    c.tokens = kv4::CHUNK_ROWS / mul;
+    const long long units = (long long)((a.n + c.tokens - 1) / c.tokens) * G;
+    const int len = a.max_len > 0 && a.max_len < kv->view.context ? a.max_len : kv->view.context;
+    const long long seen = a.window > 0 && a.window + c.tokens < len ? a.window + c.tokens : len, worth = seen / (8 * kv4::CHUNK_KEYS); // eight tiles of positions a CTA
+    long long splits = kv->sms / units;
+    if (splits > worth) splits = worth;
+    c.splits = splits < 1 ? 1 : (int)splits;
+    return c;
 }
 
 cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_args &a, int8_t *quants, float *scales, cudaStream_t stream, bool pdl) {
@@ -165,10 +187,31 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
     k.out_type = quants ? KV4_OUT_Q8 : a.out_type;
     k.scale = a.scale;
     k.out = a.out; k.quants = quants; k.scales = scales;
-    StepCut c = step_cut(kv, a, quants != nullptr);
-    if (c.splits > 1 && a.workspace && step_work_bytes(kv, a, c) <= a.workspace_bytes) c.cluster = 1;
-    else c.splits = 1;
     k.work = a.workspace;
+    const auto has_room = [&](int splits) { return a.workspace && parts_bytes(kv, a, splits) <= a.workspace_bytes; };
+    const auto join = [&](auto hs, int splits) {
+        constexpr int per_cta = hs < 64 ? 64 / hs : 1;
+        return launch(kv4::k_step_join<hs>, (unsigned)a.n * ((a.heads + per_cta - 1) / per_cta), hs < 64 ? 64 : hs, 0, 1, true, stream, k, splits);
+    };
+    ChunkCut cc = chunk_cut(kv, a, quants != nullptr);
+    if (cc.use) {
+        if (!has_room(cc.splits)) cc.splits = 1;
+        kv4::Chunk ck = {k, cc.tokens, cc.splits, aligned16(a.out, a.out_stride, 2), kv->device_error};
+        const unsigned grid = (unsigned)((a.n + cc.tokens - 1) / cc.tokens) * kv->view.kv_heads * cc.splits;
+        const auto go = [&](auto hs) {
+            constexpr size_t smem = kv4::chunk_smem_bytes(hs);
+            auto kern = kv4::k_chunk<hs>;
+            cudaError_t e = prepare(kern, smem, 1);
+            if (e == cudaSuccess) e = launch(kern, grid, kv4::CHUNK_THREADS, smem, 1, pdl, stream, ck);
+            return e != cudaSuccess || cc.splits == 1 ? e : join(hs, cc.splits);
+        };
+        if (kv->head_size == 64) return go(std::integral_constant<int, 64>());
+        if (kv->head_size == 96) return go(std::integral_constant<int, 96>());
+        return go(std::integral_constant<int, 128>());
+    }
+    StepCut c = step_cut(kv, a, quants != nullptr);
+    if (c.splits > 1 && has_room(c.splits)) c.cluster = 1;
+    else c.splits = 1;
     return by_head_size(kv->head_size, [&](auto hs) {
         auto go = [&](auto nt) {
             constexpr size_t smem = kv4::step_smem_bytes(hs, 4 * nt);
@@ -176,9 +219,7 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
             auto kern = kv4::k_step<hs, nt>;
             cudaError_t e = prepare(kern, smem, c.cluster);
             if (e == cudaSuccess) e = launch(kern, grid, kv4::STEP_WARPS * 32, smem, c.cluster, pdl, stream, k, c.per_head, c.splits);
-            if (e != cudaSuccess || c.splits == 1) return e;
-            constexpr int per_cta = hs < 64 ? 64 / hs : 1;
-            return launch(kv4::k_step_join<hs>, (unsigned)a.n * ((a.heads + per_cta - 1) / per_cta), hs < 64 ? 64 : hs, 0, 1, true, stream, k, c.splits);
+            return e != cudaSuccess || c.splits == 1 ? e : join(hs, c.splits);
         };
         if constexpr (hs < 256) if (c.heads == 8) return go(std::integral_constant<int, 2>());
         return go(std::integral_constant<int, 1>());
@@ -229,6 +270,11 @@ int b200_kv4_create(int32_t slots, int32_t context, int32_t kv_heads, int32_t he
         e = cudaMemset(kv->view.base, 0, kv->bytes);
         if (e == cudaSuccess) e = cudaDeviceSynchronize(); // the memory is zeros for every stream
     }
+    if (e == cudaSuccess && cudaHostAlloc((void **)&kv->host_error, 4, cudaHostAllocMapped) == cudaSuccess) {
+        *kv->host_error = 0;
+        if (cudaHostGetDevicePointer((void **)&kv->device_error, kv->host_error, 0) != cudaSuccess) kv->device_error = nullptr;
+    }
+    cudaGetLastError(); // (the word only reports)
     if (e != cudaSuccess) {
         cudaGetLastError();
         say(err, err_len, 0, "4-bit cache of %.3g GB: %s", (double)bytes / 1e9, cudaGetErrorString(e));
@@ -243,7 +289,8 @@ int b200_kv4_create(int32_t slots, int32_t context, int32_t kv_heads, int32_t he
 void b200_kv4_free(b200_kv4 *kv) {
     if (!kv) return;
     OnDevice on(kv->device);
-    cudaFree(kv->view.base);
+    cudaFree(kv->view.base); // (waits for the device's work)
+    cudaFreeHost(kv->host_error);
     delete kv;
 }
 
@@ -256,6 +303,12 @@ int b200_kv4_reset(b200_kv4 *kv, void *stream) {
     cudaError_t e = on.error;
     if (e == cudaSuccess) e = cudaMemsetAsync(kv->view.base, 0, kv->bytes, (cudaStream_t)stream);
     return e == cudaSuccess ? B200_OK : fail(kv, cuda_code(e), "%s", cudaGetErrorString(e));
+}
+
+static int check_error(b200_kv4 *kv) {
+    if (kv->host_error && *reinterpret_cast<volatile unsigned *>(kv->host_error))
+        return fail(kv, B200_ERR_STATE, "an earlier attention of a chunk gave up a wait on the device: its results, and what came of them, are not valid");
+    return B200_OK;
 }
 
 static int check_rows(b200_kv4 *kv, int n, const int32_t *positions, int32_t start, const int32_t *slots, int32_t slot) {
@@ -288,7 +341,8 @@ int b200_kv4_append(b200_kv4 *kv, const b200_kv4_append_args *a, void *stream) {
 int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *a, void *stream) {
     if (!kv) return B200_ERR_BAD_ARG;
     if (!a) return fail(kv, B200_ERR_BAD_ARG, "null arguments");
-    int rc = check_rows(kv, a->n, a->positions, a->start, a->slots, a->slot);
+    int rc = check_error(kv);
+    if (!rc) rc = check_rows(kv, a->n, a->positions, a->start, a->slots, a->slot);
     if (rc) return rc;
     if (a->heads <= 0 || a->heads % kv->view.kv_heads) return fail(kv, B200_ERR_BAD_ARG, "%d query heads over %d key/value heads", a->heads, kv->view.kv_heads);
     if (!known_type(a->out_type)) return fail(kv, B200_ERR_UNSUPPORTED, "results of type %d (FP32, FP16 and BF16 are known)", a->out_type);
@@ -307,7 +361,8 @@ int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *a, void *str
 
 size_t b200_kv4_attention_workspace(const b200_kv4 *kv, const b200_kv4_attention_args *a) {
     if (!kv || !a || a->n <= 0 || a->heads <= 0 || a->heads % kv->view.kv_heads) return 0;
-    return step_work_bytes(kv, *a, step_cut(kv, *a, false));
+    const ChunkCut c = chunk_cut(kv, *a, false);
+    return parts_bytes(kv, *a, c.use ? c.splits : step_cut(kv, *a, false).splits);
 }
 
 int b200_kv4_read(b200_kv4 *kv, const b200_kv4_read_args *a, void *stream) {

@@ -67,6 +67,29 @@ def attention(q, k, v, d, positions, slots, scale, window):
     return out, bound
 
 
+def chunk_bound(q, k, v, positions, slots, scale, window, want, dtype):
+    """How far the tensor-core form may be off ``want`` = attention(...)[0].  Its operands are FP16 (half a step: 2^-11 of each): queries and keys put at most 2^-10 of
+    A = scale * sum |q| |k| on a score (and hs 2^-22 for sums in FP32), a probability's relative error is twice that (numerator and sum), plus 2^-11 for its rounding and 2^-11 for the
+    value's, n 2^-22 for the sums, 2^-20 for exponentials: all relative to sum p |v|.  A probability below FP16's range (the largest is at least 2^-8 of the row's scale): 2^-25 each.
+    At last the result's own half step."""
+    n, H, hs = q.shape
+    G = k.shape[2]
+    bound = torch.zeros_like(want)
+    for r in range(n):
+        p, s = int(positions[r]), int(slots[r])
+        lo = max(0, p - window + 1) if window else 0
+        if p < 0:
+            continue
+        for h in range(H):
+            g = h // (H // G)
+            kk, vv = k[s, lo:p + 1, g], v[s, lo:p + 1, g].abs()
+            w = torch.softmax(kk @ q[r, h] * scale, 0)
+            A = (kk.abs() @ q[r, h].abs()).max() * abs(scale)
+            m = p + 1 - lo
+            bound[r, h] = (w @ vv) * (2 * A * (2.0 ** -10 + hs * 2.0 ** -22) + 2 * 2.0 ** -11 + m * 2.0 ** -22 + 2.0 ** -20) + m * 2.0 ** -25 * vv.max()
+    return bound + want.abs() * half_step(dtype) + 2.0 ** -25
+
+
 def log_probs(x, targets, top):
     """(logprobs, entropy, ids, values) in float64 of rows x."""
     x = x.double().cpu()
