@@ -12,6 +12,8 @@
 // Rows of a tile may belong to several slots and stand in any order: a run of tokens of one slot is a segment, the tiles of all segments are one list, and a row masks what is not its own.
 // Every wait is bounded: after two seconds the CTA gives up, writes the cache's error word, waits for its products under way and frees its tensor memory.
 #pragma once
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace kv4 {
@@ -46,7 +48,7 @@ __device__ __forceinline__ bool bar_wait(const void *bar, unsigned parity, unsig
         unsigned done;
         asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}" : "=r"(done) : "r"(b), "r"(parity) : "memory");
         if (done) return true;
-        if ((i & 63u) == 0u) {
+        if ((i & 255u) == 0u) {
             if (*reinterpret_cast<volatile unsigned *>(bail)) return false;
             const unsigned long long now = gtime_ns();
             if (!began) began = now;
@@ -142,10 +144,6 @@ template <int HS> struct Raw {
             get(s + 8 * NG + 2 * t * NG + c * VW, vs[0] + c * VW);
             get(s + 8 * NG + (2 * t + 1) * NG + c * VW, vs[1] + c * VW);
         }
-    }
-    __device__ __forceinline__ void clear() {
-#pragma unroll
-        for (int i = 0; i < NG; i++) k[i] = v[i] = ks[i] = vs[0][i] = vs[1][i] = 0u;
     }
 };
 
@@ -281,96 +279,116 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
         // ===== records -> FP16 operands =====
         const int d = warp - CHUNK_SOFTMAX, w = d / 2, half = d % 2, g = lane >> 2, t = lane & 3;
         const uint32_t one = magic();
-        int seg = 0, ahead = 0, block = 0, stop = 0; // tiles left in the segment, this warp's record in the next one, the segment's end
-        const unsigned char *src = nullptr;
+        int seg = 0, ahead = 0, block = 0, stop = 0, behind = 0; // tiles left in the segment, this warp's record in the next one, the segment's end; raw is a record behind it
         if (count > 0) {
             while (sh.segments[seg].tiles <= first) seg++;
             const int before = seg ? sh.segments[seg - 1].tiles : 0;
             ahead = sh.segments[seg].tiles - first;
             block = sh.segments[seg].begin + (first - before) * CHUNK_RECORDS + w;
             stop = sh.segments[seg].end;
-            src = record<HS>(a.kv, sh.segments[seg].slot, kvh, block);
         }
-        auto fetch = [&](Raw<HS> &to) { // this warp's half record of the list's next tile
+        auto fetch = [&](Raw<HS> &to) { // this warp's half record of the list's next tile; behind the segment's end its last one, whose values then count as zeros
             if (ahead == 0) {
                 seg++;
                 ahead = sh.segments[seg].tiles - sh.segments[seg - 1].tiles;
                 block = sh.segments[seg].begin + w;
                 stop = sh.segments[seg].end;
-                src = record<HS>(a.kv, sh.segments[seg].slot, kvh, block);
             }
-            if (block < stop) to.load(src, half, lane);
-            else to.clear();
+            behind = block >= stop;
+            to.load(record<HS>(a.kv, sh.segments[seg].slot, kvh, min(block, stop - 1)), half, lane);
             ahead--;
             block += CHUNK_RECORDS;
-            src += CHUNK_RECORDS * record_bytes(HS);
         };
         // row 16 w + 8 half + g of the keys; positions 16 w + 8 half + 2 t, + 1 of the values: 16-byte chunk 2 (w % 4) + half of the rows of 64 positions
         const uint32_t k_at = s32(stages) + (w * 16 + half * 8 + g) * 64 + ((t ^ (g >> 1 & 3)) << 4);
         const uint32_t v_at = s32(stages) + NG * CHUNK_KEYS * 64 + (w / 4) * (HS * 128) + g * 128 + (((w % 4 * 2 + half) ^ g) << 4) + t * 4;
         const uint32_t k_perm = half ? 0x3232 : 0x1010, v_perm = half ? 0x7632 : 0x5410;
-        auto convert = [&](int j, Raw<HS> &now) {
+        struct Held { // a half record's values, until the product two tiles before them has read its own
+            uint32_t v[NG], d[NG]; // codes, scales of positions 8 half + 2 t and + 1
+        };
+        auto keys = [&](int j, Raw<HS> &now, Held &held) {
             // a value scale that FP16 products do not hold (or a NaN) is moved into the keys: such positions get no value and a NaN key
-            uint32_t dv[NG]; // of positions 8 half + 2 t and + 1
             __half2 widest;
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                dv[i] = __byte_perm(now.vs[0][i], now.vs[1][i], v_perm);
-                const __half2 x = __habs2(*reinterpret_cast<const __half2 *>(&dv[i]));
+                held.v[i] = now.v[i];
+                held.d[i] = __byte_perm(now.vs[0][i], now.vs[1][i], v_perm);
+                const __half2 x = __habs2(*reinterpret_cast<const __half2 *>(&held.d[i]));
                 widest = i ? __hmax2_nan(widest, x) : x;
             }
             const uint32_t wide = *reinterpret_cast<const uint32_t *>(&widest);
+            if (behind)
+#pragma unroll
+                for (int i = 0; i < NG; i++) held.d[i] = 0u;
             if (__any_sync(0xffffffffu, (0xeffeeffeu - wide & 0x80008000u) != 0x80008000u)) { // a half above 0x6ffe: 8 d up to 65504
                 uint32_t bad = ((wide & 0xffffu) > 0x6ffeu ? 1u << (2 * t) : 0u) | (wide >> 16 > 0x6ffeu ? 2u << (2 * t) : 0u); // by position of the half
                 bad = __reduce_or_sync(0xffffffffu, bad);
 #pragma unroll
                 for (int i = 0; i < NG; i++) {
-                    if (bad >> (2 * t) & 1u) dv[i] &= 0xffff0000u;
-                    if (bad >> (2 * t + 1) & 1u) dv[i] &= 0x0000ffffu;
+                    if (bad >> (2 * t) & 1u) held.d[i] &= 0xffff0000u;
+                    if (bad >> (2 * t + 1) & 1u) held.d[i] &= 0x0000ffffu;
                     if (bad >> g & 1u) now.ks[i] = 0x7fff7fffu;
                 }
             }
             const int b = j & 1;
-            const uint32_t stage = b * chunk_stage_bytes(HS);
             if (j >= 2 && !__all_sync(0xffffffffu, bar_wait(&sh.s_full[b], ((j >> 1) - 1) & 1, &sh.bail))) return false; // the product of tile j - 2 has read its keys
+            const uint32_t at = k_at + b * chunk_stage_bytes(HS);
 #pragma unroll
             for (int i = 0; i < NG; i++) {
                 uint32_t x[4];
                 unpack(now.k[i], one, x);
                 const uint32_t dk = __byte_perm(now.ks[i], 0, k_perm);
-                sts128(k_at + stage + i * (CHUNK_KEYS * 64), hmul2(x[0], dk), hmul2(x[1], dk), hmul2(x[2], dk), hmul2(x[3], dk));
+                sts128(at + i * (CHUNK_KEYS * 64), hmul2(x[0], dk), hmul2(x[1], dk), hmul2(x[2], dk), hmul2(x[3], dk));
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.k_full[b]);
-            if (j >= 2 && !__all_sync(0xffffffffu, bar_wait(&sh.free[b], ((j >> 1) - 1) & 1, &sh.bail))) return false; // ... and its values
+            return true;
+        };
+        auto values = [&](int j, const Held &held) {
+            const int b = j & 1;
+            if (j >= 2 && !__all_sync(0xffffffffu, bar_wait(&sh.free[b], ((j >> 1) - 1) & 1, &sh.bail))) return false; // the product of tile j - 2 has read its values
+            const uint32_t at = v_at + b * chunk_stage_bytes(HS);
 #pragma unroll
             for (int i = 0; i < NG; i++) {
                 uint32_t x[4];
-                unpack(now.v[i], one, x);
+                unpack(held.v[i], one, x);
 #pragma unroll
-                for (int u = 0; u < 4; u++) sts32(v_at + stage + (i * 32 + u * 8) * 128, hmul2(x[u], dv[i])); // row 32 i + 8 u + g: entry 32 i + 4 g + u
+                for (int u = 0; u < 4; u++) sts32(at + (i * 32 + u * 8) * 128, hmul2(x[u], held.d[i])); // row 32 i + 8 u + g: entry 32 i + 4 g + u
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.v_full[b]);
             return true;
         };
-        Raw<HS> even, odd; // two tiles by turns: what comes next is under way while a tile is converted
-        if (count > 0) fetch(even);
-        for (int j = 0; j < count; j += 2) {
-            if (j + 1 < count) fetch(odd);
-            if (!convert(j, even)) break;
-            if (j + 1 >= count) break;
-            if (j + 2 < count) fetch(even);
-            if (!convert(j + 1, odd)) break;
+        // Keys run a tile ahead of the values, which wait for the rows; the next record is asked for when this one's registers have been read, not before: loads share their
+        // scoreboards, and a wait for the older ones would be one for both (800 cycles a tile).
+        Raw<HS> raw;
+        Held even, odd;
+        bool ok = true;
+        if (count > 0) {
+            fetch(raw);
+            ok = keys(0, raw, even);
+            if (count > 1) fetch(raw);
+        }
+        for (int j = 0; j < count && ok; j += 2) {
+            if (j + 1 < count) {
+                if (!(ok = keys(j + 1, raw, odd))) break;
+                if (j + 2 < count) fetch(raw);
+            }
+            if (!(ok = values(j, even)) || j + 1 >= count) break;
+            if (j + 2 < count) {
+                if (!(ok = keys(j + 2, raw, even))) break;
+                if (j + 3 < count) fetch(raw);
+            }
+            ok = values(j + 1, odd);
         }
     } else if (warp == CHUNK_ISSUER && lane == 0) {
         // ===== products =====
         constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(CHUNK_KEYS >> 3) << 17) | ((uint32_t)(CHUNK_ROWS >> 4) << 24);
         constexpr uint32_t idesc_o = (1u << 4) | ((uint32_t)(HS >> 3) << 17) | ((uint32_t)(CHUNK_ROWS >> 4) << 24);
         const uint32_t q = s32(sQ), st = s32(stages);
-        auto values = [&](int j) { // O += P V of tile j
+        auto product = [&](int j) { // O += P V of tile j
             const int b = j & 1;
             if (!bar_wait(&sh.v_full[b], j >> 1 & 1, &sh.bail) || !bar_wait(&sh.p_full[b], j >> 1 & 1, &sh.bail)) return false;
             fence_after();
@@ -390,9 +408,9 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
 #pragma unroll
             for (int k = 0; k < HS / 16; k++) umma_ss(tS + b * 128, desc64(q + (k / 2) * (CHUNK_ROWS * 64) + (k % 2) * 32), desc64(sK + (k / 2) * (CHUNK_KEYS * 64) + (k % 2) * 32), idesc_s, k > 0);
             umma_commit(&sh.s_full[b]);
-            if (j > 0) ok = values(j - 1);
+            if (j > 0) ok = product(j - 1);
         }
-        if (ok && count > 0) ok = values(count - 1);
+        if (ok && count > 0) ok = product(count - 1);
         if (!ok) { // given up: what is under way ends before the tensor memory goes
             unsigned none = 0;
             umma_commit(&sh.drained);
@@ -441,7 +459,7 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
             // One pass with the maximum as it stands.  It moves rarely, and a sum of more than 2^8 shows that it has to: then the tile's maximum is looked for and the pass made again.
             // (A maximum of every tile in front of or beside the exponentials cost as much as they do.)
             float sum;
-            auto exponentials = [&](float ref) {
+            const auto exponentials_of = [&](auto masked, float ref) {
                 const unsigned long long factor2 = pack_f32x2(factor, factor), ref2 = pack_f32x2(-ref, -ref);
                 unsigned long long part[2] = {0ull, 0ull};
                 uint32_t s[2][PIECE];
@@ -451,7 +469,7 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
                     uint32_t(&x)[PIECE] = s[q & 1];
                     tmem_ld_wait();
                     if (q + 1 < COLUMNS / PIECE) tmem_ld16(row_s + (q + 1) * PIECE, s[q + 1 & 1]);
-                    if (mask)
+                    if constexpr (decltype(masked)::value)
 #pragma unroll
                         for (int i = 0; i < PIECE; i++)
                             if (!(q * PIECE + i >= from && q * PIECE + i < to)) x[i] = 0xff800000u;
@@ -471,6 +489,10 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
                 unpack_f32x2(part[0], a0, a1);
                 unpack_f32x2(part[1], b0, b1);
                 sum = (a0 + a1) + (b0 + b1);
+            };
+            const auto exponentials = [&](float ref) {
+                if (mask) exponentials_of(std::true_type(), ref);
+                else exponentials_of(std::false_type(), ref);
             };
             exponentials(m == -CUDART_INF_F ? 0.0f : m);
             const bool again = __any_sync(0xffffffffu, fresh || sum > 256.0f);

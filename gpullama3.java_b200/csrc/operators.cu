@@ -155,7 +155,7 @@ static size_t parts_bytes(const b200_kv4 *kv, const b200_kv4_attention_args &a, 
 
 // Chunks on the tensor cores: 16-bit results, heads of 64, 96 or 128.  A tile takes 128 rows whether they are used or not, single rows read the cache once each: 16 tokens of 4 heads
 // over 8192 positions 38 us there and 47 here, 32 tokens 70 and 49 (heads of 128, 8 key/value heads).
-const int CHUNK_MIN_ROWS = 2;
+const int CHUNK_MIN_ROWS = 64;
 struct ChunkCut {
     int tokens, splits;
     bool use;
