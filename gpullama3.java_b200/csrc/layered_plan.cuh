@@ -1243,7 +1243,9 @@ static int ly_build(b200_plan *p, const b200_layered_config *cfg, const b200_lay
 
 // One chunk of n <= cap tokens at positions start_pos..: fills the rings; optionally returns the logits of selected rows and
 // the residual stream after every run ([runs][n][width]).
-static int ly_batch(b200_plan *p, const int32_t *tokens, int n, int start_pos, const int32_t *rows, int n_rows, float *logits_out, float *trace_out) {
+// `score`: the rows' log probabilities into the plan's result buffers (score_rows) in place of their logits.
+struct LyScore { int at, top; };
+static int ly_batch(b200_plan *p, const int32_t *tokens, int n, int start_pos, const int32_t *rows, int n_rows, float *logits_out, float *trace_out, const LyScore *score = nullptr) {
     Layered &Y = *p->ly;
     const int E = Y.c.width, V = Y.c.vocab_size;
     if (n > Y.cap) return fail(p, B200_ERR_BAD_ARG, "chunk of %d tokens exceeds prefill_batch_size %d", n, Y.cap);
@@ -1252,7 +1254,7 @@ static int ly_batch(b200_plan *p, const int32_t *tokens, int n, int start_pos, c
         if (tokens[i] < 0 || tokens[i] >= V) return fail(p, B200_ERR_BAD_ARG, "token %d out of range", tokens[i]);
     for (int i = 0; i < n_rows; i++)
         if (rows[i] < 0 || rows[i] >= n) return fail(p, B200_ERR_BAD_ARG, "row %d outside the chunk of %d tokens", rows[i], n);
-    if (n_rows > 0 && (!rows || !logits_out)) return fail(p, B200_ERR_BAD_ARG, "rows without an output buffer");
+    if (n_rows > 0 && (!rows || !(logits_out || score))) return fail(p, B200_ERR_BAD_ARG, "rows without an output buffer");
     int rc;
     if (trace_out && !Y.trace)
         if ((rc = dalloc(p, &Y.trace, Y.runs.size() * (size_t)Y.cap * E * 4))) return rc;
@@ -1296,7 +1298,9 @@ static int ly_batch(b200_plan *p, const int32_t *tokens, int n, int start_pos, c
         if ((rc = ly_project<ly::EPI_STORE>(p, false, m, Y.A32, Y.A16, Y.head, nullptr, V, E, Y.LOG, nullptr, V, 0, &t_head))) return rc;
         if (Y.c.logit_softcap > 0.0f &&
             (rc = launch_k(p, p->use_pdl, ly::k_softcap, dim3((unsigned)(((size_t)m * V + 255) / 256)), dim3(256), (size_t)0, Y.LOG, (long long)m * V, Y.c.logit_softcap))) return rc;
-        CK(cudaMemcpyAsync(logits_out + (size_t)r0 * V, Y.LOG, (size_t)m * V * 4, cudaMemcpyDeviceToHost, p->stream));
+        if (score) {
+            if ((rc = score_rows(p, Y.LOG, m, score->at + r0, score->top))) return rc;
+        } else CK(cudaMemcpyAsync(logits_out + (size_t)r0 * V, Y.LOG, (size_t)m * V * 4, cudaMemcpyDeviceToHost, p->stream));
         CK(cudaStreamSynchronize(p->stream));
     }
     CK(cudaEventElapsedTime(&p->prefill_ms, p->ev0, p->ev1));

@@ -18,9 +18,11 @@ namespace cg = cooperative_groups;
 using bf16 = __nv_bfloat16;
 typedef unsigned long long u64;
 
-constexpr int THREADS = 512, PER_THREAD = 16, BATCH = THREADS * PER_THREAD, MAX_TOP = 32, MAX_CLUSTER = 16;
+constexpr int THREADS = 256, PER_THREAD = 16, BATCH = THREADS * PER_THREAD, MAX_TOP = 32, MAX_CLUSTER = 16;
 constexpr int PUSHERS = 64;                                // threads that may add candidates in a batch: more of them raise the threshold first
-constexpr int BUFFER = MAX_TOP + 2 * PUSHERS * PER_THREAD; // what is left of the last selection, and two batches' worth
+constexpr int MANY = 96;                                   // candidates from which the best of them are chosen, so that the threshold rises
+constexpr int BUFFER = MANY + PUSHERS * PER_THREAD;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct Args {
     const void *logits;
@@ -41,16 +43,22 @@ __device__ __forceinline__ float value_of(u64 key) {
 }
 __device__ __forceinline__ unsigned index_of(u64 key) { return ~(unsigned)key; }
 
-struct Sum { // of a set of entries: its largest, and what the others add
+__device__ __forceinline__ float ex2(float x) { // 2^x
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+struct Sum { // of a set of entries: its largest, and what the others add (s in units of log2)
     float m, z, s;
 };
 __device__ __forceinline__ Sum join(const Sum &p, const Sum &q) {
     const bool first = p.m >= q.m;
     const Sum &a = first ? p : q, &b = first ? q : p;
-    const float d = b.m - a.m; // (-inf where a set is empty; NaN where both are)
+    const float d = (b.m - a.m) * LOG2E; // (-inf where a set is empty; NaN where both are)
     Sum r = a;
     if (d > -CUDART_INF_F) {
-        const float e = __expf(d);
+        const float e = ex2(d);
         r.z = fmaf(1.0f + b.z, e, a.z);
         r.s = fmaf(fmaf(d, 1.0f + b.z, b.s), e, a.s);
     }
@@ -113,25 +121,24 @@ __device__ __forceinline__ void select(Smem &sm, int total, int n) {
     __syncthreads();
 }
 
-// A cluster of CTAs reads a row, each a stretch of it in batches of 16 entries a thread.  A thread keeps the sum of its own entries; candidates for the alternatives are the entries
-// above a threshold that at least `top` known ones reach, so that after the first batch hardly any is looked at twice.
-template <typename T> __global__ void __launch_bounds__(THREADS) k_log_probs(const Args a) {
+// A cluster of CTAs reads a row, each a stretch of it in batches of 16 entries a thread, the next batch under way while one is worked on.  A warp keeps the largest entry it has met and
+// a thread the sum of its own entries in units of that; candidates for the alternatives are the entries above a threshold that at least `top` known ones reach, so that after the first
+// batch hardly any is looked at twice.  Bytes bound it: 512 rows of 128256 FP32 logits are 263 MB, 41 us.
+template <typename T> __global__ void __launch_bounds__(THREADS, 3) k_log_probs(const Args a) {
     constexpr int VEC = Load<T>::VEC;
     __shared__ Smem sm;
     cg::cluster_group cluster = cg::this_cluster();
-    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ranks, tid = threadIdx.x;
+    const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31;
     const T *x = (const T *)a.logits + row * a.ld;
     const int skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)); // entries between the 16-byte boundary in front of the row and its start
     const long long span = (long long)skew + a.vocab;
     // stretches of whole vectors, as even as that allows
     const long long vecs = (span + VEC - 1) / VEC, begin = vecs * rank / ranks * VEC, end = vecs * (rank + 1) / ranks * VEC;
     if (tid == 0) { sm.pushed = 0; sm.n_best = 0; }
-    Sum mine = {-CUDART_INF_F, 0.0f, 0.0f};
+    float m = -CUDART_INF_F, z = 0.0f, s = 0.0f; // the warp's largest; this thread's sums, without it
     u64 bar = 0; // keys that are not larger are no candidates
     float bar_value = -CUDART_INF_F;
-    __syncthreads();
-    for (long long base = begin; base < end; base += BATCH) {
-        float v[PER_THREAD];
+    const auto fetch = [&](long long base, float (&v)[PER_THREAD]) {
 #pragma unroll
         for (int i = 0; i < PER_THREAD / VEC; i++) {
             const long long at = base + ((long long)i * THREADS + tid) * VEC - skew; // index in the row
@@ -140,31 +147,47 @@ template <typename T> __global__ void __launch_bounds__(THREADS) k_log_probs(con
 #pragma unroll
                 for (int j = 0; j < VEC; j++) v[i * VEC + j] = at + j >= 0 && at + j < a.vocab && at + skew < end ? Load<T>::one(x + at + j) : -CUDART_INF_F;
         }
+    };
+    const auto take = [&](long long base, const float (&v)[PER_THREAD]) {
         float top = v[0];
 #pragma unroll
         for (int i = 1; i < PER_THREAD; i++) top = fmaxf(top, v[i]);
-        if (top > mine.m) { // a new largest entry: the sum goes on without its first one
-            Sum add = {top, 0.0f, 0.0f};
-            bool out = false;
-#pragma unroll
-            for (int i = 0; i < PER_THREAD; i++) {
-                const float y = v[i] - top;
-                const float e = !out && v[i] == top ? 0.0f : __expf(y);
-                out |= v[i] == top;
-                add.z += e;
-                add.s = fmaf(fmaxf(y, -1000.0f), e, add.s);
+        const float widest = value_of((u64)__reduce_max_sync(0xffffffffu, (unsigned)(key_of(top == top ? top : -CUDART_INF_F, 0) >> 32)) << 32); // (all NaN: none)
+        int skip = PER_THREAD; // this thread's entry that is the warp's largest from now on
+        if (widest > m) {
+            const float d = (m - widest) * LOG2E, e = d > -CUDART_INF_F ? ex2(d) : 0.0f;
+            if (e > 0.0f) s = fmaf(d, z, s) * e; else s = 0.0f;
+            z = z == z ? z * e : z;
+            if (lane == 0 && e > 0.0f) { // the largest so far becomes one of the others
+                z += e;
+                s = fmaf(d, e, s);
             }
-            mine = join(add, mine);
-        } else {
-            const float ref = mine.m == -CUDART_INF_F ? 0.0f : mine.m;
+            m = widest;
+            const unsigned owner = __ballot_sync(0xffffffffu, top == widest);
+            if (lane == __ffs(owner) - 1)
 #pragma unroll
-            for (int i = 0; i < PER_THREAD; i++) {
-                const float y = v[i] - ref, e = __expf(y);
-                mine.z += e;
-                mine.s = fmaf(fmaxf(y, -1000.0f), e, mine.s);
-            }
+                for (int i = PER_THREAD - 1; i >= 0; i--)
+                    if (v[i] == widest) skip = i;
         }
-        if (a.top == 0) continue;
+        const float ref = m == -CUDART_INF_F ? 0.0f : -m * LOG2E;
+        float zs[2] = {0.0f, 0.0f}, ss[2] = {0.0f, 0.0f};
+        if (__any_sync(0xffffffffu, skip < PER_THREAD)) {
+#pragma unroll
+            for (int i = 0; i < PER_THREAD; i++) {
+                const float y = fmaf(v[i], LOG2E, ref), e = i == skip ? 0.0f : ex2(y);
+                zs[i & 1] += e;
+                ss[i & 1] = fmaf(fmaxf(y, -1000.0f), e, ss[i & 1]); // (-inf times 0 is none)
+            }
+        } else
+#pragma unroll
+            for (int i = 0; i < PER_THREAD; i++) {
+                const float y = fmaf(v[i], LOG2E, ref), e = ex2(y);
+                zs[i & 1] += e;
+                ss[i & 1] = fmaf(fmaxf(y, -1000.0f), e, ss[i & 1]);
+            }
+        z += zs[0] + zs[1];
+        s += ss[0] + ss[1];
+        if (a.top == 0) return;
         u64 largest = 0;
         if (top >= bar_value)
 #pragma unroll
@@ -175,7 +198,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) k_log_probs(con
             }
         const bool over = largest > bar;
         const int n = __syncthreads_count(over);
-        if (n == 0) continue;
+        if (n == 0) return;
         u64 least = bar + 1;
         if (n > PUSHERS) { // at least `top` and at most PUSHERS threads hold a key from here on: half the interval at a time (the keys are no two alike, so such a bar exists)
             u64 low = bar, high = ~0ull;
@@ -186,8 +209,10 @@ template <typename T> __global__ void __launch_bounds__(THREADS) k_log_probs(con
                 else if (above < a.top) high = least;
                 else break;
             }
+            bar = least - 1; // `top` candidates reach it
+            bar_value = value_of(least);
         }
-        if (sm.pushed + PUSHERS * PER_THREAD > BUFFER) { // (the same for every thread: the barrier above follows the last push)
+        if (sm.pushed > MANY) { // (the same for every thread: the barrier above follows the last push)
             __syncthreads();
             select(sm, sm.pushed, a.top);
             if (sm.n_best == a.top && sm.buffer[a.top - 1] > bar) { bar = sm.buffer[a.top - 1]; bar_value = value_of(bar); }
@@ -200,18 +225,24 @@ template <typename T> __global__ void __launch_bounds__(THREADS) k_log_probs(con
                 const u64 k = key_of(v[i], (unsigned)(at - skew));
                 if (at >= skew && at < span && at < end && v[i] == v[i] && k >= least) sm.buffer[atomicAdd(&sm.pushed, 1)] = k;
             }
-        if (n > PUSHERS && least > bar) { // `top` candidates reach it
-            bar = least - 1;
-            bar_value = value_of(least);
-        }
+    };
+    float v0[PER_THREAD], v1[PER_THREAD];
+    if (begin < end) fetch(begin, v0);
+    __syncthreads();
+    for (long long base = begin; base < end; base += 2 * BATCH) {
+        if (base + BATCH < end) fetch(base + BATCH, v1);
+        take(base, v0);
+        if (base + BATCH >= end) break;
+        if (base + 2 * BATCH < end) fetch(base + 2 * BATCH, v0);
+        take(base + BATCH, v1);
     }
     // ---- join: threads, then CTAs -------------------------------------------------------------------------------------------------------------------------------
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const Sum other = {__shfl_xor_sync(0xffffffffu, mine.m, o), __shfl_xor_sync(0xffffffffu, mine.z, o), __shfl_xor_sync(0xffffffffu, mine.s, o)};
-        mine = join(mine, other);
+        z += __shfl_xor_sync(0xffffffffu, z, o);
+        s += __shfl_xor_sync(0xffffffffu, s, o);
     }
-    if ((tid & 31) == 0) sm.warps[tid >> 5] = mine;
+    if (lane == 0) sm.warps[tid >> 5] = {m, z, s};
     __syncthreads();
     if (a.top) select(sm, sm.pushed, a.top);
     if (tid == 0) {
@@ -231,7 +262,7 @@ template <typename T> __global__ void __launch_bounds__(THREADS) k_log_probs(con
                 const int t = a.targets ? a.targets[row] : -1;
                 a.logprobs[row] = t < 0 || t >= a.vocab ? 0.0f : none ? CUDART_NAN_F : Load<T>::one(x + t) - all.m - log_z;
             }
-            if (a.entropy) a.entropy[row] = none ? CUDART_NAN_F : log_z - all.s * inv;
+            if (a.entropy) a.entropy[row] = none ? CUDART_NAN_F : log_z - all.s * LN2 * inv;
         }
         if (a.top) {
             for (int i = tid; i < ranks * MAX_TOP; i += THREADS) {

@@ -176,7 +176,7 @@ static ChunkCut chunk_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, 
     return c;
 }
 
-cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_args &a, int8_t *quants, float *scales, cudaStream_t stream, bool pdl) {
+cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_args &a, int8_t *quants, float *scales, cudaStream_t stream, bool pdl, int *launches) {
     kv4::Step k;
     k.kv = kv->view;
     k.rows = {a.positions, a.slots, a.n, a.start, a.slot};
@@ -196,6 +196,7 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
     ChunkCut cc = chunk_cut(kv, a, quants != nullptr);
     if (cc.use) {
         if (!has_room(cc.splits)) cc.splits = 1;
+        if (launches) *launches = cc.splits > 1 ? 2 : 1;
         kv4::Chunk ck = {k, cc.tokens, cc.splits, aligned16(a.out, a.out_stride, 2), kv->device_error};
         const unsigned grid = (unsigned)((a.n + cc.tokens - 1) / cc.tokens) * kv->view.kv_heads * cc.splits;
         const auto go = [&](auto hs) {
@@ -212,6 +213,7 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
     StepCut c = step_cut(kv, a, quants != nullptr);
     if (c.splits > 1 && has_room(c.splits)) c.cluster = 1;
     else c.splits = 1;
+    if (launches) *launches = c.splits > 1 ? 2 : 1;
     return by_head_size(kv->head_size, [&](auto hs) {
         auto go = [&](auto nt) {
             constexpr size_t smem = kv4::step_smem_bytes(hs, 4 * nt);
@@ -225,6 +227,8 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
         return go(std::integral_constant<int, 1>());
     });
 }
+
+bool kv4_gave_up(const b200_kv4 *kv) { return kv->host_error && *reinterpret_cast<volatile unsigned *>(kv->host_error); }
 
 cudaError_t log_probs_launch(const b200_log_probs_args &a, cudaStream_t stream) {
     lp::Args k;
@@ -306,7 +310,7 @@ int b200_kv4_reset(b200_kv4 *kv, void *stream) {
 }
 
 static int check_error(b200_kv4 *kv) {
-    if (kv->host_error && *reinterpret_cast<volatile unsigned *>(kv->host_error))
+    if (kv4_gave_up(kv))
         return fail(kv, B200_ERR_STATE, "an earlier attention of a chunk gave up a wait on the device: its results, and what came of them, are not valid");
     return B200_OK;
 }

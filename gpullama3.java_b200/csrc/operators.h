@@ -8,5 +8,6 @@
 #define KV4_OUT_Q8 8
 
 cudaError_t kv4_append_launch(const b200_kv4 *kv, const b200_kv4_append_args &a, cudaStream_t stream, bool pdl);
-cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_args &a, int8_t *quants, float *scales, cudaStream_t stream, bool pdl);
+cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_args &a, int8_t *quants, float *scales, cudaStream_t stream, bool pdl, int *launches = nullptr);
+bool kv4_gave_up(const b200_kv4 *kv); // a wait of a chunk's attention ran out (after a synchronisation)
 cudaError_t log_probs_launch(const b200_log_probs_args &a, cudaStream_t stream);

@@ -11,6 +11,7 @@
 #include "kquant.cuh"
 #include "decode_persistent.cuh"
 #include "sampler.cuh"
+#include "operators.h"
 
 #include <math.h>
 #include <stdarg.h>
@@ -130,6 +131,13 @@ struct b200_plan {
     cudaEvent_t ev0 = nullptr, ev1 = nullptr;
 
     PrefillCtx prefill;
+    // a cache of 4-bit codes in place of key_cache / value_cache (b200_set_kv_mode): a slot per layer; rotated queries, and room for the parts of attentions that many CTAs share
+    b200_kv4 *kv4 = nullptr;
+    float *kv4_q = nullptr, *kv4_work = nullptr;
+    size_t kv4_work_bytes = 0;
+    // device-side targets and results of b200_score_tokens: int target, then logprob and entropy, then up to 32 alternatives' ids and log probabilities, each [score_rows]
+    int *score_buf = nullptr;
+    int score_rows = 0;
     // batched exact prefill (exact_prefill.cuh); rows = prefill_batch padded to whole token tiles, 0 = not built for this plan
     struct {
         int rows = 0;
@@ -712,6 +720,34 @@ bool logits_direct(const b200_plan *p, const float *logits) {
 }
 int *id_behind_logits(const b200_plan *p) { return reinterpret_cast<int *>(p->logits + p->logits_words - 1); }
 
+// n rows of a QKV product at `pos` (device positions, or null: start, start + 1, ..) into layer l's slot of the 4-bit cache, and their attention (2 or 3 launches).
+int kv4_layer(b200_plan *p, int l, int n, const float *qkv, int ld, const int *pos, int start, int max_len, void *out, int out_type, int8_t *quants, float *scales, bool pdl, int *launches) {
+    const b200_config &c = p->cfg;
+    const LayerW &L = p->layers[l];
+    b200_kv4_append_args a = {};
+    a.n = n; a.heads = c.n_heads; a.type = B200_GGML_F32;
+    a.rope_layout = p->kflags & KF_NEOX ? B200_ROPE_HALF : B200_ROPE_INTERLEAVED;
+    a.q = qkv; a.k = qkv + p->qd; a.v = qkv + p->qd + p->kvd;
+    a.q_stride = a.k_stride = a.v_stride = ld; a.q_out_stride = p->qd;
+    a.positions = pos; a.start = start; a.slot = l;
+    if (p->kflags & KF_QKNORM) { a.q_norm = L.q_norm; a.k_norm = L.k_norm; }
+    a.cos = p->rope_cr; a.sin = p->rope_ci;
+    a.eps = c.rms_norm_eps;
+    a.q_out = p->kv4_q;
+    CK(kv4_append_launch(p->kv4, a, p->stream, pdl));
+    b200_kv4_attention_args t = {};
+    t.n = n; t.heads = c.n_heads; t.max_len = max_len; t.chunk = n; t.out_type = out_type;
+    t.q = p->kv4_q; t.q_stride = t.out_stride = p->qd;
+    t.out = out;
+    t.positions = pos; t.start = start; t.slot = l;
+    t.scale = (float)(1.0 / sqrt((double)c.head_size));
+    t.workspace = p->kv4_work; t.workspace_bytes = p->kv4_work_bytes;
+    int m = 0;
+    CK(kv4_attention_launch(p->kv4, t, quants, scales, p->stream, pdl, &m));
+    if (launches) *launches += 1 + m;
+    return B200_OK;
+}
+
 // Enqueue one single-token forward on p->stream (captured into a CUDA graph at creation).
 // with_logits=false is the prefill variant (InferenceCoreBatchPrefillDecode.java:166-167).
 int enqueue_forward(b200_plan *p, bool with_logits, int *launches, bool trace = false, bool deep = false) {
@@ -751,7 +787,9 @@ int enqueue_forward(b200_plan *p, bool with_logits, int *launches, bool trace = 
         else rc = launch_matvec_f16<MODE_STORE>(p, L.qkv, p->xb, p->qkv);
         if (rc) return rc; n++;
         float *kc = p->key_cache + (size_t)l * ctx_kv, *vc = p->value_cache + (size_t)l * ctx_kv;
-        {
+        if (p->kv4) { // the row goes into the cache, then the attention over it: positions up to ATT_SPLIT, or the whole context
+            if ((rc = kv4_layer(p, l, 1, p->qkv, p->qd + 2 * p->kvd, &p->st->pos, 0, deep ? 0 : ATT_SPLIT, q8 ? nullptr : xbf, B200_GGML_F32, q8 ? p->attq : nullptr, q8 ? p->atts : nullptr, pdl, &n))) return rc;
+        } else {
             const int cluster = deep ? att_cluster(c.head_size, c.context_length) : 1;
             const size_t att_smem = att_smem_bytes(c.head_size, c.context_length, p->att_scratch != nullptr, cluster);
             auto att = [&](auto kern) {
@@ -920,6 +958,7 @@ int capture_all(b200_plan *p) {
     int rc;
     if ((rc = capture(p, true, &p->g_decode, &p->launches_decode))) return rc;
     if ((rc = capture(p, false, &p->g_prefill, nullptr))) return rc;
+    if (p->kv4) return p->cfg.context_length <= ATT_SPLIT ? B200_OK : (rc = capture(p, true, &p->g_decode_deep, nullptr, false, false, true)) ? rc : capture(p, false, &p->g_prefill_deep, nullptr, false, false, true);
     if (p->att_rows) { // two graphs, chosen by the position on the host: up to ATT_SPLIT positions the cluster's launch only costs (measured: 1 - 2 %)
         if ((rc = capture(p, true, &p->g_decode_deep, nullptr, false, false, true))) return rc;
         if ((rc = capture(p, false, &p->g_prefill_deep, nullptr, false, false, true))) return rc;
@@ -1716,12 +1755,17 @@ int prefill_forward(b200_plan *p, int n, int start_pos, int *launches) {
         nl++;
         const int qt = PA_ROWS / kv_mul;
         const dim3 ag((n + qt - 1) / qt, g.n_kv_heads);
-        if (start_pos > 0 && !c.att_simt) { // rows written by earlier chunks / decode steps
+        if (p->kv4) {
+            int rc;
+            if ((rc = kv4_layer(p, l, n, c.QKV, nqkv, nullptr, start_pos, start_pos + n, c.ATT16, B200_GGML_F16, nullptr, nullptr, false, &nl))) return rc;
+            nl -= 2; // (counted below)
+        } else if (start_pos > 0 && !c.att_simt) { // rows written by earlier chunks / decode steps
             const size_t n4 = (size_t)start_pos * p->kvd / 4;
             k_pf_kv_to_f16<<<(unsigned)((n4 + 255) / 256 < 1184 ? (n4 + 255) / 256 : 1184), 256, 0, s>>>(kc, vc, c.KH, c.VH, n4);
             nl++;
         }
-        if (g.head_size == 128) {
+        if (p->kv4) {
+        } else if (g.head_size == 128) {
             k_pf_rope_kv<128><<<n, 256, 0, s>>>(c.QKV, nqkv, kc, vc, c.KH, c.VH, p->kvd, g.n_heads, g.n_kv_heads, p->kflags, L.q_norm, L.k_norm, g.rms_norm_eps, p->rope_cr, p->rope_ci, start_pos);
             if (c.att_simt) k_pf_attention<128><<<ag, PA_THREADS, pa_smem_bytes<128>(), s>>>(c.QKV, nqkv, kc, vc, p->kvd, kv_mul, n, start_pos, inv_sqrt_hs, c.ATT16, p->qd);
             else k_pf_attention_mma<128><<<ag, PM_THREADS, pm_smem_bytes<128>(), s>>>(c.QKV, nqkv, c.KH, c.VH, p->kvd, kv_mul, n, start_pos, inv_sqrt_hs, c.ATT16, p->qd);
@@ -1782,12 +1826,46 @@ cudaGraphExec_t prefill_graph(b200_plan *p, int pos) {
 
 // After a synchronize: did a device-side wait of the persistent kernel (or a tensor-parallel flag wait) give up?
 int check_device_error(b200_plan *p) {
+    if (p->kv4 && kv4_gave_up(p->kv4)) return fail(p, B200_ERR_STATE, "a wait of the attention over the 4-bit cache gave up on the device; the plan must be freed");
     if (p->h_err && *reinterpret_cast<volatile unsigned *>(p->h_err)) {
         const unsigned code = *reinterpret_cast<volatile unsigned *>(p->h_err);
         if (code == 200u) return fail(p, B200_ERR_STATE, "a copy into the operand ring of the exact prefill's product did not arrive in time; the plan must be freed");
         return fail(p, B200_ERR_STATE, "a device-side wait timed out (code %u: 1+phase of the persistent decode kernel, 100+slot of a tensor-parallel flag): a peer "
                                        "rank is missing or the ranks' call sequences diverged; the plan must be freed", code);
     }
+    return B200_OK;
+}
+
+// The values of a layer's keys or values in a 4-bit cache, as FP32 [context][kv width].
+int kv4_read_layer(b200_plan *p, int layer, bool keys, void *dst, size_t bytes) {
+    const size_t n = (size_t)p->cfg.context_length * p->kvd;
+    float *both = nullptr;
+    CK(cudaSetDevice(p->device));
+    CK(cudaMalloc(&both, 2 * n * 4));
+    b200_kv4_read_args a = {};
+    a.n = p->cfg.context_length; a.type = B200_GGML_F32; a.k = both; a.v = both + n; a.slot = layer;
+    int rc = b200_kv4_read(p->kv4, &a, p->stream);
+    cudaError_t e = rc == B200_OK ? cudaStreamSynchronize(p->stream) : cudaSuccess;
+    if (rc == B200_OK && e == cudaSuccess) e = cudaMemcpy(dst, keys ? both : both + n, bytes, cudaMemcpyDeviceToHost);
+    cudaFree(both);
+    if (rc != B200_OK) return fail(p, rc, "%s", b200_kv4_last_error(p->kv4));
+    CK(e);
+    return B200_OK;
+}
+
+// Log probabilities of `rows` logits rows (FP32, device) into the plan's result buffers from row `at` on; targets stand there already.
+int score_rows(b200_plan *p, const float *logits, int rows, int at, int top) {
+    float *f = reinterpret_cast<float *>(p->score_buf + p->score_rows);
+    b200_log_probs_args a = {};
+    a.logits = logits; a.row_stride = p->cfg.vocab_size; a.rows = rows; a.vocab = p->cfg.vocab_size; a.type = B200_GGML_F32; a.top = top; a.device = p->device;
+    a.targets = p->score_buf + at;
+    a.logprobs = f + at;
+    a.entropy = f + p->score_rows + at;
+    if (top) {
+        a.top_ids = reinterpret_cast<int *>(f + 2 * (size_t)p->score_rows) + (size_t)at * top;
+        a.top_logprobs = f + (2 + 32) * (size_t)p->score_rows + (size_t)at * top;
+    }
+    CK(log_probs_launch(a, p->stream));
     return B200_OK;
 }
 
@@ -1949,7 +2027,7 @@ int b200_forward_batch_prefill(b200_plan *p, const int32_t *tokens, int32_t n, i
         CK(cudaEventRecord(p->ev1, p->stream));
         CK(cudaStreamSynchronize(p->stream));
         CK(cudaEventElapsedTime(&p->prefill_ms, p->ev0, p->ev1));
-        return B200_OK;
+        return p->kv4 ? check_device_error(p) : B200_OK;
     }
     // Exact path (bit-identical KV cache to the CPU batchForwardJavaPrefill, InferenceCoreBatchPrefillDecode.java:62-168): the whole chunk
     // at once where the plan has the buffers for it, else the prefill graph token by token.
@@ -2000,6 +2078,7 @@ int b200_decode_sequence(b200_plan *p, const int32_t *tokens, int32_t n, int32_t
 int b200_set_decode_mode(b200_plan *p, int32_t mode) {
     if (!p || (mode != B200_DECODE_GRAPH && mode != B200_DECODE_PERSISTENT)) return B200_ERR_BAD_ARG;
     if (!p->g_decode) return fail(p, B200_ERR_STATE, "tensor-parallel plan: call b200_tp_attach on every rank first");
+    if (mode == B200_DECODE_PERSISTENT && p->kv4) return fail(p, B200_ERR_UNSUPPORTED, "the persistent decode kernel reads an FP32 cache; this plan's holds 4 bits");
     if (mode == B200_DECODE_PERSISTENT && !p->pd_ok) return fail(p, B200_ERR_UNSUPPORTED, "%s", p->pd_why.c_str());
     p->decode_mode = mode;
     return B200_OK;
@@ -2033,6 +2112,114 @@ int b200_trace_persistent(b200_plan *p, int32_t token, int32_t position, uint64_
     if (n_rows) *n_rows = p->cfg.n_layers + 1;
     if (n_stamps) *n_stamps = PD_STAMPS;
     return B200_OK;
+}
+
+int b200_set_kv_mode(b200_plan *p, int32_t mode) {
+    if (!p || (mode != B200_KV_F32 && mode != B200_KV_Q4)) return B200_ERR_BAD_ARG;
+    if ((mode == B200_KV_Q4) == (p->kv4 != nullptr)) return B200_OK;
+    if (p->ly) return fail(p, B200_ERR_UNSUPPORTED, "layered plans keep their own caches");
+    if (mode == B200_KV_F32) return fail(p, B200_ERR_UNSUPPORTED, "the plan's FP32 cache has been given back");
+    if (p->cfg.tp_size > 1) return fail(p, B200_ERR_UNSUPPORTED, "a 4-bit cache is single-GPU");
+    const b200_config &c = p->cfg;
+    CK(cudaSetDevice(p->device));
+    CK(cudaStreamSynchronize(p->stream));
+    char err[256] = "";
+    b200_kv4 *kv4 = nullptr;
+    int rc = b200_kv4_create(c.n_layers, c.context_length, c.n_kv_heads, c.head_size, p->device, &kv4, err, sizeof err);
+    if (rc != B200_OK) return fail(p, rc, "%s", err);
+    // Everything the new cache needs in front of anything the old one gives back: a plan that cannot switch goes on as it was.
+    cudaGraphExec_t *const graphs[] = {&p->g_decode, &p->g_prefill, &p->g_trace, &p->g_decode_deep, &p->g_prefill_deep, &p->g_trace_deep, &p->g_pdecode, &p->g_pprefill, &p->g_ptrace};
+    cudaGraphExec_t old[sizeof graphs / sizeof *graphs];
+    for (size_t i = 0; i < sizeof graphs / sizeof *graphs; i++) { old[i] = *graphs[i]; *graphs[i] = nullptr; }
+    const size_t n_allocs = p->allocs.size();
+    const int64_t bytes = p->bytes;
+    const int launches = p->launches_decode, rows = p->prefill_batch > 1 ? p->prefill_batch : 1;
+    p->kv4 = kv4;
+    p->kv4_work_bytes = (size_t)p->n_sms * 128 * (c.head_size + 2) * 4; // parts of as many tiles of 128 rows as there are SMs
+    rc = dalloc(p, &p->kv4_q, (size_t)rows * p->qd * 4);
+    if (!rc) rc = dalloc(p, &p->kv4_work, p->kv4_work_bytes);
+    if (!rc) rc = capture_all(p);
+    if (rc) {
+        for (size_t i = 0; i < sizeof graphs / sizeof *graphs; i++) {
+            if (*graphs[i]) cudaGraphExecDestroy(*graphs[i]);
+            *graphs[i] = old[i];
+        }
+        for (; p->allocs.size() > n_allocs; p->allocs.pop_back()) cudaFree(p->allocs.back());
+        p->bytes = bytes;
+        p->launches_decode = launches;
+        p->kv4 = nullptr;
+        p->kv4_q = p->kv4_work = nullptr;
+        b200_kv4_free(kv4);
+        cudaGetLastError();
+        return rc;
+    }
+    for (cudaGraphExec_t g : old) if (g) cudaGraphExecDestroy(g);
+    const size_t kv_bytes = (size_t)c.n_layers * c.context_length * p->kvd_l * 4;
+    for (float **cache : {&p->key_cache, &p->value_cache}) {
+        p->allocs.erase(std::find(p->allocs.begin(), p->allocs.end(), (void *)*cache));
+        cudaFree(*cache);
+        *cache = nullptr;
+        p->bytes -= (int64_t)kv_bytes;
+    }
+    p->bytes += b200_kv4_device_bytes(kv4);
+    p->decode_mode = B200_DECODE_GRAPH;
+    p->xp.rows = 0; // the exact prefill writes FP32 rows: chunks go token by token
+    p->xp.why = "the plan's cache holds 4 bits";
+    return B200_OK;
+}
+
+int b200_kv_info(b200_plan *p, int32_t *mode, int64_t *bytes) {
+    if (!p) return B200_ERR_BAD_ARG;
+    if (p->ly) return fail(p, B200_ERR_UNSUPPORTED, "layered plans keep their own caches");
+    if (mode) *mode = p->kv4 ? B200_KV_Q4 : B200_KV_F32;
+    if (bytes) *bytes = p->kv4 ? b200_kv4_device_bytes(p->kv4) : (int64_t)p->cfg.n_layers * p->cfg.context_length * p->kvd_l * 8;
+    return B200_OK;
+}
+
+int b200_score_tokens(b200_plan *p, const int32_t *tokens, int32_t n, int32_t start_pos, const int32_t *targets, int32_t top, float *logprobs, float *entropy, int32_t *top_ids,
+                      float *top_logprobs) {
+    if (!p || !tokens) return B200_ERR_BAD_ARG;
+    if (n <= 0) return B200_OK;
+    if (!p->g_decode) return fail(p, B200_ERR_STATE, "tensor-parallel plan: call b200_tp_attach on every rank first");
+    if (p->tp.n > 1) return fail(p, B200_ERR_UNSUPPORTED, "full logits are not gathered under tensor parallelism");
+    if (top < 0 || top > 32 || top > p->cfg.vocab_size) return fail(p, B200_ERR_BAD_ARG, "%d alternatives (0 .. 32, at most the vocabulary)", top);
+    if (start_pos < 0 || n > p->cfg.context_length - start_pos) return fail(p, B200_ERR_BAD_ARG, "positions %d..%lld outside the KV cache (%d)", start_pos, (long long)start_pos + n - 1, p->cfg.context_length);
+    for (int i = 0; i < n; i++)
+        if (tokens[i] < 0 || tokens[i] >= p->cfg.vocab_size) return fail(p, B200_ERR_BAD_ARG, "token %d out of range", tokens[i]);
+    CK(cudaSetDevice(p->device));
+    int rc;
+    if (!p->score_buf) {
+        if ((rc = dalloc(p, &p->score_buf, (size_t)p->seq_cap * 4 * (1 + 2 + 2 * 32)))) return rc;
+        p->score_rows = p->seq_cap;
+    }
+    // without targets of its own a token's is the one behind it; the last has none
+    for (int i = 0; i < n; i++) p->h_ids[i] = targets ? targets[i] : i + 1 < n ? tokens[i + 1] : -1;
+    CK(cudaMemcpyAsync(p->score_buf, p->h_ids, (size_t)n * 4, cudaMemcpyHostToDevice, p->stream));
+    CK(cudaStreamSynchronize(p->stream)); // (h_ids is used again)
+    if (p->ly) {
+        std::vector<int> every(n < p->ly->cap ? n : p->ly->cap);
+        for (size_t i = 0; i < every.size(); i++) every[i] = (int)i;
+        for (int at = 0; at < n; at += p->ly->cap) {
+            const int m = n - at < p->ly->cap ? n - at : p->ly->cap;
+            const LyScore score = {at, top};
+            if ((rc = ly_batch(p, tokens + at, m, start_pos + at, every.data(), m, nullptr, nullptr, &score))) return rc;
+        }
+    } else {
+        memcpy(p->h_ids, tokens, (size_t)n * 4);
+        CK(cudaMemcpyAsync(p->seq_tokens, p->h_ids, (size_t)n * 4, cudaMemcpyHostToDevice, p->stream));
+        if ((rc = set_state(p, tokens[0], start_pos, n, 0))) return rc;
+        for (int i = 0; i < n; i++) {
+            CK(cudaGraphLaunch(decode_graph(p, start_pos + i), p->stream));
+            if ((rc = score_rows(p, p->logits, 1, i, top))) return rc;
+        }
+    }
+    const float *f = reinterpret_cast<const float *>(p->score_buf + p->score_rows);
+    if (logprobs) CK(cudaMemcpyAsync(logprobs, f, (size_t)n * 4, cudaMemcpyDeviceToHost, p->stream));
+    if (entropy) CK(cudaMemcpyAsync(entropy, f + p->score_rows, (size_t)n * 4, cudaMemcpyDeviceToHost, p->stream));
+    if (top_ids && top) CK(cudaMemcpyAsync(top_ids, f + 2 * (size_t)p->score_rows, (size_t)n * top * 4, cudaMemcpyDeviceToHost, p->stream));
+    if (top_logprobs && top) CK(cudaMemcpyAsync(top_logprobs, f + (2 + 32) * (size_t)p->score_rows, (size_t)n * top * 4, cudaMemcpyDeviceToHost, p->stream));
+    CK(cudaStreamSynchronize(p->stream));
+    return check_device_error(p);
 }
 
 int b200_set_prefill_mode(b200_plan *p, int32_t mode) {
@@ -2069,6 +2256,11 @@ int b200_kv_reset(b200_plan *p) {
     if (!p) return B200_ERR_BAD_ARG;
     CK(cudaSetDevice(p->device));
     if (p->ly) return ly_kv_reset(p);
+    if (p->kv4) {
+        if (b200_kv4_reset(p->kv4, p->stream) != B200_OK) return fail(p, B200_ERR_CUDA, "%s", b200_kv4_last_error(p->kv4));
+        CK(cudaStreamSynchronize(p->stream));
+        return B200_OK;
+    }
     size_t kv_bytes = (size_t)p->cfg.n_layers * p->cfg.context_length * p->kvd_l * 4;
     CK(cudaMemsetAsync(p->key_cache, 0, kv_bytes, p->stream));
     CK(cudaMemsetAsync(p->value_cache, 0, kv_bytes, p->stream));
@@ -2095,6 +2287,7 @@ int b200_read_buffer(b200_plan *p, const char *name, int32_t layer, void *dst, s
     else if (s == "hs") { src = p->hs; sz = (size_t)(c.hidden_dim / 32) * 4; }
     else if (s == "key_cache" || s == "value_cache") {
         if (layer < 0 || layer >= c.n_layers) return fail(p, B200_ERR_BAD_ARG, "layer out of range");
+        if (p->kv4) return kv4_read_layer(p, layer, s == "key_cache", dst, bytes < ctx_kv * 4 ? bytes : ctx_kv * 4);
         src = (s == "key_cache" ? p->key_cache : p->value_cache) + (size_t)layer * ctx_kv;
         sz = ctx_kv * 4;
     } else return fail(p, B200_ERR_BAD_ARG, "unknown buffer %s", name);
@@ -2244,6 +2437,7 @@ int b200_tp_attach(b200_plan *p, const void *handles, int32_t n) {
 
 int b200_trace_decode(b200_plan *p, int32_t token, int32_t position, uint64_t *records, int32_t cap, int32_t *n_out) {
     if (!p || !records || !n_out) return B200_ERR_BAD_ARG;
+    if (p->kv4) return fail(p, B200_ERR_UNSUPPORTED, "steps over a 4-bit cache are not traced");
     if (!p->g_trace) return fail(p, B200_ERR_UNSUPPORTED, "tracing needs a streaming path (Q8_0 tiles or the FP16 rings)");
     int rc;
     if ((rc = check_pos(p, token, position))) return rc;
@@ -2463,6 +2657,7 @@ void b200_plan_free(b200_plan *p) {
     cudaSetDevice(p->device);
     if (p->stream) cudaStreamSynchronize(p->stream);
     ly_free(p);
+    b200_kv4_free(p->kv4);
     prefill_free(p->prefill);
     if (p->g_decode) cudaGraphExecDestroy(p->g_decode);
     if (p->g_prefill) cudaGraphExecDestroy(p->g_prefill);

@@ -13,6 +13,7 @@ the oracle in the tests.
 """
 from __future__ import annotations
 
+import math
 from typing import Callable, Iterable
 
 Forward = Callable[[int, int], int]
@@ -124,3 +125,11 @@ def generate_tokens_layered(plan, prompt_tokens: list[int], stop_tokens: Iterabl
         current = nxt
         pos += 1
     return generated
+
+
+def perplexity(plan, tokens: list[int], start_position: int = 0) -> float:
+    """exp of the mean negative log probability of every token but the first, each given the ones in front of it (``plan.score_tokens``)."""
+    if len(tokens) < 2:
+        raise ValueError("a perplexity takes two tokens at least")
+    logprobs = plan.score_tokens(tokens, start_position)[0]
+    return math.exp(-sum(float(x) for x in logprobs[:-1]) / (len(tokens) - 1))

@@ -92,7 +92,7 @@ class LogProbs(C.Structure):
                [(n, C.c_void_p) for n in ("targets", "logprobs", "entropy", "top_ids", "top_logprobs")]
 
 
-EXPORTS = ["b200_kv4_create", "b200_kv4_free", "b200_kv4_reset", "b200_kv4_device_bytes", "b200_kv4_last_error", "b200_kv4_append", "b200_kv4_attention", "b200_kv4_attention_workspace", "b200_kv4_read", "b200_log_probs",
+EXPORTS = ["b200_set_kv_mode", "b200_kv_info", "b200_score_tokens", "b200_kv4_create", "b200_kv4_free", "b200_kv4_reset", "b200_kv4_device_bytes", "b200_kv4_last_error", "b200_kv4_append", "b200_kv4_attention", "b200_kv4_attention_workspace", "b200_kv4_read", "b200_log_probs",
            "b200_plan_create_layered", "b200_forward_batch_logits", "b200_layered_info", "b200_plan_create", "b200_forward_decode", "b200_forward_prefill", "b200_forward_batch_prefill", "b200_set_prefill_mode", "b200_prefill_info", "b200_exact_prefill_info",
            "b200_set_decode_mode", "b200_decode_info", "b200_trace_persistent", "b200_test_seqsum2", "b200_test_exact_prefill_wait", "b200_test_exact_prefill_wait_form", "b200_forward_decode_sample", "b200_upload_info", "b200_requant_kquant",
            "b200_decode_sequence", "b200_time_kernel", "b200_tp_handle", "b200_tp_attach", "b200_trace_decode", "b200_profile_norm", "b200_test_seqsum", "b200_gemm_f16", "b200_kv_reset", "b200_read_buffer", "b200_launches_per_decode",
@@ -146,6 +146,9 @@ def lib() -> C.CDLL:
     L.b200_last_error.argtypes = [vp]
     L.b200_last_error.restype = C.c_char_p
     L.b200_version.restype = C.c_char_p
+    L.b200_set_kv_mode.argtypes = [vp, i32]
+    L.b200_kv_info.argtypes = [vp, C.POINTER(i32), C.POINTER(C.c_int64)]
+    L.b200_score_tokens.argtypes = [vp, vp, i32, i32, vp, i32, vp, vp, vp, vp]
     L.b200_kv4_create.argtypes = [i32, i32, i32, i32, i32, C.POINTER(vp), C.c_char_p, C.c_size_t]
     L.b200_kv4_free.argtypes, L.b200_kv4_free.restype = [vp], None
     L.b200_kv4_reset.argtypes = [vp, vp]
@@ -333,6 +336,26 @@ class NativePlan:
         ms = C.c_float(0)
         self._ck(lib().b200_decode_sequence(self._p, t.ctypes.data, n, start_pos, 1 if feedback else 0, out.ctypes.data, C.byref(ms)))
         return out, ms.value
+
+    def set_kv_mode(self, mode: int):
+        self._ck(lib().b200_set_kv_mode(self._p, mode))
+
+    def kv_info(self):
+        mode, nbytes = C.c_int32(0), C.c_int64(0)
+        self._ck(lib().b200_kv_info(self._p, C.byref(mode), C.byref(nbytes)))
+        return mode.value, nbytes.value
+
+    def score_tokens(self, tokens, start_pos: int, targets=None, top: int = 0):
+        t = np.ascontiguousarray(tokens, dtype=np.int32)
+        g = None if targets is None else np.ascontiguousarray(targets, dtype=np.int32)
+        if g is not None and g.shape != t.shape:
+            raise ValueError(f"{len(g)} targets for {len(t)} tokens")
+        if not 0 <= top <= 32:
+            raise ValueError(f"{top} alternatives (0 .. 32)")
+        n = len(t)
+        lp, h, ids, values = np.empty(n, np.float32), np.empty(n, np.float32), np.empty((n, top), np.int32), np.empty((n, top), np.float32)
+        self._ck(lib().b200_score_tokens(self._p, t.ctypes.data, n, start_pos, None if g is None else g.ctypes.data, top, lp.ctypes.data, h.ctypes.data, ids.ctypes.data, values.ctypes.data))
+        return lp, h, ids, values
 
     def time_kernel(self, which: int, reps: int = 3):
         ms, nbytes = C.c_float(0), C.c_int64(0)

@@ -203,6 +203,25 @@ class B200MasterPlan:
         """(longest chunk that the exact prefill multiplies at once, 0: token by token; chunks so multiplied so far; why none are)."""
         return self._native.exact_prefill_info()
 
+    KV_F32, KV_Q4 = 0, 1
+
+    def set_kv_mode(self, mode):
+        """"f32" (what a plan is created with) or "q4": keys and values in 4 bits with a scale for 32 entries, a seventh of the memory.  The switch empties the cache and holds for
+        the rest of the plan's life; single-GPU GGUF plans."""
+        if isinstance(mode, str):
+            mode = {"f32": 0, "q4": 1}[mode]
+        self._native.set_kv_mode(int(mode))
+
+    def kv_info(self):
+        """(active cache mode, bytes of the cache)."""
+        return self._native.kv_info()
+
+    def score_tokens(self, tokens, start_pos: int = 0, targets=None, top: int = 0):
+        """Runs ``tokens`` at positions ``start_pos``.. and returns, for each, the log probability of its target in the distribution that follows it (``targets``; without them the
+        next token, 0 for the last), that distribution's entropy in nats and the ``top`` (at most 32) most likely tokens with their log probabilities: arrays (logprobs [n],
+        entropy [n], top_ids [n, top], top_logprobs [n, top]).  No logits leave the GPU."""
+        return self._native.score_tokens(tokens, start_pos, targets, top)
+
     # -Dllama.cudaGraphs-style switch of the decode implementation (both bit-identical): "graph" = one CUDA graph of
     # 5 to 7 kernels per layer, "persistent" = one persistent kernel per token (csrc/decode_persistent.cuh)
     DECODE_GRAPH, DECODE_PERSISTENT = 0, 1

@@ -360,6 +360,24 @@ int b200_forward_batch_prefill(b200_plan *plan, const int32_t *tokens, int32_t n
 #define B200_PREFILL_TENSOR_CORE 1
 int b200_set_prefill_mode(b200_plan *plan, int32_t mode);
 
+/* What a GGUF plan keeps its keys and values in.  B200_KV_F32 (what a plan is created with): FP32, as the CPU path.  B200_KV_Q4: groups of 32 entries of a head in 4 bits with an FP16
+ * scale (b200_kv4_*: 4.5 bits an entry, a seventh of the memory); decode and prefill write and read that cache, so their results are no longer those of the CPU path bit for bit.  The
+ * switch empties the cache, gives the FP32 one's memory back and holds for the rest of the plan's life; the decode graph is the only decode mode from then on, and a chunk that is not
+ * prefilled on the tensor cores goes token by token.  Single-GPU GGUF plans only (B200_ERR_UNSUPPORTED, with the reason in b200_last_error; the plan is then as it was). */
+#define B200_KV_F32 0
+#define B200_KV_Q4 1
+int b200_set_kv_mode(b200_plan *plan, int32_t mode);
+
+/* Active cache mode and the cache's bytes (any pointer may be NULL). */
+int b200_kv_info(b200_plan *plan, int32_t *mode, int64_t *bytes);
+
+/* Scores a text: runs the n tokens at positions start_pos.. (GGUF plans: single-token steps; layered plans: prefill chunks) and returns for each the log probability of its target in the
+ * distribution that follows it, that distribution's entropy in nats and its `top` (0 .. 32) most likely tokens with their log probabilities (b200_log_probs, on the device: no logits
+ * row crosses PCIe).  targets == NULL: a token's target is the next one of the text, the last one has none (0).  logprobs and entropy [n], top_ids and top_logprobs [n][top]: host,
+ * each may be NULL.  Single-GPU plans only. */
+int b200_score_tokens(b200_plan *plan, const int32_t *tokens, int32_t n, int32_t start_pos, const int32_t *targets, int32_t top, float *logprobs, float *entropy, int32_t *top_ids,
+                      float *top_logprobs);
+
 /* Active mode, kernels launched and device milliseconds of the last tensor-core chunk (any pointer may be NULL). */
 int b200_prefill_info(b200_plan *plan, int32_t *mode, int32_t *launches, float *device_ms);
 
