@@ -108,7 +108,7 @@ def _ops_command() -> list[str]:
     # torch's own libstdc++ (the shared one), also where the compiler would link a static copy into a shared object: two of them do not share their streams' tables
     inc = [f"-I{d}" for d in [*cpp_extension.include_paths(), "/usr/local/cuda/include", sysconfig.get_paths()["include"]]]
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-w", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", *inc, "-o", OPS_LIB, OPS_SRC,
-            f"-L{CSRC}", "-l:libb200llama.so", f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-nostdlib++", "-l:libstdc++.so.6", "-lm", "-Wl,-rpath,$ORIGIN",
+            f"-L{CSRC}", "-l:libb200llama.so", f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", "-nostdlib++", "-l:libstdc++.so.6", "-lm", "-Wl,-rpath,$ORIGIN",
             f"-Wl,-rpath,{lib}"]
 
 

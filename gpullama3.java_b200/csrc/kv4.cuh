@@ -139,7 +139,7 @@ template <int HS, typename T> __global__ void __launch_bounds__(256) k_append(co
             for (int o = WIDTH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         }
         if (norm && mine) {
-            const float s = (float)(1.0 / sqrt(ss / HS + (double)a.eps));
+            const float s = (float)rsqrt(ss * (1.0 / HS) + (double)a.eps);
 #pragma unroll
             for (int i = 0; i < 8; i++) x[i] = norm[li * 8 + i] * (s * x[i]);
         }
@@ -180,6 +180,7 @@ template <int HS, typename T> __global__ void __launch_bounds__(256) k_append(co
                 for (int i = 0; i < 8; i++) o[i] = x[i];
         }
     }
+    if (!__any_sync(0xffffffffu, mine && !is_q)) return; // (two thirds of the warps of a grouped model hold queries alone)
     __half scale;
     int c[8];
     quantize8(x, 0xffffffffu, scale, c);

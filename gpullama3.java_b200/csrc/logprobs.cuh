@@ -18,7 +18,7 @@ namespace cg = cooperative_groups;
 using bf16 = __nv_bfloat16;
 typedef unsigned long long u64;
 
-constexpr int THREADS = 256, PER_THREAD = 16, BATCH = THREADS * PER_THREAD, MAX_TOP = 32, MAX_CLUSTER = 16;
+constexpr int THREADS = 256, PER_THREAD = 16, BATCH = THREADS * PER_THREAD, MAX_TOP = 32, MAX_CLUSTER = 8; // (clusters of 16 start late: 37 rows took 21 us with them, 12 with 8)
 constexpr int PUSHERS = 64;                                // threads that may add candidates in a batch: more of them raise the threshold first
 constexpr int MANY = 96;                                   // candidates from which the best of them are chosen, so that the threshold rises
 constexpr int BUFFER = MANY + PUSHERS * PER_THREAD;
@@ -101,7 +101,8 @@ template <> struct Load<bf16> {
 
 struct Smem {
     u64 buffer[BUFFER], best[MAX_TOP]; // candidates; the CTA's alternatives in order
-    Sum warps[THREADS / 32], cta;
+    Sum warps[THREADS / 32], cta, parts[MAX_CLUSTER];
+    int counts[MAX_CLUSTER];
     u64 merged[MAX_TOP];
     int pushed, n_best;
 };
@@ -111,6 +112,7 @@ __device__ __forceinline__ void select(Smem &sm, int total, int n) {
     for (int i = threadIdx.x; i < total; i += THREADS) {
         const u64 k = sm.buffer[i];
         int place = 0;
+#pragma unroll 8
         for (int j = 0; j < total; j++) place += sm.buffer[j] > k;
         if (place < n) sm.best[place] = k;
     }
@@ -124,31 +126,42 @@ __device__ __forceinline__ void select(Smem &sm, int total, int n) {
 // A cluster of CTAs reads a row, each a stretch of it in batches of 16 entries a thread, the next batch under way while one is worked on.  A warp keeps the largest entry it has met and
 // a thread the sum of its own entries in units of that; candidates for the alternatives are the entries above a threshold that at least `top` known ones reach, so that after the first
 // batch hardly any is looked at twice.  Bytes bound it: 512 rows of 128256 FP32 logits are 263 MB, 41 us.
-template <typename T> __global__ void __launch_bounds__(THREADS, 3) k_log_probs(const Args a) {
+template <typename T> __global__ void __launch_bounds__(THREADS, 4) k_log_probs(const Args a) {
     constexpr int VEC = Load<T>::VEC;
     __shared__ Smem sm;
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ranks, tid = threadIdx.x, lane = tid & 31;
     const T *x = (const T *)a.logits + row * a.ld;
     const int skew = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)); // entries between the 16-byte boundary in front of the row and its start
-    const long long span = (long long)skew + a.vocab;
+    const int span = skew + a.vocab; // (vocabularies of up to 2^30)
     // stretches of whole vectors, as even as that allows
-    const long long vecs = (span + VEC - 1) / VEC, begin = vecs * rank / ranks * VEC, end = vecs * (rank + 1) / ranks * VEC;
+    const int vecs = (span + VEC - 1) / VEC, begin = (int)((long long)vecs * rank / ranks) * VEC, end = (int)((long long)vecs * (rank + 1) / ranks) * VEC;
     if (tid == 0) { sm.pushed = 0; sm.n_best = 0; }
     float m = -CUDART_INF_F, z = 0.0f, s = 0.0f; // the warp's largest; this thread's sums, without it
-    u64 bar = 0; // keys that are not larger are no candidates
-    float bar_value = -CUDART_INF_F;
-    const auto fetch = [&](long long base, float (&v)[PER_THREAD]) {
-#pragma unroll
-        for (int i = 0; i < PER_THREAD / VEC; i++) {
-            const long long at = base + ((long long)i * THREADS + tid) * VEC - skew; // index in the row
-            if (at >= 0 && at + VEC <= a.vocab && at + skew < end) Load<T>::vec(x + at, v + i * VEC);
-            else
-#pragma unroll
-                for (int j = 0; j < VEC; j++) v[i * VEC + j] = at + j >= 0 && at + j < a.vocab && at + skew < end ? Load<T>::one(x + at + j) : -CUDART_INF_F;
+    bool open = true;                // no bar yet: every entry is a candidate
+    float bar_value = -CUDART_INF_F; // entries that are not larger are none
+    const auto room = [&](float &value) { // in front of a batch's candidates, the same for every thread (a barrier follows the last ones): room for them, and a higher bar
+        if (sm.pushed <= MANY) return;
+        __syncthreads();
+        select(sm, sm.pushed, a.top);
+        if (sm.n_best == a.top) {
+            open = false;
+            value = fmaxf(value, value_of(sm.buffer[a.top - 1]));
         }
     };
-    const auto take = [&](long long base, const float (&v)[PER_THREAD]) {
+    const auto fetch = [&](int base, float (&v)[PER_THREAD]) {
+        const int from = base + tid * VEC - skew; // index in the row
+        if (base >= skew && base + BATCH <= end && base + BATCH <= span) {
+#pragma unroll
+            for (int i = 0; i < PER_THREAD / VEC; i++) Load<T>::vec(x + from + i * (THREADS * VEC), v + i * VEC);
+        } else
+#pragma unroll
+            for (int i = 0; i < PER_THREAD; i++) {
+                const int at = from + i / VEC * (THREADS * VEC) + i % VEC;
+                v[i] = at >= 0 && at < a.vocab && at + skew < end ? Load<T>::one(x + at) : -CUDART_INF_F;
+            }
+    };
+    const auto take = [&](int base, const float (&v)[PER_THREAD]) {
         float top = v[0];
 #pragma unroll
         for (int i = 1; i < PER_THREAD; i++) top = fmaxf(top, v[i]);
@@ -188,20 +201,37 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 3) k_log_probs(
         z += zs[0] + zs[1];
         s += ss[0] + ss[1];
         if (a.top == 0) return;
-        u64 largest = 0;
-        if (top >= bar_value)
+        const auto index = [&](int i) { return base + i / VEC * (THREADS * VEC) + tid * VEC + i % VEC - skew; };
+        if (!open) { // `top` entries of earlier batches reach the bar: equal ones, whose index is larger, do not beat them
+            const bool over = top > bar_value;
+            const int n = __syncthreads_count(over);
+            if (n == 0) return;
+            if (n <= PUSHERS) {
+                room(bar_value);
+                __syncthreads();
+                if (over)
 #pragma unroll
-            for (int i = 0; i < PER_THREAD; i++) {
-                const long long at = base + ((long long)(i / VEC) * THREADS + tid) * VEC + i % VEC;
-                const u64 k = key_of(v[i], (unsigned)(at - skew));
-                if (at >= skew && at < span && at < end && v[i] == v[i] && k > largest) largest = k;
+                    for (int i = 0; i < PER_THREAD; i++)
+                        if (v[i] > bar_value) sm.buffer[atomicAdd(&sm.pushed, 1)] = key_of(v[i], (unsigned)index(i));
+                return;
             }
-        const bool over = largest > bar;
+        }
+        // the first batch, and one that brings many: a bar that at least `top` and at most PUSHERS threads reach
+        u64 largest = 0;
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; i++) {
+            const int at = index(i);
+            if (at >= 0 && at < a.vocab && at + skew < end && v[i] == v[i]) {
+                const u64 k = key_of(v[i], (unsigned)at);
+                if (k > largest) largest = k;
+            }
+        }
+        const bool over = open ? largest > 0 : top > bar_value;
         const int n = __syncthreads_count(over);
-        if (n == 0) return;
-        u64 least = bar + 1;
-        if (n > PUSHERS) { // at least `top` and at most PUSHERS threads hold a key from here on: half the interval at a time (the keys are no two alike, so such a bar exists)
-            u64 low = bar, high = ~0ull;
+        u64 least = 1;
+        float next = bar_value;
+        if (n > PUSHERS) { // half the interval at a time; the keys are no two alike, so such a bar exists
+            u64 low = 0, high = ~0ull;
             for (;;) {
                 least = low + (high - low) / 2;
                 const int above = __syncthreads_count(over && largest >= least);
@@ -209,32 +239,29 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 3) k_log_probs(
                 else if (above < a.top) high = least;
                 else break;
             }
-            bar = least - 1; // `top` candidates reach it
-            bar_value = value_of(least);
+            next = value_of(least);
+            open = false;
         }
-        if (sm.pushed > MANY) { // (the same for every thread: the barrier above follows the last push)
-            __syncthreads();
-            select(sm, sm.pushed, a.top);
-            if (sm.n_best == a.top && sm.buffer[a.top - 1] > bar) { bar = sm.buffer[a.top - 1]; bar_value = value_of(bar); }
-        }
+        room(next);
         __syncthreads();
         if (over && largest >= least)
 #pragma unroll
             for (int i = 0; i < PER_THREAD; i++) {
-                const long long at = base + ((long long)(i / VEC) * THREADS + tid) * VEC + i % VEC;
-                const u64 k = key_of(v[i], (unsigned)(at - skew));
-                if (at >= skew && at < span && at < end && v[i] == v[i] && k >= least) sm.buffer[atomicAdd(&sm.pushed, 1)] = k;
+                const int at = index(i);
+                const u64 k = key_of(v[i], (unsigned)at);
+                if (at >= 0 && at < a.vocab && at + skew < end && v[i] == v[i] && k >= least) sm.buffer[atomicAdd(&sm.pushed, 1)] = k;
             }
+        bar_value = fmaxf(bar_value, next);
     };
-    float v0[PER_THREAD], v1[PER_THREAD];
-    if (begin < end) fetch(begin, v0);
+    float now[PER_THREAD], next[PER_THREAD];
+    if (begin < end) fetch(begin, next);
     __syncthreads();
-    for (long long base = begin; base < end; base += 2 * BATCH) {
-        if (base + BATCH < end) fetch(base + BATCH, v1);
-        take(base, v0);
-        if (base + BATCH >= end) break;
-        if (base + 2 * BATCH < end) fetch(base + 2 * BATCH, v0);
-        take(base + BATCH, v1);
+#pragma unroll 1
+    for (int base = begin; base < end; base += BATCH) {
+#pragma unroll
+        for (int i = 0; i < PER_THREAD; i++) now[i] = next[i];
+        if (base + BATCH < end) fetch(base + BATCH, next);
+        take(base, now);
     }
     // ---- join: threads, then CTAs -------------------------------------------------------------------------------------------------------------------------------
 #pragma unroll
@@ -252,8 +279,16 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 3) k_log_probs(
     }
     if (ranks > 1) cluster.sync(); else __syncthreads();
     if (rank == 0) {
-        Sum all = sm.cta;
-        for (int r = 1; r < ranks; r++) all = join(all, *cluster.map_shared_rank(&sm.cta, r));
+        if (tid < ranks) { // (a CTA a thread: one after the other, each is a trip to another SM)
+            sm.parts[tid] = *cluster.map_shared_rank(&sm.cta, tid);
+            sm.counts[tid] = *cluster.map_shared_rank(&sm.n_best, tid);
+        }
+        u64 mine = 0;
+        static_assert(THREADS >= MAX_CLUSTER * MAX_TOP, "a key a thread");
+        if (a.top && tid < ranks * MAX_TOP) mine = *cluster.map_shared_rank(&sm.best[tid % MAX_TOP], tid / MAX_TOP);
+        __syncthreads();
+        Sum all = sm.parts[0];
+        for (int r = 1; r < ranks; r++) all = join(all, sm.parts[r]);
         const float log_z = all.m < CUDART_INF_F ? log1pf(all.z) : CUDART_NAN_F; // (an infinite logit, or none that is not -inf)
         const float inv = 1.0f / (1.0f + all.z);
         const bool none = !(all.m > -CUDART_INF_F);
@@ -265,24 +300,24 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 3) k_log_probs(
             if (a.entropy) a.entropy[row] = none ? CUDART_NAN_F : log_z - all.s * LN2 * inv;
         }
         if (a.top) {
-            for (int i = tid; i < ranks * MAX_TOP; i += THREADS) {
-                const int r = i / MAX_TOP, j = i % MAX_TOP;
-                if (j >= *cluster.map_shared_rank(&sm.n_best, r)) continue;
-                const u64 k = *cluster.map_shared_rank(&sm.best[j], r);
+            u64 *all_keys = sm.buffer; // every CTA's alternatives, in order: [rank][MAX_TOP]; 0 behind the last
+            static_assert(BUFFER >= MAX_CLUSTER * MAX_TOP, "the lists of all CTAs");
+            if (tid < ranks * MAX_TOP) all_keys[tid] = mine = tid % MAX_TOP < sm.counts[tid / MAX_TOP] ? mine : 0;
+            __syncthreads();
+            if (mine) {
                 int place = 0;
-                for (int q = 0; q < ranks; q++) { // every CTA's keys are in order: half of them at a time
-                    const u64 *best = cluster.map_shared_rank(sm.best, q);
-                    int low = 0, high = *cluster.map_shared_rank(&sm.n_best, q);
-                    while (low < high) {
-                        const int mid = (low + high) / 2;
-                        if (best[mid] > k) low = mid + 1; else high = mid;
-                    }
-                    place += low;
+                for (int q = 0; q < ranks; q++) { // half of a list at a time
+                    const u64 *best = all_keys + q * MAX_TOP;
+                    int low = 0;
+#pragma unroll
+                    for (int step = MAX_TOP / 2; step > 0; step /= 2)
+                        if (best[low + step - 1] > mine) low += step;
+                    place += low + (best[low] > mine);
                 }
-                if (place < a.top) sm.merged[place] = k;
+                if (place < a.top) sm.merged[place] = mine;
             }
             int have = 0;
-            for (int r = 0; r < ranks; r++) have += *cluster.map_shared_rank(&sm.n_best, r);
+            for (int r = 0; r < ranks; r++) have += sm.counts[r];
             __syncthreads();
             if (tid < a.top) { // fewer than `top` numbers in the row: -1
                 const bool is = tid < have;

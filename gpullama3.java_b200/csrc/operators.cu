@@ -395,6 +395,7 @@ int b200_kv4_read(b200_kv4 *kv, const b200_kv4_read_args *a, void *stream) {
 int b200_log_probs(const b200_log_probs_args *a, void *stream, char *err, size_t err_len) {
     if (!a) return say(err, err_len, B200_ERR_BAD_ARG, "null arguments");
     if (a->rows < 0 || a->vocab <= 0) return say(err, err_len, B200_ERR_BAD_ARG, "%d rows of %d logits", a->rows, a->vocab);
+    if (a->vocab > (1 << 30)) return say(err, err_len, B200_ERR_UNSUPPORTED, "%d logits a row (at most 2^30)", a->vocab);
     if (a->top < 0 || a->top > lp::MAX_TOP || a->top > a->vocab) return say(err, err_len, B200_ERR_BAD_ARG, "%d alternatives of %d logits (at most %d)", a->top, a->vocab, lp::MAX_TOP);
     if (!known_type(a->type)) return say(err, err_len, B200_ERR_UNSUPPORTED, "logits of type %d (FP32, FP16 and BF16 are known)", a->type);
     if (a->rows == 0) return B200_OK;

@@ -1,6 +1,7 @@
 // torch_ops.cpp -- the operators of operators.cu on torch tensors (operators.py has their documentation): checks of the tensors, the current stream, results from torch's allocator.
 // A call through Python's ctypes costs 15 to 20 us of host time, more than most of these kernels run; here it is about 5.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -39,6 +40,11 @@ int type_of(at::ScalarType t, const char *what) {
     return -1;
 }
 
+// A new tensor on a device, without the dispatcher (1 us of at::empty's 2).
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, int device) {
+    return at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), std::nullopt);
+}
+
 struct Cache {
     b200_kv4 *kv;
     int64_t slots, context, kv_heads, head_size;
@@ -48,7 +54,6 @@ struct Cache {
     Cache(const Cache &) = delete;
     Cache &operator=(const Cache &) = delete;
     ~Cache() { free(); }
-    at::Device dev() const { return at::Device(at::kCUDA, (c10::DeviceIndex)device); }
     void alive() const {
         if (!kv) refused(B200_ERR_STATE, "the cache has been freed");
     }
@@ -107,7 +112,7 @@ struct Cache {
             a.heads = rows_of(q->size(1));
             a.q_stride = rows(*q, "q", n, a.heads);
             a.q = q->data_ptr();
-            if (!out) out = at::empty({n, a.heads, head_size}, q->options().dtype(at::kFloat));
+            if (!out) out = fresh({n, a.heads, head_size}, at::kFloat, device);
             NEED(out->scalar_type() == at::kFloat, "q_out is FP32");
             a.q_out_stride = rows(*out, "q_out", n, a.heads);
             a.q_out = out->data_ptr<float>();
@@ -138,7 +143,7 @@ struct Cache {
         a.q_stride = rows(q, "q", n, a.heads);
         a.positions = indices(positions, "positions", n);
         a.slots = indices(slot, "slots", n);
-        const Tensor out = given ? *given : at::empty({n, a.heads, head_size}, q.options().dtype(dtype));
+        const Tensor out = given ? *given : fresh({n, a.heads, head_size}, dtype, device);
         a.out_stride = rows(out, "out", n, a.heads);
         a.q = q.data_ptr<float>();
         a.out = out.data_ptr();
@@ -146,7 +151,7 @@ struct Cache {
         if (n == 0) return out;
         Tensor work; // from the stream's own pool: calls on other streams, and captured graphs, have theirs
         if ((a.workspace_bytes = b200_kv4_attention_workspace(kv, &a)) > 0) {
-            work = at::empty({(int64_t)(a.workspace_bytes / 4)}, q.options());
+            work = fresh({(int64_t)(a.workspace_bytes / 4)}, at::kFloat, device);
             a.workspace = work.data_ptr<float>();
         }
         check(b200_kv4_attention(kv, &a, stream()));
@@ -162,8 +167,7 @@ struct Cache {
         a.n = rows_of(n);
         a.positions = indices(positions, "positions", n);
         a.slots = indices(slot, "slots", n);
-        const auto options = at::TensorOptions().dtype(dtype).device(dev());
-        Tensor k = at::empty({n, kv_heads, head_size}, options), v = at::empty({n, kv_heads, head_size}, options);
+        Tensor k = fresh({n, kv_heads, head_size}, dtype, device), v = fresh({n, kv_heads, head_size}, dtype, device);
         a.k = k.data_ptr();
         a.v = v.data_ptr();
         if (n) check(b200_kv4_read(kv, &a, stream()));
@@ -205,8 +209,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> log_probs(const Tensor &logits, const
         NEED(targets->is_cuda() && targets->get_device() == a.device && (rows <= 1 || targets->stride(0) == 1), "targets are contiguous and on ", logits.device());
         a.targets = targets->data_ptr<int32_t>();
     }
-    const auto f32 = at::TensorOptions().dtype(at::kFloat).device(logits.device());
-    Tensor lp = at::empty({rows}, f32), entropy = at::empty({rows}, f32), ids = at::empty({rows, top}, f32.dtype(at::kInt)), values = at::empty({rows, top}, f32);
+    Tensor lp = fresh({rows}, at::kFloat, a.device), entropy = fresh({rows}, at::kFloat, a.device), ids = fresh({rows, top}, at::kInt, a.device), values = fresh({rows, top}, at::kFloat, a.device);
     if (rows) {
         a.logits = logits.data_ptr();
         a.row_stride = rows > 1 ? logits.stride(0) : vocab;
