@@ -1,16 +1,20 @@
 // kv4_chunk.cuh -- attention of prompt chunks over the 4-bit cache on the 5th-generation tensor cores, with 16-bit results.
 //
 // A CTA takes 128 rows (tokens x query heads of one key/value head) and runs through the positions that any of them sees, 128 at a time:
-//   warps 8-23  turn a tile's records (half a record a warp) into FP16 operands in shared memory: keys [position][entry], values transposed [entry][position], both K-major
-//   one thread  issues S = Q K^T (two accumulators in TMEM, so that a tile's product runs while the rows work on the one before) and O += P V, with P read from TMEM
-//   warps 0-7   half a row a thread: exponentials, P as FP16 into TMEM; O is scaled where a row's maximum has grown by too much, which is rare
-// Per tile of heads of 128: 1024 cycles of products (8192 FLOP a cycle), 1024 of exponentials (16 a cycle), about 1200 issue slots a scheduler: all three side by side.  What they
-// wait for is latency: with 4 and 8 warps in place of 8 and 16 a tile took 3000 cycles, 2000 of them in a row's exponentials and as many in a record's conversion.
+//   warps 16-23  turn a tile's records (one a warp) into FP16 operands in shared memory: keys [position][entry], values transposed [entry][position], both K-major
+//   warp 24      issues S = Q K^T and O += P V, with P read from TMEM
+//   warps 0-15   exponentials, two threads a row; P as FP16 takes the place of S; O is scaled where a row's maximum has grown by too much, which is rare
+// A tile's work is a chain: scores, exponentials, product, about 5000 cycles of which 1024 are the tensor cores' and 1024 the exponentials' (16 a cycle).  So even and odd tiles are two
+// streams with accumulators, maxima and sums of their own, each of eight warps, which the end joins: while one waits for its products the other computes.  Heads of 128, two streams of
+// scores and results: all 512 columns of TMEM.
+// Measured (512 tokens, 32 heads over 8 of 128, 8192 positions: 66.6 GFLOP): 107 us, 620 TFLOP/s, 37 % of the 1690 measured.  What bounds it is that chain and the issue slots it shares with
+// the conversion.  One stream with two S and a maximum agreed on by a row's threads in every tile took 116-123 us; 256 rows a CTA with half the conversions 133 us (two blocks of rows in
+// place of the two streams; 64 pairs of CTAs whose parts had to be joined).
 // Rounding: queries (times a power of two), keys, values and probabilities are FP16 operands, sums are FP32.  A value's NaN, or one outside FP16, is moved into its key, so that it
 // reaches the rows that see the position and no other (0 * NaN in the product would reach them all).
 //
 // Rows of a tile may belong to several slots and stand in any order: a run of tokens of one slot is a segment, the tiles of all segments are one list, and a row masks what is not its own.
-// Every wait is bounded: after two seconds the CTA gives up, writes the cache's error word, waits for its products under way and frees its tensor memory.
+// Every wait is bounded: after 2^25 tries the CTA gives up, writes the cache's error word, waits for its products under way and frees its tensor memory.
 #pragma once
 #include <type_traits>
 
@@ -18,57 +22,63 @@
 
 namespace kv4 {
 
-constexpr int CHUNK_ROWS = 128, CHUNK_KEYS = 128, CHUNK_RECORDS = CHUNK_KEYS / BLOCK;
-constexpr int CHUNK_SOFTMAX = 8, CHUNK_DEQUANT = 16, CHUNK_ISSUER = CHUNK_SOFTMAX + CHUNK_DEQUANT, CHUNK_THREADS = (CHUNK_ISSUER + 1) * 32; // warps of each kind
-__host__ __device__ constexpr int chunk_q_bytes(int hs) { return groups(hs) * CHUNK_ROWS * 64; }
-__host__ __device__ constexpr int chunk_stage_bytes(int hs) { return groups(hs) * CHUNK_KEYS * 64 + hs * CHUNK_KEYS * 2; }
+constexpr int CHUNK_ROWS = 128, CHUNK_KEYS = 128, CHUNK_K_STAGES = 3, CHUNK_V_STAGES = 2, CHUNK_RECORDS = CHUNK_KEYS / BLOCK;
+constexpr int CHUNK_SOFTMAX = 16, CHUNK_DEQUANT = CHUNK_RECORDS, CHUNK_ISSUER = CHUNK_SOFTMAX + CHUNK_DEQUANT, CHUNK_THREADS = (CHUNK_ISSUER + 1) * 32; // warps of each kind
+__host__ __device__ constexpr int chunk_tile_bytes(int hs) { return hs * CHUNK_KEYS * 2; } // of queries, keys or values
 
 struct Segment { // a run of tokens of one slot and the records that any of them sees
     int slot, begin, end, tiles; // records [begin, end); tiles of all segments up to and with this one
 };
 struct ChunkSmem { // behind the operands
-    unsigned long long k_full[2], v_full[2], free[2], s_full[2], s_empty[2], p_full[2], pair[4], drained;
-    unsigned tmem, bail;
+    unsigned long long k_full[CHUNK_K_STAGES], k_free[CHUNK_K_STAGES], v_full[CHUNK_V_STAGES], v_free[CHUNK_V_STAGES];
+    unsigned long long s_full[2], p_full[2], drained; // by stream
+    unsigned long long pair[CHUNK_SOFTMAX / 2];       // the two warps that share a stream's rows
+    unsigned tmem, bail, again[2], repeat[2];         // again: a row's maximum has to move; repeat: these are the scores of the tile before once more
     int n_segments, single;
     int slot[CHUNK_ROWS], pos[CHUNK_ROWS], segment[CHUNK_ROWS]; // by token
     float factor[CHUNK_ROWS];                                   // by row: what turns a product into a score in units of log2
-    float half_row[2][CHUNK_ROWS];                              // what the two threads of a row tell each other
-    int again[2][CHUNK_SOFTMAX];                                // by tile and warp: a row's maximum has to move
+    float half_row[2][2][CHUNK_ROWS];                           // by stream: what the two threads of a row tell each other, their sums at the end
+    float top[2][CHUNK_ROWS];
     Segment segments[CHUNK_ROWS];
 };
-__host__ __device__ constexpr size_t chunk_smem_bytes(int hs) { return 1024 + chunk_q_bytes(hs) + 2 * chunk_stage_bytes(hs) + sizeof(ChunkSmem); }
+__host__ __device__ constexpr size_t chunk_smem_bytes(int hs) { return 1024 + (1 + CHUNK_K_STAGES + CHUNK_V_STAGES) * chunk_tile_bytes(hs) + sizeof(ChunkSmem); }
 
 __device__ __forceinline__ uint32_t s32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void bar_init(const void *bar, unsigned n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s32(bar)), "r"(n)); }
 __device__ __forceinline__ void bar_arrive(const void *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(bar)) : "memory"); }
-__device__ __forceinline__ bool bar_wait(const void *bar, unsigned parity, unsigned *bail) { // false: given up
+constexpr unsigned WAIT_TRIES = 1u << 25; // a second or more
+__device__ __forceinline__ bool bar_passed(uint32_t bar, unsigned parity) {
+    unsigned done;
+    asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    return done != 0u;
+}
+// false: given up.  Warps that may come late sleep between tries: a dozen of them asking all the time took the issue slots of the one that issues the products.
+template <bool SLEEP = true> __device__ __forceinline__ bool bar_wait(const void *bar, unsigned parity, volatile unsigned *bail) {
     const uint32_t b = s32(bar);
-    unsigned long long began = 0;
-    for (unsigned i = 1;; i++) {
-        unsigned done;
-        asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}" : "=r"(done) : "r"(b), "r"(parity) : "memory");
-        if (done) return true;
-        if ((i & 255u) == 0u) {
-            if (*reinterpret_cast<volatile unsigned *>(bail)) return false;
-            const unsigned long long now = gtime_ns();
-            if (!began) began = now;
-            else if (now - began > 2000000000ull) {
-                *reinterpret_cast<volatile unsigned *>(bail) = 1u;
-                return false;
-            }
-        }
+    for (unsigned i = 1; i < WAIT_TRIES; i++) {
+        if (bar_passed(b, parity)) return true;
+        if (SLEEP) __nanosleep(20);
+        if ((i & 1023u) == 0u && *bail) return false;
     }
+    *bail = 1u;
+    return false;
 }
 // K-major operand descriptors: start >> 4 | 1 << 16 | 8 rows >> 4 << 32 | version 1 << 46 | swizzle (2: rows of 128 bytes, 4: rows of 64) << 61
 __device__ __forceinline__ uint64_t desc128(uint32_t a) { return (uint64_t)((a & 0x3ffffu) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61); }
 __device__ __forceinline__ uint64_t desc64(uint32_t a) { return (uint64_t)((a & 0x3ffffu) >> 4) | (1ull << 16) | (32ull << 32) | (1ull << 46) | (4ull << 61); }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+// The warp that issues products runs as one, so that addresses stay in its uniform registers, and one lane (lead) does it: with a single thread in that branch every operand went through
+// vector registers, and the eight products of a step took twice their time to issue.
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t lead) {
+    asm volatile("{.reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add), "r"(lead)
+                 : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) { // the first operand from TMEM
-    asm volatile("{.reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add, uint32_t lead) { // the first operand from TMEM
+    asm volatile("{.reg .pred p, q; setp.ne.b32 p, %4, 0; setp.ne.b32 q, %5, 0; @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add), "r"(lead)
+                 : "memory");
 }
-__device__ __forceinline__ void umma_commit(const void *bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(s32(bar)) : "memory"); }
+__device__ __forceinline__ void umma_commit(const void *bar, uint32_t lead) {
+    asm volatile("{.reg .pred q; setp.ne.b32 q, %1, 0; @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];}" ::"r"(s32(bar)), "r"(lead) : "memory");
+}
 __device__ __forceinline__ void tmem_ld32(uint32_t a, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -123,11 +133,11 @@ __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     return r;
 }
 
-// What a dequantising lane holds of half a record: codes, the key scales of positions g and g + 8, the value scales of positions 2 t, 2 t + 8 and 2 t + 1, 2 t + 9.
+// What a dequantising lane holds of a record: codes of both halves, the key scales of positions g and g + 8, the value scales of positions 2 t, 2 t + 8 and 2 t + 1, 2 t + 9.
 template <int HS> struct Raw {
     static constexpr int NG = groups(HS), VW = vec_words(HS);
-    uint32_t k[NG], v[NG], ks[NG], vs[2][NG];
-    __device__ __forceinline__ void load(const unsigned char *rec, int half, int lane) {
+    uint32_t k[2][NG], v[2][NG], ks[NG], vs[2][NG];
+    __device__ __forceinline__ void load(const unsigned char *rec, int lane) {
         const uint32_t *w = reinterpret_cast<const uint32_t *>(rec), *s = w + 4 * HS;
         const int g = lane >> 2, t = lane & 3;
         uint32_t x[VW];
@@ -138,8 +148,11 @@ template <int HS> struct Raw {
         };
 #pragma unroll
         for (int c = 0; c < NG / VW; c++) {
-            get(w + word_of<HS>(half, lane, c * VW), k + c * VW);
-            get(w + 2 * HS + word_of<HS>(half, lane, c * VW), v + c * VW);
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                get(w + word_of<HS>(half, lane, c * VW), k[half] + c * VW);
+                get(w + 2 * HS + word_of<HS>(half, lane, c * VW), v[half] + c * VW);
+            }
             get(s + g * NG + c * VW, ks + c * VW);
             get(s + 8 * NG + 2 * t * NG + c * VW, vs[0] + c * VW);
             get(s + 8 * NG + (2 * t + 1) * NG + c * VW, vs[1] + c * VW);
@@ -159,10 +172,10 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
     constexpr int NG = groups(HS);
     extern __shared__ unsigned char raw_smem[];
     unsigned char *smem = raw_smem + (-s32(raw_smem) & 1023u); // the operands' swizzle counts from 1024-byte boundaries
-    unsigned char *sQ = smem, *stages = smem + chunk_q_bytes(HS);
-    ChunkSmem &sh = *reinterpret_cast<ChunkSmem *>(stages + 2 * chunk_stage_bytes(HS));
+    unsigned char *sQ = smem, *sK = sQ + chunk_tile_bytes(HS), *sV = sK + CHUNK_K_STAGES * chunk_tile_bytes(HS);
+    ChunkSmem &sh = *reinterpret_cast<ChunkSmem *>(sV + CHUNK_V_STAGES * chunk_tile_bytes(HS));
     const Step &a = c.step;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int G = a.kv.kv_heads, mul = a.heads / G;
     const int n_tiles = (a.rows.n + c.tokens - 1) / c.tokens;
     const int split = blockIdx.x % c.splits, kvh = blockIdx.x / c.splits % G, tile = n_tiles - 1 - blockIdx.x / c.splits / G; // the last tokens, which see most, first
@@ -170,15 +183,18 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
 
     pdl_wait();
     if (tid == 0) {
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < CHUNK_K_STAGES; i++) {
             bar_init(&sh.k_full[i], CHUNK_DEQUANT);
-            bar_init(&sh.v_full[i], CHUNK_DEQUANT);
-            bar_init(&sh.free[i], 1);
-            bar_init(&sh.s_full[i], 1);
-            bar_init(&sh.s_empty[i], CHUNK_SOFTMAX);
-            bar_init(&sh.p_full[i], CHUNK_SOFTMAX);
+            bar_init(&sh.k_free[i], 1);
         }
-        for (int i = 0; i < 4; i++) bar_init(&sh.pair[i], 2);
+        for (int i = 0; i < 2; i++) {
+            bar_init(&sh.v_full[i], CHUNK_DEQUANT);
+            bar_init(&sh.v_free[i], 1);
+            bar_init(&sh.s_full[i], 1);
+            bar_init(&sh.p_full[i], CHUNK_SOFTMAX / 2);
+            sh.again[i] = sh.repeat[i] = 0;
+        }
+        for (int i = 0; i < CHUNK_SOFTMAX / 2; i++) bar_init(&sh.pair[i], 2);
         bar_init(&sh.drained, 1);
         sh.bail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -271,13 +287,13 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem = sh.tmem, tS = tmem, tP = tmem + 256, tO = tmem + 384;
-    const int total = sh.n_segments ? sh.segments[sh.n_segments - 1].tiles : 0;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0), tS = tmem, tO = tmem + 2 * CHUNK_KEYS;
+    const int total = __shfl_sync(0xffffffffu, sh.n_segments ? sh.segments[sh.n_segments - 1].tiles : 0, 0);
     const int first = (int)((long long)total * split / c.splits), last = (int)((long long)total * (split + 1) / c.splits), count = last - first;
 
     if (warp >= CHUNK_SOFTMAX && warp < CHUNK_ISSUER) {
         // ===== records -> FP16 operands =====
-        const int d = warp - CHUNK_SOFTMAX, w = d / 2, half = d % 2, g = lane >> 2, t = lane & 3;
+        const int w = warp - CHUNK_SOFTMAX, g = lane >> 2, t = lane & 3;
         const uint32_t one = magic();
         int seg = 0, ahead = 0, block = 0, stop = 0, behind = 0; // tiles left in the segment, this warp's record in the next one, the segment's end; raw is a record behind it
         if (count > 0) {
@@ -287,7 +303,8 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
             block = sh.segments[seg].begin + (first - before) * CHUNK_RECORDS + w;
             stop = sh.segments[seg].end;
         }
-        auto fetch = [&](Raw<HS> &to) { // this warp's half record of the list's next tile; behind the segment's end its last one, whose values then count as zeros
+        Raw<HS> raw;
+        auto fetch = [&] { // this warp's record of the list's next tile; behind the segment's end its last one, whose values then count as zeros
             if (ahead == 0) {
                 seg++;
                 ahead = sh.segments[seg].tiles - sh.segments[seg - 1].tiles;
@@ -295,171 +312,248 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
                 stop = sh.segments[seg].end;
             }
             behind = block >= stop;
-            to.load(record<HS>(a.kv, sh.segments[seg].slot, kvh, min(block, stop - 1)), half, lane);
+            raw.load(record<HS>(a.kv, sh.segments[seg].slot, kvh, min(block, stop - 1)), lane);
             ahead--;
             block += CHUNK_RECORDS;
         };
-        // row 16 w + 8 half + g of the keys; positions 16 w + 8 half + 2 t, + 1 of the values: 16-byte chunk 2 (w % 4) + half of the rows of 64 positions
-        const uint32_t k_at = s32(stages) + (w * 16 + half * 8 + g) * 64 + ((t ^ (g >> 1 & 3)) << 4);
-        const uint32_t v_at = s32(stages) + NG * CHUNK_KEYS * 64 + (w / 4) * (HS * 128) + g * 128 + (((w % 4 * 2 + half) ^ g) << 4) + t * 4;
-        const uint32_t k_perm = half ? 0x3232 : 0x1010, v_perm = half ? 0x7632 : 0x5410;
-        struct Held { // a half record's values, until the product two tiles before them has read its own
-            uint32_t v[NG], d[NG]; // codes, scales of positions 8 half + 2 t and + 1
-        };
-        auto keys = [&](int j, Raw<HS> &now, Held &held) {
-            // a value scale that FP16 products do not hold (or a NaN) is moved into the keys: such positions get no value and a NaN key
-            __half2 widest;
+        // rows 16 w + 8 half + g of the keys; positions 16 w + 8 half + 2 t, + 1 of the values: 16-byte chunk 2 (w % 4) + half of the rows of 64 positions
+        const uint32_t k_at = s32(sK) + (w * 16 + g) * 64 + ((t ^ (g >> 1 & 3)) << 4);
+        const uint32_t v_at = s32(sV) + (w / 4) * (HS * 128) + g * 128 + t * 4, v_chunk = (w % 4 * 2 ^ g) << 4;
+        if (count > 0) fetch();
+        int ks = 0; // stage of the keys
+        unsigned k_phase = 1;
+        for (int j = 0; j < count; j++) {
+            const int b = j & 1;
+            uint32_t v[2][NG], dv[2][NG]; // the values' codes and scales
+            __half2 widest = {};
 #pragma unroll
-            for (int i = 0; i < NG; i++) {
-                held.v[i] = now.v[i];
-                held.d[i] = __byte_perm(now.vs[0][i], now.vs[1][i], v_perm);
-                const __half2 x = __habs2(*reinterpret_cast<const __half2 *>(&held.d[i]));
-                widest = i ? __hmax2_nan(widest, x) : x;
-            }
-            const uint32_t wide = *reinterpret_cast<const uint32_t *>(&widest);
+            for (int i = 0; i < NG; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    v[h][i] = raw.v[h][i];
+                    dv[h][i] = __byte_perm(raw.vs[0][i], raw.vs[1][i], h ? 0x7632 : 0x5410);
+                    widest = __hmax2_nan(widest, __habs2(*reinterpret_cast<const __half2 *>(&dv[h][i])));
+                }
             if (behind)
 #pragma unroll
-                for (int i = 0; i < NG; i++) held.d[i] = 0u;
-            if (__any_sync(0xffffffffu, (0xeffeeffeu - wide & 0x80008000u) != 0x80008000u)) { // a half above 0x6ffe: 8 d up to 65504
-                uint32_t bad = ((wide & 0xffffu) > 0x6ffeu ? 1u << (2 * t) : 0u) | (wide >> 16 > 0x6ffeu ? 2u << (2 * t) : 0u); // by position of the half
+                for (int i = 0; i < NG; i++) dv[0][i] = dv[1][i] = 0u;
+            // a value scale that FP16 products do not hold (or a NaN) is moved into the keys: such positions get no value and a NaN key
+            if (__any_sync(0xffffffffu, (0xeffeeffeu - *reinterpret_cast<const uint32_t *>(&widest) & 0x80008000u) != 0x80008000u)) { // a half above 0x6ffe: 8 d up to 65504
+                uint32_t bad = 0; // by position of the record
+#pragma unroll
+                for (int i = 0; i < NG; i++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) bad |= ((dv[h][i] & 0x7fffu) > 0x6ffeu ? 1u << (8 * h + 2 * t) : 0u) | ((dv[h][i] >> 16 & 0x7fffu) > 0x6ffeu ? 2u << (8 * h + 2 * t) : 0u);
                 bad = __reduce_or_sync(0xffffffffu, bad);
 #pragma unroll
                 for (int i = 0; i < NG; i++) {
-                    if (bad >> (2 * t) & 1u) held.d[i] &= 0xffff0000u;
-                    if (bad >> (2 * t + 1) & 1u) held.d[i] &= 0x0000ffffu;
-                    if (bad >> g & 1u) now.ks[i] = 0x7fff7fffu;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        if (bad >> (8 * h + 2 * t) & 1u) dv[h][i] &= 0xffff0000u;
+                        if (bad >> (8 * h + 2 * t + 1) & 1u) dv[h][i] &= 0x0000ffffu;
+                    }
+                    if (bad >> g & 1u) raw.ks[i] |= 0x00007fffu;
+                    if (bad >> (8 + g) & 1u) raw.ks[i] |= 0x7fff0000u;
                 }
             }
-            const int b = j & 1;
-            if (j >= 2 && !__all_sync(0xffffffffu, bar_wait(&sh.s_full[b], ((j >> 1) - 1) & 1, &sh.bail))) return false; // the product of tile j - 2 has read its keys
-            const uint32_t at = k_at + b * chunk_stage_bytes(HS);
+            if (j >= CHUNK_K_STAGES && !__all_sync(0xffffffffu, bar_wait(&sh.k_free[ks], k_phase, &sh.bail))) break; // the scores of tile j - 3 stand
 #pragma unroll
-            for (int i = 0; i < NG; i++) {
-                uint32_t x[4];
-                unpack(now.k[i], one, x);
-                const uint32_t dk = __byte_perm(now.ks[i], 0, k_perm);
-                sts128(at + i * (CHUNK_KEYS * 64), hmul2(x[0], dk), hmul2(x[1], dk), hmul2(x[2], dk), hmul2(x[3], dk));
-            }
+            for (int i = 0; i < NG; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t x[4];
+                    unpack(raw.k[h][i], one, x);
+                    const uint32_t dk = __byte_perm(raw.ks[i], 0, h ? 0x3232 : 0x1010);
+                    sts128(k_at + ks * chunk_tile_bytes(HS) + h * 512 + i * (CHUNK_KEYS * 64), hmul2(x[0], dk), hmul2(x[1], dk), hmul2(x[2], dk), hmul2(x[3], dk));
+                }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            if (lane == 0) bar_arrive(&sh.k_full[b]);
-            return true;
-        };
-        auto values = [&](int j, const Held &held) {
-            const int b = j & 1;
-            if (j >= 2 && !__all_sync(0xffffffffu, bar_wait(&sh.free[b], ((j >> 1) - 1) & 1, &sh.bail))) return false; // the product of tile j - 2 has read its values
-            const uint32_t at = v_at + b * chunk_stage_bytes(HS);
-#pragma unroll
-            for (int i = 0; i < NG; i++) {
-                uint32_t x[4];
-                unpack(held.v[i], one, x);
-#pragma unroll
-                for (int u = 0; u < 4; u++) sts32(at + (i * 32 + u * 8) * 128, hmul2(x[u], held.d[i])); // row 32 i + 8 u + g: entry 32 i + 4 g + u
+            if (lane == 0) bar_arrive(&sh.k_full[ks]);
+            if (++ks == CHUNK_K_STAGES) {
+                ks = 0;
+                k_phase ^= 1;
             }
+            if (j + 1 < count) fetch(); // on its way while the values are converted
+            if (j >= 2 && !__all_sync(0xffffffffu, bar_wait(&sh.v_free[b], ((j >> 1) - 1) & 1, &sh.bail))) break; // the products of tile j - 2 have read its values
+#pragma unroll
+            for (int i = 0; i < NG; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t x[4];
+                    unpack(v[h][i], one, x);
+#pragma unroll
+                    for (int u = 0; u < 4; u++) sts32(v_at + b * chunk_tile_bytes(HS) + (v_chunk ^ h * 16) + (i * 32 + u * 8) * 128, hmul2(x[u], dv[h][i])); // row 32 i + 8 u + g: entry 32 i + 4 g + u
+                }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.v_full[b]);
-            return true;
-        };
-        // Keys run a tile ahead of the values, which wait for the rows; the next record is asked for when this one's registers have been read, not before: loads share their
-        // scoreboards, and a wait for the older ones would be one for both (800 cycles a tile).
-        Raw<HS> raw;
-        Held even, odd;
-        bool ok = true;
-        if (count > 0) {
-            fetch(raw);
-            ok = keys(0, raw, even);
-            if (count > 1) fetch(raw);
         }
-        for (int j = 0; j < count && ok; j += 2) {
-            if (j + 1 < count) {
-                if (!(ok = keys(j + 1, raw, odd))) break;
-                if (j + 2 < count) fetch(raw);
-            }
-            if (!(ok = values(j, even)) || j + 1 >= count) break;
-            if (j + 2 < count) {
-                if (!(ok = keys(j + 2, raw, even))) break;
-                if (j + 3 < count) fetch(raw);
-            }
-            ok = values(j + 1, odd);
-        }
-    } else if (warp == CHUNK_ISSUER && lane == 0) {
+    } else if (warp == CHUNK_ISSUER) {
         // ===== products =====
         constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(CHUNK_KEYS >> 3) << 17) | ((uint32_t)(CHUNK_ROWS >> 4) << 24);
         constexpr uint32_t idesc_o = (1u << 4) | ((uint32_t)(HS >> 3) << 17) | ((uint32_t)(CHUNK_ROWS >> 4) << 24);
-        const uint32_t q = s32(sQ), st = s32(stages);
-        auto product = [&](int j) { // O += P V of tile j
-            const int b = j & 1;
-            if (!bar_wait(&sh.v_full[b], j >> 1 & 1, &sh.bail) || !bar_wait(&sh.p_full[b], j >> 1 & 1, &sh.bail)) return false;
-            fence_after();
-            const uint32_t sV = st + b * chunk_stage_bytes(HS) + NG * CHUNK_KEYS * 64;
+        const uint32_t q = s32(sQ), lead = lane == 0;
+        const auto passed = [&](const void *bar, unsigned parity) { return __all_sync(0xffffffffu, bar_wait<false>(bar, parity, &sh.bail)) != 0; };
+        const auto scores = [&](int stage, int h) { // S = Q K^T
+            const uint32_t k0 = s32(sK) + stage * chunk_tile_bytes(HS);
 #pragma unroll
-            for (int k = 0; k < CHUNK_KEYS / 16; k++) umma_ts(tO, tP + b * 64 + k * 8, desc128(sV + (k / 4) * (HS * 128) + (k % 4) * 32), idesc_o, j > 0 || k > 0);
-            umma_commit(&sh.free[b]);
-            return true;
+            for (int k = 0; k < HS / 16; k++)
+                umma_ss(tS + h * CHUNK_KEYS, desc64(q + (k / 2) * (CHUNK_ROWS * 64) + (k % 2) * 32), desc64(k0 + (k / 2) * (CHUNK_KEYS * 64) + (k % 2) * 32), idesc_s, k > 0, lead);
+            umma_commit(&sh.s_full[h], lead);
         };
+        unsigned turn = 0; // bit h: the phase of the stream's next probabilities
         bool ok = true;
-        for (int j = 0; j < count && ok; j++) {
-            const int b = j & 1;
-            ok = bar_wait(&sh.k_full[b], j >> 1 & 1, &sh.bail) && (j < 2 || bar_wait(&sh.s_empty[b], ((j >> 1) - 1) & 1, &sh.bail));
-            if (!ok) break;
+        for (int j = 0; j < min(count, 2) && ok; j++) {
+            if (!(ok = passed(&sh.k_full[j], 0))) break;
             fence_after();
-            const uint32_t sK = st + b * chunk_stage_bytes(HS);
-#pragma unroll
-            for (int k = 0; k < HS / 16; k++) umma_ss(tS + b * 128, desc64(q + (k / 2) * (CHUNK_ROWS * 64) + (k % 2) * 32), desc64(sK + (k / 2) * (CHUNK_KEYS * 64) + (k % 2) * 32), idesc_s, k > 0);
-            umma_commit(&sh.s_full[b]);
-            if (j > 0) ok = product(j - 1);
+            scores(j, j);
         }
-        if (ok && count > 0) ok = product(count - 1);
+        int stage = 0, ahead = 2; // of the keys of tiles j and j + 2
+        unsigned phase = 0;
+        for (int j = 0; j < count && ok; j++) {
+            const int h = j & 1;
+            volatile unsigned *again = &sh.again[h], *repeat = &sh.repeat[h];
+            if (!(ok = passed(&sh.p_full[h], turn >> h & 1))) break;
+            turn ^= 1u << h;
+            if (__any_sync(0xffffffffu, *again != 0)) { // these probabilities do not count: the scores once more
+                if (lead) {
+                    *again = 0;
+                    *repeat = 1;
+                }
+                __syncwarp();
+                fence_after();
+                scores(stage, h);
+                if (!(ok = passed(&sh.p_full[h], turn >> h & 1))) break;
+                turn ^= 1u << h;
+            }
+            if (lead) {
+                bar_arrive(&sh.k_free[stage]);
+                *repeat = 0;
+            }
+            __syncwarp();
+            if (!(ok = passed(&sh.v_full[h], j >> 1 & 1))) break;
+            fence_after();
+            const uint32_t v0 = s32(sV) + h * chunk_tile_bytes(HS);
+#pragma unroll
+            for (int k = 0; k < CHUNK_KEYS / 16; k++) // O += P V
+                umma_ts(tO + h * CHUNK_KEYS, tS + h * CHUNK_KEYS + (k / 4) * (CHUNK_KEYS / 2) + (k % 4) * 8, desc128(v0 + (k / 4) * (HS * 128) + (k % 4) * 32), idesc_o, j > 1 || k > 0, lead);
+            umma_commit(&sh.v_free[h], lead);
+            if (j + 2 < count) {
+                if (!(ok = passed(&sh.k_full[ahead], phase))) break;
+                fence_after();
+                scores(ahead, h);
+            } else umma_commit(&sh.s_full[h], lead);
+            if (++stage == CHUNK_K_STAGES) stage = 0;
+            if (++ahead == CHUNK_K_STAGES) {
+                ahead = 0;
+                phase ^= 1;
+            }
+        }
         if (!ok) { // given up: what is under way ends before the tensor memory goes
             unsigned none = 0;
-            umma_commit(&sh.drained);
+            umma_commit(&sh.drained, lead);
             bar_wait(&sh.drained, 0, &none);
-            if (c.error) *reinterpret_cast<volatile unsigned *>(c.error) = 1u;
+            if (lead && c.error) *reinterpret_cast<volatile unsigned *>(c.error) = 1u;
         }
     } else if (warp < CHUNK_SOFTMAX) {
-        // ===== rows: warps w and w + 4 share 32 of them, 64 positions of a tile and half of the entries each =====
-        constexpr int COLUMNS = CHUNK_KEYS / 2, PIECE = 16;
-        const int side = warp / 4, r = warp % 4 * 32 + lane, token = r / mul;
-        const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16; // this warp's part of the tensor memory
-        const int group0 = side ? (NG + 1) / 2 : 0, group1 = side ? NG : (NG + 1) / 2;
+        // ===== rows: two threads a stream, 64 positions of a tile a thread =====
+        constexpr int PIECE = 16, COLUMNS = CHUNK_KEYS / 2;
+        const int side = warp / 8, stream = warp / 4 % 2, r = tid % CHUNK_ROWS, token = r / mul;
+        const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, row_s = tS + lanes + stream * CHUNK_KEYS + side * COLUMNS, row_o = tO + lanes + stream * CHUNK_KEYS;
         const float factor = sh.factor[r];
         unsigned met = 0;
         const auto meet = [&]() { // the two warps of a row; a wait with an end, as all here: one of them may have given up
             __syncwarp();
-            if (lane == 0) bar_arrive(&sh.pair[warp % 4]);
-            return __all_sync(0xffffffffu, bar_wait(&sh.pair[warp % 4], met++ & 1, &sh.bail)) != 0;
+            if (lane == 0) bar_arrive(&sh.pair[warp % 8]);
+            return __all_sync(0xffffffffu, bar_wait(&sh.pair[warp % 8], met++ & 1, &sh.bail)) != 0;
         };
         int lo = 0, hi = 0, own = -1, seg = 0;
         if (token < tokens && sh.segment[token] >= 0) {
             own = sh.segment[token];
             visible(sh.pos[token], a.window, lo, hi);
         }
-        while (seg < sh.n_segments && sh.segments[seg].tiles <= first) seg++;
-        float m = -CUDART_INF_F, l = 0.0f; // of the row; of this thread's positions
-        bool ok = true;
-        for (int j = 0; j < count; j++) {
-            const int b = j & 1;
-            while (sh.segments[seg].tiles <= first + j) seg++;
-            const int before = seg ? sh.segments[seg - 1].tiles : 0, key0 = (sh.segments[seg].begin + (first + j - before) * CHUNK_RECORDS) * BLOCK;
-            int from = lo - key0, to = hi - key0; // the tile's positions [from, to) are seen
-            if (own != seg) from = to = 0;
-            const bool fresh = m == -CUDART_INF_F && max(from, 0) < min(to, CHUNK_KEYS); // the first that the row sees
-            from -= side * COLUMNS;
-            to -= side * COLUMNS;
-            const bool mask = __any_sync(0xffffffffu, from > 0 || to < COLUMNS);
-            ok = __all_sync(0xffffffffu, bar_wait(&sh.s_full[b], j >> 1 & 1, &sh.bail));
+        float top = -CUDART_INF_F, l = 0.0f, sum = 0.0f; // the row's largest product so far; of this thread's positions the sum, and that of a tile that may yet be repeated
+        bool ok = true, fresh = false;
+        float base = 0.0f, ref = 0.0f; // top where there is one, times the factor
+        int from = 0, to = 0, j = stream - 2, next = 0; // the tile's positions [from, to) are seen, counted from this thread's first; the segment's end
+        for (unsigned turn = 0; stream < count; turn++) {
+            ok = __all_sync(0xffffffffu, bar_wait(&sh.s_full[stream], turn & 1, &sh.bail));
             if (!ok) break;
             fence_after();
-            if (j >= 2) { // P's buffer: its last product has read it
-                ok = __all_sync(0xffffffffu, bar_wait(&sh.free[b], ((j >> 1) - 1) & 1, &sh.bail));
-                if (!ok) break;
+            const bool repeat = *reinterpret_cast<volatile unsigned *>(&sh.repeat[stream]);
+            if (!repeat) {
+                l += sum;
+                if ((j += 2) >= count) break;
+                if (first + j >= next) {
+                    while (sh.segments[seg].tiles <= first + j) seg++;
+                    next = sh.segments[seg].tiles;
+                    const int before = seg ? sh.segments[seg - 1].tiles : 0, key0 = (sh.segments[seg].begin + (first + j - before) * CHUNK_RECORDS) * BLOCK + side * COLUMNS;
+                    from = own == seg ? lo - key0 : 0;
+                    to = own == seg ? hi - key0 : 0;
+                } else {
+                    from -= 2 * CHUNK_KEYS;
+                    to -= 2 * CHUNK_KEYS;
+                }
+                fresh = top == -CUDART_INF_F && max(from, -side * COLUMNS) < min(to, CHUNK_KEYS - side * COLUMNS); // the first that the row sees: no maximum yet
             }
-            const uint32_t row_s = tS + lanes + b * CHUNK_KEYS + side * COLUMNS, row_p = tP + lanes + b * (CHUNK_KEYS / 2) + side * (COLUMNS / 2);
-            // One pass with the maximum as it stands.  It moves rarely, and a sum of more than 2^8 shows that it has to: then the tile's maximum is looked for and the pass made again.
-            // (A maximum of every tile in front of or beside the exponentials cost as much as they do.)
-            float sum;
-            const auto exponentials_of = [&](auto masked, float ref) {
+            // One pass with the maximum as it stands.  It moves rarely, and a sum of more than 2^8 shows that it has to: the probabilities, which have taken the place of the scores, are
+            // dropped, the scores come once more, and the tile's maximum is looked for first.  (A maximum of every tile in front of or beside the exponentials cost as much as they do.)
+            const bool special = __any_sync(0xffffffffu, repeat || fresh || from > 0 || to < COLUMNS || !(fabsf(ref) <= 65536.0f));
+            if (special && __any_sync(0xffffffffu, repeat || fresh)) { // (the same for both warps of a row)
+                float mx = -CUDART_INF_F;
+#pragma unroll 1
+                for (int q = 0; q < COLUMNS; q += PIECE) {
+                    uint32_t x[PIECE];
+                    tmem_ld16(row_s + q, x);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < PIECE; i++) mx = fmaxf(mx, i >= from - q && i < to - q ? __uint_as_float(x[i]) : -CUDART_INF_F);
+                }
+                sh.half_row[stream][side][r] = mx;
+                ok = meet();
+                if (!ok) break;
+                mx = fmaxf(mx, sh.half_row[stream][side ^ 1][r]);
+                const float grown = fmaxf(top, mx), alpha = top == grown ? 1.0f : ex2((top - grown) * factor);
+                top = grown;
+                l *= alpha;
+                if (j > 1 && __any_sync(0xffffffffu, alpha != 1.0f)) { // (the product of tile j - 2 came before these scores)
+#pragma unroll 1
+                    for (int q = side * HS / 2; q < (side + 1) * HS / 2; q += PIECE) {
+                        uint32_t o[PIECE];
+                        tmem_ld16(row_o + q, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < PIECE; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                        tmem_st16(row_o + q, o);
+                    }
+                }
+                base = top == -CUDART_INF_F ? 0.0f : top;
+                ref = base * factor;
+            }
+            // P takes the place of S: piece q of 16 scores is read before its 8 columns are written, [8 q, 8 q + 8)
+            if (special && !__any_sync(0xffffffffu, max(from, 0) < min(to, COLUMNS))) { // other rows' tile
+                const uint32_t p[PIECE / 2] = {};
+                sum = 0.0f;
+#pragma unroll 1
+                for (int q = 0; q < COLUMNS / 2; q += PIECE / 2) tmem_st8(row_s + q, p);
+            } else if (special && __any_sync(0xffffffffu, from > 0 || to < COLUMNS || !(fabsf(ref) <= 65536.0f))) { // a border, or scores so large that their products and the maximum's round apart
+                sum = 0.0f;
+#pragma unroll 1
+                for (int q = 0; q < COLUMNS; q += PIECE) {
+                    uint32_t x[PIECE], p[PIECE / 2];
+                    tmem_ld16(row_s + q, x);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < PIECE; i++) {
+                        const float e = i >= from - q && i < to - q ? ex2((__uint_as_float(x[i]) - base) * factor) : 0.0f;
+                        sum += e;
+                        x[i] = __float_as_uint(e);
+                    }
+#pragma unroll
+                    for (int i = 0; i < PIECE / 2; i++) p[i] = pack_f16(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+                    tmem_st8(row_s + q / 2, p);
+                }
+            } else {
                 const unsigned long long factor2 = pack_f32x2(factor, factor), ref2 = pack_f32x2(-ref, -ref);
                 unsigned long long part[2] = {0ull, 0ull};
                 uint32_t s[2][PIECE];
@@ -469,10 +563,6 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
                     uint32_t(&x)[PIECE] = s[q & 1];
                     tmem_ld_wait();
                     if (q + 1 < COLUMNS / PIECE) tmem_ld16(row_s + (q + 1) * PIECE, s[q + 1 & 1]);
-                    if constexpr (decltype(masked)::value)
-#pragma unroll
-                        for (int i = 0; i < PIECE; i++)
-                            if (!(q * PIECE + i >= from && q * PIECE + i < to)) x[i] = 0xff800000u;
                     uint32_t p[PIECE / 2];
 #pragma unroll
                     for (int i = 0; i < PIECE / 2; i++) {
@@ -483,110 +573,89 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
                         part[i & 1] = add_f32x2(part[i & 1], pack_f32x2(e0, e1));
                         p[i] = pack_f16(e0, e1);
                     }
-                    tmem_st8(row_p + q * (PIECE / 2), p);
+                    tmem_st8(row_s + q * (PIECE / 2), p);
                 }
                 float a0, a1, b0, b1;
                 unpack_f32x2(part[0], a0, a1);
                 unpack_f32x2(part[1], b0, b1);
                 sum = (a0 + a1) + (b0 + b1);
-            };
-            const auto exponentials = [&](float ref) {
-                if (mask) exponentials_of(std::true_type(), ref);
-                else exponentials_of(std::false_type(), ref);
-            };
-            exponentials(m == -CUDART_INF_F ? 0.0f : m);
-            const bool again = __any_sync(0xffffffffu, fresh || sum > 256.0f);
-            if (lane == 0) sh.again[b][warp] = again;
-            ok = meet();
-            if (!ok) break;
-            if (again || sh.again[b][warp ^ 4]) {
-                float mx = -CUDART_INF_F;
-#pragma unroll 1
-                for (int q = 0; q < COLUMNS / PIECE; q++) {
-                    uint32_t x[PIECE];
-                    tmem_ld16(row_s + q * PIECE, x);
-                    tmem_ld_wait();
-                    const int lo_q = from - q * PIECE, hi_q = to - q * PIECE;
-#pragma unroll
-                    for (int i = 0; i < PIECE; i++) mx = fmaxf(mx, i >= lo_q && i < hi_q ? __uint_as_float(x[i]) : -CUDART_INF_F);
-                }
-                sh.half_row[side][r] = mx;
-                ok = meet();
-                if (!ok) break;
-                mx = fmaxf(mx, sh.half_row[side ^ 1][r]);
-                const float grown = fmaxf(m, mx * factor), alpha = m == grown ? 1.0f : ex2(m - grown);
-                m = grown;
-                l *= alpha;
-                if (j > 0) {
-                    ok = __all_sync(0xffffffffu, bar_wait(&sh.free[b ^ 1], (j - 1) >> 1 & 1, &sh.bail));
-                    if (!ok) break;
-                    fence_after();
-                    tmem_st_wait();
-#pragma unroll 1
-                    for (int q = group0 * 2; q < group1 * 2; q++) {
-                        uint32_t o[PIECE];
-                        tmem_ld16(tO + lanes + q * PIECE, o);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int i = 0; i < PIECE; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tmem_st16(tO + lanes + q * PIECE, o);
-                    }
-                }
-                exponentials(m == -CUDART_INF_F ? 0.0f : m);
             }
-            l += sum;
+            const bool over = __any_sync(0xffffffffu, !repeat && sum > 256.0f);
             tmem_st_wait();
             fence_before();
             __syncwarp();
             if (lane == 0) {
-                bar_arrive(&sh.s_empty[b]);
-                bar_arrive(&sh.p_full[b]);
+                if (over) *reinterpret_cast<volatile unsigned *>(&sh.again[stream]) = 1u;
+                bar_arrive(&sh.p_full[stream]);
             }
         }
-        if (ok && count > 0) ok = __all_sync(0xffffffffu, bar_wait(&sh.free[(count - 1) & 1], (count - 1) >> 1 & 1, &sh.bail));
+        sh.half_row[stream][side][r] = l;
+        sh.top[stream][r] = top;
+        fence_before();
+    }
+    __syncthreads();
+    // ===== results: the streams are joined; a warp takes 32 rows and 32 entries =====
+    if (warp < 4 * NG && sh.bail == 0u) {
         fence_after();
-        if (ok) {
-            sh.half_row[side][r] = l;
-            ok = meet();
-            l += sh.half_row[side ^ 1][r];
-        }
-        const bool on = token < tokens && sh.slot[min(token, CHUNK_ROWS - 1)] >= 0, some = hi > lo;
-        const int row = token0 + token, head = kvh * mul + r % mul;
-        const float inv = 1.0f / l;
-#pragma unroll 1
-        for (int q = group0; q < group1 && ok; q++) {
-            uint32_t o[32];
-            __syncwarp();
-            if (count > 0) {
-                tmem_ld32(tO + lanes + q * 32, o);
+        const int q = warp / 4, r = warp % 4 * 32 + lane, token = r / mul, row = token0 + token, head = kvh * mul + r % mul;
+        const bool on = token < tokens && sh.slot[min(token, CHUNK_ROWS - 1)] >= 0;
+        const float factor = sh.factor[r], t0 = sh.top[0][r], t1 = sh.top[1][r], top = fmaxf(t0, t1), base = top == -CUDART_INF_F ? 0.0f : top;
+        const float a0 = t0 == base ? 1.0f : ex2((t0 - base) * factor), a1 = t1 == base ? 1.0f : ex2((t1 - base) * factor);
+        const float l = a0 * (sh.half_row[0][0][r] + sh.half_row[0][1][r]) + a1 * (sh.half_row[1][0][r] + sh.half_row[1][1][r]);
+        uint32_t o[32];
+#pragma unroll
+        for (int i = 0; i < 32; i++) o[i] = 0u;
+        for (int h = 0; h < min(count, 2); h++) { // (a stream without tiles has no sums)
+#pragma unroll
+            for (int i = 0; i < 32; i += 16) {
+                uint32_t x[16];
+                tmem_ld16(tO + ((uint32_t)(warp % 4 * 32) << 16) + h * CHUNK_KEYS + q * 32 + i, x);
                 tmem_ld_wait();
-            } else
 #pragma unroll
-                for (int i = 0; i < 32; i++) o[i] = 0u;
-            if (on && c.splits > 1) {
-                float *w = a.work + (((size_t)row * a.heads + head) * c.splits + split) * (HS + 2);
-                if (q == 0) { w[0] = m; w[1] = l; }
-#pragma unroll
-                for (int i = 0; i < 32; i++) w[2 + q * 32 + i] = __uint_as_float(o[8 * (i % 4) + i / 4]); // entry i of the group is column 8 (i % 4) + i / 4
-            } else if (on) {
-                uint32_t y[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float v0 = some ? __uint_as_float(o[8 * (2 * i % 4) + 2 * i / 4]) * inv : 0.0f, v1 = some ? __uint_as_float(o[8 * ((2 * i + 1) % 4) + (2 * i + 1) / 4]) * inv : 0.0f;
-                    if (a.out_type == B200_GGML_F16) y[i] = pack_f16(v0, v1);
-                    else {
-                        const __nv_bfloat162 h = __floats2bfloat162_rn(v0, v1);
-                        y[i] = *reinterpret_cast<const uint32_t *>(&h);
-                    }
-                }
-                uint16_t *out = (uint16_t *)a.out + row * a.ldo + (size_t)head * HS + q * 32;
-                if (c.vec_out)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) reinterpret_cast<uint4 *>(out)[i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-                else
-#pragma unroll
-                    for (int i = 0; i < 32; i++) out[i] = (uint16_t)(y[i / 2] >> (i & 1) * 16);
+                for (int u = 0; u < 16; u++) o[i + u] = __float_as_uint(fmaf(h ? a1 : a0, __uint_as_float(x[u]), __uint_as_float(o[i + u])));
             }
+        }
+        if (c.splits > 1) { // parts go through shared memory, where the queries were: 64 bytes of a row at a time in place of 4 (the rows' starts are 8-byte aligned)
+            const long long part = on ? (((long long)row * a.heads + head) * c.splits + split) * (HS + 2) : -1;
+            if (on && q == 0) { a.work[part] = top * factor; a.work[part + 1] = l; }
+            const uint32_t at = s32(sQ) + warp * 2048;
+#pragma unroll 1
+            for (int e = 0; e < 32; e += 16) {
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 4; i++) // entries e + 4 i .. + 3: entry x of the group is column 8 (x % 4) + x / 4
+                    sts128(at + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4), e ? o[4 + i] : o[i], e ? o[12 + i] : o[8 + i], e ? o[20 + i] : o[16 + i], e ? o[28 + i] : o[24 + i]);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int k = 4 * i + lane / 8;
+                    float2 x;
+                    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at + k * 64 + ((lane % 8 / 2 ^ (k >> 1 & 3)) << 4) + (lane & 1) * 8) : "memory");
+                    const long long to = __shfl_sync(0xffffffffu, part, k);
+                    if (to >= 0) *reinterpret_cast<float2 *>(a.work + to + 2 + q * 32 + e + lane % 8 * 2) = x;
+                }
+            }
+        } else if (on) {
+            int lo, hi;
+            visible(sh.pos[token], a.window, lo, hi);
+            const float inv = hi > lo ? 1.0f / l : 0.0f;
+            uint32_t y[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const float v0 = __uint_as_float(o[8 * (2 * i % 4) + 2 * i / 4]) * inv, v1 = __uint_as_float(o[8 * ((2 * i + 1) % 4) + (2 * i + 1) / 4]) * inv;
+                if (a.out_type == B200_GGML_F16) y[i] = pack_f16(v0, v1);
+                else {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v0, v1);
+                    y[i] = *reinterpret_cast<const uint32_t *>(&h);
+                }
+            }
+            uint16_t *out = (uint16_t *)a.out + row * a.ldo + (size_t)head * HS + q * 32;
+            if (c.vec_out)
+#pragma unroll
+                for (int i = 0; i < 4; i++) reinterpret_cast<uint4 *>(out)[i] = make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+            else
+#pragma unroll
+                for (int i = 0; i < 32; i++) out[i] = (uint16_t)(y[i / 2] >> (i & 1) * 16);
         }
         fence_before();
     }

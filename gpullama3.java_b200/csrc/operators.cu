@@ -166,9 +166,9 @@ static ChunkCut chunk_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, 
     const int chunk = a.chunk < a.n ? a.chunk : a.n;
     c.use = !quants && a.out_type != B200_GGML_F32 && (hs == 64 || hs == 96 || hs == 128) && mul <= kv4::CHUNK_ROWS && chunk > 1 && (long long)chunk * mul >= CHUNK_MIN_ROWS;
     if (!c.use) return c;
+    const int len = a.max_len > 0 && a.max_len < kv->view.context ? a.max_len : kv->view.context;
     c.tokens = kv4::CHUNK_ROWS / mul;
     const long long units = (long long)((a.n + c.tokens - 1) / c.tokens) * G;
-    const int len = a.max_len > 0 && a.max_len < kv->view.context ? a.max_len : kv->view.context;
     const long long seen = a.window > 0 && a.window + c.tokens < len ? a.window + c.tokens : len, worth = seen / (8 * kv4::CHUNK_KEYS); // eight tiles of positions a CTA
     long long splits = kv->sms / units;
     if (splits > worth) splits = worth;
