@@ -413,6 +413,7 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
         for (int j = 0; j < count && ok; j++) {
             const int h = j & 1;
             volatile unsigned *again = &sh.again[h], *repeat = &sh.repeat[h];
+            if (!(ok = passed(&sh.v_full[h], j >> 1 & 1))) break; // (first what is ready early)
             if (!(ok = passed(&sh.p_full[h], turn >> h & 1))) break;
             turn ^= 1u << h;
             if (__any_sync(0xffffffffu, *again != 0)) { // these probabilities do not count: the scores once more
@@ -426,18 +427,15 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
                 if (!(ok = passed(&sh.p_full[h], turn >> h & 1))) break;
                 turn ^= 1u << h;
             }
-            if (lead) {
-                bar_arrive(&sh.k_free[stage]);
-                *repeat = 0;
-            }
-            __syncwarp();
-            if (!(ok = passed(&sh.v_full[h], j >> 1 & 1))) break;
+            if (lead) bar_arrive(&sh.k_free[stage]);
             fence_after();
             const uint32_t v0 = s32(sV) + h * chunk_tile_bytes(HS);
 #pragma unroll
             for (int k = 0; k < CHUNK_KEYS / 16; k++) // O += P V
                 umma_ts(tO + h * CHUNK_KEYS, tS + h * CHUNK_KEYS + (k / 4) * (CHUNK_KEYS / 2) + (k % 4) * 8, desc128(v0 + (k / 4) * (HS * 128) + (k % 4) * 32), idesc_o, j > 1 || k > 0, lead);
             umma_commit(&sh.v_free[h], lead);
+            if (lead) *repeat = 0;
+            __syncwarp();
             if (j + 2 < count) {
                 if (!(ok = passed(&sh.k_full[ahead], phase))) break;
                 fence_after();
