@@ -126,7 +126,9 @@ __device__ __forceinline__ unsigned long long add_f32x2(unsigned long long a, un
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
 }
-__device__ __forceinline__ void sts32(uint32_t a, uint32_t x) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(x) : "memory"); }
+__device__ __forceinline__ void store_matrices(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) { // four of 8 x 8 halves; lane l gives the address of row l % 8 of matrix l / 8
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -312,13 +314,15 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
                 stop = sh.segments[seg].end;
             }
             behind = block >= stop;
-            raw.load(record<HS>(a.kv, sh.segments[seg].slot, kvh, min(block, stop - 1)), lane);
+            const unsigned char *rec = record<HS>(a.kv, sh.segments[seg].slot, kvh, min(block, stop - 1));
+            raw.load(rec, lane);
             ahead--;
             block += CHUNK_RECORDS;
+            if (block < stop && lane < (record_bytes(HS) + 127) / 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(rec + (size_t)CHUNK_RECORDS * record_bytes(HS) + min(lane * 128, record_bytes(HS) - 1)));
         };
         // rows 16 w + 8 half + g of the keys; positions 16 w + 8 half + 2 t, + 1 of the values: 16-byte chunk 2 (w % 4) + half of the rows of 64 positions
         const uint32_t k_at = s32(sK) + (w * 16 + g) * 64 + ((t ^ (g >> 1 & 3)) << 4);
-        const uint32_t v_at = s32(sV) + (w / 4) * (HS * 128) + g * 128 + t * 4, v_chunk = (w % 4 * 2 ^ g) << 4;
+        const uint32_t v_at = s32(sV) + (w / 4) * (HS * 128) + lane * 128 + ((w % 4 * 2 ^ (lane & 7)) << 4);
         if (count > 0) fetch();
         int ks = 0; // stage of the keys
         unsigned k_phase = 1;
@@ -381,8 +385,8 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
                 for (int h = 0; h < 2; h++) {
                     uint32_t x[4];
                     unpack(v[h][i], one, x);
-#pragma unroll
-                    for (int u = 0; u < 4; u++) sts32(v_at + b * chunk_tile_bytes(HS) + (v_chunk ^ h * 16) + (i * 32 + u * 8) * 128, hmul2(x[u], dv[h][i])); // row 32 i + 8 u + g: entry 32 i + 4 g + u
+                    // rows 32 i + 8 u + g: entries 32 i + 4 g + u
+                    store_matrices((v_at + b * chunk_tile_bytes(HS) + i * 4096) ^ h * 16, hmul2(x[0], dv[h][i]), hmul2(x[1], dv[h][i]), hmul2(x[2], dv[h][i]), hmul2(x[3], dv[h][i]));
                 }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
