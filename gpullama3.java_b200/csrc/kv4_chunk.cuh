@@ -179,6 +179,8 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
     const Step &a = c.step;
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
     const int G = a.kv.kv_heads, mul = a.heads / G;
+    const unsigned of = (65535u + mul) / mul; // r / mul = r of >> 16: exact, as r mul < 2^16
+    const auto token_of = [&](int r) { return (int)(r * of >> 16); };
     const int n_tiles = (a.rows.n + c.tokens - 1) / c.tokens;
     const int split = blockIdx.x % c.splits, kvh = blockIdx.x / c.splits % G, tile = n_tiles - 1 - blockIdx.x / c.splits / G; // the last tokens, which see most, first
     const int token0 = tile * c.tokens, tokens = min(c.tokens, a.rows.n - token0);
@@ -221,10 +223,10 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
     float4 x[QROWS]; // entries 4 lane .. + 3
 #pragma unroll
     for (int i = 0; i < QROWS; i++) {
-        const int r = warp + i * WARPS, token = r / mul;
+        const int r = warp + i * WARPS, token = token_of(r);
         x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (token < tokens && r < CHUNK_ROWS && lane * 4 < HS) {
-            const float *q = a.q + (long long)(token0 + token) * a.ldq + (size_t)(kvh * mul + r % mul) * HS + lane * 4;
+            const float *q = a.q + (long long)(token0 + token) * a.ldq + (size_t)(kvh * mul + r - token * mul) * HS + lane * 4;
             if (a.vec) x[i] = *reinterpret_cast<const float4 *>(q);
             else x[i] = make_float4(q[0], q[1], q[2], q[3]);
         }
@@ -460,7 +462,7 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
     } else if (warp < CHUNK_SOFTMAX) {
         // ===== rows: two threads a stream, 64 positions of a tile a thread =====
         constexpr int PIECE = 16, COLUMNS = CHUNK_KEYS / 2;
-        const int side = warp / 8, stream = warp / 4 % 2, r = tid % CHUNK_ROWS, token = r / mul;
+        const int side = warp / 8, stream = warp / 4 % 2, r = tid % CHUNK_ROWS, token = token_of(r);
         const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, row_s = tS + lanes + stream * CHUNK_KEYS + side * COLUMNS, row_o = tO + lanes + stream * CHUNK_KEYS;
         const float factor = sh.factor[r];
         unsigned met = 0;
@@ -599,7 +601,7 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
     // ===== results: the streams are joined; a warp takes 32 rows and 32 entries =====
     if (warp < 4 * NG && sh.bail == 0u) {
         fence_after();
-        const int q = warp / 4, r = warp % 4 * 32 + lane, token = r / mul, row = token0 + token, head = kvh * mul + r % mul;
+        const int q = warp / 4, r = warp % 4 * 32 + lane, token = token_of(r), row = token0 + token, head = kvh * mul + r - token * mul;
         const bool on = token < tokens && sh.slot[min(token, CHUNK_ROWS - 1)] >= 0;
         const float factor = sh.factor[r], t0 = sh.top[0][r], t1 = sh.top[1][r], top = fmaxf(t0, t1), base = top == -CUDART_INF_F ? 0.0f : top;
         const float a0 = t0 == base ? 1.0f : ex2((t0 - base) * factor), a1 = t1 == base ? 1.0f : ex2((t1 - base) * factor);
