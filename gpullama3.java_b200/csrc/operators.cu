@@ -167,7 +167,9 @@ static ChunkCut chunk_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, 
     c.use = !quants && a.out_type != B200_GGML_F32 && (hs == 64 || hs == 96 || hs == 128) && mul <= kv4::CHUNK_ROWS && chunk > 1 && (long long)chunk * mul >= CHUNK_MIN_ROWS;
     if (!c.use) return c;
     const int len = a.max_len > 0 && a.max_len < kv->view.context ? a.max_len : kv->view.context;
-    c.tokens = kv4::CHUNK_ROWS / mul;
+    // even shares of a chunk, so that where all rows are chunks of that many tokens no CTA has two sequences' positions to run through (three chunks of 111, 42 tokens at most: 21 us, not 31)
+    const int most = kv4::CHUNK_ROWS / mul, shares = (chunk + most - 1) / most;
+    c.tokens = (chunk + shares - 1) / shares;
     const long long units = (long long)((a.n + c.tokens - 1) / c.tokens) * G;
     const long long seen = a.window > 0 && a.window + c.tokens < len ? a.window + c.tokens : len, worth = seen / (8 * kv4::CHUNK_KEYS); // eight tiles of positions a CTA
     long long splits = kv->sms / units;
