@@ -153,8 +153,9 @@ static StepCut step_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, bo
 }
 static size_t parts_bytes(const b200_kv4 *kv, const b200_kv4_attention_args &a, int splits) { return splits > 1 ? (size_t)a.n * a.heads * splits * (kv->head_size + 2) * 4 : 0; }
 
-// Chunks on the tensor cores: 16-bit results, heads of 64, 96 or 128.  A tile takes 128 rows whether they are used or not, single rows read the cache once each: 16 tokens of 4 heads
-// over 8192 positions 38 us there and 47 here, 32 tokens 70 and 49 (heads of 128, 8 key/value heads).
+// Chunks on the tensor cores: 16-bit results, heads of 64, 96 or 128.  A tile takes 128 rows whether they are used or not, single rows read the cache once each.  us as single rows / as a chunk,
+// by rows (tokens x query heads of a key/value head):  32/8 heads of 128, 8192 positions: 32 rows 29/25, 64 rows 53/25, 128 rows 76/27;  1024 positions: 11/21, 17/21, 29/23;
+// 32/8 heads of 64, 8192: 21/23, 33/23, 47/23;  16/16 of 64, 4096: 41/23 (32 rows), 66/23;  8/1 of 128, 8192: 17/25, 17/25, 17/27, 60/27 (512 rows).
 const int CHUNK_MIN_ROWS = 64;
 struct ChunkCut {
     int tokens, splits;
@@ -352,7 +353,7 @@ int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *a, void *str
     if (rc) return rc;
     if (a->heads <= 0 || a->heads % kv->view.kv_heads) return fail(kv, B200_ERR_BAD_ARG, "%d query heads over %d key/value heads", a->heads, kv->view.kv_heads);
     if (!known_type(a->out_type)) return fail(kv, B200_ERR_UNSUPPORTED, "results of type %d (FP32, FP16 and BF16 are known)", a->out_type);
-    if (reinterpret_cast<uintptr_t>(a->workspace) % 4) return fail(kv, B200_ERR_BAD_ARG, "the workspace is not aligned");
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(kv, B200_ERR_BAD_ARG, "the workspace is not aligned");
     if (a->window < 0 || a->max_len < 0 || a->chunk < 0) return fail(kv, B200_ERR_BAD_ARG, "a negative window, length or chunk");
     if (a->n == 0) return B200_OK;
     if (!a->q || !a->out) return fail(kv, B200_ERR_BAD_ARG, "null rows");

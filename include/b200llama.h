@@ -540,7 +540,7 @@ int b200_kv4_append(b200_kv4 *kv, const b200_kv4_append_args *args, void *stream
 /* Causal attention of n query rows over the cache: row r at position p sees the positions j <= p of its slot, the last `window` of them where window > 0; query head h reads key/value
  * head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type.  A row that sees nothing is zeros.  max_len (0: unknown) is the largest position + 1 as far as the host
  * knows, chunk (0 or 1: single steps) how many neighbouring rows are successive tokens of one sequence: both only choose how the work is split.  So does a workspace: few rows over
- * many positions fill the GPU where the call gets b200_kv4_attention_workspace(kv, args) bytes (0: it needs none) of device memory, whose content before and after does not matter
+ * many positions fill the GPU where the call gets b200_kv4_attention_workspace(kv, args) bytes (0: it needs none) of 16-byte aligned device memory, whose content before and after does not matter
  * and which no other call under way may use; NULL or fewer bytes: the call does without. */
 typedef struct b200_kv4_attention_args {
     int32_t n, heads, window, max_len, chunk, out_type;

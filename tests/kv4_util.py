@@ -55,15 +55,13 @@ def attention(q, k, v, d, positions, slots, scale, window):
         lo = max(0, p - window + 1) if window else 0
         if p < 0:
             continue
-        for h in range(H):
-            g = h // (H // G)
-            kk, vv = k[s, lo:p + 1, g], v[s, lo:p + 1, g]
-            x = kk @ q[r, h] * scale
-            w = torch.softmax(x, 0)
-            A = scale * q[r, h].abs().max() * kd[s, lo:p + 1, g].abs().sum(-1).max() * 32 * 16
-            out[r, h] = w @ vv
-            bound[r, h] = (w @ vv.abs()) * (2 * A * (2.0 ** -21 + hs * 2.0 ** -24) + 2.0 ** -16 + 2.0 ** -20 + (p + 1 - lo) * 2.0 ** -24)
-            bound[r, h] += (w @ vd[s, lo:p + 1, g].abs()).repeat_interleave(32) * 16 * ((p + 1 - lo) / 16 + 16) * 2.0 ** -22
+        kk, vv, dk, dv = (t[s, lo:p + 1].transpose(0, 1) for t in (k, v, kd, vd))  # [G, positions, ...]
+        x = q[r].view(G, H // G, hs)
+        w = torch.softmax(x @ kk.transpose(1, 2) * scale, -1)
+        A = scale * x.abs().amax(-1, keepdim=True) * dk.abs().sum(-1).amax(-1)[:, None, None] * 32 * 16
+        out[r] = (w @ vv).view(H, hs)
+        off = (w @ vv.abs()) * (2 * A * (2.0 ** -21 + hs * 2.0 ** -24) + 2.0 ** -16 + 2.0 ** -20 + (p + 1 - lo) * 2.0 ** -24)
+        bound[r] = (off + (w @ dv.abs()).repeat_interleave(32, -1) * 16 * ((p + 1 - lo) / 16 + 16) * 2.0 ** -22).view(H, hs)
     return out, bound
 
 
@@ -80,13 +78,12 @@ def chunk_bound(q, k, v, positions, slots, scale, window, want, dtype):
         lo = max(0, p - window + 1) if window else 0
         if p < 0:
             continue
-        for h in range(H):
-            g = h // (H // G)
-            kk, vv = k[s, lo:p + 1, g], v[s, lo:p + 1, g].abs()
-            w = torch.softmax(kk @ q[r, h] * scale, 0)
-            A = (kk.abs() @ q[r, h].abs()).max() * abs(scale)
-            m = p + 1 - lo
-            bound[r, h] = (w @ vv) * (2 * A * (2.0 ** -10 + hs * 2.0 ** -22) + 2 * 2.0 ** -11 + m * 2.0 ** -22 + 2.0 ** -20) + m * 2.0 ** -25 * vv.max()
+        kk, vv = k[s, lo:p + 1].transpose(0, 1), v[s, lo:p + 1].transpose(0, 1).abs()  # [G, positions, hs]
+        x, m = q[r].view(G, H // G, hs), p + 1 - lo
+        w = torch.softmax(x @ kk.transpose(1, 2) * scale, -1)
+        A = (x.abs() @ kk.abs().transpose(1, 2)).amax(-1, keepdim=True) * abs(scale)
+        off = (w @ vv) * (2 * A * (2.0 ** -10 + hs * 2.0 ** -22) + 2 * 2.0 ** -11 + m * 2.0 ** -22 + 2.0 ** -20) + m * 2.0 ** -25 * vv.flatten(1).amax(-1)[:, None, None]
+        bound[r] = off.view(H, hs)
     return bound + want.abs() * half_step(dtype) + 2.0 ** -25
 
 

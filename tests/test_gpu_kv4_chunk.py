@@ -159,3 +159,48 @@ def test_a_prompt_in_chunks_then_steps(pkg):
     d = U.quantize(x)[1], U.quantize(v)[1]
     assert (kk[0] - x).abs().max() <= d[0].abs().max() * 1.01  # a step of the cache at most
     check(torch.cat(outs), torch.cat(turned), kk, vv, [s[None] for s in d], every, torch.zeros_like(every), U.rsqrt(hs), 0, F16)
+
+
+@pytest.mark.parametrize("window", [0, 150])
+def test_scores_beyond_single_precision_exponentials(pkg, window):
+    """Exact scores, thousands apart and up to 2^23: every row is the value at its largest one, wherever that stands.  (A score and the maximum that round apart would lose it.)
+    The value is an FP16 operand and the result FP16: half a step each."""
+    H, G, hs, context, n = 4, 1, 64, 500, 100
+    g = gen(12)
+    cache = pkg.KV4Cache(1, context, G, hs)
+    order = torch.randperm(context, device="cuda", generator=g)
+    k = torch.zeros(context, G, hs, device="cuda")
+    k[:, 0, 0] = -(order + 1.0)  # the largest entry of its group: stored exactly
+    at = torch.arange(context, device="cuda", dtype=torch.int32)
+    cache.append(k, rand(g, context, G, hs), at)
+    kk, vv = cache.read(at)
+    assert torch.equal(kk, k)
+    q = torch.zeros(n, H, hs, device="cuda")
+    q[:, :, 0] = -16384.0
+    pos = at[context - n:]
+    got = cache.attention(q, pos, window=window, scale=1.0, chunk=n, dtype=F16)
+    for r, p in enumerate(pos.tolist()):
+        lo = max(0, p - window + 1) if window else 0
+        want = vv[lo + int(order[lo:p + 1].argmax()), 0].double()
+        assert ((got[r].double() - want).abs() <= want.abs() * 2 * U.half_step(F16) + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("context", [1, 16, 128, 129, 256, 257, 385])
+def test_few_tiles(pkg, context):
+    """One tile, two, three: a stream of tiles without work, or with one tile fewer than the other; all tokens at the same position, some of them twice."""
+    H, G, hs, n = 4, 2, 96, 40
+    cache, k, v, d = filled(pkg, 1, context, G, hs, context)
+    q = rand(gen(context), n, H, hs)
+    pos = torch.full((n,), context - 1, device="cuda", dtype=torch.int32)
+    pos[::3] = 0
+    check(cache.attention(q, pos, chunk=n, max_len=context, dtype=BF16), q, k, v, d, pos, torch.zeros_like(pos), U.rsqrt(hs), 0, BF16)
+
+
+def test_a_crooked_workspace_is_refused(pkg):
+    lib, raw, err = pkg.native.lib(), C.c_void_p(), C.create_string_buffer(256)
+    assert lib.b200_kv4_create(1, 64, 1, 64, 0, C.byref(raw), err, 256) == 0
+    x = torch.zeros(64, 64, device="cuda")
+    a = pkg.native.KV4Attention()
+    a.n, a.heads, a.chunk, a.q_stride, a.out_stride, a.q, a.out, a.workspace = 64, 1, 64, 64, 64, x.data_ptr(), x.data_ptr(), x.data_ptr() + 8
+    assert lib.b200_kv4_attention(raw, C.byref(a), None) == -1
+    lib.b200_kv4_free(raw)
