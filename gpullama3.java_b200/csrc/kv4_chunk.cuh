@@ -7,9 +7,10 @@
 // A tile's work is a chain: scores, exponentials, product, about 5000 cycles of which 1024 are the tensor cores' and 1024 the exponentials' (16 a cycle).  So even and odd tiles are two
 // streams with accumulators, maxima and sums of their own, each of eight warps, which the end joins: while one waits for its products the other computes.  Heads of 128, two streams of
 // scores and results: all 512 columns of TMEM.
-// Measured (512 tokens, 32 heads over 8 of 128, 8192 positions: 66.6 GFLOP): 107 us, 620 TFLOP/s, 37 % of the 1690 measured.  What bounds it is that chain and the issue slots it shares with
-// the conversion.  One stream with two S and a maximum agreed on by a row's threads in every tile took 116-123 us; 256 rows a CTA with half the conversions 133 us (two blocks of rows in
-// place of the two streams; 64 pairs of CTAs whose parts had to be joined).
+// Measured (512 tokens, 32 heads over 8 of 128, 8192 positions: 66.6 GFLOP): 102 us (99-109 from box to box), 650 TFLOP/s, 39 % of the 1690 measured.  A tile takes 2300 cycles: its 16
+// products 1400 (1024 were nothing else at shared memory), beside them the conversion of its records, one a warp, 2400 with what it waits for; 0.57 instructions a cycle and scheduler.
+// One stream with two S and a maximum agreed on by a row's threads in every tile took 116-123 us; 256 rows a CTA with half the conversions 133 us (two blocks of rows in place of the two
+// streams; 64 pairs of CTAs whose parts had to be joined).
 // Rounding: queries (times a power of two), keys, values and probabilities are FP16 operands, sums are FP32.  A value's NaN, or one outside FP16, is moved into its key, so that it
 // reaches the rows that see the position and no other (0 * NaN in the product would reach them all).
 //
