@@ -90,7 +90,6 @@ cudaError_t launch(void (*kern)(KA...), unsigned grid, int block, size_t smem, i
 // by device or by thread (0.2 us).
 template <typename K> cudaError_t prepare(K kern, size_t smem, int cluster) {
     cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
-    if (e == cudaSuccess && cluster > 8) e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     return e;
 }
 int sm_count(int device) {
