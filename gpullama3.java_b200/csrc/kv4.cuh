@@ -254,6 +254,7 @@ struct Step {
     int8_t *quants; // out_type KV4_OUT_Q8: blocks of 32
     float *scales;
     float *work; // parts of units that several clusters share
+    int by_length; // rows with the most positions first (at most STEP_ORDERED of them)
 };
 
 __device__ __forceinline__ float ex2(float x) { // 2^x
@@ -337,6 +338,36 @@ __device__ __forceinline__ void put_result(const Step &a, int row, size_t at, fl
     else put((bf16 *)a.out + row * a.ldo + at, v);
 }
 
+// The row of a rank in the order of visible positions, most first and equal ones by index, so that the long rows of a batch do not start behind the short ones: a CTA ranks all rows, a row a
+// thread.  us without / with it, 8 heads of 128 and of 64 up to 4096 positions: rows of any lengths 16: 26/23, 17/18, 24: 26/23, 19/15, 48: 43/35, 30/24; of one length (nothing to gain)
+// 29/29, 19/19, 35/37, 21/21, 56/57, 35/35.  More rows cost more than they gain (96 rows of 2048 at most: 45/42, 27/25 and 60/65, 37/39; 200: 76/90, 45/60).
+constexpr int STEP_ORDERED = 64;
+__device__ __forceinline__ int row_by_length(const Step &a, int rank, int *lengths) { // lengths: 16-byte aligned, STEP_ORDERED + 1
+    const int t = threadIdx.x;
+    int length = -1;
+    if (t < a.rows.n) {
+        const int pos = a.rows.position(t), slot = a.rows.slot_of(t);
+        int lo, hi;
+        visible(pos, a.window, lo, hi);
+        length = slot < 0 || slot >= a.kv.slots || pos >= a.kv.context || hi < lo ? 0 : hi - lo; // (padding: none)
+    }
+    if (t < STEP_ORDERED) lengths[t] = length;
+    __syncthreads();
+    if (t < a.rows.n) {
+        int r = 0;
+        for (int j = 0; j < a.rows.n; j += 4) {
+            const int4 o = *reinterpret_cast<const int4 *>(lengths + j);
+            r += (o.x > length || (o.x == length && j < t)) + (o.y > length || (o.y == length && j + 1 < t)) + (o.z > length || (o.z == length && j + 2 < t)) +
+                 (o.w > length || (o.w == length && j + 3 < t));
+        }
+        if (r == rank) lengths[STEP_ORDERED] = t;
+    }
+    __syncthreads();
+    const int row = __shfl_sync(0xffffffffu, lengths[STEP_ORDERED], 0);
+    __syncthreads(); // (the memory is the ring's)
+    return row;
+}
+
 // One query row and up to 4 NT query heads of a key/value head: the row's visible positions are split over the warps of a cluster of CTAs, each warp runs through its records
 // (cp.async ring of its own, no barrier in the loop) with its own running maximum, and the parts are joined in shared memory, then over the cluster.  Where 8 CTAs a unit leave SMs
 // idle, `splits` clusters share a unit: their parts go to the workspace, and k_step_join joins them.  Nothing depends on an order of arrival.
@@ -352,8 +383,10 @@ template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_s
     cg::cluster_group cluster = cg::this_cluster();
     const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
     const int G = a.kv.kv_heads, mul = a.heads / G;
-    const int split = blockIdx.x / ranks % splits, unit = blockIdx.x / ranks / splits, row = unit / (G * units_per_head), kvh = unit / units_per_head % G;
+    const int split = blockIdx.x / ranks % splits, unit = blockIdx.x / ranks / splits, kvh = unit / units_per_head % G;
     const int first = unit % units_per_head * H; // first head within the group
+    int row = unit / (G * units_per_head);
+    if (a.by_length) row = row_by_length(a, row, reinterpret_cast<int *>(smem));
     const int pos = a.rows.position(row), slot = a.rows.slot_of(row);
     if (slot < 0 || slot >= a.kv.slots || pos >= a.kv.context) return; // a padding row (the whole cluster leaves)
     int lo, hi;

@@ -147,7 +147,7 @@ static StepCut step_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, bo
     int most = (seen + group - 1) / group;
     if (most > kv4::STEP_MAX_CLUSTER) most = kv4::STEP_MAX_CLUSTER;
     if (quants && most > c.heads * hs / 32) most = c.heads * hs / 32; // whole blocks of 32 quants a CTA
-    c.cluster = cluster_for(units, 8 * kv->sms, most);
+    c.cluster = cluster_for(units, 4 * kv->sms, most); // (more CTAs cost more in front and behind than they spread: 16 rows of 8 heads of 128 over 4096 positions 29 us, with twice as many 39)
     return c;
 }
 static size_t parts_bytes(const b200_kv4 *kv, const b200_kv4_attention_args &a, int splits) { return splits > 1 ? (size_t)a.n * a.heads * splits * (kv->head_size + 2) * 4 : 0; }
@@ -190,6 +190,7 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
     k.scale = a.scale;
     k.out = a.out; k.quants = quants; k.scales = scales;
     k.work = a.workspace;
+    k.by_length = 0;
     const auto has_room = [&](int splits) { return a.workspace && parts_bytes(kv, a, splits) <= a.workspace_bytes; };
     const auto join = [&](auto hs, int splits) {
         constexpr int per_cta = hs < 64 ? 64 / hs : 1;
@@ -220,6 +221,7 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
         auto go = [&](auto nt) {
             constexpr size_t smem = kv4::step_smem_bytes(hs, 4 * nt);
             const unsigned grid = (unsigned)a.n * kv->view.kv_heads * c.per_head * c.splits * c.cluster;
+            k.by_length = a.positions && a.n > 1 && a.n <= kv4::STEP_ORDERED && grid > 2u * kv->sms;
             auto kern = kv4::k_step<hs, nt>;
             cudaError_t e = prepare(kern, smem, c.cluster);
             if (e == cudaSuccess) e = launch(kern, grid, kv4::STEP_WARPS * 32, smem, c.cluster, pdl, stream, k, c.per_head, c.splits);

@@ -358,3 +358,25 @@ def test_refusals(pkg):
     a.window, a.heads = 0, 3
     assert L.b200_kv4_attention(raw, C.byref(a), None) == -1 and b"heads" in L.b200_kv4_last_error(raw)
     L.b200_kv4_free(raw)
+
+
+@pytest.mark.parametrize("H,G,hs,n", [(16, 8, 64, 64), (32, 16, 128, 40), (16, 8, 32, 63)])
+def test_batches_in_the_order_of_their_lengths(pkg, H, G, hs, n):
+    """Enough rows for the order by length: equal lengths, padding, rows that see nothing, a window that makes most rows alike; the bits of every row are those it has alone in its batch's cut."""
+    slots, context = 5, 300
+    cache, k, v, d = filled(pkg, slots, context, G, hs, n)
+    g = gen(n)
+    q = rand(g, n, H, hs)
+    pos, at = torch.randint(-3, context, (n,), device="cuda", generator=g, dtype=torch.int32), (torch.arange(n, device="cuda") % slots).int()
+    pos[::7], pos[5], at[6] = 200, context, slots
+    for window in (0, 31):
+        out = torch.full((n, H, hs), 9.0, device="cuda")
+        cache.attention(q, pos, slots=at, window=window, out=out)
+        padding = (at >= slots) | (pos >= context)
+        assert (out[padding] == 9).all() and (out[(pos < 0) & ~padding] == 0).all()
+        live = ~padding
+        want, bound = U.attention(q[live].double().cpu(), k, v, d, pos[live].cpu(), at[live].cpu(), U.rsqrt(hs), window)
+        assert ((out[live].double().cpu() - want).abs() <= bound + want.abs() * U.half_step(F32)).all()
+        turned = torch.arange(n - 1, -1, -1, device="cuda")
+        again = cache.attention(q[turned], pos[turned], slots=at[turned], window=window)
+        assert torch.equal(again[turned][live], out[live])
