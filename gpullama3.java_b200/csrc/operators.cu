@@ -146,8 +146,9 @@ static StepCut step_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, bo
     if (c.splits > kv4::STEP_MAX_SPLITS) c.splits = kv4::STEP_MAX_SPLITS;
     int most = (seen + group - 1) / group;
     if (most > kv4::STEP_MAX_CLUSTER) most = kv4::STEP_MAX_CLUSTER;
-    if (quants && most > c.heads * hs / 32) most = c.heads * hs / 32; // whole blocks of 32 quants a CTA
     c.cluster = cluster_for(units, 4 * kv->sms, most); // (more CTAs cost more in front and behind than they spread: 16 rows of 8 heads of 128 over 4096 positions 29 us, with twice as many 39)
+    // whole blocks of 32 quants a CTA: heads of 96 in units of four are 12 blocks, of which 8 CTAs would have one and a half each
+    while (quants && c.heads * hs / c.cluster % 32) c.cluster /= 2;
     return c;
 }
 static size_t parts_bytes(const b200_kv4 *kv, const b200_kv4_attention_args &a, int splits) { return splits > 1 ? (size_t)a.n * a.heads * splits * (kv->head_size + 2) * 4 : 0; }
@@ -394,6 +395,20 @@ int b200_kv4_read(b200_kv4 *kv, const b200_kv4_read_args *a, void *stream) {
             });
         });
     return e == cudaSuccess ? B200_OK : fail(kv, cuda_code(e), "%s", cudaGetErrorString(e));
+}
+
+int b200_test_kv4_step_cut(int32_t head_size, int32_t kv_heads, int32_t heads, int32_t n, int32_t context, int32_t max_len, int32_t window, int32_t sms, int32_t quants, int32_t *cut) {
+    if (!cut || head_size <= 0 || head_size % 32 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || n <= 0 || context <= 0 || max_len < 0 || window < 0 || sms <= 0) return B200_ERR_BAD_ARG;
+    b200_kv4 kv;
+    kv.head_size = head_size;
+    kv.sms = sms;
+    kv.view.context = context;
+    kv.view.kv_heads = kv_heads;
+    b200_kv4_attention_args a = {};
+    a.n = n; a.heads = heads; a.max_len = max_len; a.window = window;
+    const StepCut c = step_cut(&kv, a, quants != 0);
+    cut[0] = c.heads; cut[1] = c.per_head; cut[2] = c.cluster; cut[3] = c.splits;
+    return B200_OK;
 }
 
 int b200_log_probs(const b200_log_probs_args *a, void *stream, char *err, size_t err_len) {

@@ -565,6 +565,10 @@ typedef struct b200_kv4_read_args {
 } b200_kv4_read_args;
 int b200_kv4_read(b200_kv4 *kv, const b200_kv4_read_args *args, void *stream);
 
+/* Test hook (host only): how attention of n single rows is cut on a GPU of `sms` SMs: cut[4] = {query heads of a unit, units of a row and key/value head, CTAs of a cluster, clusters of
+ * a unit}; quants: with results in blocks of 32 quants, as Q8_0 plans take them. */
+int b200_test_kv4_step_cut(int32_t head_size, int32_t kv_heads, int32_t heads, int32_t n, int32_t context, int32_t max_len, int32_t window, int32_t sms, int32_t quants, int32_t *cut);
+
 /* Of every row of logits ([rows][vocab], `type` B200_GGML_F32, _F16 or _BF16, row_stride entries apart): the log probability of token targets[row] (logprobs; 0 where the target lies
  * outside the vocabulary, as for "no target", or where targets is NULL), the entropy of the distribution in nats, and the `top` (0 .. 32, at most vocab) most likely tokens with their
  * log probabilities, in order, equal ones by index (top_ids, top_logprobs [rows][top]).  Every output may be NULL.  A row with a NaN, with an infinite logit or with none above -inf has
