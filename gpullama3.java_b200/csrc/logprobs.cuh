@@ -49,6 +49,14 @@ __device__ __forceinline__ float ex2(float x) { // 2^x
     return y;
 }
 
+// (a - ref) LOG2E of two entries in two instructions
+__device__ __forceinline__ float2 scaled(float a, float b, float ref) {
+    float2 y;
+    asm("{.reg .b64 x, r, l; mov.b64 x, {%2, %3}; mov.b64 r, {%4, %4}; mov.b64 l, {%5, %5}; add.rn.f32x2 x, x, r; mul.rn.f32x2 x, x, l; mov.b64 {%0, %1}, x;}"
+        : "=f"(y.x), "=f"(y.y) : "f"(a), "f"(b), "f"(-ref), "f"(LOG2E));
+    return y;
+}
+
 struct Sum { // of a set of entries: its largest, and what the others add (s in units of log2)
     float m, z, s;
 };
@@ -57,8 +65,8 @@ __device__ __forceinline__ Sum join(const Sum &p, const Sum &q) {
     const Sum &a = first ? p : q, &b = first ? q : p;
     const float d = (b.m - a.m) * LOG2E; // (-inf where a set is empty; NaN where both are)
     Sum r = a;
-    if (d > -CUDART_INF_F) {
-        const float e = ex2(d);
+    const float e = d > -CUDART_INF_F ? ex2(d) : 0.0f;
+    if (e > 0.0f) { // (else b adds nothing, and d (1 + b.z) may pass FP32's range)
         r.z = fmaf(1.0f + b.z, e, a.z);
         r.s = fmaf(fmaf(d, 1.0f + b.z, b.s), e, a.s);
     }
@@ -126,7 +134,7 @@ __device__ __forceinline__ void select(Smem &sm, int total, int n) {
 // A cluster of CTAs reads a row, each a stretch of it in batches of 16 entries a thread, the next batch under way while one is worked on.  A warp keeps the largest entry it has met and
 // a thread the sum of its own entries in units of that; candidates for the alternatives are the entries above a threshold that at least `top` known ones reach, so that after the first
 // batch hardly any is looked at twice.  Bytes are its floor: 512 rows of 128256 FP32 logits are 263 MB, 41 us; with
-// 20 alternatives it takes 74 (3.6 TB/s), of which a CTA's selections are the part above a plain pass.  One such row with 5: 16 us, a cluster of 8, latency.
+// 20 alternatives it takes 75 (3.5 TB/s), of which a CTA's selections are the part above a plain pass.  One such row with 5: 16 us, a cluster of 8, latency.
 template <typename T> __global__ void __launch_bounds__(THREADS, 4) k_log_probs(const Args a) {
     constexpr int VEC = Load<T>::VEC;
     __shared__ Smem sm;
@@ -183,21 +191,28 @@ template <typename T> __global__ void __launch_bounds__(THREADS, 4) k_log_probs(
                 for (int i = PER_THREAD - 1; i >= 0; i--)
                     if (v[i] == widest) skip = i;
         }
-        const float ref = m == -CUDART_INF_F ? 0.0f : -m * LOG2E;
+        // x - m first: it is exact near m, so that neither a row's offset (with m LOG2E rounded, 2^-24 of that) nor a mask of the type's lowest value, whose m LOG2E overflows, is in y
+        const float ref = m == -CUDART_INF_F ? 0.0f : m;
         float zs[2] = {0.0f, 0.0f}, ss[2] = {0.0f, 0.0f};
         if (__any_sync(0xffffffffu, skip < PER_THREAD)) {
 #pragma unroll
-            for (int i = 0; i < PER_THREAD; i++) {
-                const float y = fmaf(v[i], LOG2E, ref), e = i == skip ? 0.0f : ex2(y);
-                zs[i & 1] += e;
-                ss[i & 1] = fmaf(fmaxf(y, -1000.0f), e, ss[i & 1]); // (-inf times 0 is none)
+            for (int i = 0; i < PER_THREAD; i += 2) {
+                const float2 y = scaled(v[i], v[i + 1], ref);
+                const float e0 = i == skip ? 0.0f : ex2(y.x), e1 = i + 1 == skip ? 0.0f : ex2(y.y);
+                zs[0] += e0;
+                zs[1] += e1;
+                ss[0] = fmaf(fmaxf(y.x, -1000.0f), e0, ss[0]); // (-inf times 0 is none)
+                ss[1] = fmaf(fmaxf(y.y, -1000.0f), e1, ss[1]);
             }
         } else
 #pragma unroll
-            for (int i = 0; i < PER_THREAD; i++) {
-                const float y = fmaf(v[i], LOG2E, ref), e = ex2(y);
-                zs[i & 1] += e;
-                ss[i & 1] = fmaf(fmaxf(y, -1000.0f), e, ss[i & 1]);
+            for (int i = 0; i < PER_THREAD; i += 2) {
+                const float2 y = scaled(v[i], v[i + 1], ref);
+                const float e0 = ex2(y.x), e1 = ex2(y.y);
+                zs[0] += e0;
+                zs[1] += e1;
+                ss[0] = fmaf(fmaxf(y.x, -1000.0f), e0, ss[0]);
+                ss[1] = fmaf(fmaxf(y.y, -1000.0f), e1, ss[1]);
             }
         z += zs[0] + zs[1];
         s += ss[0] + ss[1];
