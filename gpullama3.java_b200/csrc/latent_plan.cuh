@@ -136,7 +136,7 @@ static int ly_latent_mixer_upload(b200_plan *p, int l, LyLayer &L, const b200_te
     const std::string mx = "l" + std::to_string(l) + ".mix.";
     int rc;
     if ((rc = dalloc(p, &L.w_proj, (size_t)L.P * E * 2))) return rc;
-    if (L.P > L.Pn) CK(cudaMemset(L.w_proj + (size_t)L.Pn * E, 0, (size_t)(L.P - L.Pn) * E * 2));
+    if (L.P > L.Pn) CK(zeros(p, L.w_proj + (size_t)L.Pn * E, (size_t)(L.P - L.Pn) * E * 2));
     if ((rc = ly_mat(p, tensors, nt, mx + (s.q_rank > 0 ? "dq" : "q"), L.qd, E, L.w_proj, 0))) return rc;
     if (s.q_rank > 0) {
         if ((rc = ly_vec_f32(p, tensors, nt, mx + "dq.norm", s.q_rank, &L.qnorm))) return rc;

@@ -966,7 +966,7 @@ static int ly_build(b200_plan *p, const b200_layered_config *cfg, const b200_lay
             if ((rc = ly_sandwich_mixer_upload(p, l, L, tensors, nt))) return rc;
         } else {
         if ((rc = dalloc(p, &L.w_proj, (size_t)L.P * E * 2))) return rc;
-        if (L.P > L.Pn) CK(cudaMemset(L.w_proj + (size_t)L.Pn * E, 0, (size_t)(L.P - L.Pn) * E * 2));
+        if (L.P > L.Pn) CK(zeros(p, L.w_proj + (size_t)L.Pn * E, (size_t)(L.P - L.Pn) * E * 2));
         if ((rc = ly_mat(p, tensors, nt, mx + "q", L.qd, E, L.w_proj, 0))) return rc;
         if ((rc = ly_mat(p, tensors, nt, mx + "k", L.kd, E, L.w_proj, L.qd))) return rc;
         if (L.pv > 0 && (rc = ly_mat(p, tensors, nt, mx + "v", L.pv, E, L.w_proj, L.qd + L.kd))) return rc;
@@ -1062,17 +1062,17 @@ static int ly_build(b200_plan *p, const b200_layered_config *cfg, const b200_lay
             R.kw = L.kw;
             if (L.s.kv_from >= 0) { R.own = false; R.kc = Y.runs[L.s.kv_from].kc; R.kc16 = Y.runs[L.s.kv_from].kc16; continue; }
             if ((rc = dalloc(p, &R.kc, (size_t)Y.ring * L.kw * 4))) return rc;
-            CK(cudaMemset(R.kc, 0, (size_t)Y.ring * L.kw * 4));
+            CK(zeros(p, R.kc, (size_t)Y.ring * L.kw * 4));
             if (Y.maxKX > 0) { // BF16 twin rows: the A operand of the per-chunk key / value expansion
                 if ((rc = dalloc(p, &R.kc16, (size_t)Y.ring * L.kw * 2))) return rc;
-                CK(cudaMemset(R.kc16, 0, (size_t)Y.ring * L.kw * 2));
+                CK(zeros(p, R.kc16, (size_t)Y.ring * L.kw * 2));
             }
             continue;
         }
         if (L.s.mixer == B200_MIXER_MLSTM) { // the run's matrix memory, normaliser and running maximum
             R.s_floats = ly::mlstm_state_floats(L.s.heads, L.s.key_dim, L.s.value_dim);
             if ((rc = dalloc(p, &R.S, R.s_floats * 4))) return rc;
-            CK(cudaMemset(R.S, 0, R.s_floats * 4));
+            CK(zeros(p, R.S, R.s_floats * 4));
             continue;
         }
         if (L.s.mixer == B200_MIXER_GATED_DELTA) {
@@ -1081,8 +1081,8 @@ static int ly_build(b200_plan *p, const b200_layered_config *cfg, const b200_lay
             R.s_floats = sb / 4; R.c_floats = cb / 4;
             if ((rc = dalloc(p, &R.S, sb))) return rc;
             if ((rc = dalloc(p, &R.cstate, cb))) return rc;
-            CK(cudaMemset(R.S, 0, sb));
-            CK(cudaMemset(R.cstate, 0, cb));
+            CK(zeros(p, R.S, sb));
+            CK(zeros(p, R.cstate, cb));
             continue;
         }
         if (L.s.mixer == B200_MIXER_LIGHTNING || L.s.mixer == B200_MIXER_ATTENTION_SCAN) {
@@ -1092,14 +1092,14 @@ static int ly_build(b200_plan *p, const b200_layered_config *cfg, const b200_lay
         R.kw = L.kd; R.vw = L.vd;
         if ((rc = dalloc(p, &R.kc, (size_t)Y.ring * L.kd * 4))) return rc;
         if ((rc = dalloc(p, &R.vc, (size_t)Y.ring * L.vd * 4))) return rc;
-        CK(cudaMemset(R.kc, 0, (size_t)Y.ring * L.kd * 4));
-        CK(cudaMemset(R.vc, 0, (size_t)Y.ring * L.vd * 4));
+        CK(zeros(p, R.kc, (size_t)Y.ring * L.kd * 4));
+        CK(zeros(p, R.vc, (size_t)Y.ring * L.vd * 4));
         // tensor-core prefill attention: BF16 plans, key and value sizes of an instance, a window up to the limit
         if (!Y.f32 && Y.att_mma && Y.cap > 1 && ly_mma_fits(Y, L.mixprep ? L.dk_eff : L.s.key_dim, L.s.value_dim, L.s.window) && Y.maxP % 4 == 0 && L.gd % 2 == 0) {
             if ((rc = dalloc(p, &R.kc16, (size_t)Y.ring * L.kd * 2))) return rc;
             if ((rc = dalloc(p, &R.vc16, (size_t)Y.ring * L.vd * 2))) return rc;
-            CK(cudaMemset(R.kc16, 0, (size_t)Y.ring * L.kd * 2));
-            CK(cudaMemset(R.vc16, 0, (size_t)Y.ring * L.vd * 2));
+            CK(zeros(p, R.kc16, (size_t)Y.ring * L.kd * 2));
+            CK(zeros(p, R.vc16, (size_t)Y.ring * L.vd * 2));
         }
     }
     // activations
@@ -1198,8 +1198,8 @@ static int ly_build(b200_plan *p, const b200_layered_config *cfg, const b200_lay
                 if ((rc = dalloc(p, &Y.slot_row, cap * slots * 4))) return rc;
                 if ((rc = dalloc(p, &Y.tile_group128, (size_t)Y.max_tiles128 * 4))) return rc;
             }
-            CK(cudaMemset(Y.moe_ids, 0, cap * slots * 4));
-            CK(cudaMemset(Y.moe_wts, 0, cap * slots * 4));
+            CK(zeros(p, Y.moe_ids, cap * slots * 4));
+            CK(zeros(p, Y.moe_wts, cap * slots * 4));
         }
     }
     if ((rc = dalloc(p, &Y.LOG, (size_t)(Y.f32 ? Y.logit_rows : 256) * c.vocab_size * 4))) return rc;
@@ -1216,11 +1216,11 @@ static int ly_build(b200_plan *p, const b200_layered_config *cfg, const b200_lay
             if ((rc = dalloc(p, &Y.split.o, (size_t)maxH * Y.max_splits * maxdv * 4))) return rc;
             if ((rc = dalloc(p, &Y.split.ml, (size_t)maxH * Y.max_splits * 2 * 4))) return rc;
             if ((rc = dalloc(p, &Y.split.count, (size_t)maxH * 4))) return rc;
-            CK(cudaMemset(Y.split.count, 0, (size_t)maxH * 4));
+            CK(zeros(p, Y.split.count, (size_t)maxH * 4));
         }
     }
     if ((rc = dalloc(p, &Y.st_pf, sizeof(StepState)))) return rc;
-    CK(cudaMemset(Y.st_pf, 0, sizeof(StepState)));
+    CK(zeros(p, Y.st_pf, sizeof(StepState)));
     // what the shared single-token entry points use
     if ((rc = logits_alloc(p, c.vocab_size))) return rc;
     if ((rc = dalloc(p, &p->smp_indices, (size_t)c.vocab_size * 4))) return rc;
@@ -1229,15 +1229,15 @@ static int ly_build(b200_plan *p, const b200_layered_config *cfg, const b200_lay
     if ((rc = dalloc(p, &p->st, sizeof(StepState)))) return rc;
     if ((rc = dalloc(p, &p->seq_tokens, (size_t)p->seq_cap * 4))) return rc;
     if ((rc = dalloc(p, &p->out_ids, (size_t)p->seq_cap * 4))) return rc;
-    CK(cudaMemset(p->st, 0, sizeof(StepState)));
-    CK(cudaMemset(p->seq_tokens, 0, (size_t)p->seq_cap * 4));
+    CK(zeros(p, p->st, sizeof(StepState)));
+    CK(zeros(p, p->seq_tokens, (size_t)p->seq_cap * 4));
     CK(cudaMallocHost(&p->h_st, sizeof(StepState)));
     CK(cudaMallocHost(&p->h_ids, (size_t)p->seq_cap * 4));
     p->x = Y.X;
     if (!Y.f32 && (rc = ly_tc_init(p))) return rc;
     if ((rc = ly_capture(p, true, &p->g_decode, &p->launches_decode))) return rc;
     if ((rc = ly_capture(p, false, &p->g_prefill, nullptr))) return rc;
-    CK(cudaStreamSynchronize(p->stream));
+    CK(copies_arrived(p));
     return B200_OK;
 }
 

@@ -66,7 +66,7 @@ static int ly_layernorm_embedding(b200_plan *p, const b200_tensor *tensors, int 
         if ((rc = ly_mat(p, tensors, nt, "bigram", c.bigram_buckets + 1, E, Y.bigram, 0))) return rc;
         const size_t hist = (size_t)c.context_length + Y.cap;
         if ((rc = dalloc(p, &Y.tok_hist, hist * 4))) return rc;
-        CK(cudaMemset(Y.tok_hist, 0, hist * 4));
+        CK(zeros(p, Y.tok_hist, hist * 4));
     }
     if (c.sinusoid) {
         std::vector<double> f((size_t)(E + 1) / 2);
@@ -89,7 +89,7 @@ static int ly_layernorm_upload(b200_plan *p, int l, LyLayer &L, const b200_tenso
         if ((rc = ly_latent_mixer_upload(p, l, L, tensors, nt))) return rc;
     } else {
         if ((rc = dalloc(p, &L.w_proj, (size_t)L.P * E * 2))) return rc;
-        if (L.P > L.Pn) CK(cudaMemset(L.w_proj + (size_t)L.Pn * E, 0, (size_t)(L.P - L.Pn) * E * 2));
+        if (L.P > L.Pn) CK(zeros(p, L.w_proj + (size_t)L.Pn * E, (size_t)(L.P - L.Pn) * E * 2));
         const char *nm[6] = {"q", "k", "v", "g", "i", "f"};
         const int rows[6] = {L.qd, L.kd, L.vd, L.gr, s.heads, s.heads};
         for (int k = 0, off = 0; k < 6; off += rows[k++])

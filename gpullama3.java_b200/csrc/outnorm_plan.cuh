@@ -123,7 +123,7 @@ static int ly_outnorm_upload(b200_plan *p, int l, LyLayer &L, const b200_tensor 
     if (Y.c.token_shift && (rc = ly_vec_f32(p, tensors, nt, pre + "shift", E, &L.shift))) return rc;
     if (Y.c.depth_average && (rc = ly_vec_f32(p, tensors, nt, pre + "dwa", l + 2, &L.dwa))) return rc;
     if ((rc = dalloc(p, &L.w_proj, (size_t)L.P * E * 2))) return rc;
-    if (L.P > L.Pn) CK(cudaMemset(L.w_proj + (size_t)L.Pn * E, 0, (size_t)(L.P - L.Pn) * E * 2));
+    if (L.P > L.Pn) CK(zeros(p, L.w_proj + (size_t)L.Pn * E, (size_t)(L.P - L.Pn) * E * 2));
     if (s.mixer == B200_MIXER_WINDOW_ATTENTION) {
         if ((rc = ly_mat(p, tensors, nt, mx + "q", L.qd, E, L.w_proj, 0))) return rc;
         if ((rc = ly_vec_f32(p, tensors, nt, mx + "q.norm", s.key_dim, &L.qnorm, s.qk_head_norm != 0))) return rc;
@@ -199,7 +199,7 @@ static int ly_outnorm_upload(b200_plan *p, int l, LyLayer &L, const b200_tensor 
     // mixture of experts: router rows [experts | identity experts | gate of the shared expert], stacked expert matrices
     const int F = s.ff_dim, X = s.ff_experts, XI = X + s.moe_identity, SF = s.moe_shared_ff;
     if ((rc = dalloc(p, &L.w_router, (size_t)(XI + 1) * E * 2))) return rc;
-    CK(cudaMemset(L.w_router + (size_t)XI * E, 0, (size_t)E * 2));
+    CK(zeros(p, L.w_router + (size_t)XI * E, (size_t)E * 2));
     if ((rc = ly_mat(p, tensors, nt, ff + "router", XI, E, L.w_router, 0))) return rc;
     if ((rc = ly_vec_f32(p, tensors, nt, ff + "correction", XI, &L.correction))) return rc;
     if (X > 0) {
@@ -231,7 +231,7 @@ static int ly_outnorm_run(b200_plan *p, LyRun &R, const LyLayer &L) {
     int rc;
     if (Y.c.token_shift) {
         if ((rc = dalloc(p, &R.prev, (size_t)Y.c.width * 4))) return rc;
-        CK(cudaMemset(R.prev, 0, (size_t)Y.c.width * 4));
+        CK(zeros(p, R.prev, (size_t)Y.c.width * 4));
     }
     if (s.mixer == B200_MIXER_WINDOW_ATTENTION) {
         R.kw = L.kd; R.vw = L.vd;
@@ -241,20 +241,20 @@ static int ly_outnorm_run(b200_plan *p, LyRun &R, const LyLayer &L) {
             return B200_OK;
         }
         if ((rc = dalloc(p, &R.kc, (size_t)Y.ring * L.kd * 4)) || (rc = dalloc(p, &R.vc, (size_t)Y.ring * L.vd * 4))) return rc;
-        CK(cudaMemset(R.kc, 0, (size_t)Y.ring * L.kd * 4));
-        CK(cudaMemset(R.vc, 0, (size_t)Y.ring * L.vd * 4));
+        CK(zeros(p, R.kc, (size_t)Y.ring * L.kd * 4));
+        CK(zeros(p, R.vc, (size_t)Y.ring * L.vd * 4));
         if (!Y.f32 && Y.att_mma && Y.cap > 1 && ly_mma_fits(Y, s.key_dim, s.value_dim, s.window) && Y.maxP % 4 == 0) {
             if ((rc = dalloc(p, &R.kc16, (size_t)Y.ring * L.kd * 2)) || (rc = dalloc(p, &R.vc16, (size_t)Y.ring * L.vd * 2))) return rc;
-            CK(cudaMemset(R.kc16, 0, (size_t)Y.ring * L.kd * 2));
-            CK(cudaMemset(R.vc16, 0, (size_t)Y.ring * L.vd * 2));
+            CK(zeros(p, R.kc16, (size_t)Y.ring * L.kd * 2));
+            CK(zeros(p, R.vc16, (size_t)Y.ring * L.vd * 2));
         }
         return B200_OK;
     }
     R.s_floats = s.mixer == B200_MIXER_RGLRU ? (size_t)L.qd : ly::ssd_state_floats(s.heads, s.key_dim, s.value_dim);
     R.c_floats = (size_t)Y.cring * L.dC;
     if ((rc = dalloc(p, &R.S, R.s_floats * 4)) || (rc = dalloc(p, &R.cstate, R.c_floats * 4))) return rc;
-    CK(cudaMemset(R.S, 0, R.s_floats * 4));
-    CK(cudaMemset(R.cstate, 0, R.c_floats * 4));
+    CK(zeros(p, R.S, R.s_floats * 4));
+    CK(zeros(p, R.cstate, R.c_floats * 4));
     return B200_OK;
 }
 

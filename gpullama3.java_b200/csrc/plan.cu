@@ -209,6 +209,18 @@ template <typename T> int dalloc(b200_plan *p, T **ptr, size_t n_bytes) {
     return B200_OK;
 }
 
+// Zeros for a buffer that the plan's stream, or the stream of its uploads, uses next.  (A memset on the legacy stream may still be on its way when the call returns, and neither of
+// these waits for that stream: it can clear what they have written since.)
+cudaError_t zeros(b200_plan *p, void *ptr, size_t n_bytes) {
+    const cudaError_t e = cudaMemsetAsync(ptr, 0, n_bytes, p->stream);
+    return e != cudaSuccess ? e : cudaStreamSynchronize(p->stream);
+}
+// In front of the plan's first work on what copies from pageable memory have brought: such a copy may return while its last bytes are on their way, on the legacy stream.
+cudaError_t copies_arrived(b200_plan *p) {
+    const cudaError_t e = cudaStreamSynchronize(cudaStreamLegacy);
+    return e != cudaSuccess ? e : cudaStreamSynchronize(p->stream);
+}
+
 // Buffers that a plan can do without: `alloc` allocates them with dalloc.  Where the device has no room, or its driver does not support what they are for, the ones
 // already made are given back and the plan goes on without any (*done = false, the reason in *why); every other error is returned.
 template <typename F> int alloc_optional(b200_plan *p, bool *done, F &&alloc, std::string *why = nullptr) {
@@ -702,7 +714,7 @@ int logits_alloc(b200_plan *p, int vocab) {
     const size_t words = (size_t)sampler_padded(vocab) + 1;
     int rc;
     if ((rc = dalloc(p, &p->logits, words * 4))) return rc;
-    CK(cudaMemset(p->logits, 0, words * 4));
+    CK(zeros(p, p->logits, words * 4));
     p->logits_words = words;
     return pinned_optional(p, &p->h_logits, words * 4);
 }
@@ -894,7 +906,7 @@ int pd_prepare(b200_plan *p) {
         if ((rc = dalloc(p, &p->pd_layers, h.size() * sizeof(PdLayer)))) return rc;
         CK(cudaMemcpy(p->pd_layers, h.data(), h.size() * sizeof(PdLayer), cudaMemcpyHostToDevice));
         if ((rc = dalloc(p, &p->pd_trace, (size_t)p->n_sms * (c.n_layers + 1) * PD_STAMPS * 8))) return rc;
-        CK(cudaMemset(p->pd_trace, 0, (size_t)p->n_sms * (c.n_layers + 1) * PD_STAMPS * 8));
+        CK(zeros(p, p->pd_trace, (size_t)p->n_sms * (c.n_layers + 1) * PD_STAMPS * 8));
     }
     CK(set_max_dyn(k_decode_persistent<128>, maxdyn));
     CK(set_max_dyn(k_decode_persistent<64>, maxdyn));
@@ -1146,7 +1158,7 @@ int build(b200_plan *p, const b200_tensor *tensors, int n_tensors) {
         if ((rc = dalloc(p, &p->part_val, (size_t)p->n_sms * 4))) return rc;
         if ((rc = dalloc(p, &p->part_idx, (size_t)p->n_sms * 4))) return rc;
         if ((rc = dalloc(p, &p->blk_cnt, (size_t)(c.hidden_dim / 32) * 4))) return rc;
-        CK(cudaMemset(p->blk_cnt, 0, (size_t)(c.hidden_dim / 32) * 4));
+        CK(zeros(p, p->blk_cnt, (size_t)(c.hidden_dim / 32) * 4));
     } else if (outw) {
         if (p->use_f16_stream) { // per-CTA argmax partials of the classifier launch (at most 3 CTAs per SM)
             if ((rc = dalloc(p, &p->part_val, (size_t)p->n_sms * 4 * 4))) return rc;
@@ -1261,7 +1273,7 @@ int build(b200_plan *p, const b200_tensor *tensors, int n_tensors) {
         p->pd_flags_off = (unsigned)o; o = al(o + PD_S_SLOTS * TP_MAX * 4); // epoch flags of the persistent decode kernel
         p->comm_bytes = o;
         if ((rc = dalloc(p, &p->comm, o))) return rc;
-        CK(cudaMemset(p->comm, 0, o));
+        CK(zeros(p, p->comm, o));
         p->x = reinterpret_cast<float *>(p->comm + p->tp.off_x);
     } else if ((rc = dalloc(p, &p->x, (size_t)c.dim * 4))) return rc;
     if ((rc = dalloc(p, &p->xb, (size_t)big * 4))) return rc;
@@ -1285,22 +1297,22 @@ int build(b200_plan *p, const b200_tensor *tensors, int n_tensors) {
     size_t kv_bytes = (size_t)c.n_layers * c.context_length * p->kvd_l * 4;
     if ((rc = dalloc(p, &p->key_cache, kv_bytes))) return rc;
     if ((rc = dalloc(p, &p->value_cache, kv_bytes))) return rc;
-    CK(cudaMemset(p->key_cache, 0, kv_bytes));
-    CK(cudaMemset(p->value_cache, 0, kv_bytes));
+    CK(zeros(p, p->key_cache, kv_bytes));
+    CK(zeros(p, p->value_cache, kv_bytes));
     if ((rc = dalloc(p, &p->smp_indices, (size_t)c.vocab_size * 4))) return rc;
     if ((rc = dalloc(p, &p->smp_out, 8 * 4))) return rc;
     p->seq_cap = c.context_length + 8;
     if ((rc = dalloc(p, &p->st, sizeof(StepState)))) return rc;
     if ((rc = dalloc(p, &p->seq_tokens, (size_t)p->seq_cap * 4))) return rc;
     if ((rc = dalloc(p, &p->out_ids, (size_t)p->seq_cap * 4))) return rc;
-    CK(cudaMemset(p->st, 0, sizeof(StepState)));
-    CK(cudaMemset(p->seq_tokens, 0, (size_t)p->seq_cap * 4));
+    CK(zeros(p, p->st, sizeof(StepState)));
+    CK(zeros(p, p->seq_tokens, (size_t)p->seq_cap * 4));
     CK(cudaMallocHost(&p->h_st, sizeof(StepState)));
     CK(cudaMallocHost(&p->h_ids, (size_t)p->seq_cap * 4));
 
     // epoch counters of the persistent kernel + the error word every bounded device-side wait reports through
     if ((rc = dalloc(p, &p->pd_sync, PD_S_WORDS * 4))) return rc;
-    CK(cudaMemset(p->pd_sync, 0, PD_S_WORDS * 4));
+    CK(zeros(p, p->pd_sync, PD_S_WORDS * 4));
     CK(cudaHostAlloc(&p->h_err, 64, cudaHostAllocMapped));
     *p->h_err = 0u;
     CK(cudaHostGetDevicePointer((void **)&p->d_err, p->h_err, 0));
@@ -1315,13 +1327,13 @@ int build(b200_plan *p, const b200_tensor *tensors, int n_tensors) {
         if (!done) p->att_rows = nullptr;
     }
     if ((rc = set_smem_attrs(p))) return rc;
-    if (c.tp_size > 1) { CK(cudaStreamSynchronize(p->stream)); return B200_OK; } // graphs are captured by b200_tp_attach
+    if (c.tp_size > 1) { CK(copies_arrived(p)); return B200_OK; } // graphs are captured by b200_tp_attach
     if ((rc = capture_all(p))) return rc;
     if (p->prefill_batch > 1) {
         if ((rc = prefill_init(p))) return rc;
         if ((rc = exact_prefill_init(p))) return rc;
     }
-    CK(cudaStreamSynchronize(p->stream));
+    CK(copies_arrived(p));
     return B200_OK;
 }
 
@@ -1412,10 +1424,10 @@ int exact_prefill_alloc(b200_plan *p, int rows, int nqkv, int wide) {
     if ((rc = dalloc(p, &p->xp.AS, (size_t)rows * (wide / 32) * 4))) return rc;
     if ((rc = dalloc(p, &p->xp.HQ, (size_t)rows * g.hidden_dim))) return rc;
     if ((rc = dalloc(p, &p->xp.HS, (size_t)rows * (g.hidden_dim / 32) * 4))) return rc;
-    CK(cudaMemset(p->xp.AQ, 0, (size_t)rows * wide)); // rows behind the chunk's last token are multiplied too (and dropped)
-    CK(cudaMemset(p->xp.AS, 0, (size_t)rows * (wide / 32) * 4));
-    CK(cudaMemset(p->xp.HQ, 0, (size_t)rows * g.hidden_dim));
-    CK(cudaMemset(p->xp.HS, 0, (size_t)rows * (g.hidden_dim / 32) * 4));
+    CK(zeros(p, p->xp.AQ, (size_t)rows * wide)); // rows behind the chunk's last token are multiplied too (and dropped)
+    CK(zeros(p, p->xp.AS, (size_t)rows * (wide / 32) * 4));
+    CK(zeros(p, p->xp.HQ, (size_t)rows * g.hidden_dim));
+    CK(zeros(p, p->xp.HS, (size_t)rows * (g.hidden_dim / 32) * 4));
     if (!p->prefill.tok && (rc = dalloc(p, &p->prefill.tok, (size_t)rows * 4))) return rc;
     if (xp_att_smem_bytes(g.head_size, 32, g.context_length, false) > XP_SMEM_MAX) { // one slot of 32 score rows per SM, as far as that goes
         const size_t slot = (size_t)32 * xp_score_stride(g.context_length) * 4;
@@ -1450,8 +1462,8 @@ int exact_prefill_umma_alloc(b200_plan *p, int rows, int wide) {
     if ((rc = dalloc(p, &c.AH, (size_t)rows * wide * 2))) return rc;
     if ((rc = dalloc(p, &c.HH, (size_t)rows * g.hidden_dim * 2))) return rc;
     if ((rc = dalloc(p, &c.G, (size_t)std::min(rows, XP_SLICE) * 2 * g.hidden_dim * 4))) return rc;
-    CK(cudaMemset(c.AH, 0, (size_t)rows * wide * 2)); // (as AQ and HQ)
-    CK(cudaMemset(c.HH, 0, (size_t)rows * g.hidden_dim * 2));
+    CK(zeros(p, c.AH, (size_t)rows * wide * 2)); // (as AQ and HQ)
+    CK(zeros(p, c.HH, (size_t)rows * g.hidden_dim * 2));
     bool ok = !refused("umma") && xp_map_acts(&c.hA, c.AH, true, c.AS, rows, g.dim, XT_TOK) == 0 && xp_map_acts(&c.hATT, c.AH, true, c.AS, rows, p->qd, XT_TOK) == 0 &&
               xp_map_acts(&c.hH, c.HH, true, c.HS, rows, g.hidden_dim, XT_TOK) == 0;
     c.slices.resize((rows - 1) / XP_SLICE);
@@ -1631,12 +1643,12 @@ int prefill_init(b200_plan *p) {
     if ((rc = dalloc(p, &c.tok, (size_t)c.bpad * 4))) return rc;
     if ((rc = dalloc(p, &c.KH, (size_t)g.context_length * p->kvd * 2))) return rc; // f16 K / V of the layer being processed
     if ((rc = dalloc(p, &c.VH, (size_t)g.context_length * p->kvd * 2))) return rc;
-    CK(cudaMemset(c.X, 0, (size_t)c.bpad * g.dim * 4));
-    CK(cudaMemset(c.QKV, 0, (size_t)c.bpad * nqkv * 4));
-    CK(cudaMemset(c.A16, 0, (size_t)c.bpad * g.dim * 2));
-    CK(cudaMemset(c.ATT16, 0, (size_t)c.bpad * p->qd * 2));
-    CK(cudaMemset(c.H16, 0, (size_t)c.bpad * g.hidden_dim * 2));
-    CK(cudaMemset(c.tok, 0, (size_t)c.bpad * 4));
+    CK(zeros(p, c.X, (size_t)c.bpad * g.dim * 4));
+    CK(zeros(p, c.QKV, (size_t)c.bpad * nqkv * 4));
+    CK(zeros(p, c.A16, (size_t)c.bpad * g.dim * 2));
+    CK(zeros(p, c.ATT16, (size_t)c.bpad * p->qd * 2));
+    CK(zeros(p, c.H16, (size_t)c.bpad * g.hidden_dim * 2));
+    CK(zeros(p, c.tok, (size_t)c.bpad * 4));
     bool ok = pg::make_map(&c.mA, c.A16, c.bpad, g.dim, pg::BM) == 0 && pg::make_map(&c.mATT, c.ATT16, c.bpad, p->qd, pg::BM) == 0 &&
               pg::make_map(&c.mH, c.H16, c.bpad, g.hidden_dim, pg::BM) == 0 && pg::make_map_c(&c.mX, c.X, c.bpad, g.dim) == 0 &&
               pg::make_map_c(&c.mQKV, c.QKV, c.bpad, nqkv) == 0;
@@ -2339,7 +2351,8 @@ int b200_time_kernel(b200_plan *p, int32_t which, int32_t reps, float *avg_ms, i
         CK(cudaEventElapsedTime(&ms, p->ev0, p->ev1));
         *avg_ms = ms / launches;
         if (algorithmic_bytes) *algorithmic_bytes = bytes;
-        CK(cudaMemcpy(p->x, save.data(), (size_t)c.dim * 4, cudaMemcpyHostToDevice));
+        CK(cudaMemcpyAsync(p->x, save.data(), (size_t)c.dim * 4, cudaMemcpyHostToDevice, p->stream));
+        CK(cudaStreamSynchronize(p->stream));
         return B200_OK;
     }
     auto mat_bytes = [&](const DevMat &m) -> int64_t {
@@ -2397,7 +2410,8 @@ int b200_time_kernel(b200_plan *p, int32_t which, int32_t reps, float *avg_ms, i
     CK(cudaEventElapsedTime(&ms, p->ev0, p->ev1));
     *avg_ms = ms / launches;
     if (algorithmic_bytes) *algorithmic_bytes = bytes;
-    CK(cudaMemcpy(p->x, save.data(), (size_t)c.dim * 4, cudaMemcpyHostToDevice));
+    CK(cudaMemcpyAsync(p->x, save.data(), (size_t)c.dim * 4, cudaMemcpyHostToDevice, p->stream));
+    CK(cudaStreamSynchronize(p->stream));
     return B200_OK;
 }
 
@@ -2431,7 +2445,7 @@ int b200_tp_attach(b200_plan *p, const void *handles, int32_t n) {
     p->attached = true;
     int rc;
     if ((rc = capture_all(p))) return rc;
-    CK(cudaStreamSynchronize(p->stream));
+    CK(copies_arrived(p));
     return B200_OK;
 }
 

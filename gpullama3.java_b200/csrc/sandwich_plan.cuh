@@ -105,7 +105,7 @@ static int ly_sandwich_mixer_upload(b200_plan *p, int l, LyLayer &L, const b200_
     const std::string mx = "l" + std::to_string(l) + ".mix.";
     int rc;
     if ((rc = dalloc(p, &L.w_proj, (size_t)L.P * E * 2))) return rc;
-    if (L.P > L.Pn) CK(cudaMemset(L.w_proj + (size_t)L.Pn * E, 0, (size_t)(L.P - L.Pn) * E * 2));
+    if (L.P > L.Pn) CK(zeros(p, L.w_proj + (size_t)L.Pn * E, (size_t)(L.P - L.Pn) * E * 2));
     if ((rc = dalloc(p, &L.w_o, (size_t)E * L.gd * 2))) return rc;
     const bool light = s.mixer == B200_MIXER_LIGHTNING;
     const std::string at = light ? mx : mx + "left.";
@@ -131,7 +131,7 @@ static int ly_sandwich_mixer_upload(b200_plan *p, int l, LyLayer &L, const b200_
     if ((rc = ly_vec_f32(p, tensors, nt, sc + "conv", (int64_t)I * s.conv_taps, &L.conv_w))) return rc;
     if ((rc = ly_vec_f32(p, tensors, nt, sc + "conv.b", I, &L.conv_b))) return rc;
     if ((rc = dalloc(p, &L.w_x, (size_t)L.nxp * I * 2))) return rc;
-    CK(cudaMemset(L.w_x, 0, (size_t)L.nxp * I * 2));
+    CK(zeros(p, L.w_x, (size_t)L.nxp * I * 2));
     if ((rc = ly_mat(p, tensors, nt, sc + "x", L.nx, I, L.w_x, 0))) return rc;
     if ((rc = dalloc(p, &L.w_dt, (size_t)I * s.scan_rank * 2))) return rc;
     if ((rc = ly_mat(p, tensors, nt, sc + "dt", I, s.scan_rank, L.w_dt, 0))) return rc;
@@ -166,7 +166,7 @@ static int ly_side_upload(b200_plan *p, int l, LyLayer &L, const b200_tensor *te
     const std::string sd = "l" + std::to_string(l) + ".side.";
     int rc;
     if ((rc = dalloc(p, &L.w_sgate, (size_t)Y.side_pad * E * 2))) return rc;
-    CK(cudaMemset(L.w_sgate, 0, (size_t)Y.side_pad * E * 2));
+    CK(zeros(p, L.w_sgate, (size_t)Y.side_pad * E * 2));
     if ((rc = ly_mat(p, tensors, nt, sd + "gate", D, E, L.w_sgate, 0))) return rc;
     if ((rc = dalloc(p, &L.w_sproj, (size_t)E * D * 2))) return rc;
     if ((rc = ly_mat(p, tensors, nt, sd + "proj", E, D, L.w_sproj, 0))) return rc;
@@ -183,10 +183,10 @@ static int ly_sandwich_run(b200_plan *p, LyRun &R, const LyLayer &L) {
         R.s_floats = ly::sel_state_floats(s.scan_inner, s.scan_state);
         R.c_floats = (size_t)Y.cring * L.dC;
         if ((rc = dalloc(p, &R.cstate, R.c_floats * 4))) return rc;
-        CK(cudaMemset(R.cstate, 0, R.c_floats * 4));
+        CK(zeros(p, R.cstate, R.c_floats * 4));
     }
     if ((rc = dalloc(p, &R.S, R.s_floats * 4))) return rc;
-    CK(cudaMemset(R.S, 0, R.s_floats * 4));
+    CK(zeros(p, R.S, R.s_floats * 4));
     return B200_OK;
 }
 
