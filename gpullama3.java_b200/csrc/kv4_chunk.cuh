@@ -15,7 +15,7 @@
 // reaches the rows that see the position and no other (0 * NaN in the product would reach them all).
 //
 // Rows of a tile may belong to several slots and stand in any order: a run of tokens of one slot is a segment, the tiles of all segments are one list, and a row masks what is not its own.
-// Every wait is bounded: after 2^25 tries the CTA gives up, writes the cache's error word, waits for its products under way and frees its tensor memory.
+// Every wait is bounded: after 2^25 tries the CTA gives up, waits for its products under way, frees its tensor memory and, whichever warp it was, writes the cache's error word.
 #pragma once
 #include <type_traits>
 
@@ -163,7 +163,8 @@ struct Chunk {
     unsigned *error; // the cache's error word (mapped host memory)
 };
 
-template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(const Chunk c) {
+// GIVE_UP (tests): the warps of the rows take their last wait, for the products that end a stream, as run out.
+template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(const Chunk c) {
     constexpr int NG = groups(HS);
     extern __shared__ unsigned char raw_smem[];
     unsigned char *smem = raw_smem + (-s32(raw_smem) & 1023u); // the operands' swizzle counts from 1024-byte boundaries
@@ -446,12 +447,10 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
                 phase ^= 1;
             }
         }
-        if (!ok) { // given up: what is under way ends before the tensor memory goes
-            unsigned none = 0;
-            umma_commit(&sh.drained, lead);
-            bar_wait(&sh.drained, 0, &none);
-            if (lead && c.error) *reinterpret_cast<volatile unsigned *>(c.error) = 1u;
-        }
+        // what is under way ends before the tensor memory goes: the warps of the rows have waited for it, or one of them has given up
+        unsigned none = 0;
+        umma_commit(&sh.drained, lead);
+        if (!bar_wait(&sh.drained, 0, &none)) *reinterpret_cast<volatile unsigned *>(&sh.bail) = 1u;
     } else if (warp < CHUNK_SOFTMAX) {
         // ===== rows: two threads a stream, 64 positions of a tile a thread =====
         constexpr int PIECE = 16, COLUMNS = CHUNK_KEYS / 2;
@@ -474,6 +473,10 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
         float base = 0.0f, ref = 0.0f; // top where there is one, times the factor
         int from = 0, to = 0, j = stream - 2, next = 0; // the tile's positions [from, to) are seen, counted from this thread's first; the segment's end
         for (unsigned turn = 0; stream < count; turn++) {
+            if (GIVE_UP && j + 2 >= count) {
+                *reinterpret_cast<volatile unsigned *>(&sh.bail) = 1u;
+                break;
+            }
             ok = __all_sync(0xffffffffu, bar_wait(&sh.s_full[stream], turn & 1, &sh.bail));
             if (!ok) break;
             fence_after();
@@ -657,6 +660,7 @@ template <int HS> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(co
         fence_before();
     }
     __syncthreads();
+    if (tid == 0 && sh.bail != 0u) *reinterpret_cast<volatile unsigned *>(c.error) = 1u;
     if (warp == CHUNK_SOFTMAX) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");

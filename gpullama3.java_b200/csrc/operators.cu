@@ -14,7 +14,7 @@ struct b200_kv4 {
     kv4::View view{};
     int head_size = 0, device = 0, sms = 148;
     size_t bytes = 0;
-    unsigned *host_error = nullptr, *device_error = nullptr; // a mapped word: what a wait that gave up leaves (kv4_chunk.cuh); null where the host had no memory for it
+    unsigned *host_error = nullptr, *device_error = nullptr; // a mapped word: what a wait that gave up leaves (kv4_chunk.cuh)
     char err[256] = "";
 };
 
@@ -91,6 +91,10 @@ cudaError_t launch(void (*kern)(KA...), unsigned grid, int block, size_t smem, i
 template <typename K> cudaError_t prepare(K kern, size_t smem, int cluster) {
     cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
     return e;
+}
+bool refused(const char *step) { // (as in plan.cu: what tests refuse)
+    const char *e = getenv("B200_TEST_REFUSE");
+    return e && strstr(e, step);
 }
 int sm_count(int device) {
     int n = 0;
@@ -179,7 +183,7 @@ static ChunkCut chunk_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, 
     return c;
 }
 
-cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_args &a, int8_t *quants, float *scales, cudaStream_t stream, bool pdl, int *launches) {
+static cudaError_t attention_launch(const b200_kv4 *kv, const b200_kv4_attention_args &a, int8_t *quants, float *scales, cudaStream_t stream, bool pdl, int *launches, bool give_up) {
     kv4::Step k;
     k.kv = kv->view;
     k.rows = {a.positions, a.slots, a.n, a.start, a.slot};
@@ -206,6 +210,7 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
         const auto go = [&](auto hs) {
             constexpr size_t smem = kv4::chunk_smem_bytes(hs);
             auto kern = kv4::k_chunk<hs>;
+            if constexpr (hs == 64) if (give_up) kern = kv4::k_chunk<hs, true>;
             cudaError_t e = prepare(kern, smem, 1);
             if (e == cudaSuccess) e = launch(kern, grid, kv4::CHUNK_THREADS, smem, 1, pdl, stream, ck);
             return e != cudaSuccess || cc.splits == 1 ? e : join(hs, cc.splits);
@@ -233,7 +238,11 @@ cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_ar
     });
 }
 
-bool kv4_gave_up(const b200_kv4 *kv) { return kv->host_error && *reinterpret_cast<volatile unsigned *>(kv->host_error); }
+cudaError_t kv4_attention_launch(const b200_kv4 *kv, const b200_kv4_attention_args &a, int8_t *quants, float *scales, cudaStream_t stream, bool pdl, int *launches) {
+    return attention_launch(kv, a, quants, scales, stream, pdl, launches, false);
+}
+
+bool kv4_gave_up(const b200_kv4 *kv) { return *reinterpret_cast<volatile unsigned *>(kv->host_error); }
 
 cudaError_t log_probs_launch(const b200_log_probs_args &a, cudaStream_t stream) {
     lp::Args k;
@@ -279,15 +288,17 @@ int b200_kv4_create(int32_t slots, int32_t context, int32_t kv_heads, int32_t he
         e = cudaMemset(kv->view.base, 0, kv->bytes);
         if (e == cudaSuccess) e = cudaDeviceSynchronize(); // the memory is zeros for every stream
     }
-    if (e == cudaSuccess && cudaHostAlloc((void **)&kv->host_error, 4, cudaHostAllocMapped) == cudaSuccess) {
+    // the word through which a wait that gave up is heard of: no cache without it
+    if (e == cudaSuccess) e = refused("kv4_word") ? cudaErrorMemoryAllocation : cudaHostAlloc((void **)&kv->host_error, 4, cudaHostAllocMapped);
+    if (e == cudaSuccess) {
         *kv->host_error = 0;
-        if (cudaHostGetDevicePointer((void **)&kv->device_error, kv->host_error, 0) != cudaSuccess) kv->device_error = nullptr;
+        e = cudaHostGetDevicePointer((void **)&kv->device_error, kv->host_error, 0);
     }
-    cudaGetLastError(); // (the word only reports)
     if (e != cudaSuccess) {
         cudaGetLastError();
         say(err, err_len, 0, "4-bit cache of %.3g GB: %s", (double)bytes / 1e9, cudaGetErrorString(e));
         cudaFree(kv->view.base);
+        cudaFreeHost(kv->host_error);
         delete kv;
         return cuda_code(e);
     }
@@ -316,7 +327,7 @@ int b200_kv4_reset(b200_kv4 *kv, void *stream) {
 
 static int check_error(b200_kv4 *kv) {
     if (kv4_gave_up(kv))
-        return fail(kv, B200_ERR_STATE, "an earlier attention of a chunk gave up a wait on the device: its results, and what came of them, are not valid");
+        return fail(kv, B200_ERR_STATE, "an earlier attention of a chunk gave up a wait on the device: its results, and what came of them, are not valid; the cache must be freed");
     return B200_OK;
 }
 
@@ -347,7 +358,7 @@ int b200_kv4_append(b200_kv4 *kv, const b200_kv4_append_args *a, void *stream) {
     return e == cudaSuccess ? B200_OK : fail(kv, cuda_code(e), "%s", cudaGetErrorString(e));
 }
 
-int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *a, void *stream) {
+static int attention(b200_kv4 *kv, const b200_kv4_attention_args *a, void *stream, bool give_up) {
     if (!kv) return B200_ERR_BAD_ARG;
     if (!a) return fail(kv, B200_ERR_BAD_ARG, "null arguments");
     int rc = check_error(kv);
@@ -364,8 +375,15 @@ int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *a, void *str
     if ((long long)a->n * a->heads > (1LL << 27)) return fail(kv, B200_ERR_UNSUPPORTED, "too many rows in one call");
     OnDevice on(kv->device);
     cudaError_t e = on.error;
-    if (e == cudaSuccess) e = kv4_attention_launch(kv, *a, nullptr, nullptr, (cudaStream_t)stream, false);
+    if (e == cudaSuccess) e = attention_launch(kv, *a, nullptr, nullptr, (cudaStream_t)stream, false, nullptr, give_up);
     return e == cudaSuccess ? B200_OK : fail(kv, cuda_code(e), "%s", cudaGetErrorString(e));
+}
+int b200_kv4_attention(b200_kv4 *kv, const b200_kv4_attention_args *a, void *stream) { return attention(kv, a, stream, false); }
+int b200_test_kv4_give_up(b200_kv4 *kv, const b200_kv4_attention_args *a, void *stream) {
+    if (!kv) return B200_ERR_BAD_ARG;
+    if (!a || a->n <= 0 || a->heads <= 0 || a->heads % kv->view.kv_heads || kv->head_size != 64 || !chunk_cut(kv, *a, false).use)
+        return fail(kv, B200_ERR_BAD_ARG, "no attention of a chunk with heads of 64");
+    return attention(kv, a, stream, true);
 }
 
 size_t b200_kv4_attention_workspace(const b200_kv4 *kv, const b200_kv4_attention_args *a) {

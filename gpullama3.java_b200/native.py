@@ -92,7 +92,7 @@ class LogProbs(C.Structure):
                [(n, C.c_void_p) for n in ("targets", "logprobs", "entropy", "top_ids", "top_logprobs")]
 
 
-EXPORTS = ["b200_set_kv_mode", "b200_kv_info", "b200_score_tokens", "b200_kv4_create", "b200_kv4_free", "b200_kv4_reset", "b200_kv4_device_bytes", "b200_kv4_last_error", "b200_kv4_append", "b200_kv4_attention", "b200_kv4_attention_workspace", "b200_kv4_read", "b200_test_kv4_step_cut", "b200_log_probs",
+EXPORTS = ["b200_set_kv_mode", "b200_kv_info", "b200_score_tokens", "b200_kv4_create", "b200_kv4_free", "b200_kv4_reset", "b200_kv4_device_bytes", "b200_kv4_last_error", "b200_kv4_append", "b200_kv4_attention", "b200_kv4_attention_workspace", "b200_kv4_read", "b200_test_kv4_step_cut", "b200_test_kv4_give_up", "b200_log_probs",
            "b200_plan_create_layered", "b200_forward_batch_logits", "b200_layered_info", "b200_plan_create", "b200_forward_decode", "b200_forward_prefill", "b200_forward_batch_prefill", "b200_set_prefill_mode", "b200_prefill_info", "b200_exact_prefill_info",
            "b200_set_decode_mode", "b200_decode_info", "b200_trace_persistent", "b200_test_seqsum2", "b200_test_exact_prefill_wait", "b200_test_exact_prefill_wait_form", "b200_forward_decode_sample", "b200_upload_info", "b200_requant_kquant",
            "b200_decode_sequence", "b200_time_kernel", "b200_tp_handle", "b200_tp_attach", "b200_trace_decode", "b200_profile_norm", "b200_test_seqsum", "b200_gemm_f16", "b200_kv_reset", "b200_read_buffer", "b200_launches_per_decode",
@@ -156,6 +156,7 @@ def lib() -> C.CDLL:
     L.b200_kv4_last_error.argtypes, L.b200_kv4_last_error.restype = [vp], C.c_char_p
     L.b200_kv4_append.argtypes = [vp, vp, vp]
     L.b200_kv4_attention.argtypes = [vp, vp, vp]
+    L.b200_test_kv4_give_up.argtypes = [vp, vp, vp]
     L.b200_kv4_attention_workspace.argtypes, L.b200_kv4_attention_workspace.restype = [vp, vp], C.c_size_t
     L.b200_kv4_read.argtypes = [vp, vp, vp]
     L.b200_test_kv4_step_cut.argtypes = [i32] * 9 + [C.POINTER(i32)]

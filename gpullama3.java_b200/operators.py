@@ -47,7 +47,8 @@ class KV4Cache(_ops.Cache):
     attention(q, positions, slots=None, scale=None, window=0, max_len=0, chunk=1, dtype=torch.float32, out=None)
         Causal attention of FP32 rows ``q`` [n, heads, head_size]: the row at position p sees the positions up to p of its slot, the last ``window`` of them (0: all);
         ``scale`` is head_size ** -0.5 unless given.  Results are FP32, FP16 or BF16.  ``max_len`` (largest position + 1, 0: unknown) and ``chunk`` (neighbouring rows that
-        are successive tokens of one sequence) only choose how the work is split.  A row that sees nothing is zeros.
+        are successive tokens of one sequence) only choose how the work is split.  A row that sees nothing is zeros.  (Should a wait inside
+        a chunk's kernel ever run out, its rows are not written and the cache refuses further attention: B200Error with the state's code.)
 
     read(positions, slots=None, dtype=torch.float32)
         The values held at some rows: (k, v), each [n, kv_heads, head_size] (not defined where a row is padding or has a negative position).

@@ -541,7 +541,8 @@ int b200_kv4_append(b200_kv4 *kv, const b200_kv4_append_args *args, void *stream
  * head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type.  A row that sees nothing is zeros.  max_len (0: unknown) is the largest position + 1 as far as the host
  * knows, chunk (0 or 1: single steps) how many neighbouring rows are successive tokens of one sequence: both only choose how the work is split.  So does a workspace: few rows over
  * many positions fill the GPU where the call gets b200_kv4_attention_workspace(kv, args) bytes (0: it needs none) of 16-byte aligned device memory, whose content before and after does not matter
- * and which no other call under way may use; NULL or fewer bytes: the call does without. */
+ * and which no other call under way may use; NULL or fewer bytes: the call does without.  Waits inside the kernels end after a second or more; should one ever run out, the rows are not
+ * written, and every later call, once the kernel has ended, is B200_ERR_STATE: such a cache can only be freed. */
 typedef struct b200_kv4_attention_args {
     int32_t n, heads, window, max_len, chunk, out_type;
     const float *q;
@@ -565,6 +566,8 @@ typedef struct b200_kv4_read_args {
 } b200_kv4_read_args;
 int b200_kv4_read(b200_kv4 *kv, const b200_kv4_read_args *args, void *stream);
 
+/* Test hook: the attention of a chunk (heads of 64) whose last waits count as run out. */
+int b200_test_kv4_give_up(b200_kv4 *kv, const b200_kv4_attention_args *args, void *stream);
 /* Test hook (host only): how attention of n single rows is cut on a GPU of `sms` SMs: cut[4] = {query heads of a unit, units of a row and key/value head, CTAs of a cluster, clusters of
  * a unit}; quants: with results in blocks of 32 quants, as Q8_0 plans take them. */
 int b200_test_kv4_step_cut(int32_t head_size, int32_t kv_heads, int32_t heads, int32_t n, int32_t context, int32_t max_len, int32_t window, int32_t sms, int32_t quants, int32_t *cut);
