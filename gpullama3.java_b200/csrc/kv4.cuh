@@ -28,8 +28,10 @@ __host__ __device__ constexpr int record_bytes(int hs) { return 18 * hs; }
 
 struct View {
     unsigned char *base;
+    unsigned *odd; // by slot: has it taken a group whose scale is beyond KV4_ODD or NaN (for as long as the cache is not reset)
     int slots, context, blocks, kv_heads; // blocks of a head and slot
 };
+constexpr unsigned KV4_ODD = 0x6ffe; // FP16 bits of 8184: entries of up to 8 times a larger scale may lie outside FP16
 struct Rows { // row r stands at position `positions ? positions[r] : start + r` of slot `slots ? slots[r] : slot`
     const int *positions, *slots;
     int n, start, slot;
@@ -202,7 +204,10 @@ template <int HS, typename T> __global__ void __launch_bounds__(256) k_append(co
             codes[2 * word_of<HS>(half, 4 * (2 * t + u) + ((in & 7) >> 1), grp) + (in & 1)] = (uint16_t)w;
         }
     }
-    if (t == 0) reinterpret_cast<__half *>(rec + 16 * HS + (is_v ? HS : 0))[2 * ((in & 7) * groups(HS) + grp) + half] = scale;
+    if (t == 0) {
+        reinterpret_cast<__half *>(rec + 16 * HS + (is_v ? HS : 0))[2 * ((in & 7) * groups(HS) + grp) + half] = scale;
+        if ((__half_as_ushort(scale) & 0x7fffu) > KV4_ODD) a.kv.odd[slot] = 1u; // (whoever writes it writes the same)
+    }
 }
 
 // ---- read-back: the values that the codes of some rows stand for -----------------------------------------------------------------------------------------------

@@ -11,8 +11,10 @@
 // products 1400 (1024 were nothing else at shared memory), beside them the conversion of its records, one a warp, 2400 with what it waits for; 0.57 instructions a cycle and scheduler.
 // One stream with two S and a maximum agreed on by a row's threads in every tile took 116-123 us; 256 rows a CTA with half the conversions 133 us (two blocks of rows in place of the two
 // streams; 64 pairs of CTAs whose parts had to be joined).
-// Rounding: queries (times a power of two), keys, values and probabilities are FP16 operands, sums are FP32.  A value's NaN, or one outside FP16, is moved into its key, so that it
-// reaches the rows that see the position and no other (0 * NaN in the product would reach them all).
+// Rounding: queries (times a power of two), keys, values and probabilities are FP16 operands, sums are FP32.  Entries of a position outside FP16 (a scale above 8184: codes of up to 8 times
+// that) become operands times 2^-5, and the position's scores, or its probabilities as operands, times 2^5.  A value's NaN stays out of the product, where 0 * NaN would reach every row: the
+// rows that see it note its group, and write NaN there.  The append marks the slots that have taken such an entry (kv4.cuh), and only CTAs that meet a marked slot look for them: looked for in
+// every tile they cost 9 % (104 us became 113); as it is the time of unmarked slots is what it was.
 //
 // Rows of a tile may belong to several slots and stand in any order: a run of tokens of one slot is a segment, the tiles of all segments are one list, and a row masks what is not its own.
 // Every wait is bounded: after 2^25 tries the CTA gives up, waits for its products under way, frees its tensor memory and, whichever warp it was, writes the cache's error word.
@@ -31,12 +33,14 @@ struct Segment { // a run of tokens of one slot and the records that any of them
     int slot, begin, end, tiles; // records [begin, end); tiles of all segments up to and with this one
 };
 struct ChunkSmem { // behind the operands
+    uint4 odd[CHUNK_K_STAGES][CHUNK_RECORDS]; // by record of the keys' stage: x: positions whose keys (low half) or values (high half) are held times 2^-5; y, z: whose values are NaN, 16 bits a group; w: any
     unsigned long long k_full[CHUNK_K_STAGES], k_free[CHUNK_K_STAGES], v_full[CHUNK_V_STAGES], v_free[CHUNK_V_STAGES];
     unsigned long long s_full[2], p_full[2], drained; // by stream
     unsigned long long pair[CHUNK_SOFTMAX / 2];       // the two warps that share a stream's rows
-    unsigned tmem, bail, again[2], repeat[2];         // again: a row's maximum has to move; repeat: these are the scores of the tile before once more
+    unsigned tmem, bail, again[2], repeat[2], marked; // again: a row's maximum has to move; repeat: these are the scores of the tile before once more; marked: a token's slot is
     int n_segments, single;
     int slot[CHUNK_ROWS], pos[CHUNK_ROWS], segment[CHUNK_ROWS]; // by token
+    unsigned nan[CHUNK_ROWS];                                   // by row: groups in which it has seen a NaN
     float factor[CHUNK_ROWS];                                   // by row: what turns a product into a score in units of log2
     float half_row[2][2][CHUNK_ROWS];                           // by stream: what the two threads of a row tell each other, their sums at the end
     float top[2][CHUNK_ROWS];
@@ -194,7 +198,7 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
         }
         for (int i = 0; i < CHUNK_SOFTMAX / 2; i++) bar_init(&sh.pair[i], 2);
         bar_init(&sh.drained, 1);
-        sh.bail = 0;
+        sh.bail = sh.marked = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == CHUNK_SOFTMAX) {
@@ -211,6 +215,7 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
         sh.slot[tid] = slot;
         sh.pos[tid] = pos;
         sh.segment[tid] = -1;
+        sh.nan[tid] = 0;
     }
     // queries: a row a warp, all of a warp's rows under way at once
     constexpr int WARPS = CHUNK_THREADS / 32, QROWS = (CHUNK_ROWS + WARPS - 1) / WARPS;
@@ -238,6 +243,7 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
         if (lane == 0) sh.factor[r] = a.scale == 0.0f ? 1.0f : fmaxf(down * fabsf(a.scale * 1.4426950408889634f), 1.17549435e-38f); // (0 times -inf is a NaN)
     }
     __syncthreads();
+    if (tid < tokens && sh.slot[tid] >= 0 && a.kv.odd[sh.slot[tid]] != 0u) sh.marked = 1u;
     if (warp == 0) { // one slot for all, as inside a prompt: one segment
         bool same = sh.slot[0] >= 0;
         int from = INT32_MAX, to = 0;
@@ -325,38 +331,43 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
         for (int j = 0; j < count; j++) {
             const int b = j & 1;
             uint32_t v[2][NG], dv[2][NG]; // the values' codes and scales
-            __half2 widest = {};
 #pragma unroll
             for (int i = 0; i < NG; i++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     v[h][i] = raw.v[h][i];
                     dv[h][i] = __byte_perm(raw.vs[0][i], raw.vs[1][i], h ? 0x7632 : 0x5410);
-                    widest = __hmax2_nan(widest, __habs2(*reinterpret_cast<const __half2 *>(&dv[h][i])));
                 }
             if (behind)
 #pragma unroll
                 for (int i = 0; i < NG; i++) dv[0][i] = dv[1][i] = 0u;
-            // a value scale that FP16 products do not hold (or a NaN) is moved into the keys: such positions get no value and a NaN key
-            if (__any_sync(0xffffffffu, (0xeffeeffeu - *reinterpret_cast<const uint32_t *>(&widest) & 0x80008000u) != 0x80008000u)) { // a half above 0x6ffe: 8 d up to 65504
-                uint32_t bad = 0; // by position of the record
-#pragma unroll
-                for (int i = 0; i < NG; i++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) bad |= ((dv[h][i] & 0x7fffu) > 0x6ffeu ? 1u << (8 * h + 2 * t) : 0u) | ((dv[h][i] >> 16 & 0x7fffu) > 0x6ffeu ? 2u << (8 * h + 2 * t) : 0u);
-                bad = __reduce_or_sync(0xffffffffu, bad);
+            if (j >= CHUNK_K_STAGES && !__all_sync(0xffffffffu, bar_wait(&sh.k_free[ks], k_phase, &sh.bail))) break; // the scores of tile j - 3 stand
+            if (__any_sync(0xffffffffu, sh.marked != 0u)) { // entries that FP16 does not hold, and NaN
+                const auto wide = [](uint32_t d) { return d > KV4_ODD && d <= 0x7c00u; };
+                uint32_t w5 = 0, nan[2] = {0, 0};
 #pragma unroll
                 for (int i = 0; i < NG; i++) {
+                    w5 |= (wide(raw.ks[i] & 0x7fffu) ? 1u << g : 0u) | (wide(raw.ks[i] >> 16 & 0x7fffu) ? 0x100u << g : 0u);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        if (bad >> (8 * h + 2 * t) & 1u) dv[h][i] &= 0xffff0000u;
-                        if (bad >> (8 * h + 2 * t + 1) & 1u) dv[h][i] &= 0x0000ffffu;
+                        const uint32_t a0 = dv[h][i] & 0x7fffu, a1 = dv[h][i] >> 16 & 0x7fffu, at = 8 * h + 2 * t;
+                        w5 |= (wide(a0) ? 0x10000u << at : 0u) | (wide(a1) ? 0x20000u << at : 0u);
+                        nan[i / 2] |= ((a0 > 0x7c00u ? 1u << at : 0u) | (a1 > 0x7c00u ? 2u << at : 0u)) << (16 * (i & 1));
+                        dv[h][i] &= (a0 > 0x7c00u ? 0u : 0xffffu) | (a1 > 0x7c00u ? 0u : 0xffff0000u);
                     }
-                    if (bad >> g & 1u) raw.ks[i] |= 0x00007fffu;
-                    if (bad >> (8 + g) & 1u) raw.ks[i] |= 0x7fff0000u;
                 }
+                w5 = __reduce_or_sync(0xffffffffu, w5);
+                nan[0] = __reduce_or_sync(0xffffffffu, nan[0]);
+                nan[1] = __reduce_or_sync(0xffffffffu, nan[1]);
+                const auto scale = [&](int lo, int hi) { return (w5 >> lo & 1u ? 0x2800u : 0x3c00u) | (w5 >> hi & 1u ? 0x28000000u : 0x3c000000u); }; // 2^-5 or 1
+#pragma unroll
+                for (int i = 0; i < NG; i++) {
+                    raw.ks[i] = hmul2(raw.ks[i], scale(g, 8 + g));
+#pragma unroll
+                    for (int h = 0; h < 2; h++) dv[h][i] = hmul2(dv[h][i], scale(16 + 8 * h + 2 * t, 17 + 8 * h + 2 * t));
+                }
+                if (lane == 0) sh.odd[ks][w] = make_uint4(w5, nan[0], nan[1], w5 | nan[0] | nan[1]);
             }
-            if (j >= CHUNK_K_STAGES && !__all_sync(0xffffffffu, bar_wait(&sh.k_free[ks], k_phase, &sh.bail))) break; // the scores of tile j - 3 stand
 #pragma unroll
             for (int i = 0; i < NG; i++)
 #pragma unroll
@@ -458,6 +469,14 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
         const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16, row_s = tS + lanes + stream * CHUNK_KEYS + side * COLUMNS, row_o = tO + lanes + stream * CHUNK_KEYS;
         const float factor = sh.factor[r];
         unsigned met = 0;
+        int j = stream - 2; // the tile
+        const auto times32 = [](uint32_t (&x)[PIECE], uint32_t which) { // the low bits of `which`: whose numbers
+            if (which & 0xffffu)
+#pragma unroll
+                for (int i = 0; i < PIECE; i++)
+                    if (which >> i & 1u) x[i] = __float_as_uint(__uint_as_float(x[i]) * 32.0f);
+        };
+        const auto odds = [&](int q) -> const uint4 & { return sh.odd[j % CHUNK_K_STAGES][side * (CHUNK_RECORDS / 2) + q / PIECE]; }; // of the record of columns q on
         const auto meet = [&]() { // the two warps of a row; a wait with an end, as all here: one of them may have given up
             __syncwarp();
             if (lane == 0) bar_arrive(&sh.pair[warp % 8]);
@@ -471,7 +490,9 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
         float top = -CUDART_INF_F, l = 0.0f, sum = 0.0f; // the row's largest product so far; of this thread's positions the sum, and that of a tile that may yet be repeated
         bool ok = true, fresh = false;
         float base = 0.0f, ref = 0.0f; // top where there is one, times the factor
-        int from = 0, to = 0, j = stream - 2, next = 0; // the tile's positions [from, to) are seen, counted from this thread's first; the segment's end
+        int from = 0, to = 0, next = 0; // the tile's positions [from, to) are seen, counted from this thread's first; the segment's end
+        const auto rows = [&](auto marked) {
+        constexpr bool ODD = decltype(marked)::value; // (a body of its own: the other one keeps its registers)
         for (unsigned turn = 0; stream < count; turn++) {
             if (GIVE_UP && j + 2 >= count) {
                 *reinterpret_cast<volatile unsigned *>(&sh.bail) = 1u;
@@ -498,7 +519,8 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
             }
             // One pass with the maximum as it stands.  It moves rarely, and a sum of more than 2^8 shows that it has to: the probabilities, which have taken the place of the scores, are
             // dropped, the scores come once more, and the tile's maximum is looked for first.  (A maximum of every tile in front of or beside the exponentials cost as much as they do.)
-            const bool special = __any_sync(0xffffffffu, repeat || fresh || from > 0 || to < COLUMNS || !(fabsf(ref) <= 65536.0f));
+            const bool odd = ODD && __any_sync(0xffffffffu, odds(lane % (CHUNK_RECORDS / 2) * PIECE).w != 0u);
+            const bool special = odd || __any_sync(0xffffffffu, repeat || fresh || from > 0 || to < COLUMNS || !(fabsf(ref) <= 65536.0f));
             if (special && __any_sync(0xffffffffu, repeat || fresh)) { // (the same for both warps of a row)
                 float mx = -CUDART_INF_F;
 #pragma unroll 1
@@ -506,6 +528,7 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
                     uint32_t x[PIECE];
                     tmem_ld16(row_s + q, x);
                     tmem_ld_wait();
+                    if (odd) times32(x, odds(q).x);
 #pragma unroll
                     for (int i = 0; i < PIECE; i++) mx = fmaxf(mx, i >= from - q && i < to - q ? __uint_as_float(x[i]) : -CUDART_INF_F);
                 }
@@ -536,18 +559,29 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
                 sum = 0.0f;
 #pragma unroll 1
                 for (int q = 0; q < COLUMNS / 2; q += PIECE / 2) tmem_st8(row_s + q, p);
-            } else if (special && __any_sync(0xffffffffu, from > 0 || to < COLUMNS || !(fabsf(ref) <= 65536.0f))) { // a border, or scores so large that their products and the maximum's round apart
+            } else if (special && __any_sync(0xffffffffu, odd || from > 0 || to < COLUMNS || !(fabsf(ref) <= 65536.0f))) { // a border, entries outside FP16, or scores so large that their products and the maximum's round apart
                 sum = 0.0f;
 #pragma unroll 1
                 for (int q = 0; q < COLUMNS; q += PIECE) {
                     uint32_t x[PIECE], p[PIECE / 2];
                     tmem_ld16(row_s + q, x);
                     tmem_ld_wait();
+                    if (odd) times32(x, odds(q).x);
 #pragma unroll
                     for (int i = 0; i < PIECE; i++) {
                         const float e = i >= from - q && i < to - q ? ex2((__uint_as_float(x[i]) - base) * factor) : 0.0f;
                         sum += e;
                         x[i] = __float_as_uint(e);
+                    }
+                    if (odd) {
+                        const uint4 at = odds(q);
+                        times32(x, at.x >> 16); // (at most 2^8 times that: FP16 holds it)
+                        if (at.y | at.z) {
+                            const int a = max(from - q, 0), b = min(to - q, PIECE);
+                            const unsigned seen = a < b ? (1u << b) - (1u << a) : 0u, both = seen | seen << 16;
+                            const unsigned groups = (at.y & both & 0xffffu ? 1u : 0u) | (at.y & both & 0xffff0000u ? 2u : 0u) | (at.z & both & 0xffffu ? 4u : 0u) | (at.z & both & 0xffff0000u ? 8u : 0u);
+                            if (groups) atomicOr(&sh.nan[r], groups);
+                        }
                     }
 #pragma unroll
                     for (int i = 0; i < PIECE / 2; i++) p[i] = pack_f16(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
@@ -589,6 +623,9 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
                 bar_arrive(&sh.p_full[stream]);
             }
         }
+        };
+        if (__any_sync(0xffffffffu, sh.marked != 0u)) rows(std::true_type());
+        else rows(std::false_type());
         sh.half_row[stream][side][r] = l;
         sh.top[stream][r] = top;
         fence_before();
@@ -615,6 +652,9 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
                 for (int u = 0; u < 16; u++) o[i + u] = __float_as_uint(fmaf(h ? a1 : a0, __uint_as_float(x[u]), __uint_as_float(o[i + u])));
             }
         }
+        if (sh.nan[r] >> q & 1u)
+#pragma unroll
+            for (int i = 0; i < 32; i++) o[i] = 0x7fffffffu;
         if (c.splits > 1) { // parts go through shared memory, where the queries were: 64 bytes of a row at a time in place of 4 (the rows' starts are 8-byte aligned)
             const long long part = on ? (((long long)row * a.heads + head) * c.splits + split) * (HS + 2) : -1;
             if (on && q == 0) { a.work[part] = top * factor; a.work[part + 1] = l; }

@@ -16,6 +16,7 @@ struct b200_kv4 {
     size_t bytes = 0;
     unsigned *host_error = nullptr, *device_error = nullptr; // a mapped word: what a wait that gave up leaves (kv4_chunk.cuh)
     char err[256] = "";
+    size_t marks_bytes() const { return (size_t)view.slots * 4; } // behind the records: View::odd
 };
 
 namespace {
@@ -278,14 +279,15 @@ int b200_kv4_create(int32_t slots, int32_t context, int32_t kv_heads, int32_t he
     kv->head_size = head_size;
     kv->device = device;
     kv->sms = sm_count(device);
-    kv->view = {nullptr, slots, context, (context + kv4::BLOCK - 1) / kv4::BLOCK, kv_heads};
+    kv->view = {nullptr, nullptr, slots, context, (context + kv4::BLOCK - 1) / kv4::BLOCK, kv_heads};
     const unsigned __int128 bytes = (unsigned __int128)slots * kv_heads * kv->view.blocks * kv4::record_bytes(head_size);
     OnDevice on(device);
     e = on.error;
-    if (e == cudaSuccess) e = bytes > ((unsigned __int128)1 << 48) ? cudaErrorMemoryAllocation : cudaMalloc((void **)&kv->view.base, (size_t)bytes);
+    if (e == cudaSuccess) e = bytes > ((unsigned __int128)1 << 48) ? cudaErrorMemoryAllocation : cudaMalloc((void **)&kv->view.base, (size_t)bytes + kv->marks_bytes());
     if (e == cudaSuccess) {
         kv->bytes = (size_t)bytes;
-        e = cudaMemset(kv->view.base, 0, kv->bytes);
+        kv->view.odd = reinterpret_cast<unsigned *>(kv->view.base + kv->bytes); // (records are multiples of 64 bytes)
+        e = cudaMemset(kv->view.base, 0, kv->bytes + kv->marks_bytes());
         if (e == cudaSuccess) e = cudaDeviceSynchronize(); // the memory is zeros for every stream
     }
     // the word through which a wait that gave up is heard of: no cache without it
@@ -321,7 +323,7 @@ int b200_kv4_reset(b200_kv4 *kv, void *stream) {
     if (!kv) return B200_ERR_BAD_ARG;
     OnDevice on(kv->device);
     cudaError_t e = on.error;
-    if (e == cudaSuccess) e = cudaMemsetAsync(kv->view.base, 0, kv->bytes, (cudaStream_t)stream);
+    if (e == cudaSuccess) e = cudaMemsetAsync(kv->view.base, 0, kv->bytes + kv->marks_bytes(), (cudaStream_t)stream);
     return e == cudaSuccess ? B200_OK : fail(kv, cuda_code(e), "%s", cudaGetErrorString(e));
 }
 
