@@ -177,7 +177,7 @@ static ChunkCut chunk_cut(const b200_kv4 *kv, const b200_kv4_attention_args &a, 
     const int most = kv4::CHUNK_ROWS / mul, shares = (chunk + most - 1) / most;
     c.tokens = (chunk + shares - 1) / shares;
     const long long units = (long long)((a.n + c.tokens - 1) / c.tokens) * G;
-    const long long seen = a.window > 0 && a.window + c.tokens < len ? a.window + c.tokens : len, worth = seen / (8 * kv4::CHUNK_KEYS); // eight tiles of positions a CTA
+    const long long near = (long long)a.window + c.tokens, seen = a.window > 0 && near < len ? near : len, worth = seen / (8 * kv4::CHUNK_KEYS); // eight tiles of positions a CTA
     long long splits = kv->sms / units;
     if (splits > worth) splits = worth;
     c.splits = splits < 1 ? 1 : (int)splits;
