@@ -179,9 +179,12 @@ struct Cache {
         check(b200_kv4_reset(kv, stream()));
     }
     int64_t bytes() const { return b200_kv4_device_bytes(kv); }
-    void free() {
-        b200_kv4_free(kv);
+    void free() { // waits for the device: not with the interpreter's lock, and not with a pointer that another thread could still use
+        b200_kv4 *gone = kv;
         kv = nullptr;
+        if (!gone) return;
+        py::gil_scoped_release others;
+        b200_kv4_free(gone);
     }
 };
 
@@ -189,7 +192,11 @@ Cache *create(int64_t slots, int64_t context, int64_t kv_heads, int64_t head_siz
     NEED(std::max({slots, context, kv_heads, head_size}) <= INT32_MAX && std::min({slots, context, kv_heads, head_size}) >= INT32_MIN, "sizes outside 32 bits");
     b200_kv4 *kv = nullptr;
     char err[256] = "";
-    const int rc = b200_kv4_create((int32_t)slots, (int32_t)context, (int32_t)kv_heads, (int32_t)head_size, (int32_t)device, &kv, err, sizeof err);
+    int rc;
+    {
+        py::gil_scoped_release others; // (it waits for the device)
+        rc = b200_kv4_create((int32_t)slots, (int32_t)context, (int32_t)kv_heads, (int32_t)head_size, (int32_t)device, &kv, err, sizeof err);
+    }
     if (rc != B200_OK) refused(rc, err);
     return new Cache(kv, slots, context, kv_heads, head_size, (int)device);
 }
