@@ -1,6 +1,7 @@
 // torch_ops.cpp -- the operators of operators.cu on torch tensors (operators.py has their documentation): checks of the tensors, the current stream, results from torch's allocator.
 // A call through Python's ctypes costs 15 to 20 us of host time, more than most of these kernels run; here it is about 5.
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
@@ -40,6 +41,11 @@ int type_of(at::ScalarType t, const char *what) {
     return -1;
 }
 
+// There are no backward passes: a graph that led through a call would end there without a word.
+void outside_graph(const Tensor &t, const char *name) {
+    NEED(!t.requires_grad() || !at::GradMode::is_enabled(), name, " requires a gradient, and the operators have none: detach it, or call under torch.no_grad()");
+}
+
 // A new tensor on a device, without the dispatcher (1 us of at::empty's 2).
 Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, int device) {
     return at::detail::empty_cuda(sizes, type, at::Device(at::kCUDA, (c10::DeviceIndex)device), std::nullopt);
@@ -66,6 +72,7 @@ struct Cache {
     int64_t rows(const Tensor &t, const char *name, int64_t n, int64_t heads) const {
         NEED(t.defined() && t.dim() == 3 && t.size(0) == n && t.size(1) == heads && t.size(2) == head_size, name, ": [", n, ", ", heads, ", ", head_size, "] is wanted, got ", shape(t));
         NEED(t.is_cuda() && t.get_device() == device, name, " is on ", t.device(), ", the cache on cuda:", device);
+        outside_graph(t, name);
         NEED(n == 0 || (t.stride(2) == 1 && (t.stride(1) == head_size || heads == 1)), name, ": the heads of a row have to lie one behind the other");
         return n > 1 ? t.stride(0) : heads * head_size;
     }
@@ -79,6 +86,7 @@ struct Cache {
     }
     const float *vector(const Maybe &t, const char *name, int64_t least, int64_t width) const {
         if (!t) return nullptr;
+        outside_graph(*t, name);
         NEED(t->scalar_type() == at::kFloat && t->is_cuda() && t->get_device() == device && t->is_contiguous(), name, ": a contiguous FP32 tensor on cuda:", device, " is wanted");
         NEED(least ? t->dim() == 2 && t->size(0) >= least && t->size(1) == width : t->dim() == 1 && t->size(0) == width, name, ": has the shape ", t->sizes());
         return t->data_ptr<float>();
@@ -203,6 +211,7 @@ Cache *create(int64_t slots, int64_t context, int64_t kv_heads, int64_t head_siz
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> log_probs(const Tensor &logits, const Maybe &targets, int64_t top) {
     NEED(logits.defined() && logits.dim() == 2 && logits.is_cuda(), "logits: rows [rows, vocab] on a GPU are wanted, got ", shape(logits));
+    outside_graph(logits, "logits");
     const int64_t rows = logits.size(0), vocab = logits.size(1);
     b200_log_probs_args a = {};
     a.type = type_of(logits.scalar_type(), "logits");
