@@ -87,11 +87,10 @@ cudaError_t launch(void (*kern)(KA...), unsigned grid, int block, size_t smem, i
     cfg.numAttrs = n;
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KA>(args)...);
 }
-// Shared memory limit and cluster size of a kernel, set in front of every launch of it: an attribute of the function in the current device's context, so that nothing is kept here
-// by device or by thread (0.2 us).
-template <typename K> cudaError_t prepare(K kern, size_t smem, int cluster) {
-    cudaError_t e = smem > 48 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
-    return e;
+// Shared memory limit of a kernel, set in front of every launch that needs more than the usual 48 KB: an attribute of the function in the current device's context, so that nothing is kept
+// here by device or by thread (0.2 us).
+template <typename K> cudaError_t allow_smem(K kern, size_t smem) {
+    return smem > 48 * 1024 ? cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
 }
 bool refused(const char *step) { // (as in plan.cu: what tests refuse)
     const char *e = getenv("B200_TEST_REFUSE");
@@ -161,6 +160,7 @@ static size_t parts_bytes(const b200_kv4 *kv, const b200_kv4_attention_args &a, 
 // Chunks on the tensor cores: 16-bit results, heads of 64, 96 or 128.  A tile takes 128 rows whether they are used or not, single rows read the cache once each.  us as single rows / as a chunk,
 // by rows (tokens x query heads of a key/value head):  32/8 heads of 128, 8192 positions: 32 rows 29/25, 64 rows 53/25, 128 rows 76/27;  1024 positions: 11/21, 17/21, 29/23;
 // 32/8 heads of 64, 8192: 21/23, 33/23, 47/23;  16/16 of 64, 4096: 41/23 (32 rows), 66/23;  8/1 of 128, 8192: 17/25, 17/25, 17/27, 60/27 (512 rows).
+// The rule looks at a key/value head's rows alone: 64 of them over 1024 positions, and 64 to 128 of a single head, take the slower form, by 4 to 10 us.
 const int CHUNK_MIN_ROWS = 64;
 struct ChunkCut {
     int tokens, splits;
@@ -212,7 +212,7 @@ static cudaError_t attention_launch(const b200_kv4 *kv, const b200_kv4_attention
             constexpr size_t smem = kv4::chunk_smem_bytes(hs);
             auto kern = kv4::k_chunk<hs>;
             if constexpr (hs == 64) if (give_up) kern = kv4::k_chunk<hs, true>;
-            cudaError_t e = prepare(kern, smem, 1);
+            cudaError_t e = allow_smem(kern, smem);
             if (e == cudaSuccess) e = launch(kern, grid, kv4::CHUNK_THREADS, smem, 1, pdl, stream, ck);
             return e != cudaSuccess || cc.splits == 1 ? e : join(hs, cc.splits);
         };
@@ -230,7 +230,7 @@ static cudaError_t attention_launch(const b200_kv4 *kv, const b200_kv4_attention
             const unsigned grid = (unsigned)a.n * kv->view.kv_heads * c.per_head * c.splits * c.cluster;
             k.by_length = a.positions && a.n > 1 && a.n <= kv4::STEP_ORDERED && grid > 2u * kv->sms;
             auto kern = kv4::k_step<hs, nt>;
-            cudaError_t e = prepare(kern, smem, c.cluster);
+            cudaError_t e = allow_smem(kern, smem);
             if (e == cudaSuccess) e = launch(kern, grid, kv4::STEP_WARPS * 32, smem, c.cluster, pdl, stream, k, c.per_head, c.splits);
             return e != cudaSuccess || c.splits == 1 ? e : join(hs, c.splits);
         };
@@ -256,9 +256,7 @@ cudaError_t log_probs_launch(const b200_log_probs_args &a, cudaStream_t stream) 
     const long long most = (a.vocab + 2047) / 2048;
     const int cluster = cluster_for(a.rows, 4LL * sm_count(a.device), most < lp::MAX_CLUSTER ? most : lp::MAX_CLUSTER);
     return by_type(a.type, [&](auto type) {
-        auto kern = lp::k_log_probs<decltype(type)>;
-        cudaError_t e = prepare(kern, 0, cluster);
-        return e != cudaSuccess ? e : launch(kern, (unsigned)a.rows * cluster, lp::THREADS, 0, cluster, false, stream, k);
+        return launch(lp::k_log_probs<decltype(type)>, (unsigned)a.rows * cluster, lp::THREADS, 0, cluster, false, stream, k);
     });
 }
 
