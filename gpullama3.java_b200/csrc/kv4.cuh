@@ -112,7 +112,8 @@ __device__ __forceinline__ void quantize8(const float (&x)[8], unsigned lanes, _
 
 // Lanes of a head: 8 entries each, so that pairs of neighbours lie in a lane, pairs half a head apart in lanes half the head's lanes apart, and a group in four lanes.
 // A segment of WIDTH lanes (a power of two) serves one head, 32 / WIDTH heads a warp.  Bytes are its floor: 512 rows of (32 + 2 * 8) heads of 128 with norms and
-// rotation read 12.6 MB and write 9.0, 3.8 us; it takes 16.4 with the call, of which the host and the launch are 6, the rest one wave of warps: load, reduce, normalise, turn, quantise, store.
+// rotation read 12.6 MB and write 9.0, 3.8 us; it takes 11.5 (1.12 TB/s), with the call 16.4.  1536 CTAs at 8 an SM are 1.3 waves of warps that
+// load, reduce, normalise, turn, quantise and store one after the other: per issued instruction 7.4 wait for a load, 2.7 for a fixed latency, 2.6 for shuffles; codes leave in 2 and 4 bytes.
 // (Tables asked for in front of the norm, which they do not need: more registers, 18-19 us.)
 template <int HS, typename T> __global__ void __launch_bounds__(256) k_append(const Append a) {
     constexpr int L = HS / 8, WIDTH = L == 4 ? 4 : L == 8 ? 8 : L <= 16 ? 16 : 32, PER_WARP = 32 / WIDTH;
@@ -379,8 +380,9 @@ __device__ __forceinline__ int row_by_length(const Step &a, int rank, int *lengt
 //   scores  C[16 positions x 8] = codes x queries in FP16; the eight columns are four heads, each as a high and a low part, so that a query keeps 22 bits; scaled group by group in FP32
 //   values  C[16 entries x 8] = codes x (p d), again as a high and a low part.  p d is kept in FP16's range by a power of two that follows the largest value scale seen so far
 // A lane keeps the running sums of ONE head (t); what crosses lanes in the loop is the transposition of the probabilities and, where a maximum grows by more than 2^8, its update.
-// Bytes are its floor: 131071 positions of 8 heads of 128 are 151 MB, 23.4 us; it takes 36.6 (4.1 TB/s), 43.0 with the join.  What bounds it is issue slots: a record of 2304 bytes costs a warp
-// about 300 instructions, half of them turning codes into FP16.  (The codes as they stand, subnormal FP16: fewer instructions, errors of 1e-5.)
+// Bytes are its floor: 131071 positions of 8 heads of 128 are 151 MB, 23.4 us; it takes 36.5 (4.2 TB/s), 43.0 with the join and its gap.  What bounds it is how few warps an SM
+// holds (two CTAs: 123 registers, 110 KB) and each one's chain: a record of 2304 bytes costs a warp about 300 instructions, half of them turning codes into FP16; a scheduler's four warps
+// issue in 63 % of the cycles, with 1.5 of them ready, and wait for the arithmetic pipes (1.0 per issue), fixed latencies (0.65) and their records (0.56).  (The codes as they stand, subnormal FP16: fewer instructions, errors of 1e-5.)
 template <int HS, int NT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_step(const Step a, const int units_per_head, const int splits) {
     constexpr int NG = groups(HS), VW = vec_words(HS), R = record_bytes(HS), KB = step_records(HS), S = step_stages(HS), H = 4 * NT, CHUNKS = R / 16;
     extern __shared__ __align__(16) unsigned char smem[];

@@ -7,14 +7,14 @@
 // A tile's work is a chain: scores, exponentials, product, about 5000 cycles of which 1024 are the tensor cores' and 1024 the exponentials' (16 a cycle).  So even and odd tiles are two
 // streams with accumulators, maxima and sums of their own, each of eight warps, which the end joins: while one waits for its products the other computes.  Heads of 128, two streams of
 // scores and results: all 512 columns of TMEM.
-// Measured (512 tokens, 32 heads over 8 of 128, 8192 positions: 66.6 GFLOP): 102 us (99-109 from box to box), 650 TFLOP/s, 39 % of the 1690 measured.  A tile takes 2300 cycles: its 16
+// Measured (512 tokens, 32 heads over 8 of 128, 8192 positions: 66.6 GFLOP): 104 us (99-109 from box to box), 640 TFLOP/s, 38 % of the 1690 measured.  A tile takes 2300 cycles: its 16
 // products 1400 (1024 were nothing else at shared memory), beside them the conversion of its records, one a warp, 2400 with what it waits for; 0.57 instructions a cycle and scheduler.
 // One stream with two S and a maximum agreed on by a row's threads in every tile took 116-123 us; 256 rows a CTA with half the conversions 133 us (two blocks of rows in place of the two
 // streams; 64 pairs of CTAs whose parts had to be joined).
 // Rounding: queries (times a power of two), keys, values and probabilities are FP16 operands, sums are FP32.  Entries of a position outside FP16 (a scale above 8184: codes of up to 8 times
 // that) become operands times 2^-5, and the position's scores, or its probabilities as operands, times 2^5.  A value's NaN stays out of the product, where 0 * NaN would reach every row: the
 // rows that see it note its group, and write NaN there.  The append marks the slots that have taken such an entry (kv4.cuh), and only CTAs that meet a marked slot look for them: looked for in
-// every tile they cost 9 % (104 us became 113); as it is the time of unmarked slots is what it was.
+// every tile they cost 9 % (104 us became 113); so the time of other slots is what it was, and 123 us in place of 97 for calls back to back where one position of a marked slot is such a one.
 //
 // Rows of a tile may belong to several slots and stand in any order: a run of tokens of one slot is a segment, the tiles of all segments are one list, and a row masks what is not its own.
 // Every wait is bounded: after 2^25 tries the CTA gives up, waits for its products under way, frees its tensor memory and, whichever warp it was, writes the cache's error word.
