@@ -211,6 +211,7 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
             slot = a.rows.slot_of(token0 + tid);
             pos = a.rows.position(token0 + tid);
             if (slot < 0 || slot >= a.kv.slots || pos >= a.kv.context) slot = pos = -1; // padding
+            pos = max(pos, -1); // (positions are subtracted from, and both warps of a row have to find the same)
         }
         sh.slot[tid] = slot;
         sh.pos[tid] = pos;

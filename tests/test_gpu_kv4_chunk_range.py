@@ -126,3 +126,20 @@ def test_entries_outside_fp16_beside_padding_and_other_sequences(pkg):
     assert (out[9] == 7.5).all() and (out[7] == 0).all()
     live = (at == 0) & (pos >= 0)
     check(out[live], q[live], k[:1], v[:1], (d[0][:1], d[1][:1]), pos[live], U.rsqrt(hs), 0, BF16)
+
+
+@pytest.mark.parametrize("hs", [64, 128])
+def test_rows_of_the_lowest_position_see_nothing(pkg, hs):
+    """A row of a negative position has no keys, be it -1 or the lowest number, also beside rows that see NaN and infinities: zeros."""
+    H, G, context, n = 4, 1, 300, 128
+    cache, _, _, _ = filled(pkg, 1, context, G, hs, 4)
+    at = ints(3, 150, 290)
+    odd = torch.full((3, G, hs), float("nan"), device="cuda")
+    cache.append(odd, odd, at)
+    q = rand(gen(1), n, H, hs)
+    pos = torch.arange(context - n, context, device="cuda", dtype=torch.int32)
+    pos[::5], pos[1::5], pos[2::5], pos[3::5] = -2**31, -1, -2**31 + 300, -300
+    for window in (0, 50):
+        got = cache.attention(q, pos, window=window, chunk=n, dtype=BF16)
+        assert (got[pos < 0] == 0).all()
+        assert torch.equal(torch.isnan(got), torch.isnan(cache.attention(q, pos, window=window, dtype=BF16)))
