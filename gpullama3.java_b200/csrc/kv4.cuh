@@ -28,7 +28,7 @@ __host__ __device__ constexpr int record_bytes(int hs) { return 18 * hs; }
 
 struct View {
     unsigned char *base;
-    unsigned *odd; // by slot: has it taken a group whose scale is beyond KV4_ODD or NaN (for as long as the cache is not reset)
+    unsigned *odd; // by slot: has it taken a group whose scale is beyond KV4_ODD or NaN (for as long as the cache is not reset); behind the slots: has a chunk's attention given up a wait
     int slots, context, blocks, kv_heads; // blocks of a head and slot
 };
 constexpr unsigned KV4_ODD = 0x6ffe; // FP16 bits of 8184: entries of up to 8 times a larger scale may lie outside FP16

@@ -17,7 +17,7 @@
 // every tile they cost 9 % (104 us became 113); so the time of other slots is what it was, and 123 us in place of 97 for calls back to back where one position of a marked slot is such a one.
 //
 // Rows of a tile may belong to several slots and stand in any order: a run of tokens of one slot is a segment, the tiles of all segments are one list, and a row masks what is not its own.
-// Every wait is bounded: after 2^25 tries the CTA gives up, waits for its products under way, frees its tensor memory and, whichever warp it was, writes the cache's error word.
+// Every wait is bounded: after two seconds the CTA gives up, waits for its products under way, frees its tensor memory and, whichever warp it was, writes the cache's error word.
 #pragma once
 #include <type_traits>
 
@@ -51,7 +51,7 @@ __host__ __device__ constexpr size_t chunk_smem_bytes(int hs) { return 1024 + (1
 __device__ __forceinline__ uint32_t s32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void bar_init(const void *bar, unsigned n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(s32(bar)), "r"(n)); }
 __device__ __forceinline__ void bar_arrive(const void *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(s32(bar)) : "memory"); }
-constexpr unsigned WAIT_TRIES = 1u << 25; // a second or more
+constexpr unsigned WAIT_TRIES = 1u << 19; // about two seconds of a warp's own time: a try sleeps for some 4 us where nothing comes (2^25 of them took minutes)
 __device__ __forceinline__ bool bar_passed(uint32_t bar, unsigned parity) {
     unsigned done;
     asm volatile("{.reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p;}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
@@ -167,7 +167,7 @@ struct Chunk {
     unsigned *error; // the cache's error word (mapped host memory)
 };
 
-// GIVE_UP (tests): the warps of the rows take their last wait, for the products that end a stream, as run out.
+// GIVE_UP (tests): for their last wait, that for the products that end a stream, the warps of the rows wait for a barrier at which nobody arrives.
 template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_THREADS, 1) k_chunk(const Chunk c) {
     constexpr int NG = groups(HS);
     extern __shared__ unsigned char raw_smem[];
@@ -245,6 +245,7 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
     }
     __syncthreads();
     if (tid < tokens && sh.slot[tid] >= 0 && a.kv.odd[sh.slot[tid]] != 0u) sh.marked = 1u;
+    if (tid == CHUNK_ROWS && a.kv.odd[a.kv.slots] != 0u) sh.bail = 1u; // an earlier CTA has given up: none waits as long again
     if (warp == 0) { // one slot for all, as inside a prompt: one segment
         bool same = sh.slot[0] >= 0;
         int from = INT32_MAX, to = 0;
@@ -496,7 +497,7 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
         constexpr bool ODD = decltype(marked)::value; // (a body of its own: the other one keeps its registers)
         for (unsigned turn = 0; stream < count; turn++) {
             if (GIVE_UP && j + 2 >= count) {
-                *reinterpret_cast<volatile unsigned *>(&sh.bail) = 1u;
+                bar_wait(&sh.pair[warp % 8], met & 1, &sh.bail);
                 break;
             }
             ok = __all_sync(0xffffffffu, bar_wait(&sh.s_full[stream], turn & 1, &sh.bail));
@@ -701,7 +702,7 @@ template <int HS, bool GIVE_UP = false> __global__ void __launch_bounds__(CHUNK_
         fence_before();
     }
     __syncthreads();
-    if (tid == 0 && sh.bail != 0u) *reinterpret_cast<volatile unsigned *>(c.error) = 1u;
+    if (tid == 0 && sh.bail != 0u) *reinterpret_cast<volatile unsigned *>(c.error) = a.kv.odd[a.kv.slots] = 1u;
     if (warp == CHUNK_SOFTMAX) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");

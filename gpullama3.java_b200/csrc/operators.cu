@@ -16,7 +16,7 @@ struct b200_kv4 {
     size_t bytes = 0;
     unsigned *host_error = nullptr, *device_error = nullptr; // a mapped word: what a wait that gave up leaves (kv4_chunk.cuh)
     char err[256] = "";
-    size_t marks_bytes() const { return (size_t)view.slots * 4; } // behind the records: View::odd
+    size_t marks_bytes() const { return (size_t)view.slots * 4; } // behind the records: View::odd, and a word that no reset clears
 };
 
 namespace {
@@ -281,11 +281,11 @@ int b200_kv4_create(int32_t slots, int32_t context, int32_t kv_heads, int32_t he
     const unsigned __int128 bytes = (unsigned __int128)slots * kv_heads * kv->view.blocks * kv4::record_bytes(head_size);
     OnDevice on(device);
     e = on.error;
-    if (e == cudaSuccess) e = bytes > ((unsigned __int128)1 << 48) ? cudaErrorMemoryAllocation : cudaMalloc((void **)&kv->view.base, (size_t)bytes + kv->marks_bytes());
+    if (e == cudaSuccess) e = bytes > ((unsigned __int128)1 << 48) ? cudaErrorMemoryAllocation : cudaMalloc((void **)&kv->view.base, (size_t)bytes + kv->marks_bytes() + 4);
     if (e == cudaSuccess) {
         kv->bytes = (size_t)bytes;
         kv->view.odd = reinterpret_cast<unsigned *>(kv->view.base + kv->bytes); // (records are multiples of 64 bytes)
-        e = cudaMemset(kv->view.base, 0, kv->bytes + kv->marks_bytes());
+        e = cudaMemset(kv->view.base, 0, kv->bytes + kv->marks_bytes() + 4);
         if (e == cudaSuccess) e = cudaDeviceSynchronize(); // the memory is zeros for every stream
     }
     // the word through which a wait that gave up is heard of: no cache without it

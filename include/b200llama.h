@@ -545,7 +545,7 @@ int b200_kv4_append(b200_kv4 *kv, const b200_kv4_append_args *args, void *stream
  * 2.4e-3 (1.7e-3).  FP32 results keep 22 bits of a query and exact keys and values.  What the cache holds outside FP16, and NaN, counts as it stands in every form.
  * max_len (0: unknown), the largest position + 1 as far as the host knows, only chooses how the work is split.  So does a workspace: few rows over many positions fill the GPU where the
  * call gets b200_kv4_attention_workspace(kv, args) bytes (0: it needs none) of 16-byte aligned device memory, whose content before and after does not matter
- * and which no other call under way may use; NULL or fewer bytes: the call does without.  Waits inside the kernels end after a second or more; should one ever run out, the rows are not
+ * and which no other call under way may use; NULL or fewer bytes: the call does without.  Waits inside the kernels end after two seconds; should one ever run out, the rows are not
  * written, and every later attention of this cache, once the kernel has ended, is B200_ERR_STATE: it can only be freed. */
 typedef struct b200_kv4_attention_args {
     int32_t n, heads, window, max_len, chunk, out_type;
@@ -570,7 +570,7 @@ typedef struct b200_kv4_read_args {
 } b200_kv4_read_args;
 int b200_kv4_read(b200_kv4 *kv, const b200_kv4_read_args *args, void *stream);
 
-/* Test hook: the attention of a chunk (heads of 64) whose last waits count as run out. */
+/* Test hook: the attention of a chunk (heads of 64) whose rows, at the end, wait for what never comes. */
 int b200_test_kv4_give_up(b200_kv4 *kv, const b200_kv4_attention_args *args, void *stream);
 /* Test hook (host only): how attention of n single rows is cut on a GPU of `sms` SMs: cut[4] = {query heads of a unit, units of a row and key/value head, CTAs of a cluster, clusters of
  * a unit}; quants: with results in blocks of 32 quants, as Q8_0 plans take them. */
