@@ -1249,7 +1249,7 @@ static int ly_batch(b200_plan *p, const int32_t *tokens, int n, int start_pos, c
     Layered &Y = *p->ly;
     const int E = Y.c.width, V = Y.c.vocab_size;
     if (n > Y.cap) return fail(p, B200_ERR_BAD_ARG, "chunk of %d tokens exceeds prefill_batch_size %d", n, Y.cap);
-    if (start_pos < 0 || start_pos + n > Y.c.context_length) return fail(p, B200_ERR_BAD_ARG, "positions %d..%d outside the context (%d)", start_pos, start_pos + n - 1, Y.c.context_length);
+    if (start_pos < 0 || n > Y.c.context_length - start_pos) return fail(p, B200_ERR_BAD_ARG, "positions %d..%lld outside the context (%d)", start_pos, (long long)start_pos + n - 1, Y.c.context_length);
     for (int i = 0; i < n; i++)
         if (tokens[i] < 0 || tokens[i] >= V) return fail(p, B200_ERR_BAD_ARG, "token %d out of range", tokens[i]);
     for (int i = 0; i < n_rows; i++)

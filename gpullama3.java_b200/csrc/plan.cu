@@ -2025,7 +2025,7 @@ int b200_forward_batch_prefill(b200_plan *p, const int32_t *tokens, int32_t n, i
     if (n <= 0) return B200_OK;
     if (!p->g_prefill) return fail(p, B200_ERR_STATE, "tensor-parallel plan: call b200_tp_attach on every rank first");
     if (p->prefill_batch > 1 && n > p->prefill_batch) return fail(p, B200_ERR_BAD_ARG, "chunk of %d tokens exceeds prefill_batch_size %d", n, p->prefill_batch);
-    if (start_pos < 0 || start_pos + n > p->cfg.context_length) return fail(p, B200_ERR_BAD_ARG, "positions %d..%d outside the KV cache", start_pos, start_pos + n - 1);
+    if (start_pos < 0 || n > p->cfg.context_length - start_pos) return fail(p, B200_ERR_BAD_ARG, "positions %d..%lld outside the KV cache", start_pos, (long long)start_pos + n - 1);
     for (int i = 0; i < n; i++)
         if (tokens[i] < 0 || tokens[i] >= p->cfg.vocab_size) return fail(p, B200_ERR_BAD_ARG, "token %d out of range", tokens[i]);
     CK(cudaSetDevice(p->device));
@@ -2067,7 +2067,7 @@ int b200_decode_sequence(b200_plan *p, const int32_t *tokens, int32_t n, int32_t
     if (n <= 0) return B200_OK;
     if (!p->g_decode) return fail(p, B200_ERR_STATE, "tensor-parallel plan: call b200_tp_attach on every rank first");
     if (n > p->seq_cap) return fail(p, B200_ERR_BAD_ARG, "sequence of %d steps exceeds capacity %d", n, p->seq_cap);
-    if (start_pos < 0 || start_pos + n > p->cfg.context_length) return fail(p, B200_ERR_BAD_ARG, "positions %d..%d outside the KV cache (%d)", start_pos, start_pos + n - 1, p->cfg.context_length);
+    if (start_pos < 0 || n > p->cfg.context_length - start_pos) return fail(p, B200_ERR_BAD_ARG, "positions %d..%lld outside the KV cache (%d)", start_pos, (long long)start_pos + n - 1, p->cfg.context_length);
     int nt = feedback ? 1 : n;
     for (int i = 0; i < nt; i++)
         if (tokens[i] < 0 || tokens[i] >= p->cfg.vocab_size) return fail(p, B200_ERR_BAD_ARG, "token %d out of range", tokens[i]);
