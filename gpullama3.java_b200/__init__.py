@@ -9,7 +9,7 @@ from .plan import B200MasterPlan  # noqa: F401
 
 
 def __getattr__(name):  # the operators work on torch tensors: torch is imported when they are asked for
-    if name in ("operators", "KV4Cache", "log_probs"):
+    if name in ("operators", "KV4Cache", "PagedKVCache", "log_probs", "verify_drafts"):
         import importlib
 
         operators = importlib.import_module(".operators", __name__)

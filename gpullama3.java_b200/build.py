@@ -9,20 +9,21 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libb200llama.so")
-SOURCES = ["plan.cu", "operators.cu"]
+SOURCES = ["plan.cu", "operators.cu", "serving.cu"]
 
 
-# Headers that only operators.cu reads: the other objects are not rebuilt for them.
-OPERATOR_HEADERS = ("kv4.cuh", "kv4_chunk.cuh", "logprobs.cuh")
+# Headers that plan.cu does not read: its object is not rebuilt for them.
+OPERATOR_HEADERS = {"operators.cu": ("kv4.cuh", "kv4_chunk.cuh", "logprobs.cuh", "operator_util.cuh"),
+                    "serving.cu": ("kv4.cuh", "logprobs.cuh", "operator_util.cuh", "paged.cuh", "verify.cuh")}
 
 
 def _deps(source: str | None = None):
     """What the library, or the object of one of its sources, is made from."""
     d = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    if source == "operators.cu":
-        d = [f for f in d if os.path.basename(f) in (*OPERATOR_HEADERS, "common.cuh", "operators.h")]
+    if source in OPERATOR_HEADERS:
+        d = [f for f in d if os.path.basename(f) in (*OPERATOR_HEADERS[source], "common.cuh", "operators.h")]
     elif source is not None:
-        d = [f for f in d if os.path.basename(f) not in OPERATOR_HEADERS]
+        d = [f for f in d if not any(os.path.basename(f) in h for h in OPERATOR_HEADERS.values())]
     d += [os.path.join(CSRC, f) for f in SOURCES if source in (None, f)]
     exp = os.path.join(CSRC, "experimental")
     if os.path.isdir(exp):

@@ -1,0 +1,648 @@
+// paged.cuh -- a 16-bit key/value cache in pages: append (head norms, rotation and rounding in one pass) and the attention of rows over the pages of their sequences.
+//
+// The pool is [page][key/value head][position of the page][entry], keys and values apart, FP16 or BF16; position p of a sequence lies in page table[p >> shift], row p & (2^shift - 1).
+// So the rows of a page and head are one contiguous stretch, and a row is named by one 32-bit number, (page * heads + head) * page_size + row.  A table entry outside the pool is no
+// page: nothing is stored there, and its positions are seen by nobody.
+#pragma once
+#include "kv4.cuh"
+
+namespace paged {
+
+using kv4::bf16;
+using kv4::cp_commit;
+using kv4::cp_wait;
+using kv4::ex2;
+using kv4::load8;
+using kv4::put;
+using kv4::visible;
+
+constexpr unsigned NO_ROW = 0xffffffffu;
+
+struct Pool {
+    void *keys, *values;
+    int pages, kv_heads, shift; // positions of a page: 2^shift
+};
+struct Rows { // row r stands at position positions[r] of sequence `sequences ? sequences[r] : 0`
+    const int *positions, *sequences, *tables;
+    long long ld_table;
+    int n, n_sequences, context; // context: positions that a table names
+    __device__ __forceinline__ int sequence_of(int r) const { return sequences ? sequences[r] : 0; }
+    // its sequence, or -1 for a padding row
+    __device__ __forceinline__ int place(int r, int &pos) const {
+        const int s = sequence_of(r);
+        pos = positions[r];
+        return s < 0 || s >= n_sequences || pos >= context ? -1 : s;
+    }
+    __device__ __forceinline__ const int *table(int s) const { return tables + s * ld_table; }
+};
+// The number of a head's row at a position, or NO_ROW.
+__device__ __forceinline__ unsigned row_at(const Pool &p, const int *table, int pos, int head) {
+    const int page = table[pos >> p.shift];
+    return (unsigned)page < (unsigned)p.pages ? (((unsigned)page * p.kv_heads + head) << p.shift) + (pos & ((1 << p.shift) - 1)) : NO_ROW;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) { return kv4::pack_f16(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack2<bf16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w) { return kv4::to_f32x2(w, (const T *)nullptr); }
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(bf16 v) { return __bfloat162float(v); }
+
+// ---- append ---------------------------------------------------------------------------------------------------------------------------------------------------
+struct Append {
+    Pool pool;
+    Rows rows;
+    const void *q, *k, *v;
+    long long ldq, ldk, ldv, ldo; // entries between rows
+    int heads;                    // query heads; 0: none
+    int interleaved, turned;      // turned: entries of a head that are rotated, its first ones
+    int vec, vec_out, vec_tables; // rows, query results and the rotation's rows start on 16-byte boundaries
+    const float *q_norm, *k_norm, *cos, *sin;
+    float eps;
+    void *q_out;
+};
+
+// Lanes of a head: 8 entries each; WIDTH lanes (a power of two) serve one head.  Mean of squares in 64 bits (FP32 squares leave FP32's range from 2^64 on).  Pairs of neighbours lie in a
+// lane; pairs half the rotated part apart lie in lanes a fixed distance apart where half of it is a multiple of 8, and are read once more from memory where it is not.
+template <int HS, typename T, typename C> __global__ void __launch_bounds__(256) k_paged_append(const Append a) {
+    constexpr int L = HS / 8, WIDTH = L <= 4 ? 4 : L <= 8 ? 8 : L <= 16 ? 16 : 32, PER_WARP = 32 / WIDTH;
+    const int lane = threadIdx.x & 31, li = lane & (WIDTH - 1), G = a.pool.kv_heads, total = a.heads + 2 * G;
+    const long long item = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / WIDTH;
+    const int row = (int)(item / total), which = (int)(item % total);
+    int pos = -1;
+    const int seq = row < a.rows.n ? a.rows.place(row, pos) : -1;
+    const bool on = seq >= 0 && pos >= 0, mine = on && li < L;
+    if (!__any_sync(0xffffffffu, on)) return; // (a whole warp: the shuffles below take every lane)
+    const bool is_q = which < a.heads, is_v = which >= a.heads + G;
+    const int head = is_q ? which : is_v ? which - a.heads - G : which - a.heads, e = li * 8;
+    const unsigned at = mine && !is_q ? row_at(a.pool, a.rows.table(seq), pos, head) : NO_ROW;
+    const T *src = (is_q ? (const T *)a.q + row * a.ldq : is_v ? (const T *)a.v + row * a.ldv : (const T *)a.k + row * a.ldk) + head * HS;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = 0.0f;
+    if (mine) load8(src + e, x, a.vec);
+    const float *norm = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+    float s = 1.0f;
+    if (a.q_norm || a.k_norm) {
+        double ss = 0.0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss = fma((double)x[i], (double)x[i], ss);
+#pragma unroll
+        for (int o = WIDTH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (norm && mine) {
+            s = (float)rsqrt(ss * (1.0 / HS) + (double)a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; i++) x[i] = norm[e + i] * (s * x[i]);
+        }
+    }
+    if (a.cos) {
+        const int half = a.turned / 2;
+        const float *cs = a.cos + (size_t)pos * half, *sn = a.sin + (size_t)pos * half;
+        const bool turns = mine && !is_v && e < a.turned;
+        if (a.interleaved) {
+            if (turns) {
+                float c[4], n[4];
+                if (a.vec_tables) {
+                    const float4 u = *reinterpret_cast<const float4 *>(cs + e / 2), w = *reinterpret_cast<const float4 *>(sn + e / 2);
+                    c[0] = u.x; c[1] = u.y; c[2] = u.z; c[3] = u.w;
+                    n[0] = w.x; n[1] = w.y; n[2] = w.z; n[3] = w.w;
+                } else
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const bool in = e + 2 * i < a.turned;
+                        c[i] = in ? cs[e / 2 + i] : 1.0f;
+                        n[i] = in ? sn[e / 2 + i] : 0.0f;
+                    }
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float u = x[2 * i], w = x[2 * i + 1];
+                    if (e + 2 * i >= a.turned) break;
+                    x[2 * i] = u * c[i] - w * n[i];
+                    x[2 * i + 1] = u * n[i] + w * c[i];
+                }
+            }
+        } else if (half % 8 == 0) {
+            const bool low = e < half;
+            const int partner = lane - li + (e < a.turned ? low ? li + half / 8 : li - half / 8 : li);
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i] = __shfl_sync(0xffffffffu, x[i], partner);
+            if (turns) {
+                float c[8], n[8];
+                load8(cs + (low ? e : e - half), c, a.vec_tables);
+                load8(sn + (low ? e : e - half), n, a.vec_tables);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = low ? x[i] * c[i] - y[i] * n[i] : y[i] * n[i] + x[i] * c[i];
+            }
+        } else if (turns) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int j = e + i;
+                if (j >= a.turned) break;
+                const bool low = j < half;
+                const int other = low ? j + half : j - half;
+                float y = to_f32(src[other]);
+                if (norm) y = norm[other] * (s * y);
+                const float c = cs[low ? j : j - half], n = sn[low ? j : j - half];
+                x[i] = low ? x[i] * c - y * n : y * n + x[i] * c;
+            }
+        }
+    }
+    if (!mine || (!is_q && at == NO_ROW)) return;
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = pack2<C>(x[2 * i], x[2 * i + 1]);
+    if (!is_q) *reinterpret_cast<uint4 *>((C *)(is_v ? a.pool.values : a.pool.keys) + (size_t)at * HS + e) = make_uint4(w[0], w[1], w[2], w[3]);
+    else {
+        uint16_t *o = (uint16_t *)a.q_out + row * a.ldo + head * HS + e;
+        if (a.vec_out) *reinterpret_cast<uint4 *>(o) = make_uint4(w[0], w[1], w[2], w[3]);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; i++) o[i] = (uint16_t)(w[i / 2] >> 16 * (i & 1));
+    }
+}
+
+// ---- attention ------------------------------------------------------------------------------------------------------------------------------------------------
+struct Step {
+    Pool pool;
+    Rows rows;
+    const void *q; // of the cache's type
+    long long ldq, ldo;
+    int heads, window, vec, vec_out, out_type;
+    float scale;
+    void *out;
+    int tokens, blocks, splits, share; // rows of a unit are `tokens` neighbouring ones, in `blocks` blocks; `splits` CTAs run through `share` tiles each (the last one through the rest)
+    float *work;                       // parts of units that several CTAs share: [row][head][split] entries, behind them [row][head][split] reference and sum
+};
+
+constexpr int STEP_WARPS = 4;
+__host__ __device__ constexpr int step_keys(int hs) { return hs >= 96 ? 16 : 32; }                        // positions that a warp takes at a time: a tile
+__host__ __device__ constexpr int step_stages(int hs) { return hs == 32 ? 4 : 3; }                        // tiles that it has room for
+__host__ __device__ constexpr int step_stage_bytes(int hs) { return step_keys(hs) * hs * 4; }             // keys and values
+__host__ __device__ constexpr int step_rows(int mt) { return 16 * mt; }
+__host__ __device__ constexpr int step_tokens_most() { return 32; }
+__host__ __device__ constexpr int part_stride(int hs) { return hs + 8; }
+__host__ __device__ constexpr size_t step_smem_bytes(int hs, int mt) {
+    const size_t ring = (size_t)STEP_WARPS * step_stages(hs) * step_stage_bytes(hs), parts = (size_t)STEP_WARPS * step_rows(mt) * part_stride(hs) * 4;
+    return (ring > parts ? ring : parts) + (size_t)step_rows(mt) * hs * 2;
+}
+
+__device__ __forceinline__ uint32_t s32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+template <typename T> __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) { kv4::mma_f16(d, a, b0, b1); }
+template <> __device__ __forceinline__ void mma<bf16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void cp16_or_zeros(bool on, uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
+// 16-byte piece c of row r of a tile whose rows are HS entries: eight neighbouring rows of a piece lie in different banks.
+template <int HS> __device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)(r * HS * 2 + ((HS % 64 == 0 ? c ^ (r & 7) : c ^ (r >> 1 & 3)) << 4)); }
+template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t w) { // 0xffff in the halves that are infinite or NaN
+    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    return ((w & E) == E ? 0xffffu : 0u) | ((w >> 16 & E) == E ? 0xffff0000u : 0u);
+}
+
+struct Segment { // a run of tokens of one sequence: tiles [begin, end) of its positions [lo, hi), those that any of them sees; tiles of all segments up to and with this one
+    int sequence, begin, end, lo, hi, tiles;
+};
+
+__device__ __forceinline__ void put_results(const Step &a, int row, int head, int hs, int e, float4 o) { // entries e .. e + 3 of a row's head
+    const long long at = row * a.ldo + (long long)head * hs + e;
+    const float x[4] = {o.x, o.y, o.z, o.w};
+    if (a.out_type == B200_GGML_F32) {
+        float *p = (float *)a.out + at;
+        if (a.vec_out) *reinterpret_cast<float4 *>(p) = o;
+        else
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = x[i];
+    } else {
+        const uint2 w = a.out_type == B200_GGML_F16 ? make_uint2(pack2<__half>(o.x, o.y), pack2<__half>(o.z, o.w)) : make_uint2(pack2<bf16>(o.x, o.y), pack2<bf16>(o.z, o.w));
+        uint16_t *p = (uint16_t *)a.out + at;
+        if (a.vec_out) *reinterpret_cast<uint2 *>(p) = w;
+        else {
+            p[0] = (uint16_t)w.x; p[1] = (uint16_t)(w.x >> 16);
+            p[2] = (uint16_t)w.y; p[3] = (uint16_t)(w.y >> 16);
+        }
+    }
+}
+
+// Rows (tokens x query heads of one key/value head) in blocks of 16 MT.  The tiles of positions that a block's rows see are split over CTAs and dealt to a CTA's warps in turn; each warp
+// has a cp.async ring and a running reference of its own, and no barrier in the loop.  Parts are joined in shared memory, those of several CTAs through the workspace (k_paged_join).
+// Nothing depends on an order of arrival.
+//   scores  S[16 rows x 8 positions] = Q K^T, the cache's type, exact products, FP32 sums;  p = 2^(scale log2(e) s - ref)
+//   values  O[16 rows x 8 entries] += P V with p as two numbers of the cache's type, p and what rounding it left: 16 (BF16) or 22 (FP16) bits, so that the result's rounding is what is left
+// ref follows the largest score seen so far only when that passes it by more than 2^8 (the first does), so that few tiles have anything to rescale; with FP16 it lies 2^7 below, so that
+// p reaches down to 2^-24 of 2^-15: a long tail of small ones still counts.
+// A value that is infinite or NaN would reach every row of the block as 0 * NaN, also those that do not see it.  A warp whose sums are not finite runs through its tiles once more with such
+// entries taken out of the product, and a product of zeros and ones says which rows have met one: those become NaN.  With BF16, where sums of large values may leave FP32's
+// range before they are divided, that second run has p times 2^-40.
+template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_paged_step(const Step a) {
+    constexpr int KT = step_keys(HS), NT = KT / 8, KS = KT / 16, S = step_stages(HS), ROWS = step_rows(MT), PIECES = HS / 8, STAGE = step_stage_bytes(HS), TOKENS = step_tokens_most();
+    constexpr bool F16 = std::is_same<T, __half>::value, QREG = MT == 1 && HS <= 128;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ Segment segments[TOKENS];
+    __shared__ int seq_of[TOKENS], pos_of[TOKENS], segment_of[TOKENS], n_segments;
+    __shared__ unsigned there[STEP_WARPS][S]; // positions of a tile that have a page
+    __shared__ float wref[STEP_WARPS][ROWS], wsum[STEP_WARPS][ROWS], weight[STEP_WARPS][ROWS];
+    unsigned char *sQ = smem + step_smem_bytes(HS, MT) - ROWS * HS * 2;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int G = a.pool.kv_heads, mul = a.heads / G;
+    const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % G, block = blockIdx.x / a.splits / G % a.blocks, unit = blockIdx.x / a.splits / G / a.blocks;
+    const int token0 = unit * a.tokens, tokens = min(a.tokens, a.rows.n - token0), row0 = block * ROWS, rows = min(ROWS, tokens * mul - row0);
+
+    if (tid < tokens) {
+        int pos;
+        const int s = a.rows.place(token0 + tid, pos);
+        seq_of[tid] = s;
+        pos_of[tid] = max(pos, -1);
+    }
+    for (int i = tid; i < ROWS * PIECES; i += STEP_WARPS * 32) {
+        const int r = i / PIECES, c = i % PIECES, token = (row0 + r) / mul;
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows) {
+            const uint16_t *q = (const uint16_t *)a.q + (long long)(token0 + token) * a.ldq + (size_t)(kvh * mul + row0 + r - token * mul) * HS + c * 8;
+            if (a.vec) w = *reinterpret_cast<const uint4 *>(q);
+            else w = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
+        }
+        *reinterpret_cast<uint4 *>(sQ + piece<HS>(r, c)) = w;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int n = 0, total = 0;
+        for (int i = 0; i < tokens;) {
+            const int s = seq_of[i];
+            int j = i, from = INT_MAX, to = 0;
+            for (; j < tokens && seq_of[j] == s; j++) {
+                int lo, hi;
+                visible(pos_of[j], a.window, lo, hi);
+                if (hi > lo) { from = min(from, lo); to = max(to, hi); }
+                segment_of[j] = n;
+            }
+            if (s >= 0 && to > 0) {
+                const int begin = from / KT, end = (to - 1) / KT + 1;
+                total += end - begin;
+                segments[n++] = {s, begin, end, from, to, total};
+            } else
+                for (int k = i; k < j; k++) segment_of[k] = -1;
+            i = j;
+        }
+        n_segments = n;
+    }
+    __syncthreads();
+    const int total = n_segments ? segments[n_segments - 1].tiles : 0;
+    const int first = (int)min((long long)split * a.share, (long long)total), last = split == a.splits - 1 ? total : min(total, first + a.share);
+    if (a.splits > 1 && first >= last) { // nothing for this CTA: its parts have no sum
+        float *w = a.work + (size_t)a.rows.n * a.heads * a.splits * HS;
+        if (tid < rows) {
+            const int token = (row0 + tid) / mul, head = kvh * mul + row0 + tid - token * mul;
+            reinterpret_cast<float2 *>(w)[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(-CUDART_INF_F, 0.0f);
+        }
+        return;
+    }
+
+    // rows 16 m + g and 16 m + 8 + g of this thread: what they see, within which segment
+    int lo[MT][2], hi[MT][2], own[MT][2];
+    int lo_most = 0, hi_least = INT_MAX;
+    bool one = true; // every row of the block is of the first segment
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = 16 * m + 8 * h + g, token = min((row0 + r) / mul, tokens - 1);
+            lo[m][h] = hi[m][h] = 0;
+            own[m][h] = r < rows ? segment_of[token] : 0;
+            if (r < rows && own[m][h] >= 0) visible(pos_of[token], a.window, lo[m][h], hi[m][h]);
+            if (r < rows && seq_of[token] >= 0) {
+                one &= own[m][h] == 0;
+                lo_most = max(lo_most, lo[m][h]);
+                hi_least = min(hi_least, hi[m][h]);
+            }
+        }
+    one = __all_sync(0xffffffffu, one);
+    lo_most = __reduce_max_sync(0xffffffffu, lo_most);
+    hi_least = __reduce_min_sync(0xffffffffu, hi_least);
+
+    const uint32_t ring = s32(smem) + warp * S * STAGE, q_at = s32(sQ);
+    // ldmatrix rows: keys: lanes 0-7 rows 0-7 piece 0, 8-15 the same rows piece 1, 16-31 rows 8-15; values (transposed): lanes 0-7 rows 0-7, 8-15 rows 8-15 of a piece, 16-31 of the next
+    const int k_row = (lane & 7) + (lane >> 4 << 3), k_piece = lane >> 3 & 1, v_row = lane & 15, v_piece = lane >> 4;
+    const float c = a.scale * 1.4426950408889634f;
+    uint32_t qf[QREG ? HS / 16 : 1][4];
+    if constexpr (QREG)
+#pragma unroll
+        for (int k = 0; k < HS / 16; k++) ldmatrix4(q_at + piece<HS>(v_row, 2 * k + v_piece), qf[k]);
+
+    float o[MT][HS / 8][4], l[MT][2], ref[MT][2];
+    for (int careful = 0;; careful = 1) {
+        const float below = F16 ? 7.0f : careful ? -40.0f : 0.0f;
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+#pragma unroll
+            for (int i = 0; i < HS / 8; i++) o[m][i][0] = o[m][i][1] = o[m][i][2] = o[m][i][3] = 0.0f;
+            l[m][0] = l[m][1] = 0.0f;
+            ref[m][0] = ref[m][1] = -CUDART_INF_F;
+        }
+        // this warp's tiles: numbers first + warp, + STEP_WARPS, .. of the list; `fetched` is the next to ask for, `seg_f` its segment
+        int fetched = first + warp, seg_f = 0, seg = 0;
+        auto look_up = [&]() -> unsigned { // the number of the row that this lane looks up for the tile `fetched`
+            if (fetched >= last) return NO_ROW;
+            while (segments[seg_f].tiles <= fetched) seg_f++;
+            const Segment &sg = segments[seg_f];
+            const int pos = (sg.end - (sg.tiles - fetched)) * KT + lane;
+            return lane < KT && pos >= sg.lo && pos < sg.hi ? row_at(a.pool, a.rows.table(sg.sequence), pos, kvh) : NO_ROW;
+        };
+        unsigned row = look_up();
+        auto fetch = [&](int stage) { // and look the next one up
+            if (fetched < last) {
+                const unsigned have = __ballot_sync(0xffffffffu, row != NO_ROW);
+                if (lane == 0) there[warp][stage] = have;
+                const uint32_t dst = ring + stage * STAGE;
+#pragma unroll
+                for (int i = 0; i < KT * PIECES / 32; i++) {
+                    const int n = lane + 32 * i, r = n / PIECES, p = n % PIECES;
+                    const unsigned from = __shfl_sync(0xffffffffu, row, r);
+                    const size_t off = from == NO_ROW ? 0 : ((size_t)from * HS + p * 8) * 2;
+                    cp16_or_zeros(from != NO_ROW, dst + piece<HS>(r, p), (const char *)a.pool.keys + off);
+                    cp16_or_zeros(from != NO_ROW, dst + KT * HS * 2 + piece<HS>(r, p), (const char *)a.pool.values + off);
+                }
+                fetched += STEP_WARPS;
+                row = look_up();
+            }
+            cp_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < S - 1; i++) fetch(i);
+        int stage = 0;
+        for (int tile = first + warp; tile < last; tile += STEP_WARPS) {
+            cp_wait<S - 2>();
+            __syncwarp(); // and every lane has read the tile before, whose place the next copies take
+            fetch(stage == 0 ? S - 1 : stage - 1);
+            const uint32_t kt = ring + stage * STAGE, vt = kt + KT * HS * 2;
+            float s[MT][NT][4];
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < HS / 16; k++) {
+                uint32_t qa[MT][4];
+#pragma unroll
+                for (int m = 0; m < MT; m++) {
+                    if constexpr (QREG) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) qa[m][i] = qf[k][i];
+                    } else ldmatrix4(q_at + piece<HS>(16 * m + v_row, 2 * k + v_piece), qa[m]);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t b[4];
+                    ldmatrix4(kt + piece<HS>(8 * n + k_row, 2 * k + k_piece), b);
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        mma<T>(s[m][n], qa[m], b[0], b[1]);
+                        mma<T>(s[m][n + 1], qa[m], b[2], b[3]);
+                    }
+                }
+            }
+            const unsigned have = there[warp][stage];
+            while (segments[seg].tiles <= tile) seg++;
+            const Segment &sg = segments[seg];
+            const int key0 = (sg.end - (sg.tiles - tile)) * KT;
+            // masks; the largest score of the thread's part of each row
+            const bool whole = one && key0 >= lo_most && key0 + KT <= hi_least && have == (KT == 32 ? 0xffffffffu : (1u << (KT & 31)) - 1u);
+            bool higher = false;
+            float top[MT][2];
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    float mx = -CUDART_INF_F;
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int i = 0; i < 2; i++) {
+                            float &x = s[m][n][2 * h + i];
+                            x *= c;
+                            if (!whole) {
+                                const int j = 8 * n + 2 * t + i;
+                                if (!(own[m][h] == seg && key0 + j >= lo[m][h] && key0 + j < hi[m][h] && (have >> j & 1u))) x = -CUDART_INF_F;
+                            }
+                            mx = fmaxf(mx, x);
+                        }
+                    top[m][h] = mx;
+                    higher |= mx > ref[m][h] + (below + 8.0f);
+                }
+            if (__any_sync(0xffffffffu, higher)) {
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        float mx = top[m][h];
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                        const float grown = fmaxf(ref[m][h], mx - below);
+                        if (grown != ref[m][h]) {
+                            const float f = ex2(ref[m][h] - grown);
+                            ref[m][h] = grown;
+                            l[m][h] *= f;
+#pragma unroll
+                            for (int i = 0; i < HS / 8; i++) { o[m][i][2 * h] *= f; o[m][i][2 * h + 1] *= f; }
+                        }
+                    }
+            }
+            uint32_t ph[MT][KS][4], pl[MT][KS][4];
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const float base = ref[m][h] == -CUDART_INF_F ? 0.0f : ref[m][h];
+                        const float p0 = ex2(s[m][n][2 * h] - base), p1 = ex2(s[m][n][2 * h + 1] - base);
+                        l[m][h] += p0 + p1;
+                        const uint32_t w = pack2<T>(p0, p1);
+                        const float2 r = unpack2<T>(w);
+                        ph[m][n / 2][(n & 1) * 2 + h] = w;
+                        pl[m][n / 2][(n & 1) * 2 + h] = pack2<T>(p0 - r.x, p1 - r.y);
+                    }
+            uint32_t saw[MT][KS][4]; // ones where a position is seen
+            if (careful)
+#pragma unroll
+                for (int m = 0; m < MT; m++)
+#pragma unroll
+                    for (int n = 0; n < NT; n++)
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            const int j = 8 * n + 2 * t;
+                            const auto sees = [&](int j) { return own[m][h] == seg && key0 + j >= lo[m][h] && key0 + j < hi[m][h] && (have >> j & 1u); };
+                            saw[m][n / 2][(n & 1) * 2 + h] = pack2<T>(sees(j) ? 1.0f : 0.0f, sees(j + 1) ? 1.0f : 0.0f);
+                        }
+#pragma unroll
+            for (int i = 0; i < HS / 8; i += 2)
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    uint32_t b[4];
+                    ldmatrix4_trans(vt + piece<HS>(16 * k + v_row, i + v_piece), b);
+                    if (careful) {
+                        uint32_t odd[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            odd[u] = not_finite<T>(b[u]);
+                            b[u] &= ~odd[u];
+                            odd[u] &= pack2<T>(1.0f, 1.0f);
+                        }
+                        if (__any_sync(0xffffffffu, (odd[0] | odd[1] | odd[2] | odd[3]) != 0u))
+#pragma unroll
+                            for (int m = 0; m < MT; m++) {
+                                float n0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, n1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma<T>(n0, saw[m][k], odd[0], odd[1]);
+                                mma<T>(n1, saw[m][k], odd[2], odd[3]);
+#pragma unroll
+                                for (int u = 0; u < 4; u++) {
+                                    if (n0[u] > 0.0f) o[m][i][u] = CUDART_NAN_F;
+                                    if (n1[u] > 0.0f) o[m][i + 1][u] = CUDART_NAN_F;
+                                }
+                            }
+                    }
+#pragma unroll
+                    for (int m = 0; m < MT; m++) {
+                        mma<T>(o[m][i], ph[m][k], b[0], b[1]);
+                        mma<T>(o[m][i + 1], ph[m][k], b[2], b[3]);
+                        mma<T>(o[m][i], pl[m][k], b[0], b[1]);
+                        mma<T>(o[m][i + 1], pl[m][k], b[2], b[3]);
+                    }
+                }
+            if (++stage == S) stage = 0;
+        }
+        cp_wait<0>();
+        if (careful) break;
+        bool bad = false;
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < HS / 8; i++)
+#pragma unroll
+                for (int u = 0; u < 4; u++) bad |= !(fabsf(o[m][i][u]) < CUDART_INF_F);
+        __syncwarp();
+        if (!__any_sync(0xffffffffu, bad)) break;
+    }
+
+    // ---- join: warps, then (through the workspace) CTAs ----
+    __syncthreads(); // the rings are free
+    float *parts = reinterpret_cast<float *>(smem);
+#pragma unroll
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            float sum = l[m][h];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            const int r = 16 * m + 8 * h + g;
+            if (t == 0) { wref[warp][r] = ref[m][h]; wsum[warp][r] = sum; }
+#pragma unroll
+            for (int i = 0; i < HS / 8; i++) *reinterpret_cast<float2 *>(parts + (warp * ROWS + r) * part_stride(HS) + 8 * i + 2 * t) = make_float2(o[m][i][2 * h], o[m][i][2 * h + 1]);
+        }
+    __syncthreads();
+    if (tid < rows) {
+        const int token = (row0 + tid) / mul, head = kvh * mul + row0 + tid - token * mul;
+        float M = -CUDART_INF_F, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < STEP_WARPS; w++) M = fmaxf(M, wref[w][tid]);
+        const float base = M == -CUDART_INF_F ? 0.0f : M;
+        float f[STEP_WARPS];
+#pragma unroll
+        for (int w = 0; w < STEP_WARPS; w++) {
+            f[w] = wref[w][tid] == M ? 1.0f : ex2(wref[w][tid] - base);
+            L = fmaf(f[w], wsum[w][tid], L);
+        }
+        if (a.splits > 1) reinterpret_cast<float2 *>(a.work + (size_t)a.rows.n * a.heads * a.splits * HS)[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(M, L);
+        const float scale = a.splits > 1 ? 1.0f : 1.0f / L;
+#pragma unroll
+        for (int w = 0; w < STEP_WARPS; w++) weight[w][tid] = L == 0.0f ? 0.0f : f[w] * scale; // nothing seen: zeros
+    }
+    __syncthreads();
+    for (int i = tid; i < rows * (HS / 4); i += STEP_WARPS * 32) {
+        const int r = i / (HS / 4), e = i % (HS / 4) * 4, token = (row0 + r) / mul, head = kvh * mul + row0 + r - token * mul, row = token0 + token;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < STEP_WARPS; w++) {
+            const float f = weight[w][r];
+            const float4 p = *reinterpret_cast<const float4 *>(parts + (w * ROWS + r) * part_stride(HS) + e);
+            x = make_float4(fmaf(f, p.x, x.x), fmaf(f, p.y, x.y), fmaf(f, p.z, x.z), fmaf(f, p.w, x.w));
+        }
+        if (a.splits > 1) *reinterpret_cast<float4 *>(a.work + (((size_t)row * a.heads + head) * a.splits + split) * HS + e) = x;
+        else if (seq_of[token] >= 0) put_results(a, row, head, HS, e, x);
+    }
+}
+
+// Joins the parts of a row's head: 128 threads, 4 entries each, HS / 4 threads a part.  At most MAX_SPLITS parts.
+constexpr int MAX_SPLITS = 296;
+template <int HS> __global__ void __launch_bounds__(128) k_paged_join(const Step a) {
+    constexpr int LANES = HS / 4, GROUPS = 128 / LANES;
+    __shared__ float weight[MAX_SPLITS], red[2][4];
+    __shared__ float4 sums[GROUPS][LANES];
+    pdl_wait();
+    const int tid = threadIdx.x, row = blockIdx.x / a.heads, head = blockIdx.x % a.heads;
+    int pos;
+    if (a.rows.place(row, pos) < 0) return;
+    const size_t at = ((size_t)row * a.heads + head) * a.splits;
+    const float2 *stat = reinterpret_cast<const float2 *>(a.work + (size_t)a.rows.n * a.heads * a.splits * HS) + at;
+    const float4 *part = reinterpret_cast<const float4 *>(a.work + at * HS);
+    float2 st[(MAX_SPLITS + 127) / 128];
+    float M = -CUDART_INF_F, L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < (MAX_SPLITS + 127) / 128; i++) {
+        st[i] = tid + 128 * i < a.splits ? stat[tid + 128 * i] : make_float2(-CUDART_INF_F, 0.0f);
+        M = fmaxf(M, st[i].x);
+    }
+    M = warp_max_f(M);
+    if (tid % 32 == 0) red[0][tid / 32] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    const float base = M == -CUDART_INF_F ? 0.0f : M;
+#pragma unroll
+    for (int i = 0; i < (MAX_SPLITS + 127) / 128; i++) {
+        const bool some = st[i].y != 0.0f; // (what the entries of a part without a sum hold is not defined)
+        const float f = st[i].x == M ? 1.0f : ex2(st[i].x - base);
+        if (tid + 128 * i < a.splits) weight[tid + 128 * i] = some ? f : -1.0f;
+        L += some ? f * st[i].y : 0.0f;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (tid % 32 == 0) red[1][tid / 32] = L;
+    __syncthreads();
+    L = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    const int lane = tid % LANES, group = tid / LANES;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (group < GROUPS)
+        for (int s = group; s < a.splits; s += GROUPS) {
+            const float f = weight[s];
+            if (f < 0.0f) continue;
+            const float4 p = part[(size_t)s * LANES + lane];
+            x = make_float4(fmaf(f, p.x, x.x), fmaf(f, p.y, x.y), fmaf(f, p.z, x.z), fmaf(f, p.w, x.w));
+        }
+    if (group < GROUPS) sums[group][lane] = x;
+    __syncthreads();
+    if (tid < LANES) {
+#pragma unroll
+        for (int i = 1; i < GROUPS; i++) {
+            const float4 p = sums[i][lane];
+            x = make_float4(x.x + p.x, x.y + p.y, x.z + p.z, x.w + p.w);
+        }
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        put_results(a, row, head, HS, lane * 4, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    }
+}
+
+} // namespace paged

@@ -1,0 +1,238 @@
+// serving.cu -- libb200llama.so: operators that serve many sequences from one pool of memory, and with drafted tokens (b200_paged_*, b200_verify_drafts): checks, cuts, launches.
+#include "operators.h"
+#include "operator_util.cuh"
+#include "paged.cuh"
+#include "verify.cuh"
+
+namespace {
+
+struct Fail { // the caller's message buffer
+    char *err;
+    size_t len;
+    template <typename... A> int operator()(int code, const char *fmt, A... a) const { return say(err, len, code, fmt, a...); }
+};
+
+template <typename F> cudaError_t by_cache_type(int type, F &&f) { // f(a value of the type)
+    if (type == B200_GGML_F16) return f(__half());
+    return f(__nv_bfloat16());
+}
+int shift_of(int page_size) {
+    int s = 0;
+    while (1 << s < page_size) s++;
+    return s;
+}
+
+int check_cache(const b200_paged_cache *c, const Fail &fail) {
+    if (!c) return fail(B200_ERR_BAD_ARG, "null cache");
+    if (c->type != B200_GGML_F16 && c->type != B200_GGML_BF16) return fail(B200_ERR_UNSUPPORTED, "a paged cache of type %d (FP16 and BF16 are known)", c->type);
+    if (c->head_size != 32 && c->head_size != 64 && c->head_size != 96 && c->head_size != 128 && c->head_size != 256)
+        return fail(B200_ERR_UNSUPPORTED, "a paged cache has heads of 32, 64, 96, 128 or 256 entries, not %d", c->head_size);
+    if (c->pages <= 0 || c->kv_heads <= 0) return fail(B200_ERR_BAD_ARG, "pages and kv_heads must be positive");
+    if (c->page_size < 1 || c->page_size > 65536 || (c->page_size & (c->page_size - 1))) return fail(B200_ERR_UNSUPPORTED, "pages hold a power of two of at most 65536 positions, not %d", c->page_size);
+    if ((unsigned __int128)c->pages * c->kv_heads * c->page_size > 0xfffffff0u) return fail(B200_ERR_UNSUPPORTED, "a cache of more than 2^32 rows of a head");
+    return B200_OK;
+}
+// positions, sequences and tables of a call
+int check_rows(const b200_paged_cache *c, int n, const int32_t *positions, const int32_t *tables, int64_t table_stride, int n_sequences, int table_width, const Fail &fail) {
+    if (n < 0) return fail(B200_ERR_BAD_ARG, "%d rows", n);
+    if (n_sequences < 0 || table_width < 0 || (table_stride < table_width && n_sequences > 1)) return fail(B200_ERR_BAD_ARG, "%d tables of %d pages, %lld entries apart", n_sequences, table_width, (long long)table_stride);
+    if ((long long)table_width * c->page_size > (1LL << 29)) return fail(B200_ERR_UNSUPPORTED, "a table of more than 2^29 positions");
+    if (n && (!c->keys || !c->values)) return fail(B200_ERR_BAD_ARG, "null keys or values");
+    if (reinterpret_cast<uintptr_t>(c->keys) % 16 || reinterpret_cast<uintptr_t>(c->values) % 16) return fail(B200_ERR_BAD_ARG, "keys and values have to start on 16-byte boundaries");
+    if (n && (!positions || (!tables && n_sequences && table_width))) return fail(B200_ERR_BAD_ARG, "null positions or tables");
+    return B200_OK;
+}
+
+// How the attention of n rows is cut.
+struct PagedCut {
+    int mt, tokens, blocks, splits, share; // blocks of 16 mt rows; tokens of a unit; blocks of a unit; CTAs of a block, tiles of each
+};
+// Rows of a unit: the tokens of a chunk that fit 32 rows (16 with heads of 256, whose results would leave no registers), so that they read the pages once.
+PagedCut paged_cut(const b200_paged_cache &c, const b200_paged_attention_args &a, int sms) {
+    PagedCut k;
+    const int G = c.kv_heads, mul = a.heads / G, chunk = a.chunk < 1 ? 1 : a.chunk < a.n ? a.chunk : a.n;
+    const int most = c.head_size == 256 ? 16 : 32;
+    int fit = most / mul;
+    if (fit < 1) fit = 1;
+    const int units_of_chunk = (chunk + fit - 1) / fit;
+    k.tokens = (chunk + units_of_chunk - 1) / units_of_chunk; // even shares
+    const int rows = k.tokens * mul;
+    k.mt = rows > 16 && most == 32 ? 2 : 1;
+    k.blocks = (rows + 16 * k.mt - 1) / (16 * k.mt);
+    const int KT = paged::step_keys(c.head_size);
+    const long long context = (long long)a.table_width * c.page_size;
+    long long len = a.max_len > 0 && a.max_len < context ? a.max_len : context;
+    const long long near = (long long)a.window + k.tokens;
+    if (a.window > 0 && near < len) len = near;
+    const long long tiles = (len + KT - 1) / KT + 1, units = (long long)((a.n + k.tokens - 1) / k.tokens) * G * k.blocks;
+    // One long row: two CTAs an SM, evenly.  Many rows: their lengths differ, so shares are small enough for several CTAs an SM and row; at least 8 tiles a warp, since every share leaves a part to join.
+    const long long wanted = units * tiles / (2LL * sms) + 1, least = 8 * paged::STEP_WARPS;
+    long long share = units >= sms ? (wanted + 3) / 4 : wanted;
+    if (share < least) share = least;
+    k.splits = (int)((tiles + share - 1) / share < paged::MAX_SPLITS ? (tiles + share - 1) / share : paged::MAX_SPLITS);
+    if (k.splits < 1) k.splits = 1;
+    k.share = (int)((tiles + k.splits - 1) / k.splits);
+    return k;
+}
+size_t paged_work_bytes(const b200_paged_cache &c, const b200_paged_attention_args &a, int splits) { return splits > 1 ? (size_t)a.n * a.heads * splits * (c.head_size + 2) * 4 : 0; }
+bool countable(const b200_paged_cache *c, const b200_paged_attention_args *a) {
+    return c && a && a->n > 0 && a->heads > 0 && c->kv_heads > 0 && a->heads % c->kv_heads == 0 && a->table_width >= 0 && c->page_size > 0 && c->head_size > 0;
+}
+
+cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_attention_args &a, cudaStream_t stream) {
+    paged::Step k;
+    k.pool = {c.keys, c.values, c.pages, c.kv_heads, shift_of(c.page_size)};
+    k.rows = {a.positions, a.sequences, a.tables, a.table_stride, a.n, a.n_sequences, a.table_width * c.page_size};
+    k.q = a.q; k.out = a.out;
+    k.ldq = a.q_stride; k.ldo = a.out_stride;
+    k.heads = a.heads; k.window = a.window; k.out_type = a.out_type;
+    k.scale = a.scale;
+    k.vec = aligned16(a.q, a.q_stride, 2);
+    const int four = a.out_type == B200_GGML_F32 ? 16 : 8; // bytes of the four entries that a thread writes
+    k.vec_out = reinterpret_cast<uintptr_t>(a.out) % four == 0 && a.out_stride % 4 == 0;
+    PagedCut cut = paged_cut(c, a, sm_count(c.device));
+    if (cut.splits > 1 && (!a.workspace || paged_work_bytes(c, a, cut.splits) > a.workspace_bytes)) cut.splits = 1;
+    k.tokens = cut.tokens; k.blocks = cut.blocks; k.splits = cut.splits; k.share = cut.share;
+    k.work = (float *)a.workspace;
+    const unsigned grid = (unsigned)((a.n + cut.tokens - 1) / cut.tokens) * cut.blocks * c.kv_heads * cut.splits;
+    return by_head_size(c.head_size, [&](auto hs) {
+        return by_cache_type(c.type, [&](auto type) {
+            using T = decltype(type);
+            const auto go = [&](auto mt) {
+                constexpr size_t smem = paged::step_smem_bytes(hs, mt);
+                auto kern = paged::k_paged_step<hs, T, mt>;
+                cudaError_t e = allow_smem(kern, smem);
+                if (e == cudaSuccess) e = launch(kern, grid, paged::STEP_WARPS * 32, smem, 1, false, stream, k);
+                return e != cudaSuccess || cut.splits == 1 ? e : launch(paged::k_paged_join<hs>, (unsigned)a.n * a.heads, 128, 0, 1, true, stream, k);
+            };
+            if constexpr (hs < 256) if (cut.mt == 2) return go(std::integral_constant<int, 2>());
+            return go(std::integral_constant<int, 1>());
+        });
+    });
+}
+
+int verify_stretches(int vocab) { return (vocab + verify::STRETCH - 1) / verify::STRETCH; }
+
+} // namespace
+
+extern "C" {
+
+int b200_paged_append(const b200_paged_cache *c, const b200_paged_append_args *a, void *stream, char *err, size_t err_len) {
+    const Fail fail = {err, err_len};
+    int rc = check_cache(c, fail);
+    if (rc) return rc;
+    if (!a) return fail(B200_ERR_BAD_ARG, "null arguments");
+    if ((rc = check_rows(c, a->n, a->positions, a->tables, a->table_stride, a->n_sequences, a->table_width, fail))) return rc;
+    if (a->heads < 0) return fail(B200_ERR_BAD_ARG, "%d query heads", a->heads);
+    if (!known_type(a->type)) return fail(B200_ERR_UNSUPPORTED, "rows of type %d (FP32, FP16 and BF16 are known)", a->type);
+    if (a->rope_layout != B200_ROPE_HALF && a->rope_layout != B200_ROPE_INTERLEAVED) return fail(B200_ERR_BAD_ARG, "rotation layout %d", a->rope_layout);
+    if (!a->cos != !a->sin) return fail(B200_ERR_BAD_ARG, "a rotation needs both tables");
+    if (a->cos && (a->rope_dims <= 0 || a->rope_dims % 2 || a->rope_dims > c->head_size || a->rope_rows < 0)) return fail(B200_ERR_BAD_ARG, "a rotation of %d entries of %d, %d positions", a->rope_dims, c->head_size, a->rope_rows);
+    if (a->n == 0) return B200_OK;
+    if (!a->k || !a->v || (a->heads && (!a->q || !a->q_out))) return fail(B200_ERR_BAD_ARG, "null rows");
+    const int64_t kv_width = (int64_t)c->kv_heads * c->head_size, q_width = (int64_t)a->heads * c->head_size;
+    if (a->n > 1 && (a->k_stride < kv_width || a->v_stride < kv_width || (a->heads && (a->q_stride < q_width || a->q_out_stride < q_width)))) return fail(B200_ERR_BAD_ARG, "rows overlap: a stride is smaller than its row");
+    if ((long long)a->n * (a->heads + 2LL * c->kv_heads) > (1LL << 33)) return fail(B200_ERR_UNSUPPORTED, "too many rows in one call");
+    paged::Append k;
+    k.pool = {c->keys, c->values, c->pages, c->kv_heads, shift_of(c->page_size)};
+    k.rows = {a->positions, a->sequences, a->tables, a->table_stride, a->n, a->n_sequences, a->table_width * c->page_size};
+    if (a->cos && a->rope_rows < k.rows.context) k.rows.context = a->rope_rows; // (positions behind the tables' are padding)
+    k.q = a->q; k.k = a->k; k.v = a->v;
+    k.ldq = a->q_stride; k.ldk = a->k_stride; k.ldv = a->v_stride; k.ldo = a->q_out_stride;
+    k.heads = a->heads;
+    k.interleaved = a->rope_layout == B200_ROPE_INTERLEAVED;
+    k.turned = a->cos ? a->rope_dims : 0;
+    const int b = type_bytes(a->type);
+    k.vec = aligned16(a->k, a->k_stride, b) && aligned16(a->v, a->v_stride, b) && (!a->heads || aligned16(a->q, a->q_stride, b));
+    k.vec_out = !a->heads || aligned16(a->q_out, a->q_out_stride, 2);
+    k.vec_tables = a->cos && a->rope_dims % 8 == 0 && aligned16(a->cos, 0, 4) && aligned16(a->sin, 0, 4); // rows of a multiple of 4 numbers
+    k.q_norm = a->q_norm; k.k_norm = a->k_norm; k.cos = a->cos; k.sin = a->sin;
+    k.eps = a->eps;
+    k.q_out = a->q_out;
+    OnDevice on(c->device);
+    cudaError_t e = on.error;
+    if (e == cudaSuccess)
+        e = by_head_size(c->head_size, [&](auto hs) {
+            return by_type(a->type, [&](auto type) {
+                return by_cache_type(c->type, [&](auto cache) {
+                    constexpr int L = hs / 8, per_warp = L <= 4 ? 8 : L <= 8 ? 4 : L <= 16 ? 2 : 1;
+                    const long long items = (long long)a->n * (a->heads + 2 * c->kv_heads);
+                    return launch(paged::k_paged_append<hs, decltype(type), decltype(cache)>, (unsigned)((items + 8 * per_warp - 1) / (8 * per_warp)), 256, 0, 1, false, (cudaStream_t)stream, k);
+                });
+            });
+        });
+    return e == cudaSuccess ? B200_OK : fail(cuda_code(e), "%s", cudaGetErrorString(e));
+}
+
+size_t b200_paged_attention_workspace(const b200_paged_cache *c, const b200_paged_attention_args *a) {
+    if (!countable(c, a)) return 0;
+    return paged_work_bytes(*c, *a, paged_cut(*c, *a, sm_count(c->device)).splits);
+}
+
+int b200_paged_attention(const b200_paged_cache *c, const b200_paged_attention_args *a, void *stream, char *err, size_t err_len) {
+    const Fail fail = {err, err_len};
+    int rc = check_cache(c, fail);
+    if (rc) return rc;
+    if (!a) return fail(B200_ERR_BAD_ARG, "null arguments");
+    if ((rc = check_rows(c, a->n, a->positions, a->tables, a->table_stride, a->n_sequences, a->table_width, fail))) return rc;
+    if (a->heads <= 0 || a->heads % c->kv_heads) return fail(B200_ERR_BAD_ARG, "%d query heads over %d key/value heads", a->heads, c->kv_heads);
+    if (!known_type(a->out_type)) return fail(B200_ERR_UNSUPPORTED, "results of type %d (FP32, FP16 and BF16 are known)", a->out_type);
+    if (a->window < 0 || a->max_len < 0 || a->chunk < 0) return fail(B200_ERR_BAD_ARG, "a negative window, length or chunk");
+    if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(B200_ERR_BAD_ARG, "the workspace is not aligned");
+    if (a->n == 0) return B200_OK;
+    if (!a->q || !a->out) return fail(B200_ERR_BAD_ARG, "null rows");
+    const int64_t width = (int64_t)a->heads * c->head_size;
+    if (a->n > 1 && (a->q_stride < width || a->out_stride < width)) return fail(B200_ERR_BAD_ARG, "rows overlap: a stride is smaller than its row");
+    if ((long long)a->n * a->heads > (1LL << 22)) return fail(B200_ERR_UNSUPPORTED, "too many rows in one call"); // (times MAX_SPLITS: the grid's limit)
+    OnDevice on(c->device);
+    cudaError_t e = on.error;
+    if (e == cudaSuccess) e = paged_attention_launch(*c, *a, (cudaStream_t)stream);
+    return e == cudaSuccess ? B200_OK : fail(cuda_code(e), "%s", cudaGetErrorString(e));
+}
+
+size_t b200_verify_drafts_workspace(const b200_verify_drafts_args *a) {
+    if (!a || a->sequences <= 0 || a->drafts < 0 || a->vocab <= 0) return 0;
+    const size_t rows = (size_t)a->sequences * (a->drafts + 1) + (a->draft_logits && a->temperature != 0.0f ? (size_t)a->sequences * a->drafts : 0);
+    return rows * verify_stretches(a->vocab) * sizeof(verify::Part);
+}
+
+int b200_verify_drafts(const b200_verify_drafts_args *a, void *stream, char *err, size_t err_len) {
+    const Fail fail = {err, err_len};
+    if (!a) return fail(B200_ERR_BAD_ARG, "null arguments");
+    if (a->sequences < 0 || a->drafts < 0 || a->vocab <= 0) return fail(B200_ERR_BAD_ARG, "%d sequences, %d drafts, %d logits", a->sequences, a->drafts, a->vocab);
+    if (a->drafts > verify::MAX_DRAFTS) return fail(B200_ERR_UNSUPPORTED, "%d drafts of a sequence (at most %d)", a->drafts, verify::MAX_DRAFTS);
+    if (a->vocab > (1 << 24) || a->sequences > (1 << 16)) return fail(B200_ERR_UNSUPPORTED, "%d logits a row, %d sequences (at most 2^24, 2^16)", a->vocab, a->sequences);
+    if (!known_type(a->type)) return fail(B200_ERR_UNSUPPORTED, "logits of type %d (FP32, FP16 and BF16 are known)", a->type);
+    if (!(a->temperature == 0.0f || (a->temperature >= 1e-4f && a->temperature <= 1e4f))) return fail(B200_ERR_BAD_ARG, "a temperature of %g (0, or 1e-4 to 1e4)", (double)a->temperature);
+    if (a->sequences == 0) return B200_OK;
+    if (!a->logits || !a->out_tokens || !a->accepted || (a->drafts && !a->tokens) || (!a->uniforms && a->temperature != 0.0f)) return fail(B200_ERR_BAD_ARG, "a null argument");
+    if (a->row_stride < a->vocab && a->drafts > 0) return fail(B200_ERR_BAD_ARG, "rows overlap: the stride is smaller than the row");
+    const bool both = a->draft_logits && a->temperature != 0.0f && a->drafts > 0;
+    const size_t need = b200_verify_drafts_workspace(a);
+    if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(B200_ERR_BAD_ARG, "a workspace of %zu bytes on a 16-byte boundary is needed", need);
+    verify::Args k;
+    k.logits = a->logits; k.draft_logits = both ? a->draft_logits : nullptr;
+    k.ld_s = a->sequence_stride; k.ld_r = a->row_stride; k.draft_ld_s = a->draft_sequence_stride; k.draft_ld_r = a->draft_row_stride;
+    k.sequences = a->sequences; k.drafts = a->drafts; k.vocab = a->vocab;
+    k.stretches = verify_stretches(a->vocab);
+    const int b = type_bytes(a->type);
+    k.vec = aligned16(a->logits, a->sequence_stride, b) && (a->drafts == 0 || a->row_stride * b % 16 == 0) &&
+            (!both || (aligned16(a->draft_logits, a->draft_sequence_stride, b) && a->draft_row_stride * b % 16 == 0));
+    k.temperature = a->temperature;
+    k.greedy = a->temperature == 0.0f; k.both = both;
+    k.tokens = a->tokens; k.uniforms = a->uniforms; k.out_tokens = a->out_tokens; k.accepted = a->accepted;
+    k.parts = (verify::Part *)a->workspace;
+    const unsigned long long grid = (unsigned long long)a->sequences * (a->drafts + 1 + (both ? a->drafts : 0)) * k.stretches;
+    if (grid > 0x7fffffffull) return fail(B200_ERR_UNSUPPORTED, "too many logits in one call");
+    OnDevice on(a->device);
+    cudaError_t e = on.error;
+    if (e == cudaSuccess)
+        e = by_type(a->type, [&](auto type) {
+            using T = decltype(type);
+            const cudaError_t first = launch(verify::k_verify_rows<T>, (unsigned)grid, verify::ROW_THREADS, 0, 1, false, (cudaStream_t)stream, k);
+            return first != cudaSuccess ? first : launch(verify::k_verify_token<T>, (unsigned)a->sequences * verify::CLUSTER, verify::TOKEN_THREADS, 0, verify::CLUSTER, true, (cudaStream_t)stream, k);
+        });
+    return e == cudaSuccess ? B200_OK : fail(cuda_code(e), "%s", cudaGetErrorString(e));
+}
+
+} // extern "C"

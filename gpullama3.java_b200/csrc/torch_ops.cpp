@@ -245,6 +245,205 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> log_probs(const Tensor &logits, const
     return {lp, entropy, ids, values};
 }
 
+// Checks that calls on a pool of pages and on the 4-bit cache share.
+const int32_t *int_tensor(const Tensor &t, const char *name, int device, at::IntArrayRef sizes) {
+    NEED(t.defined() && t.scalar_type() == at::kInt && t.sizes() == sizes, name, ": ", sizes, " of int32 is wanted, got ", shape(t));
+    NEED(t.is_cuda() && t.get_device() == device, name, " is on ", t.device(), ", the call on cuda:", device);
+    NEED(t.is_contiguous(), name, " has to be contiguous");
+    return t.data_ptr<int32_t>();
+}
+
+struct Paged {
+    Tensor keys, values;
+    int64_t pages, page_size, kv_heads, head_size;
+    int device;
+    b200_paged_cache cache;
+    Paged(const Tensor &k, const Tensor &v) : keys(k), values(v) {
+        NEED(k.defined() && v.defined() && k.dim() == 4 && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(), "keys and values: two of [pages, kv_heads, page_size, head_size] of one type are wanted, got ",
+             shape(k), " and ", shape(v));
+        NEED(k.is_cuda() && v.is_cuda() && k.get_device() == v.get_device(), "keys and values lie on one GPU: got ", k.device(), " and ", v.device());
+        NEED(k.is_contiguous() && v.is_contiguous(), "keys and values have to be contiguous");
+        outside_graph(k, "keys");
+        outside_graph(v, "values");
+        for (int i = 0; i < 4; i++) NEED(k.size(i) <= INT32_MAX, "sizes outside 32 bits");
+        pages = k.size(0); kv_heads = k.size(1); page_size = k.size(2); head_size = k.size(3);
+        device = k.get_device();
+        cache = {k.data_ptr(), v.data_ptr(), (int32_t)pages, (int32_t)page_size, (int32_t)kv_heads, (int32_t)head_size, type_of(k.scalar_type(), "keys and values"), device};
+        // what the library refuses of a cache it refuses here
+        b200_paged_append_args none = {};
+        none.rope_layout = B200_ROPE_HALF;
+        char err[256] = "";
+        const int rc = b200_paged_append(&cache, &none, nullptr, err, sizeof err);
+        if (rc != B200_OK) refused(rc, err);
+    }
+    at::ScalarType dtype() const { return keys.scalar_type(); }
+    void *stream() const { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
+
+    // rows [n, heads, head_size] whose heads lie one behind the other: entries between rows
+    int64_t rows(const Tensor &t, const char *name, int64_t n, int64_t heads) const {
+        NEED(t.defined() && t.dim() == 3 && t.size(0) == n && t.size(1) == heads && t.size(2) == head_size, name, ": [", n, ", ", heads, ", ", head_size, "] is wanted, got ", shape(t));
+        NEED(t.is_cuda() && t.get_device() == device, name, " is on ", t.device(), ", the cache on cuda:", device);
+        outside_graph(t, name);
+        NEED(n == 0 || (t.stride(2) == 1 && (t.stride(1) == head_size || heads == 1)), name, ": the heads of a row have to lie one behind the other");
+        return n > 1 ? t.stride(0) : heads * head_size;
+    }
+    const float *floats(const Maybe &t, const char *name) const {
+        if (!t) return nullptr;
+        outside_graph(*t, name);
+        NEED(t->scalar_type() == at::kFloat && t->is_cuda() && t->get_device() == device && t->is_contiguous(), name, ": a contiguous FP32 tensor on cuda:", device, " is wanted");
+        return t->data_ptr<float>();
+    }
+    const float *norm(const Maybe &t, const char *name) const {
+        if (t) NEED(t->dim() == 1 && t->size(0) == head_size, name, ": has the shape ", t->sizes());
+        return floats(t, name);
+    }
+    template <typename A> void places(A &a, int64_t n, const Tensor &positions, const Tensor &tables, const Maybe &sequences) const {
+        NEED(n <= INT32_MAX, n, " rows in one call");
+        a.n = (int32_t)n;
+        a.positions = int_tensor(positions, "positions", device, {n});
+        a.sequences = sequences ? int_tensor(*sequences, "sequences", device, {n}) : nullptr;
+        NEED(tables.defined() && tables.scalar_type() == at::kInt && tables.dim() == 2, "tables: [sequences, pages] of int32 is wanted, got ", shape(tables));
+        NEED(tables.is_cuda() && tables.get_device() == device, "tables are on ", tables.device(), ", the cache on cuda:", device);
+        NEED(tables.size(0) <= INT32_MAX && tables.size(1) <= INT32_MAX, "sizes outside 32 bits");
+        NEED(tables.size(1) <= 1 || tables.size(0) == 0 || tables.stride(1) == 1, "the pages of a table have to lie one behind the other");
+        a.tables = tables.data_ptr<int32_t>();
+        a.n_sequences = (int32_t)tables.size(0);
+        a.table_width = (int32_t)tables.size(1);
+        a.table_stride = tables.size(0) > 1 ? tables.stride(0) : tables.size(1);
+    }
+
+    Maybe append(const Tensor &k, const Tensor &v, const Tensor &positions, const Tensor &tables, const Maybe &sequences, const Maybe &q, const Maybe &q_norm, const Maybe &k_norm, double eps,
+                 const Maybe &cos, const Maybe &sin, const std::string &layout, const Maybe &q_out) const {
+        NEED(k.defined() && v.defined() && k.dim() == 3, "k: [n, ", kv_heads, ", ", head_size, "] is wanted, got ", shape(k));
+        const int64_t n = k.size(0);
+        b200_paged_append_args a = {};
+        places(a, n, positions, tables, sequences);
+        a.type = type_of(k.scalar_type(), "k");
+        NEED(v.scalar_type() == k.scalar_type(), "k and v have the same type: got ", k.scalar_type(), " and ", v.scalar_type());
+        NEED(layout == "half" || layout == "interleaved", "layout ", layout);
+        a.rope_layout = layout == "half" ? B200_ROPE_HALF : B200_ROPE_INTERLEAVED;
+        a.eps = (float)eps;
+        a.k_stride = rows(k, "k", n, kv_heads);
+        a.v_stride = rows(v, "v", n, kv_heads);
+        a.k = k.data_ptr();
+        a.v = v.data_ptr();
+        Maybe out = q_out;
+        if (q) {
+            NEED(q->defined() && q->scalar_type() == k.scalar_type() && q->dim() == 3, "q: rows of k's type are wanted");
+            NEED(q->size(1) <= INT32_MAX, "sizes outside 32 bits");
+            a.heads = (int32_t)q->size(1);
+            a.q_stride = rows(*q, "q", n, a.heads);
+            a.q = q->data_ptr();
+            if (!out) out = fresh({n, a.heads, head_size}, dtype(), device);
+            NEED(out->defined() && out->scalar_type() == dtype(), "q_out is of the cache's type, ", dtype());
+            a.q_out_stride = rows(*out, "q_out", n, a.heads);
+            a.q_out = out->data_ptr();
+        } else NEED(!q_out && !q_norm, "q_out and q_norm belong to q");
+        a.q_norm = norm(q_norm, "q_norm");
+        a.k_norm = norm(k_norm, "k_norm");
+        NEED(cos.has_value() == sin.has_value(), "a rotation needs cos and sin");
+        if (cos) {
+            NEED(cos->dim() == 2 && cos->sizes() == sin->sizes() && cos->size(1) > 0 && 2 * cos->size(1) <= head_size, "cos and sin: [positions, up to ", head_size / 2, "] are wanted, got ", shape(*cos), " and ",
+                 shape(*sin));
+            a.cos = floats(cos, "cos");
+            a.sin = floats(sin, "sin");
+            a.rope_dims = (int32_t)(2 * cos->size(1));
+            a.rope_rows = (int32_t)std::min<int64_t>(cos->size(0), INT32_MAX);
+            if (a.rope_rows == 0) return out; // every row is padding
+        }
+        if (n) {
+            char err[256] = "";
+            const int rc = b200_paged_append(&cache, &a, stream(), err, sizeof err);
+            if (rc != B200_OK) refused(rc, err);
+        }
+        return out;
+    }
+
+    Tensor attention(const Tensor &q, const Tensor &positions, const Tensor &tables, const Maybe &sequences, std::optional<double> scale, int64_t window, int64_t max_len, int64_t chunk,
+                     std::optional<at::ScalarType> dtype_, const Maybe &given) const {
+        NEED(q.defined() && q.dim() == 3 && q.scalar_type() == dtype(), "q: rows [n, heads, head_size] of the cache's type, ", dtype(), ", are wanted, got ", shape(q));
+        NEED(q.size(1) > 0 && q.size(1) % kv_heads == 0, q.size(1), " query heads over ", kv_heads, " key/value heads");
+        NEED(window >= 0 && max_len >= 0 && chunk >= 0, "a negative window, length or chunk");
+        const int64_t n = q.size(0);
+        b200_paged_attention_args a = {};
+        places(a, n, positions, tables, sequences);
+        if (given) NEED(given->defined(), "out is wanted");
+        const at::ScalarType type = given ? given->scalar_type() : dtype_ ? *dtype_ : dtype();
+        a.out_type = type_of(type, "results");
+        NEED(q.size(1) <= INT32_MAX, "sizes outside 32 bits");
+        a.heads = (int32_t)q.size(1);
+        a.window = (int32_t)std::min<int64_t>(window, INT32_MAX);
+        a.max_len = (int32_t)std::min<int64_t>(max_len, INT32_MAX);
+        a.chunk = (int32_t)std::min<int64_t>(chunk, INT32_MAX);
+        a.q_stride = rows(q, "q", n, a.heads);
+        const Tensor out = given ? *given : fresh({n, a.heads, head_size}, type, device);
+        a.out_stride = rows(out, "out", n, a.heads);
+        a.q = q.data_ptr();
+        a.out = out.data_ptr();
+        a.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)head_size));
+        if (n == 0) return out;
+        Tensor work; // from the stream's own pool: calls on other streams, and captured graphs, have theirs
+        if ((a.workspace_bytes = b200_paged_attention_workspace(&cache, &a)) > 0) {
+            work = fresh({(int64_t)(a.workspace_bytes / 4)}, at::kFloat, device);
+            a.workspace = work.data_ptr();
+        }
+        char err[256] = "";
+        const int rc = b200_paged_attention(&cache, &a, stream(), err, sizeof err);
+        if (rc != B200_OK) refused(rc, err);
+        return out;
+    }
+};
+
+std::pair<Tensor, Tensor> verify_drafts(const Tensor &logits, const Tensor &drafts, const Maybe &uniforms, const Maybe &draft_logits, double temperature) {
+    NEED(logits.defined() && logits.dim() == 3 && logits.is_cuda(), "logits: [sequences, drafts + 1, vocab] on a GPU is wanted, got ", shape(logits));
+    outside_graph(logits, "logits");
+    const int64_t S = logits.size(0), K = logits.size(1) - 1, V = logits.size(2);
+    NEED(K >= 0 && V > 0 && S <= INT32_MAX && K <= INT32_MAX && V <= INT32_MAX, "logits: [sequences, drafts + 1, vocab] is wanted, got ", shape(logits));
+    NEED(V == 1 || logits.stride(2) == 1, "the logits of a row have to lie one behind the other");
+    b200_verify_drafts_args a = {};
+    a.device = logits.get_device();
+    a.type = type_of(logits.scalar_type(), "logits");
+    a.sequences = (int32_t)S;
+    a.drafts = (int32_t)K;
+    a.vocab = (int32_t)V;
+    a.temperature = (float)temperature;
+    a.logits = logits.data_ptr();
+    a.row_stride = K > 0 ? logits.stride(1) : V;
+    a.sequence_stride = S > 1 ? logits.stride(0) : 0;
+    a.tokens = int_tensor(drafts, "drafts", a.device, {S, K});
+    if (uniforms) {
+        NEED(uniforms->defined() && uniforms->scalar_type() == at::kFloat && uniforms->sizes() == at::IntArrayRef({S, K + 1}), "uniforms: [", S, ", ", K + 1, "] of FP32 is wanted, got ", shape(*uniforms));
+        NEED(uniforms->is_cuda() && uniforms->get_device() == a.device && uniforms->is_contiguous(), "uniforms are contiguous and on ", logits.device());
+        outside_graph(*uniforms, "uniforms");
+        a.uniforms = uniforms->data_ptr<float>();
+    } else NEED(temperature == 0.0, "uniforms are wanted unless the temperature is 0");
+    if (draft_logits) {
+        const Tensor &y = *draft_logits;
+        NEED(y.defined() && y.dim() == 3 && y.size(0) == S && y.size(1) == K && y.size(2) == V && y.scalar_type() == logits.scalar_type(), "draft_logits: [", S, ", ", K, ", ", V, "] of ", logits.scalar_type(),
+             " is wanted, got ", shape(y));
+        NEED(y.is_cuda() && y.get_device() == a.device, "draft_logits are on ", y.device(), ", the logits on ", logits.device());
+        outside_graph(y, "draft_logits");
+        NEED(V == 1 || y.numel() == 0 || y.stride(2) == 1, "the logits of a row have to lie one behind the other");
+        if (K > 0) {
+            a.draft_logits = y.data_ptr();
+            a.draft_row_stride = K > 1 ? y.stride(1) : V;
+            a.draft_sequence_stride = S > 1 ? y.stride(0) : 0;
+        }
+    }
+    Tensor tokens = fresh({S, K + 1}, at::kInt, a.device), accepted = fresh({S}, at::kInt, a.device);
+    a.out_tokens = tokens.data_ptr<int32_t>();
+    a.accepted = accepted.data_ptr<int32_t>();
+    Tensor work; // from the stream's own pool
+    if ((a.workspace_bytes = b200_verify_drafts_workspace(&a)) > 0) {
+        work = fresh({(int64_t)(a.workspace_bytes / 4)}, at::kFloat, a.device);
+        a.workspace = work.data_ptr();
+    }
+    char err[256] = "";
+    const int rc = b200_verify_drafts(&a, c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)a.device).stream(), err, sizeof err);
+    if (rc != B200_OK) refused(rc, err);
+    return {tokens, accepted};
+}
+
 } // namespace
 
 PYBIND11_MODULE(_b200ops, m) {
@@ -265,5 +464,19 @@ PYBIND11_MODULE(_b200ops, m) {
         .def("read", &Cache::read, arg("positions").none(false), arg("slots") = py::none(), arg("dtype") = at::kFloat)
         .def("reset", &Cache::reset)
         .def("free", &Cache::free);
+    py::class_<Paged>(m, "Paged")
+        .def(py::init<const Tensor &, const Tensor &>(), arg("keys").none(false), arg("values").none(false))
+        .def_readonly("keys", &Paged::keys)
+        .def_readonly("values", &Paged::values)
+        .def_readonly("pages", &Paged::pages)
+        .def_readonly("page_size", &Paged::page_size)
+        .def_readonly("kv_heads", &Paged::kv_heads)
+        .def_readonly("head_size", &Paged::head_size)
+        .def_readonly("device_index", &Paged::device)
+        .def("append", &Paged::append, arg("k"), arg("v"), arg("positions").none(false), arg("tables").none(false), arg("sequences") = py::none(), arg("q") = py::none(), arg("q_norm") = py::none(),
+             arg("k_norm") = py::none(), arg("eps") = 1e-6, arg("cos") = py::none(), arg("sin") = py::none(), arg("layout") = "half", arg("q_out") = py::none())
+        .def("attention", &Paged::attention, arg("q"), arg("positions").none(false), arg("tables").none(false), arg("sequences") = py::none(), arg("scale") = py::none(), arg("window") = 0,
+             arg("max_len") = 0, arg("chunk") = 1, arg("dtype") = py::none(), arg("out") = py::none());
+    m.def("verify_drafts", &verify_drafts, arg("logits"), arg("drafts").none(false), arg("uniforms").none(true), arg("draft_logits") = py::none(), arg("temperature") = 1.0);
     m.def("log_probs", &log_probs, arg("logits"), arg("targets").none(true), arg("top") = 0);
 }

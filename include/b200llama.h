@@ -591,6 +591,79 @@ typedef struct b200_log_probs_args {
 } b200_log_probs_args;
 int b200_log_probs(const b200_log_probs_args *args, void *stream, char *err, size_t err_len);
 
+/* A key/value cache in pages, in the caller's memory: keys and values are each [pages][kv_heads][page_size][head_size] entries of `type` (B200_GGML_F16 or _BF16), 16-byte aligned;
+ * page_size is a power of two of at most 65536, head sizes are 32, 64, 96, 128, 256.  Position p of a sequence lies in page table[p / page_size], position p % page_size of it.  Tables may
+ * share pages; a table entry outside [0, pages) is no page. */
+typedef struct b200_paged_cache {
+    void *keys, *values;
+    int32_t pages, page_size, kv_heads, head_size, type, device;
+} b200_paged_cache;
+
+/* The rows of a call on a paged cache: row r stands at positions[r] of sequence `sequences ? sequences[r] : 0`, whose table is the table_width entries from tables + sequence * table_stride
+ * on (device arrays).  A row whose sequence lies outside [0, n_sequences) or whose position lies behind its table is padding: nothing is read, stored or written for it.  A negative
+ * position is a row without keys.  At most 2^29 positions a table. */
+
+/* Rows of a QKV product -> pages, as b200_kv4_append: head norms (the mean of squares in 64 bits) and rotation in FP32, rounded once to the cache's type.  The rotation turns the first
+ * rope_dims entries of a head (an even number): cos / sin are FP32 [rope_rows][rope_dims / 2], pairs by rope_layout within that part; a position behind rope_rows is padding.  q_out receives
+ * the queries in the cache's type (it may not overlap q).  A row of a negative position is not stored and its q_out not written, one whose page is none is not stored.  Two rows of a call
+ * must not name the same place. */
+typedef struct b200_paged_append_args {
+    int32_t n, heads, type, rope_layout, rope_dims, rope_rows; /* type: of the rows, F32, F16 or BF16 */
+    const void *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride, q_out_stride;
+    const int32_t *positions, *sequences, *tables;
+    int64_t table_stride;
+    int32_t n_sequences, table_width;
+    const float *q_norm, *k_norm, *cos, *sin;
+    void *q_out;
+    float eps;
+} b200_paged_append_args;
+int b200_paged_append(const b200_paged_cache *cache, const b200_paged_append_args *args, void *stream, char *err, size_t err_len);
+
+/* Causal attention of n query rows of the cache's type over the pages of their sequences: the row at position p sees the positions j <= p that have a page, the last `window` of them
+ * where window > 0; query head h reads key/value head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type (F32, F16, BF16).  Queries and keys are multiplied as they are,
+ * probabilities keep 16 bits (BF16 caches) or 22 (FP16), sums are FP32.  A row that sees nothing, or only scores of -inf, is zeros.  A value that is infinite or NaN makes its entry NaN in the
+ * rows that see it, and only in those.  chunk (0 or 1: single steps; how many neighbouring rows are successive tokens of one sequence) and max_len (0: unknown; the largest position + 1)
+ * only choose how the work is split.  So does a workspace: few rows over many positions fill the GPU where the call gets b200_paged_attention_workspace(cache, args) bytes (0: it needs
+ * none) of 16-byte aligned device memory, whose content before and after does not matter and which no other call under way may use; NULL or fewer bytes: the call does without. */
+typedef struct b200_paged_attention_args {
+    int32_t n, heads, window, max_len, chunk, out_type;
+    const void *q;
+    void *out;
+    int64_t q_stride, out_stride;
+    const int32_t *positions, *sequences, *tables;
+    int64_t table_stride;
+    int32_t n_sequences, table_width;
+    float scale;
+    void *workspace;
+    size_t workspace_bytes;
+} b200_paged_attention_args;
+size_t b200_paged_attention_workspace(const b200_paged_cache *cache, const b200_paged_attention_args *args);
+int b200_paged_attention(const b200_paged_cache *cache, const b200_paged_attention_args *args, void *stream, char *err, size_t err_len);
+
+/* Verification of drafted tokens.  Of each of `sequences` sequences: logits rows x_0 .. x_drafts of the target ([vocab] of `type`; sequence_stride, row_stride entries apart), tokens
+ * [sequences][drafts] drafted behind them (the first outside [0, vocab) ends a sequence's drafts), draft_logits rows y_0 .. y_{drafts - 1} that they were sampled from, at the same
+ * temperature (NULL: the drafts were not sampled: all of q_i is on its draft), and uniforms [sequences][drafts + 1] in [0, 1).  With p_i = softmax(x_i / temperature), q_i = softmax(y_i / temperature), a
+ * draft is accepted when uniforms[i] * q_i(draft) < p_i(draft) and all in front of it were.  n of them are: accepted[s] = n, out_tokens [sequences][drafts + 1] = the n drafts, the token
+ * behind them, then -1.  The token is the first index whose running sum of weights passes uniforms[drafts] times their sum; weights: p_n where no draft was left, else
+ * max(p_n - q_n, 0) (without draft_logits p_n without the draft; p_n where that is all 0).  So the tokens are distributed as the target's own samples.  temperature 0 (else 1e-4 to 1e4): a draft is
+ * accepted where it is its row's largest logit (the first of equal ones), the token is that of its row; uniforms and draft_logits are not read.  A row reached that has no distribution
+ * (a NaN, an infinite logit or none above -inf) ends its sequence: its draft is not accepted, the token is -1.  Running sums of the drawn row, and decisions that FP32 cannot make, are in 64 bits.
+ * The workspace: b200_verify_drafts_workspace(args) bytes, 16-byte aligned, content does not matter, of no other call under way.  At most 64 drafts, 2^24 logits, 2^16 sequences. */
+typedef struct b200_verify_drafts_args {
+    const void *logits, *draft_logits;
+    int64_t sequence_stride, row_stride, draft_sequence_stride, draft_row_stride;
+    int32_t sequences, drafts, vocab, type, device;
+    float temperature;
+    const int32_t *tokens;
+    const float *uniforms;
+    int32_t *out_tokens, *accepted;
+    void *workspace;
+    size_t workspace_bytes;
+} b200_verify_drafts_args;
+size_t b200_verify_drafts_workspace(const b200_verify_drafts_args *args);
+int b200_verify_drafts(const b200_verify_drafts_args *args, void *stream, char *err, size_t err_len);
+
 /* Number of kernels one decode step launches (bench.py's gpu_launches). */
 int b200_launches_per_decode(b200_plan *plan);
 
