@@ -14,7 +14,7 @@ SOURCES = ["plan.cu", "operators.cu", "serving.cu"]
 
 # Headers that plan.cu does not read: its object is not rebuilt for them.
 OPERATOR_HEADERS = {"operators.cu": ("kv4.cuh", "kv4_chunk.cuh", "logprobs.cuh", "operator_util.cuh"),
-                    "serving.cu": ("kv4.cuh", "logprobs.cuh", "operator_util.cuh", "paged.cuh", "verify.cuh")}
+                    "serving.cu": ("kv4.cuh", "kv4_chunk.cuh", "logprobs.cuh", "operator_util.cuh", "paged.cuh", "paged_chunk.cuh", "verify.cuh")}
 
 
 def _deps(source: str | None = None):

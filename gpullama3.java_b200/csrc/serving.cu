@@ -1,7 +1,7 @@
 // serving.cu -- libb200llama.so: operators that serve many sequences from one pool of memory, and with drafted tokens (b200_paged_*, b200_verify_drafts): checks, cuts, launches.
 #include "operators.h"
 #include "operator_util.cuh"
-#include "paged.cuh"
+#include "paged_chunk.cuh"
 #include "verify.cuh"
 
 namespace {
@@ -74,12 +74,35 @@ PagedCut paged_cut(const b200_paged_cache &c, const b200_paged_attention_args &a
     k.share = (int)((tiles + k.splits - 1) / k.splits);
     return k;
 }
+// Chunks on the tensor cores: 16-bit results, heads of 64, 96 or 128.  A tile takes 128 rows whether they are used or not.
+const int CHUNK_MIN_ROWS = 64;
+struct PagedChunkCut {
+    int tokens, splits;
+    bool use;
+};
+PagedChunkCut paged_chunk_cut(const b200_paged_cache &c, const b200_paged_attention_args &a, int sms) {
+    PagedChunkCut k = {};
+    const int G = c.kv_heads, mul = a.heads / G, hs = c.head_size, chunk = a.chunk < a.n ? a.chunk : a.n;
+    k.use = a.out_type != B200_GGML_F32 && (hs == 64 || hs == 96 || hs == 128) && mul <= paged::C_ROWS && chunk > 1 && (long long)chunk * mul >= CHUNK_MIN_ROWS;
+    if (!k.use) return k;
+    const int most = paged::C_ROWS / mul, shares = (chunk + most - 1) / most;
+    k.tokens = (chunk + shares - 1) / shares; // even shares of a chunk: where all rows are chunks of that many tokens no CTA has two sequences' positions to run through
+    const long long context = (long long)a.table_width * c.page_size, near = (long long)a.window + k.tokens;
+    long long len = a.max_len > 0 && a.max_len < context ? a.max_len : context;
+    if (a.window > 0 && near < len) len = near;
+    const long long units = (long long)((a.n + k.tokens - 1) / k.tokens) * G, worth = len / (8 * paged::C_KEYS); // eight tiles of positions a CTA
+    long long splits = sms / units;
+    if (splits > worth) splits = worth;
+    if (splits > paged::MAX_SPLITS) splits = paged::MAX_SPLITS;
+    k.splits = splits < 1 ? 1 : (int)splits;
+    return k;
+}
 size_t paged_work_bytes(const b200_paged_cache &c, const b200_paged_attention_args &a, int splits) { return splits > 1 ? (size_t)a.n * a.heads * splits * (c.head_size + 2) * 4 : 0; }
 bool countable(const b200_paged_cache *c, const b200_paged_attention_args *a) {
     return c && a && a->n > 0 && a->heads > 0 && c->kv_heads > 0 && a->heads % c->kv_heads == 0 && a->table_width >= 0 && c->page_size > 0 && c->head_size > 0;
 }
 
-cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_attention_args &a, cudaStream_t stream) {
+cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_attention_args &a, cudaStream_t stream, bool give_up) {
     paged::Step k;
     k.pool = {c.keys, c.values, c.pages, c.kv_heads, shift_of(c.page_size)};
     k.rows = {a.positions, a.sequences, a.tables, a.table_stride, a.n, a.n_sequences, a.table_width * c.page_size};
@@ -90,10 +113,33 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
     k.vec = aligned16(a.q, a.q_stride, 2);
     const int four = a.out_type == B200_GGML_F32 ? 16 : 8; // bytes of the four entries that a thread writes
     k.vec_out = reinterpret_cast<uintptr_t>(a.out) % four == 0 && a.out_stride % 4 == 0;
-    PagedCut cut = paged_cut(c, a, sm_count(c.device));
-    if (cut.splits > 1 && (!a.workspace || paged_work_bytes(c, a, cut.splits) > a.workspace_bytes)) cut.splits = 1;
-    k.tokens = cut.tokens; k.blocks = cut.blocks; k.splits = cut.splits; k.share = cut.share;
     k.work = (float *)a.workspace;
+    const int sms = sm_count(c.device);
+    const auto has_room = [&](int splits) { return a.workspace && paged_work_bytes(c, a, splits) <= a.workspace_bytes; };
+    if (PagedChunkCut cc = paged_chunk_cut(c, a, sms); cc.use) {
+        if (!has_room(cc.splits)) cc.splits = 1;
+        k.tokens = cc.tokens; k.splits = cc.splits;
+        k.blocks = k.share = 1;
+        k.vec_out = aligned16(a.out, a.out_stride, 2);
+        const unsigned grid = (unsigned)((a.n + cc.tokens - 1) / cc.tokens) * c.kv_heads * cc.splits;
+        return by_cache_type(c.type, [&](auto type) {
+            using T = decltype(type);
+            const auto go = [&](auto hs) {
+                constexpr size_t smem = paged::c_smem_bytes(hs);
+                auto kern = paged::k_paged_chunk<hs, T>;
+                if constexpr (hs == 64 && std::is_same<T, __half>::value) if (give_up) kern = paged::k_paged_chunk<hs, T, true>;
+                cudaError_t e = allow_smem(kern, smem);
+                if (e == cudaSuccess) e = launch(kern, grid, paged::C_THREADS, smem, 1, false, stream, k);
+                return e != cudaSuccess || cc.splits == 1 ? e : launch(paged::k_paged_join<hs>, (unsigned)a.n * a.heads, 128, 0, 1, true, stream, k);
+            };
+            if (c.head_size == 64) return go(std::integral_constant<int, 64>());
+            if (c.head_size == 96) return go(std::integral_constant<int, 96>());
+            return go(std::integral_constant<int, 128>());
+        });
+    }
+    PagedCut cut = paged_cut(c, a, sms);
+    if (!has_room(cut.splits)) cut.splits = 1;
+    k.tokens = cut.tokens; k.blocks = cut.blocks; k.splits = cut.splits; k.share = cut.share;
     const unsigned grid = (unsigned)((a.n + cut.tokens - 1) / cut.tokens) * cut.blocks * c.kv_heads * cut.splits;
     return by_head_size(c.head_size, [&](auto hs) {
         return by_cache_type(c.type, [&](auto type) {
@@ -166,10 +212,12 @@ int b200_paged_append(const b200_paged_cache *c, const b200_paged_append_args *a
 
 size_t b200_paged_attention_workspace(const b200_paged_cache *c, const b200_paged_attention_args *a) {
     if (!countable(c, a)) return 0;
-    return paged_work_bytes(*c, *a, paged_cut(*c, *a, sm_count(c->device)).splits);
+    const int sms = sm_count(c->device);
+    const PagedChunkCut cc = paged_chunk_cut(*c, *a, sms);
+    return paged_work_bytes(*c, *a, cc.use ? cc.splits : paged_cut(*c, *a, sms).splits);
 }
 
-int b200_paged_attention(const b200_paged_cache *c, const b200_paged_attention_args *a, void *stream, char *err, size_t err_len) {
+static int paged_attention(const b200_paged_cache *c, const b200_paged_attention_args *a, void *stream, char *err, size_t err_len, bool give_up) {
     const Fail fail = {err, err_len};
     int rc = check_cache(c, fail);
     if (rc) return rc;
@@ -186,8 +234,13 @@ int b200_paged_attention(const b200_paged_cache *c, const b200_paged_attention_a
     if ((long long)a->n * a->heads > (1LL << 22)) return fail(B200_ERR_UNSUPPORTED, "too many rows in one call"); // (times MAX_SPLITS: the grid's limit)
     OnDevice on(c->device);
     cudaError_t e = on.error;
-    if (e == cudaSuccess) e = paged_attention_launch(*c, *a, (cudaStream_t)stream);
+    if (e == cudaSuccess) e = paged_attention_launch(*c, *a, (cudaStream_t)stream, give_up);
     return e == cudaSuccess ? B200_OK : fail(cuda_code(e), "%s", cudaGetErrorString(e));
+}
+int b200_paged_attention(const b200_paged_cache *c, const b200_paged_attention_args *a, void *stream, char *err, size_t err_len) { return paged_attention(c, a, stream, err, err_len, false); }
+int b200_test_paged_give_up(const b200_paged_cache *c, const b200_paged_attention_args *a, void *stream, char *err, size_t err_len) {
+    if (!countable(c, a) || c->head_size != 64 || c->type != B200_GGML_F16 || !paged_chunk_cut(*c, *a, 148).use) return say(err, err_len, B200_ERR_BAD_ARG, "no attention of a chunk with heads of 64 in FP16");
+    return paged_attention(c, a, stream, err, err_len, true);
 }
 
 size_t b200_verify_drafts_workspace(const b200_verify_drafts_args *a) {

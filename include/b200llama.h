@@ -622,9 +622,11 @@ int b200_paged_append(const b200_paged_cache *cache, const b200_paged_append_arg
 
 /* Causal attention of n query rows of the cache's type over the pages of their sequences: the row at position p sees the positions j <= p that have a page, the last `window` of them
  * where window > 0; query head h reads key/value head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type (F32, F16, BF16).  Queries and keys are multiplied as they are,
- * probabilities keep 16 bits (BF16 caches) or 22 (FP16), sums are FP32.  A row that sees nothing, or only scores of -inf, is zeros.  A value that is infinite or NaN makes its entry NaN in the
- * rows that see it, and only in those.  chunk (0 or 1: single steps; how many neighbouring rows are successive tokens of one sequence) and max_len (0: unknown; the largest position + 1)
- * only choose how the work is split.  So does a workspace: few rows over many positions fill the GPU where the call gets b200_paged_attention_workspace(cache, args) bytes (0: it needs
+ * sums are FP32.  A row that sees nothing, or only scores of -inf, is zeros.  A value that is infinite or NaN makes its entry not finite in the
+ * rows that see it, and only in those.  chunk (0 or 1: single steps) is how many neighbouring rows are successive tokens of one sequence.  It chooses how the work is split and, with 16-bit results, what is
+ * left of a probability: chunks of 64 rows (tokens x query heads of a key/value head) and more with heads of 64, 96 or 128 keep one number of the cache's type (8 bits BF16, 11 FP16), all others two
+ * (16 bits, 22).  Waits inside the kernel of such chunks end after half a second; should one ever run out, its rows are NaN.  max_len (0: unknown; the largest position + 1) only chooses how
+ * the work is split.  So does a workspace: few rows over many positions fill the GPU where the call gets b200_paged_attention_workspace(cache, args) bytes (0: it needs
  * none) of 16-byte aligned device memory, whose content before and after does not matter and which no other call under way may use; NULL or fewer bytes: the call does without. */
 typedef struct b200_paged_attention_args {
     int32_t n, heads, window, max_len, chunk, out_type;
@@ -640,6 +642,9 @@ typedef struct b200_paged_attention_args {
 } b200_paged_attention_args;
 size_t b200_paged_attention_workspace(const b200_paged_cache *cache, const b200_paged_attention_args *args);
 int b200_paged_attention(const b200_paged_cache *cache, const b200_paged_attention_args *args, void *stream, char *err, size_t err_len);
+
+/* Test hook: the attention of a chunk (FP16, heads of 64) whose rows, at the end, wait for what never comes. */
+int b200_test_paged_give_up(const b200_paged_cache *cache, const b200_paged_attention_args *args, void *stream, char *err, size_t err_len);
 
 /* Verification of drafted tokens.  Of each of `sequences` sequences: logits rows x_0 .. x_drafts of the target ([vocab] of `type`; sequence_stride, row_stride entries apart), tokens
  * [sequences][drafts] drafted behind them (the first outside [0, vocab) ends a sequence's drafts), draft_logits rows y_0 .. y_{drafts - 1} that they were sampled from, at the same

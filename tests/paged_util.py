@@ -20,13 +20,14 @@ def rounding(want, off, dtype):
     return off + (want.abs() + off) * U.half_step(dtype) + (2.0 ** -25 if dtype == torch.float16 else 2.0 ** -126)
 
 
-def attention(q, keys, values, positions, sequences, tables, scale=None, window=0, dtype=torch.float64):
+def attention(q, keys, values, positions, sequences, tables, scale=None, window=0, dtype=torch.float64, probability=0.0):
     """(out, bound) in float64: a row at a time, over the positions that have a page.
 
     The bound.  Products of two 16-bit numbers are exact; a score's sum of hs of them, which the tensor core may cut rather than round, is off by at most hs 2^-22 of A = |scale| sum |q| |k|, its scaling and
     the subtraction of the reference by 4 of 2^-24 of that.  A probability's relative error is twice that (numerator and sum), 2^-20 for its exponential, 2^-17 for the two numbers that hold
     it (BF16; FP16's 2^-22 is less).  FP16 loses what is below 2^-25 of a row whose largest is at least 2^7: 2^-32 a position.  Sums of m products, 16 an instruction, two instructions each:
-    (m / 8 + 32) 2^-22.  Then the result's own half step."""
+    (m / 8 + 32) 2^-22.  Chunks on the tensor cores hold a probability as one number, half a step off (``probability``), while their sum has it as it was: that much more of sum p |v|.  Then the
+    result's own half step."""
     n, H, hs = q.shape
     pages, G, page, _ = keys.shape
     scale = 1.0 / math.sqrt(hs) if scale is None else scale
@@ -47,7 +48,7 @@ def attention(q, keys, values, positions, sequences, tables, scale=None, window=
         w = torch.softmax(x @ k.transpose(1, 2) * scale, -1)
         out[r] = (w @ v).view(H, hs)
         A = (x.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * abs(scale)
-        off = (w @ v.abs()) * (2 * A * (hs * 2.0 ** -22 + 4 * 2.0 ** -24) + 2.0 ** -20 + 2.0 ** -17 + (len(at) / 8 + 32) * 2.0 ** -22)
+        off = (w @ v.abs()) * (2 * A * (hs * 2.0 ** -22 + 4 * 2.0 ** -24) + 2.0 ** -20 + 2.0 ** -17 + probability + (len(at) / 8 + 32) * 2.0 ** -22)
         bound[r] = (off + len(at) * 2.0 ** -32 * v.abs().amax(1, keepdim=True)).reshape(H, hs)
     return out, rounding(out, bound, dtype) if dtype != torch.float64 else bound
 

@@ -43,9 +43,15 @@ def paged(pkg, g, lengths, page, G, hs, dtype, gain=1.0):
     return cache, tables
 
 
+def probability(cache, q, dtype, chunk):
+    """What the documentation says of chunks with 16-bit results: half a step of the cache's type where they are 64 rows and more."""
+    rows = min(chunk, len(q)) * (q.shape[1] // cache.kv_heads)
+    return U.half_step(cache.keys.dtype) if dtype != F32 and cache.head_size in (64, 96, 128) and min(chunk, len(q)) > 1 and rows >= 64 else 0.0
+
+
 def check(cache, q, positions, tables, sequences=None, dtype=None, **kw):
     got = cache.attention(q, positions, tables, sequences=sequences, dtype=dtype, **kw)
-    want, bound = P.attention(q, cache.keys, cache.values, positions, sequences, tables, kw.get("scale"), kw.get("window", 0), got.dtype)
+    want, bound = P.attention(q, cache.keys, cache.values, positions, sequences, tables, kw.get("scale"), kw.get("window", 0), got.dtype, probability(cache, q, got.dtype, kw.get("chunk", 1)))
     written = positions.cpu() < tables.shape[1] * cache.page_size
     if sequences is not None:
         written &= (sequences.cpu() >= 0) & (sequences.cpu() < tables.shape[0])  # (padding's rows are not)
@@ -155,7 +161,7 @@ def test_chunks(pkg, H, G, hs, page, dtype, out, window):
     check(cache, rand(g, 227, H, hs, dtype=dtype), pos, tables, seq, out, window=window, chunk=150, max_len=333)
 
 
-@pytest.mark.parametrize("dtype,out", [(BF16, F32), (F16, F16)])
+@pytest.mark.parametrize("dtype,out", [(BF16, F32), (F16, F16), (BF16, BF16)])
 @pytest.mark.parametrize("chunk", [1, 7, 50, 10**9])
 def test_rows_in_any_order(pkg, dtype, out, chunk):
     """What ``chunk`` and ``max_len`` say may be wrong: rows of many sequences, positions up and down, padding in between."""
@@ -224,19 +230,19 @@ def test_pages_that_are_none_and_shared_ones(pkg):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
-@pytest.mark.parametrize("chunk,hs", [(1, 128), (6, 64), (40, 64), (40, 128)])
-def test_values_that_are_not_finite_reach_who_sees_them(pkg, dtype, bad, chunk, hs):
-    g = gen(4)
+@pytest.mark.parametrize("chunk,hs,out", [(1, 128, F32), (6, 64, F32), (40, 64, F32), (40, 128, F32), (40, 64, None), (40, 96, None), (40, 128, None), (3, 128, None)])
+def test_values_that_are_not_finite_reach_who_sees_them(pkg, dtype, bad, chunk, hs, out):
+    g, out = gen(4), out or dtype
     cache, tables = paged(pkg, g, [90], 16, 2, hs, dtype)
     q = rand(g, 40, 8, hs, dtype=dtype)
     pos = torch.arange(50, 90, device="cuda", dtype=torch.int32)
-    clean = cache.attention(q, pos, tables, chunk=chunk, window=20, dtype=F32)
+    clean = cache.attention(q, pos, tables, chunk=chunk, window=20, dtype=out)
     cache.values[tables[0, 4], 1, 6, 5] = bad  # position 70: rows 70 .. 89 see it, in heads 4 .. 7, entry 5
-    got = cache.attention(q, pos, tables, chunk=chunk, window=20, dtype=F32)
+    got = cache.attention(q, pos, tables, chunk=chunk, window=20, dtype=out)
     hit = torch.zeros_like(got, dtype=torch.bool)
     hit[20:, 4:, 5] = True
-    assert torch.isnan(got[hit]).all()
-    want, bound = P.attention(q, cache.keys, torch.where(torch.isfinite(cache.values), cache.values, 0), pos, None, tables, window=20, dtype=F32)
+    assert not torch.isfinite(got[hit]).any()
+    want, bound = P.attention(q, cache.keys, torch.where(torch.isfinite(cache.values), cache.values, 0), pos, None, tables, window=20, dtype=out, probability=probability(cache, q, out, chunk))
     assert ((got.double().cpu() - want).abs() <= bound)[~hit.cpu()].all() and clean.isfinite().all()
 
 
@@ -245,7 +251,7 @@ def test_keys_that_are_not_finite(pkg):
     cache, tables = paged(pkg, g, [90], 16, 2, 64, BF16)
     q, pos = rand(g, 40, 8, 64, dtype=BF16), torch.arange(50, 90, device="cuda", dtype=torch.int32)
     cache.keys[tables[0, 4], 1, 6, 5] = float("nan")
-    for chunk in (1, 6, 40):
+    for chunk in (1, 6, 40):  # the last on the tensor cores
         got = cache.attention(q, pos, tables, chunk=chunk)
         assert got[20:, 4:].isnan().all() and got[:20].isfinite().all() and got[:, :4].isfinite().all()
 
@@ -261,6 +267,9 @@ def test_values_near_the_types_end(pkg):
     for chunk in (1, 3):
         got = cache.attention(q, pos, tables, chunk=chunk, dtype=F32).cpu() / top
         assert torch.allclose(got[..., 0], torch.ones(3, 4), atol=1e-4) and torch.allclose(got[..., 1], -torch.ones(3, 4), atol=1e-4)
+    q, pos = torch.zeros(40, 4, 64, device="cuda", dtype=BF16), torch.arange(360, 400, device="cuda", dtype=torch.int32)
+    got = cache.attention(q, pos, tables, chunk=40).float().cpu() / top  # (on the tensor cores, then once more)
+    assert torch.allclose(got[..., 0], torch.ones(40, 4), atol=2.0 ** -7) and torch.allclose(got[..., 1], -torch.ones(40, 4), atol=2.0 ** -7)
 
 
 @pytest.mark.parametrize("gain,scale", [(30.0, None), (1.0, 0.0), (1.0, -0.3), (3.0, 1.0), (1e-3, None)])
@@ -306,6 +315,45 @@ def test_rows_of_wider_ones(pkg, pad, out):
         want, bound = P.attention(q, cache.keys, cache.values, pos, seq, tables, dtype=out)
         assert ((place.double().cpu() - want).abs() <= bound).all()
         assert (wide[:, :pad] == 7).all() and (wide[:, -pad:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("H,G,hs,page,lengths,chunk,window", [(8, 2, 64, 16, [3000, 777], 64, 0), (4, 1, 128, 64, [4100], 128, 0), (4, 1, 128, 32, [9000], 33, 0), (3, 1, 96, 16, [2500, 40, 700], 40, 1500),
+                                                              (64, 1, 64, 8, [5000], 3, 0), (128, 1, 64, 16, [300], 5, 0), (16, 8, 96, 1, [1000, 900], 50, 333)])
+def test_chunks_of_long_sequences(pkg, dtype, H, G, hs, page, lengths, chunk, window):
+    """Few rows over many positions (shared by several CTAs) and many rows; sequences with holes and scores that grow."""
+    g = gen(chunk)
+    cache, tables = paged(pkg, g, lengths, page, G, hs, dtype)
+    for n, t in zip(lengths, tables):
+        at = torch.arange(n, device="cuda")
+        cache.keys[t.long()[at // page], :, at % page] *= (0.2 + 3 * at / n)[:, None, None]  # a maximum that keeps growing
+    if page > 1:
+        tables[:, 1] = -1
+    pos = torch.cat([torch.arange(n - min(chunk, n), n, device="cuda") for n in lengths]).int()
+    seq = torch.cat([torch.full((min(chunk, n),), s, device="cuda") for s, n in enumerate(lengths)]).int()
+    check(cache, rand(g, len(pos), H, hs, dtype=dtype), pos, tables, seq, dtype, chunk=chunk, window=window)
+    check(cache, rand(g, len(pos), H, hs, dtype=dtype), pos, tables, seq, dtype, chunk=chunk, window=window, max_len=max(lengths), scale=-0.2)
+
+
+def test_a_wait_that_runs_out_is_heard_of(pkg):
+    """Rows of a block whose wait ran out are NaN, whether they are joined or not, and the next call is as it was."""
+    g, N = gen(3), pkg.native
+    for length, heads in ((300, 8), (5000, 4)):
+        cache, tables = paged(pkg, g, [length], 16, heads // 4, 64, F16)
+        q, pos = rand(g, 32, heads, 64, dtype=F16), torch.arange(length - 32, length, device="cuda", dtype=torch.int32)
+        want = cache.attention(q, pos, tables, chunk=32)
+        out = torch.zeros(32, heads, 64, device="cuda", dtype=F16)
+        c, a, err = N.PagedCache(cache.keys.data_ptr(), cache.values.data_ptr(), cache.pages, 16, heads // 4, 64, 1, 0), N.PagedAttention(), C.create_string_buffer(256)
+        a.n, a.heads, a.q, a.out, a.q_stride, a.out_stride, a.positions, a.tables, a.table_stride, a.n_sequences, a.table_width, a.scale, a.chunk, a.out_type = 32, heads, q.data_ptr(), out.data_ptr(), \
+            heads * 64, heads * 64, pos.data_ptr(), tables.data_ptr(), tables.shape[1], 1, tables.shape[1], 0.125, 32, 1
+        need = N.lib().b200_paged_attention_workspace(C.byref(c), C.byref(a))
+        work = torch.zeros(need // 4 + 4, device="cuda")
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
+        assert (need > 0) == (length == 5000)
+        assert N.lib().b200_test_paged_give_up(C.byref(c), C.byref(a), torch.cuda.current_stream().cuda_stream, err, 256) == 0
+        torch.cuda.synchronize()
+        assert out.isnan().all()
+        assert torch.equal(cache.attention(q, pos, tables, chunk=32), want)
 
 
 # ---- streams, graphs, repeats ------------------------------------------------------------------------------------------------------------
