@@ -1,8 +1,8 @@
 // paged_chunk.cuh -- attention of prompt chunks over the pages on the 5th-generation tensor cores, with 16-bit results.
 //
 // A CTA takes 128 rows (tokens x query heads of one key/value head) and runs through the positions that any of them sees, 128 at a time:
-//   warps 16-23  copy a tile's keys and values from their pages as they are, [position][entry] in swizzled rows: even and odd tiles are two groups of four warps
-//   warp 24      issues S = Q K^T (both K-major) and O += P V (P from TMEM, V entry-major)
+//   warps 16-25  copy keys and values from their pages as they are, [position][entry] in swizzled rows: two warps for each of the three tiles of keys and two of values that there is room for
+//   warp 26      issues S = Q K^T (both K-major) and O += P V (P from TMEM, V entry-major)
 //   warps 0-15   exponentials, two threads a row; P in the cache's type takes the place of S; O is scaled where a row's maximum has grown by too much, which is rare
 // Even and odd tiles are two streams with accumulators, maxima and sums of their own, each of eight warps, which the end joins: while one waits for its products the other computes.
 // Rows of a tile may belong to several sequences and stand in any order: a run of tokens of one sequence is a segment, the tiles of all segments are one list, and a row masks what is not its own.
@@ -19,7 +19,7 @@ namespace paged {
 
 using namespace kv4; // barriers, products, tensor memory
 
-constexpr int C_ROWS = 128, C_KEYS = 128, C_K = 3, C_V = 2, C_SOFTMAX = 16, C_COPY = 8, C_ISSUER = C_SOFTMAX + C_COPY, C_THREADS = (C_ISSUER + 1) * 32;
+constexpr int C_ROWS = 128, C_KEYS = 128, C_K = 3, C_V = 2, C_SOFTMAX = 16, C_PAIR = 2, C_COPY = (C_K + C_V) * C_PAIR, C_ISSUER = C_SOFTMAX + C_COPY, C_THREADS = (C_ISSUER + 1) * 32;
 __host__ __device__ constexpr int c_tile_bytes(int hs) { return hs * C_KEYS * 2; }
 __host__ __device__ constexpr int c_width(int hs) { return hs % 64 == 0 ? 64 : 32; } // entries of a swizzled row: 128 or 64 bytes
 template <int HS> __device__ __forceinline__ uint32_t c_at(int r, int c) {          // of the 8 entries 8 c .. of row r in a tile
@@ -99,11 +99,11 @@ template <int HS, typename T, bool GIVE_UP = false> __global__ void __launch_bou
 
     if (tid == 0) {
         for (int i = 0; i < C_K; i++) {
-            bar_init(&sh.k_full[i], C_COPY / 2);
+            bar_init(&sh.k_full[i], C_PAIR);
             bar_init(&sh.k_free[i], 1);
         }
         for (int i = 0; i < 2; i++) {
-            bar_init(&sh.v_full[i], C_COPY / 2);
+            bar_init(&sh.v_full[i], C_PAIR);
             bar_init(&sh.v_free[i], 1);
             bar_init(&sh.s_full[i], 1);
             bar_init(&sh.p_full[i], C_SOFTMAX / 2);
@@ -190,38 +190,39 @@ template <int HS, typename T, bool GIVE_UP = false> __global__ void __launch_bou
     };
 
     if (warp >= C_SOFTMAX && warp < C_ISSUER) {
-        // ===== pages -> operands =====
-        const int group = (warp - C_SOFTMAX) / 4, part = (warp - C_SOFTMAX) % 4;
-        constexpr int PIECES = HS / 8;
+        // ===== pages -> operands: a pair of warps for every place that a tile of keys or of values has =====
+        constexpr int PIECES = HS / 8, PART = C_KEYS / C_PAIR;
+        const int place = (warp - C_SOFTMAX) / C_PAIR, part = (warp - C_SOFTMAX) % C_PAIR;
+        const bool is_k = place < C_K;
+        const int at = is_k ? place : place - C_K, step = is_k ? C_K : C_V;
+        const char *pool = (const char *)(is_k ? a.pool.keys : a.pool.values);
+        const uint32_t to = kv4::s32(is_k ? sK : sV) + at * c_tile_bytes(HS);
+        const void *full = is_k ? &sh.k_full[at] : &sh.v_full[at], *free = is_k ? &sh.k_free[at] : &sh.v_free[at];
         int seg = 0;
-        for (int j = group; j < count; j += 2) {
+        for (int j = at, turn = 0; j < count; j += step, turn++) {
             while (sh.segments[seg].tiles <= first + j) seg++;
-            const int pos = begin_of(seg, first + j) + part * 32 + lane;
-            const unsigned row = pos < sh.segments[seg].end ? row_at(a.pool, a.rows.table(sh.segments[seg].sequence), pos, kvh) : NO_ROW;
-            const unsigned have = __ballot_sync(0xffffffffu, row != NO_ROW);
-            const auto copy = [&](const void *pool, uint32_t to) {
+            const int pos = begin_of(seg, first + j) + part * PART + lane, end = sh.segments[seg].end;
+            const int *table = a.rows.table(sh.segments[seg].sequence);
+            unsigned row[PART / 32];
+#pragma unroll
+            for (int h = 0; h < PART / 32; h++) row[h] = pos + 32 * h < end ? row_at(a.pool, table, pos + 32 * h, kvh) : NO_ROW;
+            if (turn > 0 && !__all_sync(0xffffffffu, c_wait(free, (turn - 1) & 1, &sh.bail))) break; // keys: the scores of tile j - 3 stand; values: the products of tile j - 2 have read them
+#pragma unroll
+            for (int h = 0; h < PART / 32; h++) {
+                const unsigned have = __ballot_sync(0xffffffffu, row[h] != NO_ROW);
+                if (is_k && lane == 0) sh.have[at][part * (PART / 32) + h] = have;
 #pragma unroll
                 for (int i = 0; i < PIECES; i++) {
                     const int n = lane + 32 * i, r = n / PIECES, p = n % PIECES;
-                    const unsigned from = __shfl_sync(0xffffffffu, row, r);
-                    cp16_or_zeros(from != NO_ROW, to + c_at<HS>(part * 32 + r, p), (const char *)pool + (from == NO_ROW ? 0 : ((size_t)from * HS + p * 8) * 2));
+                    const unsigned from = __shfl_sync(0xffffffffu, row[h], r);
+                    cp16_or_zeros(from != NO_ROW, to + c_at<HS>(part * PART + 32 * h + r, p), pool + (from == NO_ROW ? 0 : ((size_t)from * HS + p * 8) * 2));
                 }
-                cp_commit();
-            };
-            const auto there = [&](const void *bar) { // the copies have landed
-                cp_wait<0>();
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) bar_arrive(bar);
-            };
-            const int ks = j % C_K;
-            if (j >= C_K && !__all_sync(0xffffffffu, c_wait(&sh.k_free[ks], (j / C_K - 1) & 1, &sh.bail))) break; // the scores of tile j - 3 stand
-            if (lane == 0) sh.have[ks][part] = have;
-            copy(a.pool.keys, kv4::s32(sK) + ks * c_tile_bytes(HS));
-            there(&sh.k_full[ks]);
-            if (j >= 2 && !__all_sync(0xffffffffu, c_wait(&sh.v_free[group], ((j >> 1) - 1) & 1, &sh.bail))) break; // the products of tile j - 2 have read its values
-            copy(a.pool.values, kv4::s32(sV) + group * c_tile_bytes(HS));
-            there(&sh.v_full[group]);
+            }
+            cp_commit();
+            cp_wait<0>();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(full);
         }
     } else if (warp == C_ISSUER) {
         // ===== products =====
@@ -331,21 +332,27 @@ template <int HS, typename T, bool GIVE_UP = false> __global__ void __launch_bou
                 }
                 fresh = top == -CUDART_INF_F && max(from, -side * COLUMNS) < min(to, C_KEYS - side * COLUMNS); // the first that the row sees: no maximum yet
             }
-            const unsigned *have = sh.have[j % C_K];
-            const unsigned have_lo = have[2 * side], have_hi = have[2 * side + 1]; // of this thread's positions
-            const auto seen = [&](int i) { return i >= from && i < to && ((i < 32 ? have_lo >> i : have_hi >> (i - 32)) & 1u); };
+            // bits of this thread's positions that its row sees, where not all do
+            const unsigned have_lo = sh.have[j % C_K][2 * side], have_hi = sh.have[j % C_K][2 * side + 1];
+            const auto bits = [](int from, int to) { // [from, to) of 32
+                const unsigned below = to <= 0 ? 0u : to >= 32 ? 0xffffffffu : (1u << to) - 1u;
+                return from <= 0 ? below : from >= 32 ? 0u : below & (0xffffffffu << from);
+            };
+            const unsigned seen_lo = bits(from, to) & have_lo, seen_hi = bits(from - 32, to - 32) & have_hi;
+            const bool whole = (seen_lo & seen_hi) == 0xffffffffu;
             // One pass with the maximum as it stands.  It moves rarely, and a sum of more than 2^8 shows that it has to: the probabilities, which have taken the place of the scores, are
             // dropped, the scores come once more, and the tile's maximum is looked for first.  (A maximum of every tile in front of the exponentials would read the scores twice.)
-            const bool special = __any_sync(0xffffffffu, repeat || fresh || from > 0 || to < COLUMNS || (have_lo & have_hi) != 0xffffffffu || !(fabsf(ref) <= 65536.0f));
+            const bool special = __any_sync(0xffffffffu, repeat || fresh || !whole || !(fabsf(ref) <= 65536.0f));
             if (special && __any_sync(0xffffffffu, repeat || fresh)) { // (the same for both warps of a row)
                 float mx = -CUDART_INF_F;
 #pragma unroll 1
                 for (int q = 0; q < COLUMNS; q += PIECE) {
                     uint32_t x[PIECE];
                     tmem_ld16(row_s + q, x);
+                    const unsigned seen = (q < 32 ? seen_lo : seen_hi) >> q % 32;
                     tmem_ld_wait();
 #pragma unroll
-                    for (int i = 0; i < PIECE; i++) mx = fmaxf(mx, seen(q + i) ? __uint_as_float(x[i]) : -CUDART_INF_F);
+                    for (int i = 0; i < PIECE; i++) mx = fmaxf(mx, seen & (1u << i) ? __uint_as_float(x[i]) : -CUDART_INF_F);
                 }
                 sh.half_row[stream][side][r] = mx;
                 ok = meet();
@@ -369,21 +376,22 @@ template <int HS, typename T, bool GIVE_UP = false> __global__ void __launch_bou
                 ref = base * factor - LIFT;
             }
             // P takes the place of S: piece q of 16 scores is read before its 8 columns are written, [8 q, 8 q + 8)
-            if (special && !__any_sync(0xffffffffu, max(from, 0) < min(to, COLUMNS))) { // other rows' tile
+            if (special && !__any_sync(0xffffffffu, (seen_lo | seen_hi) != 0u)) { // other rows' tile
                 const uint32_t p[PIECE / 2] = {};
                 sum = 0.0f;
 #pragma unroll 1
                 for (int q = 0; q < COLUMNS / 2; q += PIECE / 2) tmem_st8(row_s + q, p);
-            } else if (special && __any_sync(0xffffffffu, from > 0 || to < COLUMNS || (have_lo & have_hi) != 0xffffffffu || !(fabsf(ref) <= 65536.0f))) { // a border, or scores so large that their products and the maximum's round apart
+            } else if (special && __any_sync(0xffffffffu, !whole || !(fabsf(ref) <= 65536.0f))) { // a border, or scores so large that their products and the maximum's round apart
                 sum = 0.0f;
 #pragma unroll 1
                 for (int q = 0; q < COLUMNS; q += PIECE) {
                     uint32_t x[PIECE], p[PIECE / 2];
                     tmem_ld16(row_s + q, x);
+                    const unsigned seen = (q < 32 ? seen_lo : seen_hi) >> q % 32;
                     tmem_ld_wait();
 #pragma unroll
                     for (int i = 0; i < PIECE; i++) {
-                        const float e = seen(q + i) ? ex2(fmaf(__uint_as_float(x[i]) - base, factor, LIFT)) : 0.0f;
+                        const float e = seen & (1u << i) ? ex2(fmaf(__uint_as_float(x[i]) - base, factor, LIFT)) : 0.0f;
                         sum += e;
                         x[i] = __float_as_uint(e);
                     }
