@@ -180,9 +180,10 @@ struct Step {
 };
 
 constexpr int STEP_WARPS = 4;
-__host__ __device__ constexpr int step_keys(int hs) { return hs >= 96 ? 16 : 32; }                        // positions that a warp takes at a time: a tile
-__host__ __device__ constexpr int step_stages(int hs) { return hs == 32 ? 4 : 3; }                        // tiles that it has room for
-__host__ __device__ constexpr int step_stage_bytes(int hs) { return step_keys(hs) * hs * 4; }             // keys and values
+__host__ __device__ constexpr int step_keys(int hs) { return hs >= 96 ? 16 : 32; }            // positions that a warp takes at a time: a tile
+__host__ __device__ constexpr int step_stages(int hs) { return hs == 32 ? 4 : hs == 64 ? 2 : 3; } // tiles that it has room for
+__host__ __device__ constexpr int step_stage_bytes(int hs) { return step_keys(hs) * hs * 4; } // keys and values
+__host__ __device__ constexpr int step_ctas(int hs, int mt) { return mt == 2 ? 2 : hs <= 64 ? 4 : hs <= 128 ? 3 : 1; } // of an SM, as far as registers go
 __host__ __device__ constexpr int step_rows(int mt) { return 16 * mt; }
 __host__ __device__ constexpr int step_tokens_most() { return 32; }
 __host__ __device__ constexpr int part_stride(int hs) { return hs + 8; }
@@ -242,13 +243,13 @@ __device__ __forceinline__ void put_results(const Step &a, int row, int head, in
 // has a cp.async ring and a running reference of its own, and no barrier in the loop.  Parts are joined in shared memory, those of several CTAs through the workspace (k_paged_join).
 // Nothing depends on an order of arrival.
 //   scores  S[16 rows x 8 positions] = Q K^T, the cache's type, exact products, FP32 sums;  p = 2^(scale log2(e) s - ref)
-//   values  O[16 rows x 8 entries] += P V with p as two numbers of the cache's type, p and what rounding it left: 16 (BF16) or 22 (FP16) bits, so that the result's rounding is what is left
+//   values  O[16 rows x 8 entries] += P V with p in the cache's type, half a step off, as the result will be; TWO (FP32 results): and what that left, 16 (BF16) or 22 (FP16) bits in all
 // ref follows the largest score seen so far only when that passes it by more than 2^8 (the first does), so that few tiles have anything to rescale; with FP16 it lies 2^7 below, so that
 // p reaches down to 2^-24 of 2^-15: a long tail of small ones still counts.
 // A value that is infinite or NaN would reach every row of the block as 0 * NaN, also those that do not see it.  A warp whose sums are not finite runs through its tiles once more with such
 // entries taken out of the product, and a product of zeros and ones says which rows have met one: those become NaN.  With BF16, where sums of large values may leave FP32's
 // range before they are divided, that second run has p times 2^-40.
-template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WARPS * 32) k_paged_step(const Step a) {
+template <int HS, typename T, int MT, bool TWO> __global__ void __launch_bounds__(STEP_WARPS * 32, step_ctas(HS, MT)) k_paged_step(const Step a) {
     constexpr int KT = step_keys(HS), NT = KT / 8, KS = KT / 16, S = step_stages(HS), ROWS = step_rows(MT), PIECES = HS / 8, STAGE = step_stage_bytes(HS), TOKENS = step_tokens_most();
     constexpr bool F16 = std::is_same<T, __half>::value, QREG = MT == 1 && HS <= 128;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -262,13 +263,99 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
     const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % G, block = blockIdx.x / a.splits / G % a.blocks, unit = blockIdx.x / a.splits / G / a.blocks;
     const int token0 = unit * a.tokens, tokens = min(a.tokens, a.rows.n - token0), row0 = block * ROWS, rows = min(ROWS, tokens * mul - row0);
 
-    if (tid < tokens) {
+    Segment only = {-1, 0, 0, 0, 0, 0}; // the first segment, which mostly is the only one
+    if (tokens == 1) { // every thread by itself
         int pos;
-        const int s = a.rows.place(token0 + tid, pos);
-        seq_of[tid] = s;
-        pos_of[tid] = max(pos, -1);
+        const int s = a.rows.place(token0, pos);
+        pos = max(pos, -1);
+        if (s >= 0 && pos >= 0) {
+            visible(pos, a.window, only.lo, only.hi);
+            only.sequence = s;
+            only.begin = only.lo / KT;
+            only.end = (only.hi - 1) / KT + 1;
+            only.tiles = only.end - only.begin;
+        }
+        if (tid == 0) { // (read behind the next barrier)
+            seq_of[0] = s;
+            pos_of[0] = pos;
+            segment_of[0] = s >= 0 && pos >= 0 ? 0 : -1;
+        }
+    } else {
+        if (tid < tokens) {
+            int pos;
+            const int s = a.rows.place(token0 + tid, pos);
+            seq_of[tid] = s;
+            pos_of[tid] = max(pos, -1);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int n = 0, total = 0;
+            for (int i = 0; i < tokens;) {
+                const int s = seq_of[i];
+                int j = i, from = INT_MAX, to = 0;
+                for (; j < tokens && seq_of[j] == s; j++) {
+                    int lo, hi;
+                    visible(pos_of[j], a.window, lo, hi);
+                    if (hi > lo) { from = min(from, lo); to = max(to, hi); }
+                    segment_of[j] = n;
+                }
+                if (s >= 0 && to > 0) {
+                    const int begin = from / KT, end = (to - 1) / KT + 1;
+                    total += end - begin;
+                    segments[n++] = {s, begin, end, from, to, total};
+                } else
+                    for (int k = i; k < j; k++) segment_of[k] = -1;
+                i = j;
+            }
+            n_segments = n;
+        }
+        __syncthreads();
+        if (n_segments) only = segments[0];
     }
-    for (int i = tid; i < ROWS * PIECES; i += STEP_WARPS * 32) {
+    const int total = tokens == 1 ? only.tiles : n_segments ? segments[n_segments - 1].tiles : 0;
+    const int first = (int)min((long long)split * a.share, (long long)total), last = split == a.splits - 1 ? total : min(total, first + a.share);
+    if (a.splits > 1 && first >= last) { // nothing for this CTA: its parts have no sum
+        float *w = a.work + (size_t)a.rows.n * a.heads * a.splits * HS;
+        if (tid < rows) {
+            const int token = (row0 + tid) / mul, head = kvh * mul + row0 + tid - token * mul;
+            reinterpret_cast<float2 *>(w)[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(-CUDART_INF_F, 0.0f);
+        }
+        return;
+    }
+
+    const uint32_t ring = s32(smem) + warp * S * STAGE, q_at = s32(sQ);
+    // this warp's tiles: numbers first + warp, + STEP_WARPS, .. of the list; `fetched` is the next to ask for
+    int fetched = first + warp, seg_f = 0;
+    Segment ahead = only;
+    auto look_up = [&]() -> unsigned { // the number of the row that this lane looks up for the tile `fetched`
+        if (fetched >= last) return NO_ROW;
+        while (ahead.tiles <= fetched) ahead = segments[++seg_f];
+        const int pos = (ahead.end - (ahead.tiles - fetched)) * KT + lane;
+        return lane < KT && pos >= ahead.lo && pos < ahead.hi ? row_at(a.pool, a.rows.table(ahead.sequence), pos, kvh) : NO_ROW;
+    };
+    unsigned row = look_up();
+    auto fetch = [&](int stage) { // and look the next one up
+        if (fetched < last) {
+            const unsigned have = __ballot_sync(0xffffffffu, row != NO_ROW);
+            if (lane == 0) there[warp][stage] = have;
+            const uint32_t dst = ring + stage * STAGE;
+#pragma unroll
+            for (int i = 0; i < KT * PIECES / 32; i++) {
+                const int n = lane + 32 * i, r = n / PIECES, p = n % PIECES;
+                const unsigned from = __shfl_sync(0xffffffffu, row, r);
+                const size_t off = from == NO_ROW ? 0 : ((size_t)from * HS + p * 8) * 2;
+                cp16_or_zeros(from != NO_ROW, dst + piece<HS>(r, p), (const char *)a.pool.keys + off);
+                cp16_or_zeros(from != NO_ROW, dst + KT * HS * 2 + piece<HS>(r, p), (const char *)a.pool.values + off);
+            }
+            fetched += STEP_WARPS;
+            row = look_up();
+        }
+        cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < S - 1; i++) fetch(i);
+
+    for (int i = tid; i < ROWS * PIECES; i += STEP_WARPS * 32) { // queries
         const int r = i / PIECES, c = i % PIECES, token = (row0 + r) / mul;
         uint4 w = make_uint4(0u, 0u, 0u, 0u);
         if (r < rows) {
@@ -279,38 +366,6 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
         *reinterpret_cast<uint4 *>(sQ + piece<HS>(r, c)) = w;
     }
     __syncthreads();
-    if (tid == 0) {
-        int n = 0, total = 0;
-        for (int i = 0; i < tokens;) {
-            const int s = seq_of[i];
-            int j = i, from = INT_MAX, to = 0;
-            for (; j < tokens && seq_of[j] == s; j++) {
-                int lo, hi;
-                visible(pos_of[j], a.window, lo, hi);
-                if (hi > lo) { from = min(from, lo); to = max(to, hi); }
-                segment_of[j] = n;
-            }
-            if (s >= 0 && to > 0) {
-                const int begin = from / KT, end = (to - 1) / KT + 1;
-                total += end - begin;
-                segments[n++] = {s, begin, end, from, to, total};
-            } else
-                for (int k = i; k < j; k++) segment_of[k] = -1;
-            i = j;
-        }
-        n_segments = n;
-    }
-    __syncthreads();
-    const int total = n_segments ? segments[n_segments - 1].tiles : 0;
-    const int first = (int)min((long long)split * a.share, (long long)total), last = split == a.splits - 1 ? total : min(total, first + a.share);
-    if (a.splits > 1 && first >= last) { // nothing for this CTA: its parts have no sum
-        float *w = a.work + (size_t)a.rows.n * a.heads * a.splits * HS;
-        if (tid < rows) {
-            const int token = (row0 + tid) / mul, head = kvh * mul + row0 + tid - token * mul;
-            reinterpret_cast<float2 *>(w)[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(-CUDART_INF_F, 0.0f);
-        }
-        return;
-    }
 
     // rows 16 m + g and 16 m + 8 + g of this thread: what they see, within which segment
     int lo[MT][2], hi[MT][2], own[MT][2];
@@ -334,7 +389,6 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
     lo_most = __reduce_max_sync(0xffffffffu, lo_most);
     hi_least = __reduce_min_sync(0xffffffffu, hi_least);
 
-    const uint32_t ring = s32(smem) + warp * S * STAGE, q_at = s32(sQ);
     // ldmatrix rows: keys: lanes 0-7 rows 0-7 piece 0, 8-15 the same rows piece 1, 16-31 rows 8-15; values (transposed): lanes 0-7 rows 0-7, 8-15 rows 8-15 of a piece, 16-31 of the next
     const int k_row = (lane & 7) + (lane >> 4 << 3), k_piece = lane >> 3 & 1, v_row = lane & 15, v_piece = lane >> 4;
     const float c = a.scale * 1.4426950408889634f;
@@ -345,6 +399,14 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
 
     float o[MT][HS / 8][4], l[MT][2], ref[MT][2];
     for (int careful = 0;; careful = 1) {
+        if (careful) { // once more from the first tile
+            fetched = first + warp;
+            seg_f = 0;
+            ahead = only;
+            row = look_up();
+#pragma unroll
+            for (int i = 0; i < S - 1; i++) fetch(i);
+        }
         const float below = F16 ? 7.0f : careful ? -40.0f : 0.0f;
 #pragma unroll
         for (int m = 0; m < MT; m++) {
@@ -353,36 +415,8 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
             l[m][0] = l[m][1] = 0.0f;
             ref[m][0] = ref[m][1] = -CUDART_INF_F;
         }
-        // this warp's tiles: numbers first + warp, + STEP_WARPS, .. of the list; `fetched` is the next to ask for, `seg_f` its segment
-        int fetched = first + warp, seg_f = 0, seg = 0;
-        auto look_up = [&]() -> unsigned { // the number of the row that this lane looks up for the tile `fetched`
-            if (fetched >= last) return NO_ROW;
-            while (segments[seg_f].tiles <= fetched) seg_f++;
-            const Segment &sg = segments[seg_f];
-            const int pos = (sg.end - (sg.tiles - fetched)) * KT + lane;
-            return lane < KT && pos >= sg.lo && pos < sg.hi ? row_at(a.pool, a.rows.table(sg.sequence), pos, kvh) : NO_ROW;
-        };
-        unsigned row = look_up();
-        auto fetch = [&](int stage) { // and look the next one up
-            if (fetched < last) {
-                const unsigned have = __ballot_sync(0xffffffffu, row != NO_ROW);
-                if (lane == 0) there[warp][stage] = have;
-                const uint32_t dst = ring + stage * STAGE;
-#pragma unroll
-                for (int i = 0; i < KT * PIECES / 32; i++) {
-                    const int n = lane + 32 * i, r = n / PIECES, p = n % PIECES;
-                    const unsigned from = __shfl_sync(0xffffffffu, row, r);
-                    const size_t off = from == NO_ROW ? 0 : ((size_t)from * HS + p * 8) * 2;
-                    cp16_or_zeros(from != NO_ROW, dst + piece<HS>(r, p), (const char *)a.pool.keys + off);
-                    cp16_or_zeros(from != NO_ROW, dst + KT * HS * 2 + piece<HS>(r, p), (const char *)a.pool.values + off);
-                }
-                fetched += STEP_WARPS;
-                row = look_up();
-            }
-            cp_commit();
-        };
-#pragma unroll
-        for (int i = 0; i < S - 1; i++) fetch(i);
+        Segment sg = only;
+        int seg = 0;
         int stage = 0;
         for (int tile = first + warp; tile < last; tile += STEP_WARPS) {
             cp_wait<S - 2>();
@@ -416,8 +450,7 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
                 }
             }
             const unsigned have = there[warp][stage];
-            while (segments[seg].tiles <= tile) seg++;
-            const Segment &sg = segments[seg];
+            while (sg.tiles <= tile) sg = segments[++seg];
             const int key0 = (sg.end - (sg.tiles - tile)) * KT;
             // masks; the largest score of the thread's part of each row
             const bool whole = one && key0 >= lo_most && key0 + KT <= hi_least && have == (KT == 32 ? 0xffffffffu : (1u << (KT & 31)) - 1u);
@@ -472,9 +505,11 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
                         const float p0 = ex2(s[m][n][2 * h] - base), p1 = ex2(s[m][n][2 * h + 1] - base);
                         l[m][h] += p0 + p1;
                         const uint32_t w = pack2<T>(p0, p1);
-                        const float2 r = unpack2<T>(w);
                         ph[m][n / 2][(n & 1) * 2 + h] = w;
-                        pl[m][n / 2][(n & 1) * 2 + h] = pack2<T>(p0 - r.x, p1 - r.y);
+                        if constexpr (TWO) {
+                            const float2 r = unpack2<T>(w);
+                            pl[m][n / 2][(n & 1) * 2 + h] = pack2<T>(p0 - r.x, p1 - r.y);
+                        }
                     }
             uint32_t saw[MT][KS][4]; // ones where a position is seen
             if (careful)
@@ -519,8 +554,10 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
                     for (int m = 0; m < MT; m++) {
                         mma<T>(o[m][i], ph[m][k], b[0], b[1]);
                         mma<T>(o[m][i + 1], ph[m][k], b[2], b[3]);
-                        mma<T>(o[m][i], pl[m][k], b[0], b[1]);
-                        mma<T>(o[m][i + 1], pl[m][k], b[2], b[3]);
+                        if constexpr (TWO) {
+                            mma<T>(o[m][i], pl[m][k], b[0], b[1]);
+                            mma<T>(o[m][i + 1], pl[m][k], b[2], b[3]);
+                        }
                     }
                 }
             if (++stage == S) stage = 0;
@@ -550,8 +587,9 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             const int r = 16 * m + 8 * h + g;
             if (t == 0) { wref[warp][r] = ref[m][h]; wsum[warp][r] = sum; }
+            if (r < rows)
 #pragma unroll
-            for (int i = 0; i < HS / 8; i++) *reinterpret_cast<float2 *>(parts + (warp * ROWS + r) * part_stride(HS) + 8 * i + 2 * t) = make_float2(o[m][i][2 * h], o[m][i][2 * h + 1]);
+                for (int i = 0; i < HS / 8; i++) *reinterpret_cast<float2 *>(parts + (warp * ROWS + r) * part_stride(HS) + 8 * i + 2 * t) = make_float2(o[m][i][2 * h], o[m][i][2 * h + 1]);
         }
     __syncthreads();
     if (tid < rows) {
@@ -583,6 +621,56 @@ template <int HS, typename T, int MT> __global__ void __launch_bounds__(STEP_WAR
         }
         if (a.splits > 1) *reinterpret_cast<float4 *>(a.work + (((size_t)row * a.heads + head) * a.splits + split) * HS + e) = x;
         else if (seq_of[token] >= 0) put_results(a, row, head, HS, e, x);
+    }
+}
+
+// Joins the parts of a row's head, at most 32 of them: a warp each, the weight of a part a lane.
+template <int HS> __global__ void __launch_bounds__(128) k_paged_join_few(const Step a) {
+    constexpr int V = HS % 128 == 0 ? 4 : HS % 64 == 0 ? 2 : 1, N = HS / (32 * V); // entries of a lane at a time, how many times
+    pdl_wait();
+    const int lane = threadIdx.x & 31, item = blockIdx.x * 4 + (threadIdx.x >> 5), row = item / a.heads, head = item % a.heads;
+    int pos;
+    if (row >= a.rows.n || a.rows.place(row, pos) < 0) return;
+    const float *part = a.work + (size_t)item * a.splits * HS;
+    const float2 st = lane < a.splits ? (reinterpret_cast<const float2 *>(a.work + (size_t)a.rows.n * a.heads * a.splits * HS) + (size_t)item * a.splits)[lane] : make_float2(-CUDART_INF_F, 0.0f);
+    const float M = warp_max_f(st.x), base = M == -CUDART_INF_F ? 0.0f : M, f = st.x == M ? 1.0f : ex2(st.x - base);
+    const unsigned some = __ballot_sync(0xffffffffu, st.y != 0.0f); // (what the entries of a part without a sum hold is not defined)
+    float L = st.y != 0.0f ? f * st.y : 0.0f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    float x[N][V];
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < V; i++) x[n][i] = 0.0f;
+    for (int s = 0; s < a.splits; s++) {
+        const float w = __shfl_sync(0xffffffffu, f, s);
+        if (!(some >> s & 1u)) continue;
+#pragma unroll
+        for (int n = 0; n < N; n++) {
+            const float *p = part + (size_t)s * HS + (n * 32 + lane) * V;
+            float v[V];
+            if constexpr (V == 4) { const float4 u = *reinterpret_cast<const float4 *>(p); v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w; }
+            else if constexpr (V == 2) { const float2 u = *reinterpret_cast<const float2 *>(p); v[0] = u.x; v[1] = u.y; }
+            else v[0] = *p;
+#pragma unroll
+            for (int i = 0; i < V; i++) x[n][i] = fmaf(w, v[i], x[n][i]);
+        }
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const long long at = row * a.ldo + (long long)head * HS + (n * 32 + lane) * V;
+#pragma unroll
+        for (int i = 0; i < V; i++) x[n][i] *= inv;
+        if constexpr (V == 4) put_results(a, row, head, HS, (n * 32 + lane) * 4, make_float4(x[n][0], x[n][1], x[n][2], x[n][3]));
+        else
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                if (a.out_type == B200_GGML_F32) ((float *)a.out)[at + i] = x[n][i];
+                else if (a.out_type == B200_GGML_F16) put((__half *)a.out + at + i, x[n][i]);
+                else put((bf16 *)a.out + at + i, x[n][i]);
+            }
     }
 }
 

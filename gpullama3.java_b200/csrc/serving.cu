@@ -116,6 +116,11 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
     k.work = (float *)a.workspace;
     const int sms = sm_count(c.device);
     const auto has_room = [&](int splits) { return a.workspace && paged_work_bytes(c, a, splits) <= a.workspace_bytes; };
+    const auto join = [&](auto hs, int splits) { // a warp a row and head, a CTA where there are more parts than lanes
+        const unsigned items = (unsigned)a.n * a.heads;
+        if (splits <= 32) return launch(paged::k_paged_join_few<hs>, (items + 3) / 4, 128, 0, 1, true, stream, k);
+        return launch(paged::k_paged_join<hs>, items, 128, 0, 1, true, stream, k);
+    };
     if (PagedChunkCut cc = paged_chunk_cut(c, a, sms); cc.use) {
         if (!has_room(cc.splits)) cc.splits = 1;
         k.tokens = cc.tokens; k.splits = cc.splits;
@@ -130,7 +135,7 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
                 if constexpr (hs == 64 && std::is_same<T, __half>::value) if (give_up) kern = paged::k_paged_chunk<hs, T, true>;
                 cudaError_t e = allow_smem(kern, smem);
                 if (e == cudaSuccess) e = launch(kern, grid, paged::C_THREADS, smem, 1, false, stream, k);
-                return e != cudaSuccess || cc.splits == 1 ? e : launch(paged::k_paged_join<hs>, (unsigned)a.n * a.heads, 128, 0, 1, true, stream, k);
+                return e != cudaSuccess || cc.splits == 1 ? e : join(hs, cc.splits);
             };
             if (c.head_size == 64) return go(std::integral_constant<int, 64>());
             if (c.head_size == 96) return go(std::integral_constant<int, 96>());
@@ -146,10 +151,10 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
             using T = decltype(type);
             const auto go = [&](auto mt) {
                 constexpr size_t smem = paged::step_smem_bytes(hs, mt);
-                auto kern = paged::k_paged_step<hs, T, mt>;
+                auto kern = a.out_type == B200_GGML_F32 ? paged::k_paged_step<hs, T, mt, true> : paged::k_paged_step<hs, T, mt, false>;
                 cudaError_t e = allow_smem(kern, smem);
                 if (e == cudaSuccess) e = launch(kern, grid, paged::STEP_WARPS * 32, smem, 1, false, stream, k);
-                return e != cudaSuccess || cut.splits == 1 ? e : launch(paged::k_paged_join<hs>, (unsigned)a.n * a.heads, 128, 0, 1, true, stream, k);
+                return e != cudaSuccess || cut.splits == 1 ? e : join(hs, cut.splits);
             };
             if constexpr (hs < 256) if (cut.mt == 2) return go(std::integral_constant<int, 2>());
             return go(std::integral_constant<int, 1>());

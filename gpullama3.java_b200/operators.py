@@ -94,10 +94,10 @@ class PagedKVCache(_ops.Paged):
 
     attention(q, positions, tables, sequences=None, scale=None, window=0, max_len=0, chunk=1, dtype=None, out=None)
         Causal attention of rows ``q`` [n, heads, head_size] of the cache's type: the row at position p sees the positions up to p of its sequence, the last ``window`` of them (0: all);
-        ``scale`` is head_size ** -0.5 unless given.  Results are of the cache's type unless ``dtype`` says FP32, FP16 or BF16.  ``max_len`` (largest position + 1, 0: unknown) only
-        chooses how the work is split.  ``chunk`` (neighbouring rows that are successive tokens of one sequence: drafted tokens, a prompt's chunk) does too, and with 16-bit results it chooses
-        what is left of a probability: chunks of 64 rows (tokens x query heads of a key/value head) and more with heads of 64, 96 or 128 keep one number of the cache's type (8 bits BF16, 11
-        FP16), all others two (16 bits, 22).  A row that sees nothing is zeros; a value that is infinite or NaN reaches the rows that see it, and only those."""
+        ``scale`` is head_size ** -0.5 unless given.  Results are of the cache's type unless ``dtype`` says FP32, FP16 or BF16.  ``chunk`` (neighbouring rows that are successive tokens of one
+        sequence: drafted tokens, a prompt's chunk) and ``max_len`` (largest position + 1, 0: unknown) only choose how the work is split.  ``dtype`` chooses the precision too: 16-bit results come
+        from probabilities of the cache's type, half a step off each, FP32 results from two such numbers (16 bits BF16, 22 FP16).  A row that sees nothing is zeros; a value that is
+        infinite or NaN reaches the rows that see it, and only those."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_size: int, dtype: torch.dtype = torch.bfloat16, device: int | torch.device | str | None = None):
         device = torch.device("cuda", device) if isinstance(device, int) else torch.device("cuda" if device is None else device)

@@ -622,11 +622,11 @@ int b200_paged_append(const b200_paged_cache *cache, const b200_paged_append_arg
 
 /* Causal attention of n query rows of the cache's type over the pages of their sequences: the row at position p sees the positions j <= p that have a page, the last `window` of them
  * where window > 0; query head h reads key/value head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type (F32, F16, BF16).  Queries and keys are multiplied as they are,
- * sums are FP32.  A row that sees nothing, or only scores of -inf, is zeros.  A value that is infinite or NaN makes its entry not finite in the
- * rows that see it, and only in those.  chunk (0 or 1: single steps) is how many neighbouring rows are successive tokens of one sequence.  It chooses how the work is split and, with 16-bit results, what is
- * left of a probability: chunks of 64 rows (tokens x query heads of a key/value head) and more with heads of 64, 96 or 128 keep one number of the cache's type (8 bits BF16, 11 FP16), all others two
- * (16 bits, 22).  Waits inside the kernel of such chunks end after half a second; should one ever run out, its rows are NaN.  max_len (0: unknown; the largest position + 1) only chooses how
- * the work is split.  So does a workspace: few rows over many positions fill the GPU where the call gets b200_paged_attention_workspace(cache, args) bytes (0: it needs
+ * sums are FP32, and a probability is a number of the cache's type (8 bits BF16, 11 FP16: with results of 16 bits, which round as much) or two of them (16 bits, 22: with FP32 results).  A row
+ * that sees nothing, or only scores of -inf, is zeros.  A value that is infinite or NaN makes its entry not finite in the rows that see it, and only in those.  chunk (0 or 1: single
+ * steps; how many neighbouring rows are successive tokens of one sequence) and max_len (0: unknown; the largest position + 1) only choose how the work is split.  Chunks of 64 rows (tokens x query
+ * heads of a key/value head) and more with 16-bit results and heads of 64, 96 or 128 run on the tensor cores' own memory; waits inside that kernel end after half a second, and should one ever run
+ * out, its rows are NaN.  So does a workspace: few rows over many positions fill the GPU where the call gets b200_paged_attention_workspace(cache, args) bytes (0: it needs
  * none) of 16-byte aligned device memory, whose content before and after does not matter and which no other call under way may use; NULL or fewer bytes: the call does without. */
 typedef struct b200_paged_attention_args {
     int32_t n, heads, window, max_len, chunk, out_type;

@@ -26,7 +26,7 @@ def attention(q, keys, values, positions, sequences, tables, scale=None, window=
     The bound.  Products of two 16-bit numbers are exact; a score's sum of hs of them, which the tensor core may cut rather than round, is off by at most hs 2^-22 of A = |scale| sum |q| |k|, its scaling and
     the subtraction of the reference by 4 of 2^-24 of that.  A probability's relative error is twice that (numerator and sum), 2^-20 for its exponential, 2^-17 for the two numbers that hold
     it (BF16; FP16's 2^-22 is less).  FP16 loses what is below 2^-25 of a row whose largest is at least 2^7: 2^-32 a position.  Sums of m products, 16 an instruction, two instructions each:
-    (m / 8 + 32) 2^-22.  Chunks on the tensor cores hold a probability as one number, half a step off (``probability``), while their sum has it as it was: that much more of sum p |v|.  Then the
+    (m / 8 + 32) 2^-22.  With 16-bit results a probability is one number, half a step off (``probability``), while their sum has it as it was: that much more of sum p |v|.  Then the
     result's own half step."""
     n, H, hs = q.shape
     pages, G, page, _ = keys.shape

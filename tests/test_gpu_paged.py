@@ -43,15 +43,14 @@ def paged(pkg, g, lengths, page, G, hs, dtype, gain=1.0):
     return cache, tables
 
 
-def probability(cache, q, dtype, chunk):
-    """What the documentation says of chunks with 16-bit results: half a step of the cache's type where they are 64 rows and more."""
-    rows = min(chunk, len(q)) * (q.shape[1] // cache.kv_heads)
-    return U.half_step(cache.keys.dtype) if dtype != F32 and cache.head_size in (64, 96, 128) and min(chunk, len(q)) > 1 and rows >= 64 else 0.0
+def probability(cache, dtype):
+    """What the documentation says: with 16-bit results a probability is one number of the cache's type, half a step off."""
+    return 0.0 if dtype == F32 else U.half_step(cache.keys.dtype)
 
 
 def check(cache, q, positions, tables, sequences=None, dtype=None, **kw):
     got = cache.attention(q, positions, tables, sequences=sequences, dtype=dtype, **kw)
-    want, bound = P.attention(q, cache.keys, cache.values, positions, sequences, tables, kw.get("scale"), kw.get("window", 0), got.dtype, probability(cache, q, got.dtype, kw.get("chunk", 1)))
+    want, bound = P.attention(q, cache.keys, cache.values, positions, sequences, tables, kw.get("scale"), kw.get("window", 0), got.dtype, probability(cache, got.dtype))
     written = positions.cpu() < tables.shape[1] * cache.page_size
     if sequences is not None:
         written &= (sequences.cpu() >= 0) & (sequences.cpu() < tables.shape[0])  # (padding's rows are not)
@@ -242,7 +241,7 @@ def test_values_that_are_not_finite_reach_who_sees_them(pkg, dtype, bad, chunk, 
     hit = torch.zeros_like(got, dtype=torch.bool)
     hit[20:, 4:, 5] = True
     assert not torch.isfinite(got[hit]).any()
-    want, bound = P.attention(q, cache.keys, torch.where(torch.isfinite(cache.values), cache.values, 0), pos, None, tables, window=20, dtype=out, probability=probability(cache, q, out, chunk))
+    want, bound = P.attention(q, cache.keys, torch.where(torch.isfinite(cache.values), cache.values, 0), pos, None, tables, window=20, dtype=out, probability=probability(cache, out))
     assert ((got.double().cpu() - want).abs() <= bound)[~hit.cpu()].all() and clean.isfinite().all()
 
 
@@ -312,7 +311,7 @@ def test_rows_of_wider_ones(pkg, pad, out):
     for chunk in (1, 3, 5):
         place.fill_(7.0)
         cache.attention(q, pos, wide_tables[:, 1:-2], sequences=seq, chunk=chunk, out=place)
-        want, bound = P.attention(q, cache.keys, cache.values, pos, seq, tables, dtype=out)
+        want, bound = P.attention(q, cache.keys, cache.values, pos, seq, tables, dtype=out, probability=probability(cache, out))
         assert ((place.double().cpu() - want).abs() <= bound).all()
         assert (wide[:, :pad] == 7).all() and (wide[:, -pad:] == 7).all()
 
