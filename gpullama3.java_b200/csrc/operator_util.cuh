@@ -56,9 +56,9 @@ int type_bytes(int type) { return type == B200_GGML_F32 ? 4 : 2; }
 bool aligned16(const void *p, long long stride, int bytes) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * bytes % 16 == 0; }
 
 template <typename... KA, typename... A>
-cudaError_t launch(void (*kern)(KA...), unsigned grid, int block, size_t smem, int cluster, bool pdl, cudaStream_t stream, A... args) {
+cudaError_t launch(void (*kern)(KA...), dim3 grid, int block, size_t smem, int cluster, bool pdl, cudaStream_t stream, A... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(block);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;

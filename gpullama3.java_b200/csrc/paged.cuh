@@ -9,6 +9,7 @@
 namespace paged {
 
 using kv4::bf16;
+using kv4::cp16;
 using kv4::cp_commit;
 using kv4::cp_wait;
 using kv4::ex2;
@@ -175,21 +176,22 @@ struct Step {
     int heads, window, vec, vec_out, out_type;
     float scale;
     void *out;
+    int mul, of;                       // query heads of a key/value head; r / mul = r of >> 16 for the rows of a unit of several tokens
     int tokens, blocks, splits, share; // rows of a unit are `tokens` neighbouring ones, in `blocks` blocks; `splits` CTAs run through `share` tiles each (the last one through the rest)
     float *work;                       // parts of units that several CTAs share: [row][head][split] entries, behind them [row][head][split] reference and sum
 };
 
 constexpr int STEP_WARPS = 4;
-__host__ __device__ constexpr int step_keys(int hs) { return hs >= 96 ? 16 : 32; }            // positions that a warp takes at a time: a tile
-__host__ __device__ constexpr int step_stages(int hs) { return hs == 32 ? 4 : hs == 64 ? 2 : 3; } // tiles that it has room for
-__host__ __device__ constexpr int step_stage_bytes(int hs) { return step_keys(hs) * hs * 4; } // keys and values
-__host__ __device__ constexpr int step_ctas(int hs, int mt) { return mt == 2 ? 2 : hs <= 64 ? 4 : hs <= 128 ? 3 : 1; } // of an SM, as far as registers go
-__host__ __device__ constexpr int step_rows(int mt) { return 16 * mt; }
+__host__ __device__ constexpr int step_keys(int hs) { return hs >= 96 ? 16 : 32; }               // positions that a warp takes at a time: a tile
+__host__ __device__ constexpr int step_stages(int hs) { return hs == 32 ? 4 : 3; }               // tiles that it has room for
+__host__ __device__ constexpr int step_stage_bytes(int hs) { return step_keys(hs) * hs * 4; }    // keys and values
+__host__ __device__ constexpr int step_ctas(int hs, int nr) { return hs * nr <= 64 ? 5 : hs * nr <= 128 ? 4 : hs * nr <= 256 ? 3 : 2; } // of an SM, as far as registers go
+__host__ __device__ constexpr int step_rows(int nr) { return 8 * nr; }
 __host__ __device__ constexpr int step_tokens_most() { return 32; }
-__host__ __device__ constexpr int part_stride(int hs) { return hs + 8; }
-__host__ __device__ constexpr size_t step_smem_bytes(int hs, int mt) {
-    const size_t ring = (size_t)STEP_WARPS * step_stages(hs) * step_stage_bytes(hs), parts = (size_t)STEP_WARPS * step_rows(mt) * part_stride(hs) * 4;
-    return (ring > parts ? ring : parts) + (size_t)step_rows(mt) * hs * 2;
+__host__ __device__ constexpr int part_stride(int hs) { return hs + 4; } // (rows 8 banks apart two by two)
+__host__ __device__ constexpr size_t step_smem_bytes(int hs, int nr) {
+    const size_t ring = (size_t)STEP_WARPS * step_stages(hs) * step_stage_bytes(hs), parts = (size_t)STEP_WARPS * step_rows(nr) * part_stride(hs) * 4;
+    return (ring > parts ? ring : parts) + (size_t)step_rows(nr) * hs * 2;
 }
 
 __device__ __forceinline__ uint32_t s32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -205,15 +207,13 @@ template <> __device__ __forceinline__ void mma<bf16>(float (&d)[4], const uint3
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+using kv4::transpose8x8;
 __device__ __forceinline__ void cp16_or_zeros(bool on, uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
 }
 // 16-byte piece c of row r of a tile whose rows are HS entries: eight neighbouring rows of a piece lie in different banks.
-template <int HS> __device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)(r * HS * 2 + ((HS % 64 == 0 ? c ^ (r & 7) : c ^ (r >> 1 & 3)) << 4)); }
-template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t w) { // 0xffff in the halves that are infinite or NaN
-    constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-    return ((w & E) == E ? 0xffffu : 0u) | ((w >> 16 & E) == E ? 0xffff0000u : 0u);
-}
+template <int HS> __device__ __forceinline__ int turn_of(int r) { return HS % 64 == 0 ? r & 7 : r >> 1 & 3; }
+template <int HS> __device__ __forceinline__ uint32_t piece(int r, int c) { return (uint32_t)(r * HS * 2 + ((c ^ turn_of<HS>(r)) << 4)); }
 
 struct Segment { // a run of tokens of one sequence: tiles [begin, end) of its positions [lo, hi), those that any of them sees; tiles of all segments up to and with this one
     int sequence, begin, end, lo, hi, tiles;
@@ -239,32 +239,89 @@ __device__ __forceinline__ void put_results(const Step &a, int row, int head, in
     }
 }
 
-// Rows (tokens x query heads of one key/value head) in blocks of 16 MT.  The tiles of positions that a block's rows see are split over CTAs and dealt to a CTA's warps in turn; each warp
-// has a cp.async ring and a running reference of its own, and no barrier in the loop.  Parts are joined in shared memory, those of several CTAs through the workspace (k_paged_join).
-// Nothing depends on an order of arrival.
-//   scores  S[16 rows x 8 positions] = Q K^T, the cache's type, exact products, FP32 sums;  p = 2^(scale log2(e) s - ref)
-//   values  O[16 rows x 8 entries] += P V with p in the cache's type, half a step off, as the result will be; TWO (FP32 results): and what that left, 16 (BF16) or 22 (FP16) bits in all
+// Rows (tokens x query heads of one key/value head) in blocks of 8 NR; LONE: of a single token, all on the same positions.  The tiles of positions that a block's rows see are split over CTAs
+// and dealt to a CTA's warps in turn; each warp has a cp.async ring and a running reference of its own, and no barrier in the loop.  Parts are joined in shared memory, those of several CTAs
+// through the workspace (k_paged_join).  Nothing depends on an order of arrival.
+//   scores  S[16 positions x 8 rows] = K Q^T, the cache's type, exact products, FP32 sums;  p = 2^(factor s - ref), factor = |scale| log2(e), the scale's sign is the queries'
+//   values  O[16 entries x 8 rows] += V^T P with p in the cache's type, half a step off, as the result will be; TWO (FP32 results): and what that left, 16 (BF16) or 22 (FP16) bits in all
+// (Rows as the products' eight columns: four query heads of a key/value head, the usual number, leave half of them empty, as rows they would leave three quarters, with twice the registers.)
 // ref follows the largest score seen so far only when that passes it by more than 2^8 (the first does), so that few tiles have anything to rescale; with FP16 it lies 2^7 below, so that
 // p reaches down to 2^-24 of 2^-15: a long tail of small ones still counts.
-// A value that is infinite or NaN would reach every row of the block as 0 * NaN, also those that do not see it.  A warp whose sums are not finite runs through its tiles once more with such
-// entries taken out of the product, and a product of zeros and ones says which rows have met one: those become NaN.  With BF16, where sums of large values may leave FP32's
-// range before they are divided, that second run has p times 2^-40.
-template <int HS, typename T, int MT, bool TWO> __global__ void __launch_bounds__(STEP_WARPS * 32, step_ctas(HS, MT)) k_paged_step(const Step a) {
-    constexpr int KT = step_keys(HS), NT = KT / 8, KS = KT / 16, S = step_stages(HS), ROWS = step_rows(MT), PIECES = HS / 8, STAGE = step_stage_bytes(HS), TOKENS = step_tokens_most();
-    constexpr bool F16 = std::is_same<T, __half>::value, QREG = MT == 1 && HS <= 128;
+// A value that is infinite or NaN would reach every row of the block as 0 * NaN, also those that do not see it, and sums of large BF16 values may leave FP32's range before they are divided: a
+// warp whose sums are not finite computes its share once more at the end, a row after the other in FP32, from what each sees, 2^-40 below its maximum (slow_rows).
+template <int HS, typename T> __device__ __noinline__ void slow_rows(const Step &a, const unsigned char *sQ, int rows, int row0, int token0, int kvh, int first, int last, int warp, const Segment *segments, const int *segment_of,
+                                                                     const int *pos_of, float factor, float *parts, float *wref, float *wsum) {
+    constexpr int KT = step_keys(HS), E = HS / 32; // entries of a lane
+    const int lane = threadIdx.x & 31;
+    for (int r = 0; r < rows; r++) {
+        const int token = (row0 + r) / a.mul, own = segment_of[token];
+        int lo, hi, seg = 0;
+        visible(pos_of[token], a.window, lo, hi);
+        float top = -CUDART_INF_F, l = 0.0f, o[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = 0.0f;
+        for (int tile = first + warp; tile < last && own >= 0; tile += STEP_WARPS) {
+            while (segments[seg].tiles <= tile) seg++;
+            if (seg != own) continue;
+            const int pos = (segments[seg].end - (segments[seg].tiles - tile)) * KT + lane;
+            const unsigned at = lane < KT && pos >= lo && pos < hi ? row_at(a.pool, a.rows.table(segments[seg].sequence), pos, kvh) : NO_ROW;
+            float s = -CUDART_INF_F;
+            if (at != NO_ROW) {
+                s = 0.0f;
+                for (int c = 0; c < HS / 8; c++) {
+                    const uint4 x = reinterpret_cast<const uint4 *>((const T *)a.pool.keys + (size_t)at * HS)[c], q = *reinterpret_cast<const uint4 *>(sQ + piece<HS>(r, c));
+                    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, qs[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const float2 x2 = unpack2<T>(xs[u]), q2 = unpack2<T>(qs[u]);
+                        s = fmaf(x2.x, q2.x, s);
+                        s = fmaf(x2.y, q2.y, s);
+                    }
+                }
+            }
+            const float grown = fmaxf(top, warp_max_f(s)), base = grown == -CUDART_INF_F ? 0.0f : grown, alpha = top == grown ? 1.0f : ex2((top - base) * factor);
+            top = grown;
+            const float p = at != NO_ROW ? ex2(fmaf(s - base, factor, -40.0f)) : 0.0f;
+            l = l * alpha + p;
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] *= alpha;
+            const unsigned seen = __ballot_sync(0xffffffffu, at != NO_ROW);
+            for (int k = 0; k < KT; k++) {
+                const float w = __shfl_sync(0xffffffffu, p, k);
+                const unsigned from = __shfl_sync(0xffffffffu, at, k);
+                if (!(seen >> k & 1u)) continue;
+#pragma unroll
+                for (int e = 0; e < E; e++) o[e] = fmaf(w, to_f32(((const T *)a.pool.values + (size_t)from * HS)[e * 32 + lane]), o[e]);
+            }
+        }
+#pragma unroll
+        for (int i = 16; i > 0; i >>= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+#pragma unroll
+        for (int e = 0; e < E; e++) parts[r * part_stride(HS) + e * 32 + lane] = o[e];
+        if (lane == 0) {
+            wref[r] = top * factor + 40.0f;
+            wsum[r] = l;
+        }
+    }
+}
+
+template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __launch_bounds__(STEP_WARPS * 32, step_ctas(HS, NR)) k_paged_step(const Step a) {
+    constexpr int KT = step_keys(HS), KB = KT / 16, S = step_stages(HS), ROWS = step_rows(NR), PIECES = HS / 8, STAGE = step_stage_bytes(HS), TOKENS = LONE ? 1 : step_tokens_most(), RB = HS * 2;
+    constexpr bool F16 = std::is_same<T, __half>::value, QREG = HS * NR <= 256;
+    constexpr float LIFT = F16 ? 7.0f : 0.0f;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ Segment segments[TOKENS];
     __shared__ int seq_of[TOKENS], pos_of[TOKENS], segment_of[TOKENS], n_segments;
     __shared__ unsigned there[STEP_WARPS][S]; // positions of a tile that have a page
     __shared__ float wref[STEP_WARPS][ROWS], wsum[STEP_WARPS][ROWS], weight[STEP_WARPS][ROWS];
-    unsigned char *sQ = smem + step_smem_bytes(HS, MT) - ROWS * HS * 2;
+    unsigned char *sQ = smem + step_smem_bytes(HS, NR) - ROWS * RB;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int G = a.pool.kv_heads, mul = a.heads / G;
-    const int split = blockIdx.x % a.splits, kvh = blockIdx.x / a.splits % G, block = blockIdx.x / a.splits / G % a.blocks, unit = blockIdx.x / a.splits / G / a.blocks;
-    const int token0 = unit * a.tokens, tokens = min(a.tokens, a.rows.n - token0), row0 = block * ROWS, rows = min(ROWS, tokens * mul - row0);
+    const int mul = a.mul, kvh = blockIdx.y, split = blockIdx.z, block = a.blocks > 1 ? blockIdx.x % a.blocks : 0, unit = a.blocks > 1 ? blockIdx.x / a.blocks : blockIdx.x;
+    const int token0 = LONE ? unit : unit * a.tokens, tokens = LONE ? 1 : min(a.tokens, a.rows.n - token0), row0 = block * ROWS, rows = min(ROWS, tokens * mul - row0);
+    const auto token_of = [&](int r) { return LONE ? 0 : (row0 + r) * a.of >> 16; };
 
     Segment only = {-1, 0, 0, 0, 0, 0}; // the first segment, which mostly is the only one
-    if (tokens == 1) { // every thread by itself
+    if constexpr (LONE) { // every thread by itself
         int pos;
         const int s = a.rows.place(token0, pos);
         pos = max(pos, -1);
@@ -279,6 +336,7 @@ template <int HS, typename T, int MT, bool TWO> __global__ void __launch_bounds_
             seq_of[0] = s;
             pos_of[0] = pos;
             segment_of[0] = s >= 0 && pos >= 0 ? 0 : -1;
+            segments[0] = only;
         }
     } else {
         if (tid < tokens) {
@@ -312,13 +370,13 @@ template <int HS, typename T, int MT, bool TWO> __global__ void __launch_bounds_
         __syncthreads();
         if (n_segments) only = segments[0];
     }
-    const int total = tokens == 1 ? only.tiles : n_segments ? segments[n_segments - 1].tiles : 0;
+    const int total = LONE ? only.tiles : n_segments ? segments[n_segments - 1].tiles : 0;
     const int first = (int)min((long long)split * a.share, (long long)total), last = split == a.splits - 1 ? total : min(total, first + a.share);
+    float2 *stats = reinterpret_cast<float2 *>(a.work + (size_t)a.rows.n * a.heads * a.splits * HS);
     if (a.splits > 1 && first >= last) { // nothing for this CTA: its parts have no sum
-        float *w = a.work + (size_t)a.rows.n * a.heads * a.splits * HS;
         if (tid < rows) {
-            const int token = (row0 + tid) / mul, head = kvh * mul + row0 + tid - token * mul;
-            reinterpret_cast<float2 *>(w)[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(-CUDART_INF_F, 0.0f);
+            const int token = token_of(tid), head = kvh * mul + row0 + tid - token * mul;
+            stats[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(-CUDART_INF_F, 0.0f);
         }
         return;
     }
@@ -329,24 +387,40 @@ template <int HS, typename T, int MT, bool TWO> __global__ void __launch_bounds_
     Segment ahead = only;
     auto look_up = [&]() -> unsigned { // the number of the row that this lane looks up for the tile `fetched`
         if (fetched >= last) return NO_ROW;
-        while (ahead.tiles <= fetched) ahead = segments[++seg_f];
+        if constexpr (!LONE)
+            while (ahead.tiles <= fetched) ahead = segments[++seg_f];
         const int pos = (ahead.end - (ahead.tiles - fetched)) * KT + lane;
         return lane < KT && pos >= ahead.lo && pos < ahead.hi ? row_at(a.pool, a.rows.table(ahead.sequence), pos, kvh) : NO_ROW;
     };
     unsigned row = look_up();
     auto fetch = [&](int stage) { // and look the next one up
         if (fetched < last) {
-            const unsigned have = __ballot_sync(0xffffffffu, row != NO_ROW);
+            const unsigned have = __ballot_sync(0xffffffffu, row != NO_ROW), row_0 = __shfl_sync(0xffffffffu, row, 0);
             if (lane == 0) there[warp][stage] = have;
             const uint32_t dst = ring + stage * STAGE;
+            // rows one behind the other, as inside a page: one address, the others a fixed distance from it
+            const bool together = 32 % PIECES == 0 && __all_sync(0xffffffffu, lane >= KT || (row != NO_ROW && row == row_0 + lane));
+            if (together) {
+                constexpr int RPI = 32 % PIECES == 0 ? 32 / PIECES : 1; // rows of a copy of the whole warp
+                const int r0 = lane / PIECES, p = lane % PIECES;
+                const size_t off = (size_t)(row_0 + r0) * RB + p * 16;
+                const char *ks = (const char *)a.pool.keys + off, *vs = (const char *)a.pool.values + off;
+                const uint32_t x = (uint32_t)(p ^ turn_of<HS>(r0)) << 4, to = dst + r0 * RB;
 #pragma unroll
-            for (int i = 0; i < KT * PIECES / 32; i++) {
-                const int n = lane + 32 * i, r = n / PIECES, p = n % PIECES;
-                const unsigned from = __shfl_sync(0xffffffffu, row, r);
-                const size_t off = from == NO_ROW ? 0 : ((size_t)from * HS + p * 8) * 2;
-                cp16_or_zeros(from != NO_ROW, dst + piece<HS>(r, p), (const char *)a.pool.keys + off);
-                cp16_or_zeros(from != NO_ROW, dst + KT * HS * 2 + piece<HS>(r, p), (const char *)a.pool.values + off);
-            }
+                for (int i = 0; i < KT / RPI; i++) {
+                    const uint32_t at = to + RPI * i * RB + (x ^ turn_of<HS>(RPI * i) << 4); // (r0 and RPI i have no bit in common)
+                    cp16(at, ks + RPI * i * RB);
+                    cp16(at + KT * RB, vs + RPI * i * RB);
+                }
+            } else
+#pragma unroll
+                for (int i = 0; i < KT * PIECES / 32; i++) {
+                    const int n = lane + 32 * i, r = n / PIECES, p = n % PIECES;
+                    const unsigned from = __shfl_sync(0xffffffffu, row, r);
+                    const size_t off = from == NO_ROW ? 0 : (size_t)from * RB + p * 16;
+                    cp16_or_zeros(from != NO_ROW, dst + piece<HS>(r, p), (const char *)a.pool.keys + off);
+                    cp16_or_zeros(from != NO_ROW, dst + KT * RB + piece<HS>(r, p), (const char *)a.pool.values + off);
+                }
             fetched += STEP_WARPS;
             row = look_up();
         }
@@ -355,245 +429,205 @@ template <int HS, typename T, int MT, bool TWO> __global__ void __launch_bounds_
 #pragma unroll
     for (int i = 0; i < S - 1; i++) fetch(i);
 
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u; // scores times a positive factor
+    const float factor = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale * 1.4426950408889634f), 1.17549435e-38f), slack = fminf(8.0f / factor, 1e30f);
     for (int i = tid; i < ROWS * PIECES; i += STEP_WARPS * 32) { // queries
-        const int r = i / PIECES, c = i % PIECES, token = (row0 + r) / mul;
+        const int r = i / PIECES, c = i % PIECES, token = token_of(r);
         uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows) {
+        if (r < rows && a.scale != 0.0f) {
             const uint16_t *q = (const uint16_t *)a.q + (long long)(token0 + token) * a.ldq + (size_t)(kvh * mul + row0 + r - token * mul) * HS + c * 8;
             if (a.vec) w = *reinterpret_cast<const uint4 *>(q);
             else w = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
         }
-        *reinterpret_cast<uint4 *>(sQ + piece<HS>(r, c)) = w;
+        *reinterpret_cast<uint4 *>(sQ + piece<HS>(r, c)) = make_uint4(w.x ^ flip, w.y ^ flip, w.z ^ flip, w.w ^ flip);
     }
     __syncthreads();
 
-    // rows 16 m + g and 16 m + 8 + g of this thread: what they see, within which segment
-    int lo[MT][2], hi[MT][2], own[MT][2];
-    int lo_most = 0, hi_least = INT_MAX;
+    // rows 8 n + 2 t and 8 n + 2 t + 1 of this thread: what they see, within which segment
+    int lo[NR][2], hi[NR][2], own[NR][2];
+    int lo_most = only.lo, hi_least = only.hi;
     bool one = true; // every row of the block is of the first segment
+    if constexpr (!LONE) {
+        lo_most = 0;
+        hi_least = INT_MAX;
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+        for (int n = 0; n < NR; n++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int r = 16 * m + 8 * h + g, token = min((row0 + r) / mul, tokens - 1);
-            lo[m][h] = hi[m][h] = 0;
-            own[m][h] = r < rows ? segment_of[token] : 0;
-            if (r < rows && own[m][h] >= 0) visible(pos_of[token], a.window, lo[m][h], hi[m][h]);
-            if (r < rows && seq_of[token] >= 0) {
-                one &= own[m][h] == 0;
-                lo_most = max(lo_most, lo[m][h]);
-                hi_least = min(hi_least, hi[m][h]);
+            for (int h = 0; h < 2; h++) {
+                const int r = 8 * n + 2 * t + h, token = min(token_of(r), tokens - 1);
+                lo[n][h] = hi[n][h] = 0;
+                own[n][h] = r < rows ? segment_of[token] : 0;
+                if (r < rows && own[n][h] >= 0) visible(pos_of[token], a.window, lo[n][h], hi[n][h]);
+                if (r < rows && seq_of[token] >= 0) {
+                    one &= own[n][h] == 0;
+                    lo_most = max(lo_most, lo[n][h]);
+                    hi_least = min(hi_least, hi[n][h]);
+                }
             }
-        }
-    one = __all_sync(0xffffffffu, one);
-    lo_most = __reduce_max_sync(0xffffffffu, lo_most);
-    hi_least = __reduce_min_sync(0xffffffffu, hi_least);
+        one = __all_sync(0xffffffffu, one);
+        lo_most = __reduce_max_sync(0xffffffffu, lo_most);
+        hi_least = __reduce_min_sync(0xffffffffu, hi_least);
+    }
 
-    // ldmatrix rows: keys: lanes 0-7 rows 0-7 piece 0, 8-15 the same rows piece 1, 16-31 rows 8-15; values (transposed): lanes 0-7 rows 0-7, 8-15 rows 8-15 of a piece, 16-31 of the next
-    const int k_row = (lane & 7) + (lane >> 4 << 3), k_piece = lane >> 3 & 1, v_row = lane & 15, v_piece = lane >> 4;
-    const float c = a.scale * 1.4426950408889634f;
-    uint32_t qf[QREG ? HS / 16 : 1][4];
+    // ldmatrix rows: keys: lanes 0-15 rows 0-15 of a piece, 16-31 of the next; values (transposed): lanes 0-7 rows 0-7 of a piece, 8-15 of the next, 16-31 rows 8-15 likewise; queries:
+    // lanes 0-7 rows 0-7 of a piece, 8-15, 16-23, 24-31 of the next three
+    const int k_row = lane & 15, k_piece = lane >> 4, v_row = (lane & 7) + (lane >> 4 << 3), v_piece = lane >> 3 & 1, q_row = lane & 7, q_piece = lane >> 3;
+    const uint32_t k_off = k_row * RB, k_x = (uint32_t)(k_piece ^ turn_of<HS>(k_row)) << 4, v_off = KT * RB + v_row * RB, v_x = (uint32_t)(v_piece ^ turn_of<HS>(v_row)) << 4;
+    uint32_t qf[QREG ? NR : 1][QREG ? HS / 32 : 1][4]; // two steps of 16 entries each
     if constexpr (QREG)
 #pragma unroll
-        for (int k = 0; k < HS / 16; k++) ldmatrix4(q_at + piece<HS>(v_row, 2 * k + v_piece), qf[k]);
+        for (int n = 0; n < NR; n++)
+#pragma unroll
+            for (int k = 0; k < HS / 32; k++) ldmatrix4(q_at + piece<HS>(8 * n + q_row, 4 * k + q_piece), qf[n][k]);
 
-    float o[MT][HS / 8][4], l[MT][2], ref[MT][2];
-    for (int careful = 0;; careful = 1) {
-        if (careful) { // once more from the first tile
-            fetched = first + warp;
-            seg_f = 0;
-            ahead = only;
-            row = look_up();
+    float o[NR][HS / 16][4], l[NR][2], top[NR][2], ref[NR][2]; // ref = top factor - LIFT
 #pragma unroll
-            for (int i = 0; i < S - 1; i++) fetch(i);
-        }
-        const float below = F16 ? 7.0f : careful ? -40.0f : 0.0f;
+    for (int n = 0; n < NR; n++) {
 #pragma unroll
-        for (int m = 0; m < MT; m++) {
+        for (int i = 0; i < HS / 16; i++) o[n][i][0] = o[n][i][1] = o[n][i][2] = o[n][i][3] = 0.0f;
+        l[n][0] = l[n][1] = ref[n][0] = ref[n][1] = 0.0f;
+        top[n][0] = top[n][1] = -CUDART_INF_F;
+    }
+    Segment sg = only;
+    int seg = 0, stage = 0;
+    for (int tile = first + warp; tile < last; tile += STEP_WARPS) {
+        cp_wait<S - 2>();
+        __syncwarp(); // and every lane has read the tile before, whose place the next copies take
+        fetch(stage == 0 ? S - 1 : stage - 1);
+        const uint32_t at = ring + stage * STAGE;
+        float s[NR][KB][4];
 #pragma unroll
-            for (int i = 0; i < HS / 8; i++) o[m][i][0] = o[m][i][1] = o[m][i][2] = o[m][i][3] = 0.0f;
-            l[m][0] = l[m][1] = 0.0f;
-            ref[m][0] = ref[m][1] = -CUDART_INF_F;
-        }
-        Segment sg = only;
-        int seg = 0;
-        int stage = 0;
-        for (int tile = first + warp; tile < last; tile += STEP_WARPS) {
-            cp_wait<S - 2>();
-            __syncwarp(); // and every lane has read the tile before, whose place the next copies take
-            fetch(stage == 0 ? S - 1 : stage - 1);
-            const uint32_t kt = ring + stage * STAGE, vt = kt + KT * HS * 2;
-            float s[MT][NT][4];
+        for (int n = 0; n < NR; n++)
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+            for (int b = 0; b < KB; b++) s[n][b][0] = s[n][b][1] = s[n][b][2] = s[n][b][3] = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NT; n++) s[m][n][0] = s[m][n][1] = s[m][n][2] = s[m][n][3] = 0.0f;
+        for (int k = 0; k < HS / 32; k++) {
+            uint32_t q[NR][4];
 #pragma unroll
-            for (int k = 0; k < HS / 16; k++) {
-                uint32_t qa[MT][4];
+            for (int n = 0; n < NR; n++) {
+                if constexpr (QREG) {
 #pragma unroll
-                for (int m = 0; m < MT; m++) {
-                    if constexpr (QREG) {
-#pragma unroll
-                        for (int i = 0; i < 4; i++) qa[m][i] = qf[k][i];
-                    } else ldmatrix4(q_at + piece<HS>(16 * m + v_row, 2 * k + v_piece), qa[m]);
-                }
-#pragma unroll
-                for (int n = 0; n < NT; n += 2) {
-                    uint32_t b[4];
-                    ldmatrix4(kt + piece<HS>(8 * n + k_row, 2 * k + k_piece), b);
-#pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        mma<T>(s[m][n], qa[m], b[0], b[1]);
-                        mma<T>(s[m][n + 1], qa[m], b[2], b[3]);
-                    }
-                }
+                    for (int i = 0; i < 4; i++) q[n][i] = qf[n][k][i];
+                } else ldmatrix4(q_at + piece<HS>(8 * n + q_row, 4 * k + q_piece), q[n]);
             }
-            const unsigned have = there[warp][stage];
-            while (sg.tiles <= tile) sg = segments[++seg];
-            const int key0 = (sg.end - (sg.tiles - tile)) * KT;
-            // masks; the largest score of the thread's part of each row
-            const bool whole = one && key0 >= lo_most && key0 + KT <= hi_least && have == (KT == 32 ? 0xffffffffu : (1u << (KT & 31)) - 1u);
-            bool higher = false;
-            float top[MT][2];
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int b = 0; b < KB; b++) {
+                    uint32_t ka[4];
+                    ldmatrix4(at + k_off + 16 * b * RB + (k_x ^ (2 * k + u) << 5), ka);
+#pragma unroll
+                    for (int n = 0; n < NR; n++) mma<T>(s[n][b], ka, q[n][2 * u], q[n][2 * u + 1]);
+                }
+        }
+        const unsigned have = there[warp][stage];
+        if constexpr (!LONE)
+            while (sg.tiles <= tile) sg = segments[++seg];
+        const int key0 = (sg.end - (sg.tiles - tile)) * KT;
+        // masks; has the largest score of some row grown by too much?
+        if (!(one && key0 >= lo_most && key0 + KT <= hi_least && have == (KT == 32 ? 0xffffffffu : (1u << (KT & 31)) - 1u)))
+#pragma unroll
+            for (int n = 0; n < NR; n++)
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    float mx = -CUDART_INF_F;
+                    const int from = LONE ? lo_most - key0 : lo[n][h] - key0, to = LONE ? hi_least - key0 : own[n][h] == seg ? hi[n][h] - key0 : INT_MIN;
 #pragma unroll
-                    for (int n = 0; n < NT; n++)
+                    for (int b = 0; b < KB; b++)
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            float &x = s[m][n][2 * h + i];
-                            x *= c;
-                            if (!whole) {
-                                const int j = 8 * n + 2 * t + i;
-                                if (!(own[m][h] == seg && key0 + j >= lo[m][h] && key0 + j < hi[m][h] && (have >> j & 1u))) x = -CUDART_INF_F;
-                            }
-                            mx = fmaxf(mx, x);
+                            const int j = 16 * b + 8 * i + g;
+                            if (!(j >= from && j < to && (have >> j & 1u))) s[n][b][2 * i + h] = -CUDART_INF_F;
                         }
-                    top[m][h] = mx;
-                    higher |= mx > ref[m][h] + (below + 8.0f);
                 }
-            if (__any_sync(0xffffffffu, higher)) {
+        const auto highest = [&](int n, int h) {
+            float mx = s[n][0][h];
 #pragma unroll
-                for (int m = 0; m < MT; m++)
+            for (int b = 0; b < KB; b++) mx = fmaxf(mx, fmaxf(s[n][b][h], s[n][b][2 + h]));
+            return mx;
+        };
+        bool higher = false;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        float mx = top[m][h];
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const float grown = fmaxf(ref[m][h], mx - below);
-                        if (grown != ref[m][h]) {
-                            const float f = ex2(ref[m][h] - grown);
-                            ref[m][h] = grown;
-                            l[m][h] *= f;
+        for (int n = 0; n < NR; n++) higher |= highest(n, 0) > top[n][0] + slack || highest(n, 1) > top[n][1] + slack;
+        if (__any_sync(0xffffffffu, higher)) {
 #pragma unroll
-                            for (int i = 0; i < HS / 8; i++) { o[m][i][2 * h] *= f; o[m][i][2 * h + 1] *= f; }
-                        }
-                    }
-            }
-            uint32_t ph[MT][KS][4], pl[MT][KS][4];
+            for (int n = 0; n < NR; n++)
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+                for (int h = 0; h < 2; h++) {
+                    float mx = highest(n, h);
 #pragma unroll
-                for (int n = 0; n < NT; n++)
+                    for (int i = 4; i < 32; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
+                    if (mx > top[n][h]) {
+                        const float next = mx * factor - LIFT, f = top[n][h] == -CUDART_INF_F ? 0.0f : ex2(ref[n][h] - next);
+                        top[n][h] = mx;
+                        ref[n][h] = next;
+                        l[n][h] *= f;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const float base = ref[m][h] == -CUDART_INF_F ? 0.0f : ref[m][h];
-                        const float p0 = ex2(s[m][n][2 * h] - base), p1 = ex2(s[m][n][2 * h + 1] - base);
-                        l[m][h] += p0 + p1;
-                        const uint32_t w = pack2<T>(p0, p1);
-                        ph[m][n / 2][(n & 1) * 2 + h] = w;
-                        if constexpr (TWO) {
-                            const float2 r = unpack2<T>(w);
-                            pl[m][n / 2][(n & 1) * 2 + h] = pack2<T>(p0 - r.x, p1 - r.y);
-                        }
-                    }
-            uint32_t saw[MT][KS][4]; // ones where a position is seen
-            if (careful)
-#pragma unroll
-                for (int m = 0; m < MT; m++)
-#pragma unroll
-                    for (int n = 0; n < NT; n++)
-#pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            const int j = 8 * n + 2 * t;
-                            const auto sees = [&](int j) { return own[m][h] == seg && key0 + j >= lo[m][h] && key0 + j < hi[m][h] && (have >> j & 1u); };
-                            saw[m][n / 2][(n & 1) * 2 + h] = pack2<T>(sees(j) ? 1.0f : 0.0f, sees(j + 1) ? 1.0f : 0.0f);
-                        }
-#pragma unroll
-            for (int i = 0; i < HS / 8; i += 2)
-#pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    uint32_t b[4];
-                    ldmatrix4_trans(vt + piece<HS>(16 * k + v_row, i + v_piece), b);
-                    if (careful) {
-                        uint32_t odd[4];
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            odd[u] = not_finite<T>(b[u]);
-                            b[u] &= ~odd[u];
-                            odd[u] &= pack2<T>(1.0f, 1.0f);
-                        }
-                        if (__any_sync(0xffffffffu, (odd[0] | odd[1] | odd[2] | odd[3]) != 0u))
-#pragma unroll
-                            for (int m = 0; m < MT; m++) {
-                                float n0[4] = {0.0f, 0.0f, 0.0f, 0.0f}, n1[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                mma<T>(n0, saw[m][k], odd[0], odd[1]);
-                                mma<T>(n1, saw[m][k], odd[2], odd[3]);
-#pragma unroll
-                                for (int u = 0; u < 4; u++) {
-                                    if (n0[u] > 0.0f) o[m][i][u] = CUDART_NAN_F;
-                                    if (n1[u] > 0.0f) o[m][i + 1][u] = CUDART_NAN_F;
-                                }
-                            }
-                    }
-#pragma unroll
-                    for (int m = 0; m < MT; m++) {
-                        mma<T>(o[m][i], ph[m][k], b[0], b[1]);
-                        mma<T>(o[m][i + 1], ph[m][k], b[2], b[3]);
-                        if constexpr (TWO) {
-                            mma<T>(o[m][i], pl[m][k], b[0], b[1]);
-                            mma<T>(o[m][i + 1], pl[m][k], b[2], b[3]);
-                        }
+                        for (int i = 0; i < HS / 16; i++) { o[n][i][h] *= f; o[n][i][2 + h] *= f; }
                     }
                 }
-            if (++stage == S) stage = 0;
         }
-        cp_wait<0>();
-        if (careful) break;
-        bool bad = false;
+        uint32_t ph[NR][KB][2], pl[NR][KB][2]; // of 8 positions each: of positions 2 t, 2 t + 1 and row g
 #pragma unroll
-        for (int m = 0; m < MT; m++)
+        for (int n = 0; n < NR; n++)
 #pragma unroll
-            for (int i = 0; i < HS / 8; i++)
+            for (int b = 0; b < KB; b++)
 #pragma unroll
-                for (int u = 0; u < 4; u++) bad |= !(fabsf(o[m][i][u]) < CUDART_INF_F);
-        __syncwarp();
-        if (!__any_sync(0xffffffffu, bad)) break;
+                for (int i = 0; i < 2; i++) {
+                    const float p0 = ex2(fmaf(s[n][b][2 * i], factor, -ref[n][0])), p1 = ex2(fmaf(s[n][b][2 * i + 1], factor, -ref[n][1]));
+                    l[n][0] += p0;
+                    l[n][1] += p1;
+                    const uint32_t w = pack2<T>(p0, p1);
+                    ph[n][b][i] = transpose8x8(w);
+                    if constexpr (TWO) {
+                        const float2 r = unpack2<T>(w);
+                        pl[n][b][i] = transpose8x8(pack2<T>(p0 - r.x, p1 - r.y));
+                    }
+                }
+#pragma unroll
+        for (int i = 0; i < HS / 16; i++)
+#pragma unroll
+            for (int b = 0; b < KB; b++) {
+                uint32_t va[4];
+                ldmatrix4_trans(at + v_off + 16 * b * RB + (v_x ^ i << 5), va);
+#pragma unroll
+                for (int n = 0; n < NR; n++) {
+                    mma<T>(o[n][i], va, ph[n][b][0], ph[n][b][1]);
+                    if constexpr (TWO) mma<T>(o[n][i], va, pl[n][b][0], pl[n][b][1]);
+                }
+            }
+        if (++stage == S) stage = 0;
     }
+    cp_wait<0>();
 
     // ---- join: warps, then (through the workspace) CTAs ----
     __syncthreads(); // the rings are free
     float *parts = reinterpret_cast<float *>(smem);
+    float sum = 0.0f; // not finite where an entry is not
 #pragma unroll
-    for (int m = 0; m < MT; m++)
+    for (int n = 0; n < NR; n++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            float sum = l[m][h];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            const int r = 16 * m + 8 * h + g;
-            if (t == 0) { wref[warp][r] = ref[m][h]; wsum[warp][r] = sum; }
-            if (r < rows)
+            float all = l[n][h];
 #pragma unroll
-                for (int i = 0; i < HS / 8; i++) *reinterpret_cast<float2 *>(parts + (warp * ROWS + r) * part_stride(HS) + 8 * i + 2 * t) = make_float2(o[m][i][2 * h], o[m][i][2 * h + 1]);
+            for (int i = 4; i < 32; i <<= 1) all += __shfl_xor_sync(0xffffffffu, all, i);
+            const int r = 8 * n + 2 * t + h;
+            if (g == 0) { wref[warp][r] = top[n][h] == -CUDART_INF_F ? -CUDART_INF_F : ref[n][h]; wsum[warp][r] = all; }
+            if (r < rows) {
+                float *to = parts + (warp * ROWS + r) * part_stride(HS) + g;
+#pragma unroll
+                for (int i = 0; i < HS / 16; i++) {
+                    to[16 * i] = o[n][i][h];
+                    to[16 * i + 8] = o[n][i][2 + h];
+                    sum += 0.0f * o[n][i][h] + 0.0f * o[n][i][2 + h];
+                }
+            }
         }
+    __syncwarp();
+    if (__any_sync(0xffffffffu, sum != 0.0f))
+        slow_rows<HS, T>(a, sQ, rows, row0, token0, kvh, first, last, warp, segments, segment_of, pos_of, factor, parts + warp * ROWS * part_stride(HS), wref[warp], wsum[warp]);
     __syncthreads();
     if (tid < rows) {
-        const int token = (row0 + tid) / mul, head = kvh * mul + row0 + tid - token * mul;
+        const int token = token_of(tid), head = kvh * mul + row0 + tid - token * mul;
         float M = -CUDART_INF_F, L = 0.0f;
 #pragma unroll
         for (int w = 0; w < STEP_WARPS; w++) M = fmaxf(M, wref[w][tid]);
@@ -604,14 +638,14 @@ template <int HS, typename T, int MT, bool TWO> __global__ void __launch_bounds_
             f[w] = wref[w][tid] == M ? 1.0f : ex2(wref[w][tid] - base);
             L = fmaf(f[w], wsum[w][tid], L);
         }
-        if (a.splits > 1) reinterpret_cast<float2 *>(a.work + (size_t)a.rows.n * a.heads * a.splits * HS)[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(M, L);
+        if (a.splits > 1) stats[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(M, L);
         const float scale = a.splits > 1 ? 1.0f : 1.0f / L;
 #pragma unroll
         for (int w = 0; w < STEP_WARPS; w++) weight[w][tid] = L == 0.0f ? 0.0f : f[w] * scale; // nothing seen: zeros
     }
     __syncthreads();
     for (int i = tid; i < rows * (HS / 4); i += STEP_WARPS * 32) {
-        const int r = i / (HS / 4), e = i % (HS / 4) * 4, token = (row0 + r) / mul, head = kvh * mul + row0 + r - token * mul, row = token0 + token;
+        const int r = i / (HS / 4), e = i % (HS / 4) * 4, token = token_of(r), head = kvh * mul + row0 + r - token * mul, row = token0 + token;
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < STEP_WARPS; w++) {

@@ -45,20 +45,19 @@ int check_rows(const b200_paged_cache *c, int n, const int32_t *positions, const
 
 // How the attention of n rows is cut.
 struct PagedCut {
-    int mt, tokens, blocks, splits, share; // blocks of 16 mt rows; tokens of a unit; blocks of a unit; CTAs of a block, tiles of each
+    int nr, tokens, blocks, splits, share; // blocks of 8 nr rows; tokens of a unit; blocks of a unit; CTAs of a block, tiles of each
 };
-// Rows of a unit: the tokens of a chunk that fit 32 rows (16 with heads of 256, whose results would leave no registers), so that they read the pages once.
+// Rows of a unit: the tokens of a chunk that fit 32 rows (16 with heads of 256, for more their results would leave no registers), so that they read the pages once.
 PagedCut paged_cut(const b200_paged_cache &c, const b200_paged_attention_args &a, int sms) {
     PagedCut k;
     const int G = c.kv_heads, mul = a.heads / G, chunk = a.chunk < 1 ? 1 : a.chunk < a.n ? a.chunk : a.n;
-    const int most = c.head_size == 256 ? 16 : 32;
-    int fit = most / mul;
+    int fit = (c.head_size == 256 ? 16 : 32) / mul;
     if (fit < 1) fit = 1;
     const int units_of_chunk = (chunk + fit - 1) / fit;
     k.tokens = (chunk + units_of_chunk - 1) / units_of_chunk; // even shares
-    const int rows = k.tokens * mul;
-    k.mt = rows > 16 && most == 32 ? 2 : 1;
-    k.blocks = (rows + 16 * k.mt - 1) / (16 * k.mt);
+    // (a token of more than 16 query heads of a key/value head reads the pages once for 16 of them)
+    k.nr = k.tokens > 1 ? (k.tokens * mul <= 16 ? 2 : (k.tokens * mul + 7) / 8) : mul <= 8 ? 1 : 2;
+    k.blocks = (k.tokens * mul + 8 * k.nr - 1) / (8 * k.nr);
     const int KT = paged::step_keys(c.head_size);
     const long long context = (long long)a.table_width * c.page_size;
     long long len = a.max_len > 0 && a.max_len < context ? a.max_len : context;
@@ -109,6 +108,8 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
     k.q = a.q; k.out = a.out;
     k.ldq = a.q_stride; k.ldo = a.out_stride;
     k.heads = a.heads; k.window = a.window; k.out_type = a.out_type;
+    k.mul = a.heads / c.kv_heads;
+    k.of = (65535 + k.mul) / k.mul;
     k.scale = a.scale;
     k.vec = aligned16(a.q, a.q_stride, 2);
     const int four = a.out_type == B200_GGML_F32 ? 16 : 8; // bytes of the four entries that a thread writes
@@ -145,19 +146,23 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
     PagedCut cut = paged_cut(c, a, sms);
     if (!has_room(cut.splits)) cut.splits = 1;
     k.tokens = cut.tokens; k.blocks = cut.blocks; k.splits = cut.splits; k.share = cut.share;
-    const unsigned grid = (unsigned)((a.n + cut.tokens - 1) / cut.tokens) * cut.blocks * c.kv_heads * cut.splits;
+    const dim3 grid((unsigned)((a.n + cut.tokens - 1) / cut.tokens) * cut.blocks, c.kv_heads, cut.splits);
     return by_head_size(c.head_size, [&](auto hs) {
         return by_cache_type(c.type, [&](auto type) {
             using T = decltype(type);
-            const auto go = [&](auto mt) {
-                constexpr size_t smem = paged::step_smem_bytes(hs, mt);
-                auto kern = a.out_type == B200_GGML_F32 ? paged::k_paged_step<hs, T, mt, true> : paged::k_paged_step<hs, T, mt, false>;
+            const auto go = [&](auto nr, auto lone) {
+                constexpr size_t smem = paged::step_smem_bytes(hs, nr);
+                auto kern = a.out_type == B200_GGML_F32 ? paged::k_paged_step<hs, T, nr, true, lone> : paged::k_paged_step<hs, T, nr, false, lone>;
                 cudaError_t e = allow_smem(kern, smem);
                 if (e == cudaSuccess) e = launch(kern, grid, paged::STEP_WARPS * 32, smem, 1, false, stream, k);
                 return e != cudaSuccess || cut.splits == 1 ? e : join(hs, cut.splits);
             };
-            if constexpr (hs < 256) if (cut.mt == 2) return go(std::integral_constant<int, 2>());
-            return go(std::integral_constant<int, 1>());
+            if (cut.tokens == 1) return cut.nr == 1 ? go(std::integral_constant<int, 1>(), std::true_type()) : go(std::integral_constant<int, 2>(), std::true_type());
+            if constexpr (hs < 256) {
+                if (cut.nr == 3) return go(std::integral_constant<int, 3>(), std::false_type());
+                if (cut.nr == 4) return go(std::integral_constant<int, 4>(), std::false_type());
+            }
+            return go(std::integral_constant<int, 2>(), std::false_type());
         });
     });
 }
@@ -234,6 +239,7 @@ static int paged_attention(const b200_paged_cache *c, const b200_paged_attention
     if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(B200_ERR_BAD_ARG, "the workspace is not aligned");
     if (a->n == 0) return B200_OK;
     if (!a->q || !a->out) return fail(B200_ERR_BAD_ARG, "null rows");
+    if (c->kv_heads > 65535) return fail(B200_ERR_UNSUPPORTED, "%d key/value heads (at most 65535)", c->kv_heads);
     const int64_t width = (int64_t)a->heads * c->head_size;
     if (a->n > 1 && (a->q_stride < width || a->out_stride < width)) return fail(B200_ERR_BAD_ARG, "rows overlap: a stride is smaller than its row");
     if ((long long)a->n * a->heads > (1LL << 22)) return fail(B200_ERR_UNSUPPORTED, "too many rows in one call"); // (times MAX_SPLITS: the grid's limit)
