@@ -177,21 +177,27 @@ struct Step {
     float scale;
     void *out;
     int mul, of;                       // query heads of a key/value head; r / mul = r of >> 16 for the rows of a unit of several tokens
-    int tokens, blocks, splits, share; // rows of a unit are `tokens` neighbouring ones, in `blocks` blocks; `splits` CTAs run through `share` tiles each (the last one through the rest)
-    float *work;                       // parts of units that several CTAs share: [row][head][split] entries, behind them [row][head][split] reference and sum
+    int tokens, blocks; // rows of a group are `tokens` neighbouring ones; a unit is one of its `blocks` blocks of one key/value head
+    int ctas;           // that find room on the GPU, where units are shared out (0: a CTA a unit)
+    int splits;         // (chunks) CTAs of a unit
+    float *work;        // parts of units that several CTAs share.  ctas: [CTA][row] entries, behind them reference and sum; splits: [row][head][split] likewise
 };
 
-constexpr int STEP_WARPS = 4;
-__host__ __device__ constexpr int step_keys(int hs) { return hs >= 96 ? 16 : 32; }               // positions that a warp takes at a time: a tile
-__host__ __device__ constexpr int step_stages(int hs) { return hs == 32 ? 4 : 3; }               // tiles that it has room for
-__host__ __device__ constexpr int step_stage_bytes(int hs) { return step_keys(hs) * hs * 4; }    // keys and values
-__host__ __device__ constexpr int step_ctas(int hs, int nr) { return hs * nr <= 64 ? 5 : hs * nr <= 128 ? 4 : hs * nr <= 256 ? 3 : 2; } // of an SM, as far as registers go
+constexpr int STEP_WARPS = 2, STEP_GROUPS = 256; // warps of a CTA; units of tokens that it shares out by their lengths
+constexpr int STEP_SHARED_ROWS = 4 * STEP_GROUPS; // rows of all groups, then
+__host__ __device__ constexpr int step_keys(int hs) { return hs == 256 ? 16 : 32; }           // positions that a warp takes at a time: a tile
+__host__ __device__ constexpr int step_stages(int hs) { return hs == 32 || hs == 256 ? 3 : 2; } // tiles that it has room for
+__host__ __device__ constexpr int step_stage_bytes(int hs) { return step_keys(hs) * hs * 4; } // keys and values
 __host__ __device__ constexpr int step_rows(int nr) { return 8 * nr; }
 __host__ __device__ constexpr int step_tokens_most() { return 32; }
 __host__ __device__ constexpr int part_stride(int hs) { return hs + 4; } // (rows 8 banks apart two by two)
 __host__ __device__ constexpr size_t step_smem_bytes(int hs, int nr) {
     const size_t ring = (size_t)STEP_WARPS * step_stages(hs) * step_stage_bytes(hs), parts = (size_t)STEP_WARPS * step_rows(nr) * part_stride(hs) * 4;
     return (ring > parts ? ring : parts) + (size_t)step_rows(nr) * hs * 2;
+}
+__host__ __device__ constexpr int step_ctas(int hs, int nr) { // of an SM, as far as its shared memory and registers go
+    const int n = (int)(233472 / (step_smem_bytes(hs, nr) + 3072)), most = hs <= 64 && nr >= 3 ? 4 : 8;
+    return n < 1 ? 1 : n > most ? most : n;
 }
 
 __device__ __forceinline__ uint32_t s32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -239,9 +245,128 @@ __device__ __forceinline__ void put_results(const Step &a, int row, int head, in
     }
 }
 
-// Rows (tokens x query heads of one key/value head) in blocks of 8 NR; LONE: of a single token, all on the same positions.  The tiles of positions that a block's rows see are split over CTAs
-// and dealt to a CTA's warps in turn; each warp has a cp.async ring and a running reference of its own, and no barrier in the loop.  Parts are joined in shared memory, those of several CTAs
-// through the workspace (k_paged_join).  Nothing depends on an order of arrival.
+// The segments of a group of tokens, in order: emit(first token, last token + 1, segment), sequence -1 for a run that sees nothing.
+template <typename P, typename F> __device__ __forceinline__ void segments_of_group(const Step &a, int tokens, int KT, P place, F emit) {
+    int total = 0;
+    for (int i = 0; i < tokens;) {
+        int pos;
+        const int s = place(i, pos);
+        int j = i, from = INT_MAX, to = 0;
+        for (int sj = s; sj == s;) {
+            int lo, hi;
+            visible(max(pos, -1), a.window, lo, hi);
+            if (hi > lo) { from = min(from, lo); to = max(to, hi); }
+            if (++j == tokens) break;
+            sj = place(j, pos);
+        }
+        Segment sg = {-1, 0, 0, 0, 0, total};
+        if (s >= 0 && to > 0) {
+            sg = {s, from / KT, (to - 1) / KT + 1, from, to, 0};
+            total += sg.end - sg.begin;
+            sg.tiles = total;
+        }
+        emit(i, j, sg);
+        i = j;
+    }
+}
+// How units are shared out over CTAs, by what their rows see: with S tiles a CTA at most, a unit of t tiles gets n = ceil(t / S) CTAs, even shares.  S is the smallest, to a sixteenth, with which
+// all CTAs find room on the GPU at once (where there are many units: an even share of all tiles).  Every CTA finds its own place: all of them look at the rows' positions.
+constexpr int SHARE_LEAST = 8; // tiles of a CTA, where a unit has so many
+struct Shares {
+    int before[STEP_GROUPS + 1]; // CTAs of the groups in front
+    int tiles[STEP_GROUPS];      // of a group, for one head and block
+    int2 at[STEP_GROUPS];        // LONE: its sequence and position
+    long long sums[8];
+};
+template <int THREADS> __device__ __forceinline__ long long block_sum(long long v, long long *sums) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = v;
+    __syncthreads();
+    v = sums[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 32; w++) v += sums[w];
+    return v;
+}
+static_assert(STEP_SHARED_ROWS * 8 + sizeof(Shares) <= (size_t)STEP_WARPS * step_stages(32) * step_stage_bytes(32), "the smallest ring holds what is needed before it");
+// The whole CTA; stage: room for the rows' sequences and positions, where groups have several of them.
+template <int KT, bool LONE, int THREADS> __device__ __forceinline__ void share_out(const Step &a, Shares &sh, int2 *stage) {
+    constexpr int PER = STEP_GROUPS / THREADS;
+    const int tid = threadIdx.x, lane = tid & 31, groups = (a.rows.n + a.tokens - 1) / a.tokens, per_group = a.pool.kv_heads * a.blocks;
+    if constexpr (LONE) {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            const int g = tid + i * THREADS;
+            int pos = -1, lo, hi, s = -1;
+            if (g < groups) s = a.rows.place(g, pos);
+            pos = max(pos, -1);
+            visible(pos, a.window, lo, hi);
+            sh.at[g] = make_int2(s, pos);
+            sh.tiles[g] = s >= 0 && hi > lo ? (hi - 1) / KT + 1 - lo / KT : 0;
+        }
+    } else {
+#pragma unroll 4
+        for (int r = tid; r < a.rows.n; r += THREADS) {
+            int pos;
+            const int s = a.rows.place(r, pos);
+            stage[r] = make_int2(s, pos);
+        }
+        __syncthreads();
+        for (int g = tid; g < STEP_GROUPS; g += THREADS) {
+            int tiles = 0;
+            const int token0 = g * a.tokens;
+            if (g < groups)
+                segments_of_group(a, min(a.tokens, a.rows.n - token0), KT, [&](int t, int &pos) { pos = stage[token0 + t].y; return stage[token0 + t].x; },
+                                  [&](int, int, const Segment &sg) { tiles = sg.tiles; });
+            sh.tiles[g] = tiles;
+        }
+    }
+    __syncthreads();
+    int mine[PER];
+    long long sum = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        mine[i] = sh.tiles[tid * PER + i];
+        sum += mine[i];
+    }
+    const long long total = block_sum<THREADS>(sum, sh.sums) * per_group;
+    int share = (int)min(max((total + a.ctas - 1) / a.ctas, (long long)SHARE_LEAST), 1LL << 30);
+    if (groups * per_group <= a.ctas / 4 * 3)
+        for (;;) { // (at most a few dozen times: the units alone take three quarters of the room)
+            long long ctas = 0;
+#pragma unroll
+            for (int i = 0; i < PER; i++) ctas += (mine[i] + share - 1) / share;
+            if (block_sum<THREADS>(ctas, sh.sums) * per_group <= a.ctas) break;
+            share += max(1, share / 16);
+        }
+    int ctas = 0;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int n = (mine[i] + share - 1) / share * per_group;
+        mine[i] = ctas;
+        ctas += n;
+    }
+    int run = ctas;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run += x;
+    }
+    __syncthreads();
+    if (lane == 31) sh.sums[tid / 32] = run;
+    __syncthreads();
+    run -= ctas;
+    for (int w = 0; w < tid / 32; w++) run += (int)sh.sums[w];
+#pragma unroll
+    for (int i = 0; i < PER; i++) sh.before[tid * PER + i] = run + mine[i];
+    if (tid == THREADS - 1) sh.before[STEP_GROUPS] = run + ctas;
+    __syncthreads();
+}
+
+// Rows (tokens x query heads of one key/value head) in blocks of 8 NR; LONE: of a single token, all on the same positions.  A CTA takes a unit, or an even
+// share of its tiles (Shares), and deals them to its warps in turn; each warp has a cp.async ring and a running reference of its own, and no barrier in the loop.  Parts
+// are joined in shared memory, those of several CTAs through the workspace (k_paged_join_shares).  Nothing depends on an order of arrival.
 //   scores  S[16 positions x 8 rows] = K Q^T, the cache's type, exact products, FP32 sums;  p = 2^(factor s - ref), factor = |scale| log2(e), the scale's sign is the queries'
 //   values  O[16 entries x 8 rows] += V^T P with p in the cache's type, half a step off, as the result will be; TWO (FP32 results): and what that left, 16 (BF16) or 22 (FP16) bits in all
 // (Rows as the products' eight columns: four query heads of a key/value head, the usual number, leave half of them empty, as rows they would leave three quarters, with twice the registers.)
@@ -305,6 +430,11 @@ template <int HS, typename T> __device__ __noinline__ void slow_rows(const Step 
     }
 }
 
+// CTAs of the grid where units are shared out; in the workspace, behind the parts' entries and statistics: Shares::before.
+__host__ __device__ inline size_t shared_grid(const Step &a, int groups) { return (size_t)a.ctas + (size_t)groups * a.pool.kv_heads * a.blocks; }
+template <int HS, int NR> __device__ __forceinline__ float2 *stats_of(const Step &a, int groups) { return reinterpret_cast<float2 *>(a.work + shared_grid(a, groups) * step_rows(NR) * HS); }
+template <int HS, int NR> __device__ __forceinline__ int *plan_of(const Step &a, int groups) { return reinterpret_cast<int *>(stats_of<HS, NR>(a, groups) + shared_grid(a, groups) * step_rows(NR)); }
+
 template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __launch_bounds__(STEP_WARPS * 32, step_ctas(HS, NR)) k_paged_step(const Step a) {
     constexpr int KT = step_keys(HS), KB = KT / 16, S = step_stages(HS), ROWS = step_rows(NR), PIECES = HS / 8, STAGE = step_stage_bytes(HS), TOKENS = LONE ? 1 : step_tokens_most(), RB = HS * 2;
     constexpr bool F16 = std::is_same<T, __half>::value, QREG = HS * NR <= 256;
@@ -316,15 +446,47 @@ template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __lau
     __shared__ float wref[STEP_WARPS][ROWS], wsum[STEP_WARPS][ROWS], weight[STEP_WARPS][ROWS];
     unsigned char *sQ = smem + step_smem_bytes(HS, NR) - ROWS * RB;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int mul = a.mul, kvh = blockIdx.y, split = blockIdx.z, block = a.blocks > 1 ? blockIdx.x % a.blocks : 0, unit = a.blocks > 1 ? blockIdx.x / a.blocks : blockIdx.x;
+    Shares &shares = *reinterpret_cast<Shares *>(smem + STEP_SHARED_ROWS * 8); // (where the rings will be)
+    const int mul = a.mul, groups = (a.rows.n + a.tokens - 1) / a.tokens, per_group = a.pool.kv_heads * a.blocks;
+    pdl_launch_dependents();
+    int unit = blockIdx.x / per_group, within = blockIdx.x % per_group, part = 0, n_parts = 1;
+    int2 sequence_position;
+    if (a.ctas) {
+        share_out<KT, LONE, STEP_WARPS * 32>(a, shares, reinterpret_cast<int2 *>(smem));
+        if (blockIdx.x == 0) // for the join
+            for (int i = tid; i <= groups; i += STEP_WARPS * 32) plan_of<HS, NR>(a, groups)[i] = shares.before[i];
+        if ((int)blockIdx.x >= shares.before[groups]) return;
+        int low = 0, high = groups - 1; // the last group that starts with this CTA or in front of it
+        while (low < high) {
+            const int mid = (low + high + 1) / 2;
+            if (shares.before[mid] <= (int)blockIdx.x) low = mid;
+            else high = mid - 1;
+        }
+        unit = low;
+        n_parts = (shares.before[low + 1] - shares.before[low]) / per_group;
+        const int at = blockIdx.x - shares.before[low];
+        within = at % per_group; // (CTAs that run side by side read neighbouring heads of the same pages)
+        part = at / per_group;
+        if constexpr (LONE) sequence_position = shares.at[low];
+        __syncthreads(); // (before the rings' first copies)
+    }
+    const bool whole = n_parts == 1;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u; // scores times a positive factor
+    const float factor = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale * 1.4426950408889634f), 1.17549435e-38f), slack = fminf(8.0f / factor, 1e30f);
+    const int kvh = within % a.pool.kv_heads, block = within / a.pool.kv_heads;
     const int token0 = LONE ? unit : unit * a.tokens, tokens = LONE ? 1 : min(a.tokens, a.rows.n - token0), row0 = block * ROWS, rows = min(ROWS, tokens * mul - row0);
     const auto token_of = [&](int r) { return LONE ? 0 : (row0 + r) * a.of >> 16; };
 
     Segment only = {-1, 0, 0, 0, 0, 0}; // the first segment, which mostly is the only one
     if constexpr (LONE) { // every thread by itself
-        int pos;
-        const int s = a.rows.place(token0, pos);
-        pos = max(pos, -1);
+        int pos, s;
+        if (a.ctas) {
+            s = sequence_position.x;
+            pos = sequence_position.y;
+        } else {
+            s = a.rows.place(token0, pos);
+            pos = max(pos, -1);
+        }
         if (s >= 0 && pos >= 0) {
             visible(pos, a.window, only.lo, only.hi);
             only.sequence = s;
@@ -347,39 +509,19 @@ template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __lau
         }
         __syncthreads();
         if (tid == 0) {
-            int n = 0, total = 0;
-            for (int i = 0; i < tokens;) {
-                const int s = seq_of[i];
-                int j = i, from = INT_MAX, to = 0;
-                for (; j < tokens && seq_of[j] == s; j++) {
-                    int lo, hi;
-                    visible(pos_of[j], a.window, lo, hi);
-                    if (hi > lo) { from = min(from, lo); to = max(to, hi); }
-                    segment_of[j] = n;
-                }
-                if (s >= 0 && to > 0) {
-                    const int begin = from / KT, end = (to - 1) / KT + 1;
-                    total += end - begin;
-                    segments[n++] = {s, begin, end, from, to, total};
-                } else
-                    for (int k = i; k < j; k++) segment_of[k] = -1;
-                i = j;
-            }
+            int n = 0;
+            segments_of_group(a, tokens, KT, [&](int t, int &pos) { pos = pos_of[t]; return seq_of[t]; }, [&](int i, int j, const Segment &sg) {
+                for (int k = i; k < j; k++) segment_of[k] = sg.sequence < 0 ? -1 : n;
+                if (sg.sequence >= 0) segments[n++] = sg;
+            });
             n_segments = n;
         }
         __syncthreads();
         if (n_segments) only = segments[0];
     }
+
     const int total = LONE ? only.tiles : n_segments ? segments[n_segments - 1].tiles : 0;
-    const int first = (int)min((long long)split * a.share, (long long)total), last = split == a.splits - 1 ? total : min(total, first + a.share);
-    float2 *stats = reinterpret_cast<float2 *>(a.work + (size_t)a.rows.n * a.heads * a.splits * HS);
-    if (a.splits > 1 && first >= last) { // nothing for this CTA: its parts have no sum
-        if (tid < rows) {
-            const int token = token_of(tid), head = kvh * mul + row0 + tid - token * mul;
-            stats[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(-CUDART_INF_F, 0.0f);
-        }
-        return;
-    }
+    const int first = whole ? 0 : (int)((long long)total * part / n_parts), last = whole ? total : (int)((long long)total * (part + 1) / n_parts);
 
     const uint32_t ring = s32(smem) + warp * S * STAGE, q_at = s32(sQ);
     // this warp's tiles: numbers first + warp, + STEP_WARPS, .. of the list; `fetched` is the next to ask for
@@ -429,8 +571,6 @@ template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __lau
 #pragma unroll
     for (int i = 0; i < S - 1; i++) fetch(i);
 
-    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u; // scores times a positive factor
-    const float factor = a.scale == 0.0f ? 1.0f : fmaxf(fabsf(a.scale * 1.4426950408889634f), 1.17549435e-38f), slack = fminf(8.0f / factor, 1e30f);
     for (int i = tid; i < ROWS * PIECES; i += STEP_WARPS * 32) { // queries
         const int r = i / PIECES, c = i % PIECES, token = token_of(r);
         uint4 w = make_uint4(0u, 0u, 0u, 0u);
@@ -638,14 +778,14 @@ template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __lau
             f[w] = wref[w][tid] == M ? 1.0f : ex2(wref[w][tid] - base);
             L = fmaf(f[w], wsum[w][tid], L);
         }
-        if (a.splits > 1) stats[((size_t)(token0 + token) * a.heads + head) * a.splits + split] = make_float2(M, L);
-        const float scale = a.splits > 1 ? 1.0f : 1.0f / L;
+        if (!whole) stats_of<HS, NR>(a, groups)[(size_t)blockIdx.x * ROWS + tid] = make_float2(M, L);
+        const float scale = whole ? 1.0f / L : 1.0f;
 #pragma unroll
         for (int w = 0; w < STEP_WARPS; w++) weight[w][tid] = L == 0.0f ? 0.0f : f[w] * scale; // nothing seen: zeros
     }
     __syncthreads();
     for (int i = tid; i < rows * (HS / 4); i += STEP_WARPS * 32) {
-        const int r = i / (HS / 4), e = i % (HS / 4) * 4, token = token_of(r), head = kvh * mul + row0 + r - token * mul, row = token0 + token;
+        const int r = i / (HS / 4), e = i % (HS / 4) * 4, token = token_of(r);
         float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < STEP_WARPS; w++) {
@@ -653,8 +793,94 @@ template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __lau
             const float4 p = *reinterpret_cast<const float4 *>(parts + (w * ROWS + r) * part_stride(HS) + e);
             x = make_float4(fmaf(f, p.x, x.x), fmaf(f, p.y, x.y), fmaf(f, p.z, x.z), fmaf(f, p.w, x.w));
         }
-        if (a.splits > 1) *reinterpret_cast<float4 *>(a.work + (((size_t)row * a.heads + head) * a.splits + split) * HS + e) = x;
-        else if (seq_of[token] >= 0) put_results(a, row, head, HS, e, x);
+        if (!whole) *reinterpret_cast<float4 *>(a.work + ((size_t)blockIdx.x * ROWS + r) * HS + e) = x;
+        else if (seq_of[token] >= 0) put_results(a, token0 + token, kvh * mul + row0 + r - token * mul, HS, e, x);
+    }
+}
+
+// Joins the parts of units that several CTAs shared, and clears rows that see nothing.  FEW (where a unit has few CTAs): eight rows a CTA, four entries a thread, part by part; else a row a
+// CTA, whose HS / 4 threads a part take parts in turn.
+template <int HS, int NR, bool LONE, bool FEW> __global__ void __launch_bounds__(128) k_paged_join_shares(const Step a) {
+    constexpr int ROWS = step_rows(NR), LANES = HS / 4, GROUPS = 128 / LANES, AT_ONCE = 128;
+    pdl_wait();
+    const int tid = threadIdx.x, per_group = a.pool.kv_heads * a.blocks, group = blockIdx.x / per_group, within = blockIdx.x % per_group, groups = (a.rows.n + a.tokens - 1) / a.tokens;
+    const int kvh = within % a.pool.kv_heads, block = within / a.pool.kv_heads, token0 = group * a.tokens, tokens = min(a.tokens, a.rows.n - token0), row0 = block * ROWS, rows = min(ROWS, tokens * a.mul - row0);
+    const int *plan = plan_of<HS, NR>(a, groups);
+    const int before = plan[group], parts = (plan[group + 1] - before) / per_group;
+    if (parts == 1) return; // one CTA's
+    const auto place = [&](int r, int &row, int &head) {
+        const int token = LONE ? 0 : (row0 + r) / a.mul;
+        row = token0 + token;
+        head = kvh * a.mul + row0 + r - token * a.mul;
+        int pos;
+        return a.rows.place(row, pos) >= 0;
+    };
+    const auto slot = [&](int p) { return (size_t)(before + p * per_group + within) * ROWS; };
+    const float2 *stats = stats_of<HS, NR>(a, groups);
+    int row, head;
+    if constexpr (FEW) {
+        for (int i = tid; i < 8 * LANES; i += 128) {
+            const int r = blockIdx.y * 8 + i / LANES, e = i % LANES * 4;
+            if (r >= rows || !place(r, row, head)) continue;
+            float M = -CUDART_INF_F, L = 0.0f;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+            for (int p = 0; p < parts; p++) {
+                const float2 st = stats[slot(p) + r];
+                const float4 v = *reinterpret_cast<const float4 *>(a.work + (slot(p) + r) * HS + e);
+                const float grown = fmaxf(M, st.x), base = grown == -CUDART_INF_F ? 0.0f : grown, f = M == grown ? 1.0f : ex2(M - base), w = st.x == grown ? 1.0f : ex2(st.x - base);
+                M = grown;
+                L = fmaf(w, st.y, L * f);
+                x = make_float4(fmaf(w, v.x, x.x * f), fmaf(w, v.y, x.y * f), fmaf(w, v.z, x.z * f), fmaf(w, v.w, x.w * f));
+            }
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            put_results(a, row, head, HS, e, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+        }
+    } else {
+        __shared__ float2 stat[AT_ONCE];
+        __shared__ float red[4], sums_l[GROUPS];
+        __shared__ float4 sums[GROUPS][LANES];
+        const int r = blockIdx.y, lane = tid % LANES, mine = tid / LANES;
+        if (r >= rows || !place(r, row, head)) return;
+        float M = -CUDART_INF_F, L = 0.0f;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p0 = 0; p0 < parts; p0 += AT_ONCE) { // (more than 128 parts: what was joined so far is moved to the larger reference)
+            const int n = min(AT_ONCE, parts - p0);
+            const float2 st = tid < n ? stats[slot(p0 + tid) + r] : make_float2(-CUDART_INF_F, 0.0f);
+            const float most = warp_max_f(st.x);
+            __syncthreads();
+            if (tid % 32 == 0) red[tid / 32] = most;
+            __syncthreads();
+            const float grown = fmaxf(M, fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]))), base = grown == -CUDART_INF_F ? 0.0f : grown, f = M == grown ? 1.0f : ex2(M - base);
+            M = grown;
+            L *= f;
+            x = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+            stat[tid] = make_float2(st.x == M ? 1.0f : ex2(st.x - base), st.y);
+            __syncthreads();
+            if (mine < GROUPS)
+#pragma unroll 8
+                for (int p = mine; p < n; p += GROUPS) {
+                    const float4 v = *reinterpret_cast<const float4 *>(a.work + (slot(p0 + p) + r) * HS + lane * 4);
+                    const float2 w = stat[p];
+                    L = fmaf(w.x, w.y, L);
+                    x = make_float4(fmaf(w.x, v.x, x.x), fmaf(w.x, v.y, x.y), fmaf(w.x, v.z, x.z), fmaf(w.x, v.w, x.w));
+                }
+        }
+        if (mine < GROUPS) {
+            sums[mine][lane] = x;
+            if (lane == 0) sums_l[mine] = L;
+        }
+        __syncthreads();
+        if (tid < LANES) {
+#pragma unroll
+            for (int i = 1; i < GROUPS; i++) {
+                const float4 p = sums[i][lane];
+                x = make_float4(x.x + p.x, x.y + p.y, x.z + p.z, x.w + p.w);
+                L += sums_l[i];
+            }
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+            put_results(a, row, head, HS, lane * 4, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+        }
     }
 }
 

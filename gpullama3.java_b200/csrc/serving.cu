@@ -45,34 +45,35 @@ int check_rows(const b200_paged_cache *c, int n, const int32_t *positions, const
 
 // How the attention of n rows is cut.
 struct PagedCut {
-    int nr, tokens, blocks, splits, share; // blocks of 8 nr rows; tokens of a unit; blocks of a unit; CTAs of a block, tiles of each
+    int nr, tokens, blocks, ctas; // blocks of 8 nr rows; tokens of a group; blocks of a group and key/value head; CTAs that units are shared out over (0: a CTA a unit)
+    size_t units;
 };
-// Rows of a unit: the tokens of a chunk that fit 32 rows (16 with heads of 256, for more their results would leave no registers), so that they read the pages once.
+// Rows of a group: the tokens of a chunk that fit 32 rows (16 with heads of 256, for more their results would leave no registers), so that they read the pages once.
 PagedCut paged_cut(const b200_paged_cache &c, const b200_paged_attention_args &a, int sms) {
-    PagedCut k;
+    PagedCut k = {};
     const int G = c.kv_heads, mul = a.heads / G, chunk = a.chunk < 1 ? 1 : a.chunk < a.n ? a.chunk : a.n;
     int fit = (c.head_size == 256 ? 16 : 32) / mul;
     if (fit < 1) fit = 1;
-    const int units_of_chunk = (chunk + fit - 1) / fit;
-    k.tokens = (chunk + units_of_chunk - 1) / units_of_chunk; // even shares
+    const int groups_of_chunk = (chunk + fit - 1) / fit;
+    k.tokens = (chunk + groups_of_chunk - 1) / groups_of_chunk; // even shares
     // (a token of more than 16 query heads of a key/value head reads the pages once for 16 of them)
     k.nr = k.tokens > 1 ? (k.tokens * mul <= 16 ? 2 : (k.tokens * mul + 7) / 8) : mul <= 8 ? 1 : 2;
     k.blocks = (k.tokens * mul + 8 * k.nr - 1) / (8 * k.nr);
-    const int KT = paged::step_keys(c.head_size);
+    const int KT = paged::step_keys(c.head_size), groups = (a.n + k.tokens - 1) / k.tokens;
     const long long context = (long long)a.table_width * c.page_size;
     long long len = a.max_len > 0 && a.max_len < context ? a.max_len : context;
     const long long near = (long long)a.window + k.tokens;
     if (a.window > 0 && near < len) len = near;
-    const long long tiles = (len + KT - 1) / KT + 1, units = (long long)((a.n + k.tokens - 1) / k.tokens) * G * k.blocks;
-    // One long row: two CTAs an SM, evenly.  Many rows: their lengths differ, so shares are small enough for several CTAs an SM and row; at least 8 tiles a warp, since every share leaves a part to join.
-    const long long wanted = units * tiles / (2LL * sms) + 1, least = 8 * paged::STEP_WARPS;
-    long long share = units >= sms ? (wanted + 3) / 4 : wanted;
-    if (share < least) share = least;
-    k.splits = (int)((tiles + share - 1) / share < paged::MAX_SPLITS ? (tiles + share - 1) / share : paged::MAX_SPLITS);
-    if (k.splits < 1) k.splits = 1;
-    k.share = (int)((tiles + k.splits - 1) / k.splits);
+    k.units = (size_t)groups * G * k.blocks;
+    // Shared out where a unit is worth more than two CTAs, and where a CTA finds its place quickly: it looks at all rows' positions.
+    if (len > 2LL * paged::SHARE_LEAST * KT && groups <= paged::STEP_GROUPS && a.n <= paged::STEP_SHARED_ROWS) {
+        const long long most = ((len + KT - 1) / KT + 1) * (long long)k.units / paged::SHARE_LEAST + 1, room = (long long)sms * paged::step_ctas(c.head_size, k.nr);
+        k.ctas = (int)(most < room ? most : room);
+    }
     return k;
 }
+size_t paged_cut_bytes(const b200_paged_cache &c, const PagedCut &k) { return k.ctas ? (k.ctas + k.units) * 8 * k.nr * (c.head_size + 2) * 4 + (paged::STEP_GROUPS + 1) * 4 : 0; } // (paged::shared_grid)
+
 // Chunks on the tensor cores: 16-bit results, heads of 64, 96 or 128.  A tile takes 128 rows whether they are used or not.
 const int CHUNK_MIN_ROWS = 64;
 struct PagedChunkCut {
@@ -125,7 +126,8 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
     if (PagedChunkCut cc = paged_chunk_cut(c, a, sms); cc.use) {
         if (!has_room(cc.splits)) cc.splits = 1;
         k.tokens = cc.tokens; k.splits = cc.splits;
-        k.blocks = k.share = 1;
+        k.blocks = 1;
+        k.ctas = 0;
         k.vec_out = aligned16(a.out, a.out_stride, 2);
         const unsigned grid = (unsigned)((a.n + cc.tokens - 1) / cc.tokens) * c.kv_heads * cc.splits;
         return by_cache_type(c.type, [&](auto type) {
@@ -144,9 +146,9 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
         });
     }
     PagedCut cut = paged_cut(c, a, sms);
-    if (!has_room(cut.splits)) cut.splits = 1;
-    k.tokens = cut.tokens; k.blocks = cut.blocks; k.splits = cut.splits; k.share = cut.share;
-    const dim3 grid((unsigned)((a.n + cut.tokens - 1) / cut.tokens) * cut.blocks, c.kv_heads, cut.splits);
+    if (!a.workspace || paged_cut_bytes(c, cut) > a.workspace_bytes) cut.ctas = 0;
+    k.tokens = cut.tokens; k.blocks = cut.blocks; k.ctas = cut.ctas; k.splits = 1;
+    const unsigned units = (unsigned)cut.units;
     return by_head_size(c.head_size, [&](auto hs) {
         return by_cache_type(c.type, [&](auto type) {
             using T = decltype(type);
@@ -154,8 +156,10 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
                 constexpr size_t smem = paged::step_smem_bytes(hs, nr);
                 auto kern = a.out_type == B200_GGML_F32 ? paged::k_paged_step<hs, T, nr, true, lone> : paged::k_paged_step<hs, T, nr, false, lone>;
                 cudaError_t e = allow_smem(kern, smem);
-                if (e == cudaSuccess) e = launch(kern, grid, paged::STEP_WARPS * 32, smem, 1, false, stream, k);
-                return e != cudaSuccess || cut.splits == 1 ? e : join(hs, cut.splits);
+                if (e == cudaSuccess) e = launch(kern, cut.ctas ? cut.ctas + units : units, paged::STEP_WARPS * 32, smem, 1, false, stream, k);
+                if (e != cudaSuccess || !cut.ctas) return e;
+                if ((unsigned)cut.ctas <= 8 * units) return launch(paged::k_paged_join_shares<hs, nr, lone, true>, dim3(units, nr), 128, 0, 1, true, stream, k);
+                return launch(paged::k_paged_join_shares<hs, nr, lone, false>, dim3(units, 8 * nr), 128, 0, 1, true, stream, k);
             };
             if (cut.tokens == 1) return cut.nr == 1 ? go(std::integral_constant<int, 1>(), std::true_type()) : go(std::integral_constant<int, 2>(), std::true_type());
             if constexpr (hs < 256) {
@@ -224,7 +228,7 @@ size_t b200_paged_attention_workspace(const b200_paged_cache *c, const b200_page
     if (!countable(c, a)) return 0;
     const int sms = sm_count(c->device);
     const PagedChunkCut cc = paged_chunk_cut(*c, *a, sms);
-    return paged_work_bytes(*c, *a, cc.use ? cc.splits : paged_cut(*c, *a, sms).splits);
+    return cc.use ? paged_work_bytes(*c, *a, cc.splits) : paged_cut_bytes(*c, paged_cut(*c, *a, sms));
 }
 
 static int paged_attention(const b200_paged_cache *c, const b200_paged_attention_args *a, void *stream, char *err, size_t err_len, bool give_up) {
@@ -239,7 +243,6 @@ static int paged_attention(const b200_paged_cache *c, const b200_paged_attention
     if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(B200_ERR_BAD_ARG, "the workspace is not aligned");
     if (a->n == 0) return B200_OK;
     if (!a->q || !a->out) return fail(B200_ERR_BAD_ARG, "null rows");
-    if (c->kv_heads > 65535) return fail(B200_ERR_UNSUPPORTED, "%d key/value heads (at most 65535)", c->kv_heads);
     const int64_t width = (int64_t)a->heads * c->head_size;
     if (a->n > 1 && (a->q_stride < width || a->out_stride < width)) return fail(B200_ERR_BAD_ARG, "rows overlap: a stride is smaller than its row");
     if ((long long)a->n * a->heads > (1LL << 22)) return fail(B200_ERR_UNSUPPORTED, "too many rows in one call"); // (times MAX_SPLITS: the grid's limit)
