@@ -368,7 +368,8 @@ template <int KT, bool LONE, int THREADS> __device__ __forceinline__ void share_
 // share of its tiles (Shares), and deals them to its warps in turn; each warp has a cp.async ring and a running reference of its own, and no barrier in the loop.  Parts
 // are joined in shared memory, those of several CTAs through the workspace (k_paged_join_shares).  Nothing depends on an order of arrival.
 //   scores  S[16 positions x 8 rows] = K Q^T, the cache's type, exact products, FP32 sums;  p = 2^(factor s - ref), factor = |scale| log2(e), the scale's sign is the queries'
-//   values  O[16 entries x 8 rows] += V^T P with p in the cache's type, half a step off, as the result will be; TWO (FP32 results): and what that left, 16 (BF16) or 22 (FP16) bits in all
+//   values  O[16 entries x 8 rows] += V^T P with p in the cache's type, half a step off, as the result will be; with FP32 results as PARTS numbers, each what the ones before left: two of FP16
+//           (22 bits), three of BF16 (24: two, 16 bits, put FP32 results three times as far off as FP32 sums are)
 // (Rows as the products' eight columns: four query heads of a key/value head, the usual number, leave half of them empty, as rows they would leave three quarters, with twice the registers.)
 // ref follows the largest score seen so far only when that passes it by more than 2^8 (the first does), so that few tiles have anything to rescale; with FP16 it lies 2^7 below, so that
 // p reaches down to 2^-24 of 2^-15: a long tail of small ones still counts.
@@ -435,7 +436,7 @@ __host__ __device__ inline size_t shared_grid(const Step &a, int groups) { retur
 template <int HS, int NR> __device__ __forceinline__ float2 *stats_of(const Step &a, int groups) { return reinterpret_cast<float2 *>(a.work + shared_grid(a, groups) * step_rows(NR) * HS); }
 template <int HS, int NR> __device__ __forceinline__ int *plan_of(const Step &a, int groups) { return reinterpret_cast<int *>(stats_of<HS, NR>(a, groups) + shared_grid(a, groups) * step_rows(NR)); }
 
-template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __launch_bounds__(STEP_WARPS * 32, step_ctas(HS, NR)) k_paged_step(const Step a) {
+template <int HS, typename T, int NR, int PARTS, bool LONE> __global__ void __launch_bounds__(STEP_WARPS * 32, step_ctas(HS, NR)) k_paged_step(const Step a) {
     constexpr int KT = step_keys(HS), KB = KT / 16, S = step_stages(HS), ROWS = step_rows(NR), PIECES = HS / 8, STAGE = step_stage_bytes(HS), TOKENS = LONE ? 1 : step_tokens_most(), RB = HS * 2;
     constexpr bool F16 = std::is_same<T, __half>::value, QREG = HS * NR <= 256;
     constexpr float LIFT = F16 ? 7.0f : 0.0f;
@@ -706,7 +707,7 @@ template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __lau
                     }
                 }
         }
-        uint32_t ph[NR][KB][2], pl[NR][KB][2]; // of 8 positions each: of positions 2 t, 2 t + 1 and row g
+        uint32_t pp[PARTS][NR][KB][2]; // of 8 positions each: of positions 2 t, 2 t + 1 and row g
 #pragma unroll
         for (int n = 0; n < NR; n++)
 #pragma unroll
@@ -716,11 +717,13 @@ template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __lau
                     const float p0 = ex2(fmaf(s[n][b][2 * i], factor, -ref[n][0])), p1 = ex2(fmaf(s[n][b][2 * i + 1], factor, -ref[n][1]));
                     l[n][0] += p0;
                     l[n][1] += p1;
-                    const uint32_t w = pack2<T>(p0, p1);
-                    ph[n][b][i] = transpose8x8(w);
-                    if constexpr (TWO) {
+                    float2 left = make_float2(p0, p1);
+#pragma unroll
+                    for (int c = 0; c < PARTS; c++) {
+                        const uint32_t w = pack2<T>(left.x, left.y);
+                        pp[c][n][b][i] = transpose8x8(w);
                         const float2 r = unpack2<T>(w);
-                        pl[n][b][i] = transpose8x8(pack2<T>(p0 - r.x, p1 - r.y));
+                        left = make_float2(left.x - r.x, left.y - r.y);
                     }
                 }
 #pragma unroll
@@ -730,10 +733,9 @@ template <int HS, typename T, int NR, bool TWO, bool LONE> __global__ void __lau
                 uint32_t va[4];
                 ldmatrix4_trans(at + v_off + 16 * b * RB + (v_x ^ i << 5), va);
 #pragma unroll
-                for (int n = 0; n < NR; n++) {
-                    mma<T>(o[n][i], va, ph[n][b][0], ph[n][b][1]);
-                    if constexpr (TWO) mma<T>(o[n][i], va, pl[n][b][0], pl[n][b][1]);
-                }
+                for (int n = 0; n < NR; n++)
+#pragma unroll
+                    for (int c = 0; c < PARTS; c++) mma<T>(o[n][i], va, pp[c][n][b][0], pp[c][n][b][1]);
             }
         if (++stage == S) stage = 0;
     }

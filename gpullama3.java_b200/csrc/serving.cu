@@ -154,7 +154,7 @@ cudaError_t paged_attention_launch(const b200_paged_cache &c, const b200_paged_a
             using T = decltype(type);
             const auto go = [&](auto nr, auto lone) {
                 constexpr size_t smem = paged::step_smem_bytes(hs, nr);
-                auto kern = a.out_type == B200_GGML_F32 ? paged::k_paged_step<hs, T, nr, true, lone> : paged::k_paged_step<hs, T, nr, false, lone>;
+                auto kern = a.out_type == B200_GGML_F32 ? paged::k_paged_step<hs, T, nr, std::is_same<T, __half>::value ? 2 : 3, lone> : paged::k_paged_step<hs, T, nr, 1, lone>;
                 cudaError_t e = allow_smem(kern, smem);
                 if (e == cudaSuccess) e = launch(kern, cut.ctas ? cut.ctas + units : units, paged::STEP_WARPS * 32, smem, 1, false, stream, k);
                 if (e != cudaSuccess || !cut.ctas) return e;

@@ -96,7 +96,7 @@ class PagedKVCache(_ops.Paged):
         Causal attention of rows ``q`` [n, heads, head_size] of the cache's type: the row at position p sees the positions up to p of its sequence, the last ``window`` of them (0: all);
         ``scale`` is head_size ** -0.5 unless given.  Results are of the cache's type unless ``dtype`` says FP32, FP16 or BF16.  ``chunk`` (neighbouring rows that are successive tokens of one
         sequence: drafted tokens, a prompt's chunk) and ``max_len`` (largest position + 1, 0: unknown) only choose how the work is split.  ``dtype`` chooses the precision too: 16-bit results come
-        from probabilities of the cache's type, half a step off each, FP32 results from two such numbers (16 bits BF16, 22 FP16).  A row that sees nothing is zeros; a value that is
+        from probabilities of the cache's type, half a step off each, FP32 results from several such numbers (24 bits BF16, 22 FP16).  A row that sees nothing is zeros; a value that is
         infinite or NaN reaches the rows that see it, and only those."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_size: int, dtype: torch.dtype = torch.bfloat16, device: int | torch.device | str | None = None):

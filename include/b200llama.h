@@ -622,7 +622,7 @@ int b200_paged_append(const b200_paged_cache *cache, const b200_paged_append_arg
 
 /* Causal attention of n query rows of the cache's type over the pages of their sequences: the row at position p sees the positions j <= p that have a page, the last `window` of them
  * where window > 0; query head h reads key/value head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type (F32, F16, BF16).  Queries and keys are multiplied as they are,
- * sums are FP32, and a probability is a number of the cache's type (8 bits BF16, 11 FP16: with results of 16 bits, which round as much) or two of them (16 bits, 22: with FP32 results).  A row
+ * sums are FP32, and a probability is a number of the cache's type (8 bits BF16, 11 FP16: with results of 16 bits, which round as much) or several of them (24 bits, 22: with FP32 results).  A row
  * that sees nothing, or only scores of -inf, is zeros.  A value that is infinite or NaN makes its entry not finite in the rows that see it, and only in those.  chunk (0 or 1: single
  * steps; how many neighbouring rows are successive tokens of one sequence) and max_len (0: unknown; the largest position + 1) only choose how the work is split.  Chunks of 64 rows (tokens x query
  * heads of a key/value head) and more with 16-bit results and heads of 64, 96 or 128 run on the tensor cores' own memory; waits inside that kernel end after half a second, and should one ever run
