@@ -297,6 +297,7 @@ int b200_verify_drafts(const b200_verify_drafts_args *a, void *stream, char *err
         e = by_type(a->type, [&](auto type) {
             using T = decltype(type);
             const cudaError_t first = launch(verify::k_verify_rows<T>, (unsigned)grid, verify::ROW_THREADS, 0, 1, false, (cudaStream_t)stream, k);
+            if (first == cudaSuccess && k.greedy) return launch(verify::k_verify_greedy, (unsigned)a->sequences, 256, 0, 1, true, (cudaStream_t)stream, k);
             return first != cudaSuccess ? first : launch(verify::k_verify_token<T>, (unsigned)a->sequences * verify::CLUSTER, verify::TOKEN_THREADS, 0, verify::CLUSTER, true, (cudaStream_t)stream, k);
         });
     return e == cudaSuccess ? B200_OK : fail(cuda_code(e), "%s", cudaGetErrorString(e));

@@ -10,6 +10,7 @@
 // 64 bits; and where FP32's error could turn a decision, its row's sum is taken once more in 64 bits.
 // Nothing depends on an order of arrival.
 #pragma once
+#include "kv4.cuh"
 #include "logprobs.cuh"
 
 namespace verify {
@@ -39,6 +40,8 @@ struct Args {
     Part *parts; // [target rows, then draft rows][stretch]
 };
 
+__host__ __device__ inline int share_of(int vocab) { return ((vocab + CLUSTER * TOKEN_WARPS - 1) / (CLUSTER * TOKEN_WARPS) + 7) / 8 * 8; } // entries of a warp: whole vectors
+
 // Drafts of a sequence in front of the first that is no token (at most `most` looked at): a warp.
 __device__ __forceinline__ int given(const Args &a, int s, int most) {
     const int lane = threadIdx.x & 31;
@@ -57,6 +60,7 @@ template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 5) k_verify
     __shared__ float warp_top[ROW_THREADS / 32], warp_sum[ROW_THREADS / 32];
     __shared__ int warp_at[ROW_THREADS / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
     const int row = blockIdx.x / a.stretches, stretch = blockIdx.x % a.stretches, per = a.drafts + 1, n_target = a.sequences * per;
     const bool target = row < n_target;
     const int s = target ? row / per : (row - n_target) / a.drafts, i = target ? row % per : (row - n_target) % a.drafts;
@@ -122,228 +126,310 @@ struct Row { // a row's largest entry and its sum; without a distribution: a sum
     int at;
     double sum;
 };
-// 64-bit sums of weights over the vocabulary, by warp, CTA and cluster.
+// The parts of a row joined: a warp.
+__device__ __forceinline__ Row join_parts(const Args &a, size_t row, float to_log2) {
+    const int lane = threadIdx.x & 31;
+    float top = -CUDART_INF_F;
+    double sum = 0.0;
+    int at = INT_MAX;
+    bool nan = false;
+    for (int j = lane; j < a.stretches; j += 32) {
+        const Part p = a.parts[row * a.stretches + j];
+        nan |= p.sum != p.sum;
+        if (p.top > top) {
+            sum *= (double)ex2((top - p.top) * to_log2);
+            top = p.top;
+            at = p.at;
+            sum += (double)p.sum;
+        } else if (p.top > -CUDART_INF_F) sum += (double)p.sum * (double)(p.top == top ? 1.0f : ex2((p.top - top) * to_log2));
+    }
+    const float all = warp_max_f(top);
+    sum = top == -CUDART_INF_F ? 0.0 : sum * (double)(top == all ? 1.0f : ex2((top - all) * to_log2));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    at = __reduce_min_sync(0xffffffffu, top == all ? at : INT_MAX);
+    nan = __any_sync(0xffffffffu, nan);
+    return {all, at, nan || !(fabsf(all) < CUDART_INF_F) ? -1.0 : a.greedy ? 1.0 : sum};
+}
+
+// Temperature 0: a CTA a sequence, a row a warp.
+__global__ void __launch_bounds__(256) k_verify_greedy(const Args a) {
+    __shared__ int best[MAX_DRAFTS + 1];
+    pdl_wait();
+    const int tid = threadIdx.x, s = blockIdx.x, c = given(a, s, a.drafts);
+    const long long out = (long long)s * (a.drafts + 1);
+    for (int r = tid / 32; r <= c; r += 8) {
+        const Row row = join_parts(a, (size_t)out + r, 0.0f);
+        if (tid % 32 == 0) best[r] = row.sum > 0.0 ? row.at : -1;
+    }
+    __syncthreads();
+    if (tid >= 32) return;
+    int n = 0;
+    while (n < c && best[n] == a.tokens[(long long)s * a.drafts + n]) n++;
+    for (int i = tid; i <= a.drafts; i += 32) a.out_tokens[out + i] = i <= n ? best[i] : -1;
+    if (tid == 0) a.accepted[s] = n;
+}
+
+// 64-bit sums over the vocabulary: of p = exp((x - top) / T), of q likewise, and of both where p weighs more.
+constexpr int SUMS = 4;
 struct Sums {
-    double warp[TOKEN_WARPS], cta[CLUSTER]; // this CTA's warps; every CTA
+    double warp[SUMS][TOKEN_WARPS], cta[SUMS][CLUSTER]; // this CTA's warps; every CTA
+};
+__device__ __forceinline__ float4 load4(const float *x) { return __ldcs(reinterpret_cast<const float4 *>(x)); }
+template <typename T> __device__ __forceinline__ float4 load4(const T *x) {
+    const uint2 w = __ldcs(reinterpret_cast<const uint2 *>(x));
+    const float2 a = kv4::to_f32x2(w.x, x), b = kv4::to_f32x2(w.y, x);
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+// exp((x - top) / T) for x <= top, within 4e-15 of itself: 2^(k / 32) from a table, the rest, at most ln(2) / 64, by its series (P. T. P. Tang's table-driven exponential, 1989); below -690 it is 0.
+constexpr int EXP_TABLE = 32;
+struct Weight {
+    const unsigned (*table)[EXP_TABLE]; // low, high words of 2^(i / 32): 32 banks each, no conflicts
+    double scale;                       // 32 log2(e) / T
+    float reach;                        // 690 T
+    __device__ __forceinline__ double operator()(float x, float top) const {
+        constexpr double MAGIC = 6755399441055744.0, A = 0.693147180559945309417232 / EXP_TABLE; // 1.5 * 2^52: its last bits are those of the whole number added
+        const double u = ((double)x - (double)top) * scale, d = u + MAGIC, r = u - (d - MAGIC);
+        const int k = __double2loint(d);
+        const double p = fma(fma(fma(fma(fma(A * A * A * A * A / 120.0, r, A * A * A * A / 24.0), r, A * A * A / 6.0), r, A * A / 2.0), r, A), r, 1.0) *
+                         __hiloint2double((int)table[1][k & (EXP_TABLE - 1)], (int)table[0][k & (EXP_TABLE - 1)]);
+        const bool some = x >= top - reach;
+        return __hiloint2double(some ? __double2hiint(p) + (k >> 5 << 20) : 0, some ? __double2loint(p) : 0);
+    }
 };
 
-template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS) k_verify_token(const Args a) {
-    constexpr int VEC = Load<T>::VEC;
-    __shared__ Row rows[2 * MAX_DRAFTS + 1]; // target rows, then draft rows
+template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_verify_token(const Args a) {
+    __shared__ Row rows[2 * MAX_DRAFTS + 1];    // target rows, then draft rows
     __shared__ signed char verdict[MAX_DRAFTS]; // 1 accepted, 0 not, -1 too close, -2 no distribution
-    __shared__ Sums sums[2];
+    __shared__ Sums sums;
     __shared__ double scan[TOKEN_WARPS];
+    __shared__ unsigned table[2][EXP_TABLE];
     __shared__ int found;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = (int)cluster.block_rank(), s = blockIdx.x / CLUSTER;
-    pdl_wait();
-    cluster.sync(); // every CTA is there before another writes into its memory
+    if (tid < EXP_TABLE) {
+        const double x = exp2((double)tid / EXP_TABLE);
+        table[0][tid] = (unsigned)__double2loint(x);
+        table[1][tid] = (unsigned)__double2hiint(x);
+    }
     const int c = given(a, s, a.drafts);
     const int *d = a.tokens + (long long)s * a.drafts;
     const float *u = a.uniforms + (long long)s * (a.drafts + 1);
-    const int greedy = a.greedy, both = a.both;
-    const float to_log2 = greedy ? 0.0f : LOG2E / a.temperature;
-    const double inv_t = greedy ? 0.0 : 1.0 / (double)a.temperature;
+    const int both = a.both;
+    const Weight weight = {table, EXP_TABLE * 1.44269504088896340736 / (double)a.temperature, 690.0f * a.temperature};
     const auto target = [&](int i) { return (const T *)a.logits + s * a.ld_s + i * a.ld_r; };
     const auto draft = [&](int i) { return (const T *)a.draft_logits + s * a.draft_ld_s + i * a.draft_ld_r; };
+    cluster.sync(); // every CTA is there before another writes into its memory
+    pdl_wait();
 
     // ---- the rows' parts, a row a warp ----
     for (int r = warp; r < (both ? 2 * c + 1 : c + 1); r += TOKEN_WARPS) {
         const bool first = r <= c;
-        const size_t row = first ? (size_t)s * (a.drafts + 1) + r : (size_t)a.sequences * (a.drafts + 1) + (size_t)s * a.drafts + r - c - 1;
-        float top = -CUDART_INF_F;
-        for (int j = lane; j < a.stretches; j += 32) top = fmaxf(top, a.parts[row * a.stretches + j].top);
-        top = warp_max_f(top);
-        double sum = 0.0;
-        int at = INT_MAX;
-        bool nan = false;
-        for (int j = lane; j < a.stretches; j += 32) {
-            const Part p = a.parts[row * a.stretches + j];
-            nan |= p.sum != p.sum;
-            if (p.top == -CUDART_INF_F) continue;
-            sum += (double)p.sum * (double)(p.top == top ? 1.0f : ex2((p.top - top) * to_log2));
-            if (p.top == top) at = min(at, p.at);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        at = __reduce_min_sync(0xffffffffu, at);
-        nan = __any_sync(0xffffffffu, nan);
-        if (lane == 0) rows[first ? r : MAX_DRAFTS + r - c] = {top, at, nan || !(fabsf(top) < CUDART_INF_F) ? -1.0 : greedy ? 1.0 : sum};
+        const Row row = join_parts(a, first ? (size_t)s * (a.drafts + 1) + r : (size_t)a.sequences * (a.drafts + 1) + (size_t)s * a.drafts + r - c - 1, LOG2E / a.temperature);
+        if (lane == 0) rows[first ? r : MAX_DRAFTS + r - c] = row;
     }
     __syncthreads();
     const auto of_draft = [&](int i) -> Row & { return rows[MAX_DRAFTS + 1 + i]; };
-    const auto chance = [&](const Row &r, const T *x, int j) { return exp(((double)Load<T>::one(x + j) - (double)r.top) * inv_t) / r.sum; };
-    const auto decide = [&](int i) { // u q < p, and by how much
-        const Row &p = rows[i];
-        if (!(p.sum > 0.0) || (both && !(of_draft(i).sum > 0.0))) return -2;
-        if (greedy) return p.at == d[i] ? 1 : 0;
-        const double x = (double)u[i] * (both ? chance(of_draft(i), draft(i), d[i]) : 1.0), y = chance(p, target(i), d[i]);
-        return fabs(x - y) <= 1e-5 * fmax(x, y) && y > 0.0 ? -1 : x < y ? 1 : 0;
+    const auto decide = [&](int i, double sum, double draft_sum) { // u q < p; 2 and 3: too close for sums of FP32
+        const double q = both ? weight(Load<T>::one(draft(i) + d[i]), of_draft(i).top) / draft_sum : 1.0;
+        const double x = (double)u[i] * q, y = weight(Load<T>::one(target(i) + d[i]), rows[i].top) / sum;
+        return fabs(x - y) <= 1e-5 * fmax(x, y) && y > 0.0 ? x < y ? 3 : 2 : x < y ? 1 : 0;
     };
-    if (tid < c) verdict[tid] = (signed char)decide(tid);
+    if (tid < c) {
+        const int v = !(rows[tid].sum > 0.0) || (both && !(of_draft(tid).sum > 0.0)) ? -2 : decide(tid, rows[tid].sum, of_draft(tid).sum);
+        verdict[tid] = (signed char)(v >= 2 ? -1 : v);
+    }
     __syncthreads();
 
-    // Sums of weights f(j, x_j, y_j) over the vocabulary, which the cluster's warps share in order; y may be null.
-    const int share = ((a.vocab + CLUSTER * TOKEN_WARPS - 1) / (CLUSTER * TOKEN_WARPS) + 7) / 8 * 8; // (whole vectors)
+    // One pass over target row i, without entry `without`, and draft row i (two), which the cluster's warps share in order: sums of p, of q, and of both where p / sum_p > q / sum_q.
+    const int share = share_of(a.vocab);
     const auto begin_of = [&](int w) { return (int)min((long long)w * share, (long long)a.vocab); };
-    const auto add = [&](Sums &to, const T *x, const T *y, auto f) {
-        const int begin = begin_of(rank * TOKEN_WARPS + warp), end = begin_of(rank * TOKEN_WARPS + warp + 1);
-        double sum = 0.0;
-        for (int j0 = begin; j0 < end; j0 += 2 * 32 * VEC) {
-            float p[2][VEC], q[2][VEC];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int j = j0 + (h * 32 + lane) * VEC;
-                if (a.vec && j + VEC <= end) {
-                    Load<T>::vec(x + j, p[h]);
-                    if (y) Load<T>::vec(y + j, q[h]);
-                } else
-#pragma unroll
-                    for (int k = 0; k < VEC; k++) {
-                        p[h][k] = j + k < end ? Load<T>::one(x + j + k) : -CUDART_INF_F;
-                        q[h][k] = y && j + k < end ? Load<T>::one(y + j + k) : -CUDART_INF_F;
-                    }
+    int n = 0, kind = -1, without = -1; // kind: of the pass.  -1: for a verdict; 0: weights p; 1: p - q; 2: p - q once more, by exact sums; 3: p whole
+    double sum_p = 1.0, sum_q = 1.0;    // of the rows that the pass is for
+    bool fails = false;
+    for (;;) {
+        if (kind < 0) { // the next draft whose verdict takes a pass, or the token
+            int v = 1;
+            while (n < c && (v = verdict[n]) == 1) n++;
+            fails = n < c ? v == -2 : !(rows[c].sum > 0.0);
+            if (fails) break;
+            if (n == c || v == 0) {
+                kind = n < c && both ? 1 : 0;
+                without = n < c && !both ? d[n] : -1; // a looked-up draft that did not stand
             }
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int k = 0; k < VEC; k++) sum += f(j0 + (h * 32 + lane) * VEC + k, p[h][k], y ? q[h][k] : 0.0f);
+        }
+        const bool two = both && n < c;
+        const T *x = target(n), *y = two ? draft(n) : nullptr;
+        const float top_p = rows[n].top, top_q = two ? of_draft(n).top : 0.0f;
+        if (kind != 2) {
+            sum_p = rows[n].sum;
+            sum_q = two ? of_draft(n).sum : 1.0;
+        }
+        const double by_p = 1.0 / sum_p, by_q = 1.0 / sum_q;
+        double part[SUMS] = {0.0, 0.0, 0.0, 0.0};
+        const int begin = begin_of(rank * TOKEN_WARPS + warp), end = begin_of(rank * TOKEN_WARPS + warp + 1);
+        const float nothing = -CUDART_INF_F;
+#pragma unroll 1
+        for (int j0 = begin; j0 < end; j0 += 128) {
+            const int j = j0 + lane * 4;
+            float4 xs = make_float4(nothing, nothing, nothing, nothing), ys = xs;
+            if (two) { // (needed last)
+                if (a.vec && j + 4 <= end) ys = load4(y + j);
+                else {
+                    if (j < end) ys.x = Load<T>::one(y + j);
+                    if (j + 1 < end) ys.y = Load<T>::one(y + j + 1);
+                    if (j + 2 < end) ys.z = Load<T>::one(y + j + 2);
+                    if (j + 3 < end) ys.w = Load<T>::one(y + j + 3);
+                }
+            }
+            if (a.vec && j + 4 <= end) xs = load4(x + j);
+            else {
+                if (j < end) xs.x = Load<T>::one(x + j);
+                if (j + 1 < end) xs.y = Load<T>::one(x + j + 1);
+                if (j + 2 < end) xs.z = Load<T>::one(x + j + 2);
+                if (j + 3 < end) xs.w = Load<T>::one(x + j + 3);
+            }
+            if (without >= j && without < j + 4) {
+                if (without == j) xs.x = nothing;
+                if (without == j + 1) xs.y = nothing;
+                if (without == j + 2) xs.z = nothing;
+                if (without == j + 3) xs.w = nothing;
+            }
+            const double p0 = weight(xs.x, top_p), p1 = weight(xs.y, top_p), p2 = weight(xs.z, top_p), p3 = weight(xs.w, top_p);
+            part[0] += (p0 + p1) + (p2 + p3);
+            if (two) {
+                const auto also = [&](double p, float yi) {
+                    const double q = weight(yi, top_q);
+                    part[1] += q;
+                    const bool more = p * by_p > q * by_q;
+                    part[2] += more ? p : 0.0;
+                    part[3] += more ? q : 0.0;
+                };
+                also(p0, ys.x);
+                also(p1, ys.y);
+                also(p2, ys.z);
+                also(p3, ys.w);
+            }
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) to.warp[warp] = sum;
+        for (int k = 0; k < SUMS; k++)
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) part[k] += __shfl_xor_sync(0xffffffffu, part[k], o);
+        cluster.sync(); // what was added before has been read
+        if (lane == 0)
+#pragma unroll
+            for (int k = 0; k < SUMS; k++) sums.warp[k][warp] = part[k];
         __syncthreads();
-        if (tid < CLUSTER) { // to every CTA of the cluster
+        if (tid < SUMS * CLUSTER) { // to every CTA of the cluster
             double cta = 0.0;
 #pragma unroll
-            for (int w = 0; w < TOKEN_WARPS; w++) cta += to.warp[w];
-            *cluster.map_shared_rank(&to.cta[rank], tid) = cta;
+            for (int w = 0; w < TOKEN_WARPS; w++) cta += sums.warp[tid / CLUSTER][w];
+            *cluster.map_shared_rank(&sums.cta[tid / CLUSTER][rank], tid % CLUSTER) = cta;
         }
         cluster.sync();
-        double all = 0.0;
+        double all[SUMS] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-        for (int r = 0; r < CLUSTER; r++) all += to.cta[r];
-        return all;
-    };
-    const auto weight = [&](const Row &r, float x) { return exp(((double)x - (double)r.top) * inv_t); };
-
-    int n = 0;
-    bool fails = false;
-    for (; n < c; n++) {
-        int v = verdict[n];
-        if (v == -1) { // (all CTAs of the cluster come to the same)
-            Row &p = rows[n];
-            const Row was = p;
-            const double sp = add(sums[0], target(n), (const T *)nullptr, [&](int, float x, float) { return weight(was, x); });
-            double sq = 1.0;
-            if (both) {
-                const Row wasq = of_draft(n);
-                sq = add(sums[1], draft(n), (const T *)nullptr, [&](int, float x, float) { return weight(wasq, x); });
-            }
-            const double x = (double)u[n] * (both ? exp(((double)Load<T>::one(draft(n) + d[n]) - (double)of_draft(n).top) * inv_t) / sq : 1.0);
-            v = x < exp(((double)Load<T>::one(target(n) + d[n]) - (double)was.top) * inv_t) / sp;
-            cluster.sync(); // (the sums' memory is used again)
+        for (int r = 0; r < CLUSTER; r++)
+#pragma unroll
+            for (int k = 0; k < SUMS; k++) all[k] += sums.cta[k][r];
+        // (all CTAs of the cluster come to the same)
+        if (kind < 0) {
+            if (tid == 0) verdict[n] = (signed char)(decide(n, all[0], all[1]) & 1);
+            __syncthreads();
+        } else if (kind == 0 || kind == 3) {
+            if (all[0] > 0.0) break;
+            kind = 3; // nothing but the draft: p as it is
+            without = -1;
+        } else {
+            sum_p = all[0];
+            sum_q = all[1];
+            const double left = all[2] / sum_p - all[3] / sum_q;
+            // Which entries weigh more was told by FP32's sums, off by 1e-6 at most: an entry on the wrong side adds no more than that of itself, and few are that near.  Where little is left over they
+            // might count.
+            if (kind == 2 || left > 0.05) {
+                if (left > 0.0) break;
+                kind = 3; // the same distributions
+            } else kind = 2;
         }
-        fails = v == -2;
-        if (v != 1) break;
     }
-    if (n == c) fails = !(rows[c].sum > 0.0);
     if (rank == 0) {
         for (int i = tid; i <= a.drafts; i += TOKEN_THREADS)
             if (i != n) a.out_tokens[(long long)s * (a.drafts + 1) + i] = i < n ? d[i] : -1;
         if (tid == 0) {
             a.accepted[s] = n;
-            if (fails || greedy) a.out_tokens[(long long)s * (a.drafts + 1) + n] = fails ? -1 : rows[n].at;
+            if (fails) a.out_tokens[(long long)s * (a.drafts + 1) + n] = -1;
         }
     }
-    if (fails || greedy) return; // (the same in every CTA of the cluster)
+    if (fails) return; // (the same in every CTA of the cluster)
 
-    // ---- the token ----
-    const bool left = n < c; // a draft that did not stand
-    const Row p = rows[n], q = rows[both && left ? MAX_DRAFTS + 1 + n : n];
-    const int without = left && !both ? d[n] : -1; // it was looked up
-    const auto whole = [&](int, float x, float) { return weight(p, x); };
-    const auto rest = [&](int j, float x, float) { return j == without ? 0.0 : weight(p, x); };
-    double total = add(sums[0], target(n), (const T *)nullptr, rest), sp = total, sq = 1.0;
-    int kind = 0; // of weights: rest, difference, whole
-    Sums *by = &sums[0];
-    if (both && left) {
-        sq = add(sums[1], draft(n), (const T *)nullptr, [&](int, float x, float) { return weight(q, x); });
-        cluster.sync();
-        const auto more = [&](int, float x, float y) { return fmax(weight(p, x) / sp - weight(q, y) / sq, 0.0); };
-        total = add(sums[1], target(n), draft(n), more);
-        by = &sums[1];
-        kind = 1;
-        if (!(total > 0.0)) { // the same distributions
-            by = &sums[0];
-            kind = 0;
-            total = sp;
-        }
-    } else if (without >= 0 && !(total > 0.0)) { // nothing but the draft
-        cluster.sync();
-        total = add(sums[0], target(n), (const T *)nullptr, whole);
-        kind = 2;
-    }
+    // ---- the token: which CTA, which warp's share, which entry: the first whose running sum passes the border, or the last that weighs anything ----
+    const bool differ = kind == 1 || kind == 2;
+    const double by_p = 1.0 / sum_p, by_q = 1.0 / sum_q;
+    const auto weight_of = [&](const double *p, const double *more_p, const double *more_q, int i) { return differ ? more_p[i] * by_p - more_q[i] * by_q : p[i]; };
+    const auto cta_weight = [&](int r) { return weight_of(sums.cta[0], sums.cta[2], sums.cta[3], r); };
+    const auto warp_weight = [&](int w) { return weight_of(sums.warp[0], sums.warp[2], sums.warp[3], w); };
+    const T *x = target(n), *y = differ ? draft(n) : nullptr;
+    const float top_p = rows[n].top, top_q = differ ? of_draft(n).top : 0.0f;
     const auto one = [&](int j) -> double {
-        const float x = Load<T>::one(target(n) + j);
-        return kind == 1 ? fmax(weight(p, x) / sp - weight(q, Load<T>::one(draft(n) + j)) / sq, 0.0) : kind == 0 ? rest(j, x, 0.0f) : whole(j, x, 0.0f);
+        const double p = j == without ? 0.0 : weight(Load<T>::one(x + j), top_p);
+        return differ ? fmax(p * by_p - weight(Load<T>::one(y + j), top_q) * by_q, 0.0) : p;
     };
-    // which CTA, which warp's share, which entry: the first whose running sum passes the border, or the last that weighs anything
+    double total = 0.0;
+    for (int r = 0; r < CLUSTER; r++) total += cta_weight(r);
     const double border = (double)u[a.drafts] * total;
     double before = 0.0, sum = 0.0;
     int chosen = -1;
     for (int r = 0; r < CLUSTER; r++) {
-        const double x = by->cta[r];
-        if (x > 0.0) { chosen = r; before = sum; }
-        sum += x;
-        if (x > 0.0 && sum > border) break;
+        const double w = cta_weight(r);
+        if (w > 0.0) { chosen = r; before = sum; }
+        sum += w;
+        if (w > 0.0 && sum > border) break;
     }
-    if (chosen == rank) { // (the others are done: nothing of theirs is read any more)
-        int w_chosen = 0;
-        double at = before;
-        sum = before;
-        for (int w = 0; w < TOKEN_WARPS; w++) {
-            const double x = by->warp[w];
-            if (x > 0.0) { w_chosen = w; at = sum; }
-            sum += x;
-            if (x > 0.0 && sum > border) break;
+    if (chosen != rank) return; // (the others are done: nothing of theirs is read any more)
+    int w_chosen = 0;
+    double at = before;
+    sum = before;
+    for (int w = 0; w < TOKEN_WARPS; w++) {
+        const double v = warp_weight(w);
+        if (v > 0.0) { w_chosen = w; at = sum; }
+        sum += v;
+        if (v > 0.0 && sum > border) break;
+    }
+    const int begin = begin_of(rank * TOKEN_WARPS + w_chosen), end = begin_of(rank * TOKEN_WARPS + w_chosen + 1);
+    int last = -1; // this thread's last entry that weighs anything
+    if (tid == 0) found = INT_MAX;
+    __syncthreads();
+    for (int j0 = begin; j0 < end; j0 += TOKEN_THREADS) {
+        const int j = j0 + tid;
+        const double v = j < end ? one(j) : 0.0;
+        double run = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double w = __shfl_up_sync(0xffffffffu, run, o);
+            if (lane >= o) run += w;
         }
-        const int begin = begin_of(rank * TOKEN_WARPS + w_chosen), end = begin_of(rank * TOKEN_WARPS + w_chosen + 1);
-        int last = -1; // this thread's last entry that weighs anything
-        if (tid == 0) found = INT_MAX;
+        if (lane == 31) scan[warp] = run;
         __syncthreads();
-        for (int j0 = begin; j0 < end; j0 += TOKEN_THREADS) {
-            const int j = j0 + tid;
-            const double x = j < end ? one(j) : 0.0;
-            double run = x;
+        double front = at, all = at;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double y = __shfl_up_sync(0xffffffffu, run, o);
-                if (lane >= o) run += y;
-            }
-            if (lane == 31) scan[warp] = run;
-            __syncthreads();
-            double front = at, all = at;
-#pragma unroll
-            for (int w = 0; w < TOKEN_WARPS; w++) {
-                if (w == warp) front = all;
-                all += scan[w];
-            }
-            if (x > 0.0) last = j;
-            if (x > 0.0 && front + run > border) atomicMin(&found, j);
-            __syncthreads();
-            at = all;
-            if (found != INT_MAX) break;
+        for (int w = 0; w < TOKEN_WARPS; w++) {
+            if (w == warp) front = all;
+            all += scan[w];
         }
-        if (found == INT_MAX) { // (the sums round apart by a last bit)
-            __syncthreads();
-            if (tid == 0) found = -1;
-            __syncthreads();
-            atomicMax(&found, last);
-            __syncthreads();
-        }
-        if (tid == 0) a.out_tokens[(long long)s * (a.drafts + 1) + n] = found;
+        if (v > 0.0) last = j;
+        if (v > 0.0 && front + run > border) atomicMin(&found, j);
+        __syncthreads();
+        at = all;
+        if (found != INT_MAX) break;
     }
+    if (found == INT_MAX) { // (the sums round apart by a last bit)
+        __syncthreads();
+        if (tid == 0) found = -1;
+        __syncthreads();
+        atomicMax(&found, last);
+        __syncthreads();
+    }
+    if (tid == 0) a.out_tokens[(long long)s * (a.drafts + 1) + n] = found;
 }
 
 } // namespace verify
