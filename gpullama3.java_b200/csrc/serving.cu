@@ -245,7 +245,7 @@ static int paged_attention(const b200_paged_cache *c, const b200_paged_attention
     if (!a->q || !a->out) return fail(B200_ERR_BAD_ARG, "null rows");
     const int64_t width = (int64_t)a->heads * c->head_size;
     if (a->n > 1 && (a->q_stride < width || a->out_stride < width)) return fail(B200_ERR_BAD_ARG, "rows overlap: a stride is smaller than its row");
-    if ((long long)a->n * a->heads > (1LL << 22)) return fail(B200_ERR_UNSUPPORTED, "too many rows in one call"); // (times MAX_SPLITS: the grid's limit)
+    if ((long long)a->n * a->heads > (1LL << 27)) return fail(B200_ERR_UNSUPPORTED, "too many rows in one call");
     OnDevice on(c->device);
     cudaError_t e = on.error;
     if (e == cudaSuccess) e = paged_attention_launch(*c, *a, (cudaStream_t)stream, give_up);

@@ -336,6 +336,7 @@ struct Paged {
             a.q = q->data_ptr();
             if (!out) out = fresh({n, a.heads, head_size}, dtype(), device);
             NEED(out->defined() && out->scalar_type() == dtype(), "q_out is of the cache's type, ", dtype());
+            NEED(n == 0 || out->data_ptr() != q->data_ptr(), "q_out may not overlap q");
             a.q_out_stride = rows(*out, "q_out", n, a.heads);
             a.q_out = out->data_ptr();
         } else NEED(!q_out && !q_norm, "q_out and q_norm belong to q");

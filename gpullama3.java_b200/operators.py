@@ -90,7 +90,7 @@ class PagedKVCache(_ops.Paged):
         Stores rows ``k``, ``v`` [n, kv_heads, head_size] (FP32, FP16 or BF16; parts of a wider row are fine), rounded once.  ``q`` [n, heads, head_size] of the same type comes back in the
         cache's type.  On the way the heads of q and k are RMS-normed (``q_norm`` / ``k_norm`` [head_size]) and their first 2 r entries rotated (``cos`` / ``sin`` [positions, r]; r is
         head_size / 2 for whole heads; scaled or stretched positions are a matter of these tables; pairs by ``layout``: "half": i and i + r, or "interleaved": 2 i and 2 i + 1).  A position
-        behind these tables is padding.  Two rows of a call must not name the same place; ``q_out`` is left as it was where a row is padding or has a negative position.
+        behind these tables is padding.  Two rows of a call must not name the same place; ``q_out``, which may not overlap ``q``, is left as it was where a row is padding or has a negative position.
 
     attention(q, positions, tables, sequences=None, scale=None, window=0, max_len=0, chunk=1, dtype=None, out=None)
         Causal attention of rows ``q`` [n, heads, head_size] of the cache's type: the row at position p sees the positions up to p of its sequence, the last ``window`` of them (0: all);

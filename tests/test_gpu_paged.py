@@ -318,7 +318,7 @@ def test_rows_of_wider_ones(pkg, pad, out):
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("H,G,hs,page,lengths,chunk,window", [(8, 2, 64, 16, [3000, 777], 64, 0), (4, 1, 128, 64, [4100], 128, 0), (4, 1, 128, 32, [9000], 33, 0), (3, 1, 96, 16, [2500, 40, 700], 40, 1500),
-                                                              (64, 1, 64, 8, [5000], 3, 0), (128, 1, 64, 16, [300], 5, 0), (16, 8, 96, 1, [1000, 900], 50, 333)])
+                                                              (64, 1, 64, 8, [5000], 3, 0), (4, 1, 64, 64, [40000], 32, 0), (128, 1, 64, 16, [300], 5, 0), (16, 8, 96, 1, [1000, 900], 50, 333)])
 def test_chunks_of_long_sequences(pkg, dtype, H, G, hs, page, lengths, chunk, window):
     """Few rows over many positions (shared by several CTAs) and many rows; sequences with holes and scores that grow."""
     g = gen(chunk)
@@ -332,6 +332,34 @@ def test_chunks_of_long_sequences(pkg, dtype, H, G, hs, page, lengths, chunk, wi
     seq = torch.cat([torch.full((min(chunk, n),), s, device="cuda") for s, n in enumerate(lengths)]).int()
     check(cache, rand(g, len(pos), H, hs, dtype=dtype), pos, tables, seq, dtype, chunk=chunk, window=window)
     check(cache, rand(g, len(pos), H, hs, dtype=dtype), pos, tables, seq, dtype, chunk=chunk, window=window, max_len=max(lengths), scale=-0.2)
+
+
+@pytest.mark.parametrize("n,chunk,out", [(300, 1, F32), (1500, 1500, F32), (700, 3, F16)])
+def test_more_rows_than_are_shared_out(pkg, n, chunk, out):
+    """Many groups of rows take a CTA a unit, whatever their lengths are; results of another 16-bit type than the cache's."""
+    g = gen(n)
+    cache, tables = paged(pkg, g, [500, 40, 1400], 16, 1, 32, BF16)
+    seq = torch.randint(-1, 3, (n,), device="cuda", generator=g).int() if chunk < n else torch.full((n,), 2, device="cuda", dtype=torch.int32)
+    pos = (torch.rand(n, device="cuda", generator=g) * ints(500, 40, 1400).float()[seq.clamp(min=0).long()]).int() if chunk < n else torch.arange(n, device="cuda").int() - 100
+    check(cache, rand(g, n, 2, 32, dtype=BF16), pos, tables, seq, out, chunk=chunk)
+
+
+def test_offsets_beyond_32_bits(pkg):
+    """A pool of 2 x 5.2 GB: entries behind 2^31 and bytes behind 2^32."""
+    g, G, hs, page, pages = gen(12), 8, 128, 256, 10000
+    cache = pkg.PagedKVCache(pages, page, G, hs, dtype=BF16)
+    tables = ints(pages - 1, 3, pages - 2).view(1, 3)
+    n = 600
+    k, v, pos = rand(g, n, G, hs, dtype=BF16), rand(g, n, G, hs, dtype=BF16), torch.arange(n, device="cuda", dtype=torch.int32)
+    cache.append(k, v, pos, tables)
+    assert torch.equal(cache.keys[pages - 1].transpose(0, 1), k[:256]) and torch.equal(cache.values[pages - 2, :, :88].transpose(0, 1), v[512:])
+    small, q = pkg.PagedKVCache(3, page, G, hs, dtype=BF16), rand(g, 64, 2 * G, hs, dtype=BF16)
+    for name in ("keys", "values"):
+        getattr(small, name).copy_(getattr(cache, name)[tables[0].long()])
+    for chunk, out in ((1, F32), (64, BF16)):
+        got = cache.attention(q, pos[-64:], tables, chunk=chunk, dtype=out)
+        assert torch.equal(got, small.attention(q, pos[-64:], ints(0, 1, 2).view(1, 3), chunk=chunk, dtype=out))
+    check(small, q, pos[-64:], ints(0, 1, 2).view(1, 3), None, F32)
 
 
 def test_a_wait_that_runs_out_is_heard_of(pkg):
@@ -412,7 +440,7 @@ def test_refusals(pkg):
            lambda: cache.append(k, k, pos.long(), tables), lambda: cache.append(k, k, pos[:2], tables), lambda: cache.append(k, k, pos, tables.long()), lambda: cache.append(k, k, pos, tables[0]),
            lambda: cache.append(k, k, pos, tables.cpu()), lambda: cache.append(k, k, pos, tables, sequences=pos[:2]), lambda: cache.append(k, k, pos, tables, cos=cos), lambda: cache.append(k, k, pos, tables, cos=cos, sin=cos[:10]),
            lambda: cache.append(k, k, pos, tables, cos=torch.ones(20, 33, device="cuda"), sin=torch.ones(20, 33, device="cuda")), lambda: cache.append(k, k, pos, tables, layout="other"), lambda: cache.append(k, k, pos, tables, q_norm=w),
-           lambda: cache.append(k, k, pos, tables, k_norm=w[:3]), lambda: cache.append(k, k, pos, tables, q=k, q_out=k), lambda: cache.append(k.transpose(1, 2), k, pos, tables), lambda: cache.append(on(k), k, pos, tables),
+           lambda: cache.append(k, k, pos, tables, k_norm=w[:3]), lambda: cache.append(k, k, pos, tables, q=k, q_out=k), lambda: cache.append(k.bfloat16(), k.bfloat16(), pos, tables, q=q, q_out=q), lambda: cache.append(k.transpose(1, 2), k, pos, tables), lambda: cache.append(on(k), k, pos, tables),
            lambda: cache.append(k, k, pos, tables, q=on(k)), lambda: cache.append(k, k, pos, tables, k_norm=on(w)), lambda: cache.attention(q.float(), pos, tables), lambda: cache.attention(q[:, :3], pos, tables),
            lambda: cache.attention(on(q), pos, tables), lambda: cache.attention(q, pos, tables, window=-1), lambda: cache.attention(q, pos, tables, dtype=torch.float64), lambda: cache.attention(q, pos, tables, out=q[:2]),
            lambda: cache.attention(q, pos, tables, chunk=-1), lambda: cache.attention(q[:, :, ::2], pos, tables), lambda: cache.attention(q, pos[::2], tables), lambda: cache.attention(q, pos, tables.repeat(2, 1).T)]

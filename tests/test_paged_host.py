@@ -55,7 +55,7 @@ def test_attention_refuses(pkg):
     L, err = pkg.native.lib(), C.create_string_buffer(256)
     good = dict(n=3, heads=4, out_type=0, q=256, out=256, q_stride=256, out_stride=256, positions=256, sequences=256, tables=256, table_stride=5, n_sequences=2, table_width=5, scale=1.0)
     for bad, code in ((dict(n=-1), -1), (dict(heads=0), -1), (dict(heads=3), -1), (dict(out_type=8), -2), (dict(window=-1), -1), (dict(max_len=-1), -1), (dict(chunk=-1), -1), (dict(workspace=8), -1), (dict(q=None), -1),
-                      (dict(out=None), -1), (dict(q_stride=255), -1), (dict(out_stride=255), -1), (dict(positions=None), -1), (dict(tables=None), -1), (dict(n=2**21 + 1), -2)):
+                      (dict(out=None), -1), (dict(q_stride=255), -1), (dict(out_stride=255), -1), (dict(positions=None), -1), (dict(tables=None), -1), (dict(n=2**25 + 1), -2)):
         a = pkg.native.PagedAttention()
         for k, v in dict(good, **bad).items():
             setattr(a, k, v)
