@@ -67,25 +67,24 @@ struct Append {
     void *q_out;
 };
 
-// Lanes of a head: 8 entries each; WIDTH lanes (a power of two) serve one head.  Mean of squares in 64 bits (FP32 squares leave FP32's range from 2^64 on).  Pairs of neighbours lie in a
+// A CTA takes a row, or some of its heads.  Lanes of a head: 8 entries each; WIDTH lanes (a power of two) serve one head.  Mean of squares in 64 bits (FP32 squares leave FP32's range from 2^64 on).  Pairs of neighbours lie in a
 // lane; pairs half the rotated part apart lie in lanes a fixed distance apart where half of it is a multiple of 8, and are read once more from memory where it is not.
 template <int HS, typename T, typename C> __global__ void __launch_bounds__(256) k_paged_append(const Append a) {
     constexpr int L = HS / 8, WIDTH = L <= 4 ? 4 : L <= 8 ? 8 : L <= 16 ? 16 : 32, PER_WARP = 32 / WIDTH;
     const int lane = threadIdx.x & 31, li = lane & (WIDTH - 1), G = a.pool.kv_heads, total = a.heads + 2 * G;
-    const long long item = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / WIDTH;
-    const int row = (int)(item / total), which = (int)(item % total);
-    int pos = -1;
-    const int seq = row < a.rows.n ? a.rows.place(row, pos) : -1;
-    const bool on = seq >= 0 && pos >= 0, mine = on && li < L;
-    if (!__any_sync(0xffffffffu, on)) return; // (a whole warp: the shuffles below take every lane)
-    const bool is_q = which < a.heads, is_v = which >= a.heads + G;
+    const int row = blockIdx.x, which = (blockIdx.y * 8 + (threadIdx.x >> 5)) * PER_WARP + lane / WIDTH;
+    const bool is_q = which < a.heads, is_v = which >= a.heads + G, there = which < total && li < L;
     const int head = is_q ? which : is_v ? which - a.heads - G : which - a.heads, e = li * 8;
-    const unsigned at = mine && !is_q ? row_at(a.pool, a.rows.table(seq), pos, head) : NO_ROW;
-    const T *src = (is_q ? (const T *)a.q + row * a.ldq : is_v ? (const T *)a.v + row * a.ldv : (const T *)a.k + row * a.ldk) + head * HS;
-    float x[8];
+    const T *src = (is_q ? (const T *)a.q + (long long)row * a.ldq : is_v ? (const T *)a.v + (long long)row * a.ldv : (const T *)a.k + (long long)row * a.ldk) + (size_t)head * HS;
+    float x[8]; // (on its way while its place is looked up)
 #pragma unroll
     for (int i = 0; i < 8; i++) x[i] = 0.0f;
-    if (mine) load8(src + e, x, a.vec);
+    if (there) load8(src + e, x, a.vec);
+    int pos = -1;
+    const int seq = a.rows.place(row, pos);
+    if (seq < 0 || pos < 0) return; // (the whole CTA)
+    const bool mine = there;
+    const unsigned at = mine && !is_q ? row_at(a.pool, a.rows.table(seq), pos, head) : NO_ROW;
     const float *norm = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
     float s = 1.0f;
     if (a.q_norm || a.k_norm) {
@@ -159,7 +158,7 @@ template <int HS, typename T, typename C> __global__ void __launch_bounds__(256)
     for (int i = 0; i < 4; i++) w[i] = pack2<C>(x[2 * i], x[2 * i + 1]);
     if (!is_q) *reinterpret_cast<uint4 *>((C *)(is_v ? a.pool.values : a.pool.keys) + (size_t)at * HS + e) = make_uint4(w[0], w[1], w[2], w[3]);
     else {
-        uint16_t *o = (uint16_t *)a.q_out + row * a.ldo + head * HS + e;
+        uint16_t *o = (uint16_t *)a.q_out + (long long)row * a.ldo + (size_t)head * HS + e;
         if (a.vec_out) *reinterpret_cast<uint4 *>(o) = make_uint4(w[0], w[1], w[2], w[3]);
         else
 #pragma unroll

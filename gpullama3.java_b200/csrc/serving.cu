@@ -65,9 +65,14 @@ PagedCut paged_cut(const b200_paged_cache &c, const b200_paged_attention_args &a
     const long long near = (long long)a.window + k.tokens;
     if (a.window > 0 && near < len) len = near;
     k.units = (size_t)groups * G * k.blocks;
-    // Shared out where a unit is worth more than two CTAs, and where a CTA finds its place quickly: it looks at all rows' positions.
-    if (len > 2LL * paged::SHARE_LEAST * KT && groups <= paged::STEP_GROUPS && a.n <= paged::STEP_SHARED_ROWS) {
-        const long long most = ((len + KT - 1) / KT + 1) * (long long)k.units / paged::SHARE_LEAST + 1, room = (long long)sms * paged::step_ctas(c.head_size, k.nr);
+    // Shared out where the rows are long enough to pay for it (about 6 us: every CTA looks at all rows' positions, the parts are joined by a kernel of their own) and the units leave room.  us of a
+    // captured call, a CTA a unit / shared out, by positions: one row of 8 heads of 128: 384: 8.3/10.1, 512: 9.7/10.8, 768: 12.8/11.0, 2048: 28.4/11.4; 8 rows of 8 heads of 64 (of room for 888 units):
+    // 768: 10.3/11.4, 1024: 12.6/11.6, 2048: 21.6/12.7; 4 rows of a head of 256: 256: 11.4/11.1, 512: 17.7/11.4; 32 rows of 8 heads of 128 (256 units where 444 have room: no two CTAs for each) all of
+    // one length: 1024: 27.5/34.7, 2048: 48.6/56.2; 24 rows of up to 4099: 74/49.
+    const long long room = (long long)sms * paged::step_ctas(c.head_size, k.nr), units = (long long)k.units;
+    const long long worth = 65536 / c.head_size * (room + 4 * units) / room * (2 * units > room ? 2 : 1);
+    if (len > worth && groups <= paged::STEP_GROUPS && a.n <= paged::STEP_SHARED_ROWS) {
+        const long long most = ((len + KT - 1) / KT + 1) * units / paged::SHARE_LEAST + 1;
         k.ctas = (int)(most < room ? most : room);
     }
     return k;
@@ -192,7 +197,7 @@ int b200_paged_append(const b200_paged_cache *c, const b200_paged_append_args *a
     if (!a->k || !a->v || (a->heads && (!a->q || !a->q_out))) return fail(B200_ERR_BAD_ARG, "null rows");
     const int64_t kv_width = (int64_t)c->kv_heads * c->head_size, q_width = (int64_t)a->heads * c->head_size;
     if (a->n > 1 && (a->k_stride < kv_width || a->v_stride < kv_width || (a->heads && (a->q_stride < q_width || a->q_out_stride < q_width)))) return fail(B200_ERR_BAD_ARG, "rows overlap: a stride is smaller than its row");
-    if ((long long)a->n * (a->heads + 2LL * c->kv_heads) > (1LL << 33)) return fail(B200_ERR_UNSUPPORTED, "too many rows in one call");
+    if (a->heads + 2LL * c->kv_heads > (1LL << 18)) return fail(B200_ERR_UNSUPPORTED, "too many heads"); // (the grid's second dimension)
     paged::Append k;
     k.pool = {c->keys, c->values, c->pages, c->kv_heads, shift_of(c->page_size)};
     k.rows = {a->positions, a->sequences, a->tables, a->table_stride, a->n, a->n_sequences, a->table_width * c->page_size};
@@ -216,8 +221,8 @@ int b200_paged_append(const b200_paged_cache *c, const b200_paged_append_args *a
             return by_type(a->type, [&](auto type) {
                 return by_cache_type(c->type, [&](auto cache) {
                     constexpr int L = hs / 8, per_warp = L <= 4 ? 8 : L <= 8 ? 4 : L <= 16 ? 2 : 1;
-                    const long long items = (long long)a->n * (a->heads + 2 * c->kv_heads);
-                    return launch(paged::k_paged_append<hs, decltype(type), decltype(cache)>, (unsigned)((items + 8 * per_warp - 1) / (8 * per_warp)), 256, 0, 1, false, (cudaStream_t)stream, k);
+                    const unsigned heads = (unsigned)(a->heads + 2 * c->kv_heads), per_cta = 8 * per_warp;
+                    return launch(paged::k_paged_append<hs, decltype(type), decltype(cache)>, dim3((unsigned)a->n, (heads + per_cta - 1) / per_cta), 256, 0, 1, false, (cudaStream_t)stream, k);
                 });
             });
         });

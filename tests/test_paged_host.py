@@ -40,7 +40,7 @@ def test_append_refuses(pkg):
     for bad, code in ((dict(n=-1), -1), (dict(heads=-1), -1), (dict(type=8), -2), (dict(rope_layout=7), -1), (dict(sin=None), -1), (dict(rope_dims=0), -1), (dict(rope_dims=66), -1), (dict(rope_dims=31), -1),
                       (dict(rope_rows=-1), -1), (dict(k=None), -1), (dict(v=None), -1), (dict(q=None), -1), (dict(q_out=None), -1), (dict(k_stride=127), -1), (dict(q_stride=255), -1), (dict(q_out_stride=0), -1),
                       (dict(positions=None), -1), (dict(tables=None), -1), (dict(table_stride=4), -1), (dict(table_width=-1), -1), (dict(n_sequences=-1), -1),
-                      (dict(table_width=2**26, table_stride=2**26), -2), (dict(n=2**30, heads=2**10, q_stride=2**17, q_out_stride=2**17), -2)):
+                      (dict(table_width=2**26, table_stride=2**26), -2), (dict(heads=2**18, q_stride=2**25, q_out_stride=2**25), -2)):
         a = pkg.native.PagedAppend()
         for k, v in dict(good, **bad).items():
             setattr(a, k, v)
