@@ -69,6 +69,8 @@ struct Append {
 
 // A CTA takes a row, or some of its heads.  Lanes of a head: 8 entries each; WIDTH lanes (a power of two) serve one head.  Mean of squares in 64 bits (FP32 squares leave FP32's range from 2^64 on).  Pairs of neighbours lie in a
 // lane; pairs half the rotated part apart lie in lanes a fixed distance apart where half of it is a multiple of 8, and are read once more from memory where it is not.
+// Bytes are its floor: 512 rows of (32 + 2 * 8) heads of 128 in BF16 read and write 12.8 MB, 2.0 us; in a captured graph it takes 7.3 (10.2 as a call), a step's row 2.4: latency, a chain of loads (position, then
+// page and angles) and 64-bit sums; a warp's index by division of a flat one was 1.2 us more.
 template <int HS, typename T, typename C> __global__ void __launch_bounds__(256) k_paged_append(const Append a) {
     constexpr int L = HS / 8, WIDTH = L <= 4 ? 4 : L <= 8 ? 8 : L <= 16 ? 16 : 32, PER_WARP = 32 / WIDTH;
     const int lane = threadIdx.x & 31, li = lane & (WIDTH - 1), G = a.pool.kv_heads, total = a.heads + 2 * G;
@@ -374,6 +376,10 @@ template <int KT, bool LONE, int THREADS> __device__ __forceinline__ void share_
 // p reaches down to 2^-24 of 2^-15: a long tail of small ones still counts.
 // A value that is infinite or NaN would reach every row of the block as 0 * NaN, also those that do not see it, and sums of large BF16 values may leave FP32's range before they are divided: a
 // warp whose sums are not finite computes its share once more at the end, a row after the other in FP32, from what each sees, 2^-40 below its maximum (slow_rows).
+// Bytes are its floor.  One row of 8 key/value heads of 128 over 131071 positions, 537 MB: 84-85 us (6.3 TB/s; floor 83), with the join 88 in a graph; 48 rows of up to 4099 positions of 8 heads of 64, 206 MB: 45
+// (floor 32), with the join 47; 16 sequences of 5 drafted tokens, 20 rows, over up to 8191 positions, 285 MB: 62 (floor 44), with the join 67, where the chains of products of six warps an SM (tensor pipes 22 %)
+// keep the copies from running ahead.  What a CTA holds was measured on these three: two warps with two tiles of 32 positions each; tiles of 16 with three places: 91, 47, 61-66; four warps: 90, 53-56, 62; products with
+// positions as columns (16 rows at least): 90, 46, 86.  An even share of all tiles for every CTA, whichever units they are of, was slower (88, 53, 72): a second unit costs a CTA another 5 us.
 template <int HS, typename T> __device__ __noinline__ void slow_rows(const Step &a, const unsigned char *sQ, int rows, int row0, int token0, int kvh, int first, int last, int warp, const Segment *segments, const int *segment_of,
                                                                      const int *pos_of, float factor, float *parts, float *wref, float *wsum) {
     constexpr int KT = step_keys(HS), E = HS / 32; // entries of a lane

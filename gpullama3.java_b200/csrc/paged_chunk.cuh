@@ -10,6 +10,9 @@
 // largest are kept.
 // A row whose sums are not finite (a value that is infinite or NaN reaches every row of the tile as 0 * NaN, also those that do not see it; sums of large BF16 values) is computed once more at
 // the end, by the whole CTA in FP32, from what it sees.
+// Measured (512 tokens of 32 heads over 8 of 128, 8192 positions, 66.6 GFLOP, pages of 64): 90 us in a graph, 740 TFLOP/s, 45 % of the 1647 measured; floor 40.  128 CTAs leave 20 SMs idle.  Of a tile's 2300 cycles the
+// products take 1490 to issue (1024 alone): their operands and the copies of the next tiles share the bandwidth of shared memory; exponentials keep their unit busy in 44 % of the cycles.  One group of warps for a
+// tile's keys and values one after the other 100-102 us, a warp a place 104, two 100; what a row sees as bits in place of comparisons 92 (and 31 -> 22 us for three chunks of 111 tokens through a window of 500).
 // Every wait is bounded: after half a second the CTA gives up, waits for its products under way, frees its tensor memory and writes NaN for its rows.
 #pragma once
 #include "kv4_chunk.cuh"

@@ -79,7 +79,9 @@ PagedCut paged_cut(const b200_paged_cache &c, const b200_paged_attention_args &a
 }
 size_t paged_cut_bytes(const b200_paged_cache &c, const PagedCut &k) { return k.ctas ? (k.ctas + k.units) * 8 * k.nr * (c.head_size + 2) * 4 + (paged::STEP_GROUPS + 1) * 4 : 0; } // (paged::shared_grid)
 
-// Chunks on the tensor cores: 16-bit results, heads of 64, 96 or 128.  A tile takes 128 rows whether they are used or not.
+// Chunks on tcgen05: 16-bit results, heads of 64, 96 or 128.  A tile takes 128 rows whether they are used or not.  us of a captured call in groups of 32 rows / as a chunk, by rows: 32/8 heads of 128, 8192
+// positions: 64: 30.5/23.4, 128: 41.6/25.9, 512: 119/35; 1024 positions: 64: 22.9/19.3, 512: 33.5/20.9; 32/8 of 64, 8192: 64: 21.3/19.0; 16/16 of 64, 4096: 64: 23.9/18.7; 8/1 of 128, 8192: 64: 21.0/22.5,
+// 128: 21.6/25.2, 512: 30.1/25.5 (the rule looks at a key/value head's rows alone: a few rows of a single head lose up to 4 us).
 const int CHUNK_MIN_ROWS = 64;
 struct PagedChunkCut {
     int tokens, splits;

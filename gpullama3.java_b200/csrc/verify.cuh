@@ -8,6 +8,10 @@
 // k_verify_rows reads every row once: a CTA a stretch of it, its largest entry and the sum of exp((x - largest) / T) in FP32.  k_verify_token, a cluster a sequence, joins them, decides, and
 // draws the token: that is a whole number which one more bit would change where u falls near a border, and a vocabulary has 10^5 of them, so the drawn row's weights and their sums are in
 // 64 bits; and where FP32's error could turn a decision, its row's sum is taken once more in 64 bits.
+// Where the token comes from max(p - q, 0), one pass takes both rows' sums and, on either side of which p / sum_p > q / sum_q by FP32's sums, those of the entries that weigh more in p: their difference is the
+// weight, whatever the sums come out as (a pass for the sums and one for the weights took 70 us in place of 37).
+// Bytes are the floor: 32 sequences of 5 drafts and 128256 FP32 logits of two models are 181 MB, 28 us; the call takes 53 (51 in a graph): the rows 23 (less is read where drafts are missing), the tokens 27-37, of
+// which a pass over two rows in 64 bits is 18: two exponentials an entry, 64-bit units at 23 % on average, their chains and the loads in between on the clusters that have one.  One sequence: 16.5, latency.
 // Nothing depends on an order of arrival.
 #pragma once
 #include "kv4.cuh"
@@ -53,7 +57,7 @@ __device__ __forceinline__ int given(const Args &a, int s, int most) {
     return most;
 }
 
-// A stretch is read whole into registers: largest entry, then the sum.  FP32: an exponential's argument is off by at most 2^-24 of itself, so a row's sum by sum p |log2 p| 2^-24 and 2^-20 for
+// A stretch is read whole into registers, so that all of its loads are under way at once: largest entry, then the sum.  FP32: an exponential's argument is off by at most 2^-24 of itself, so a row's sum by sum p |log2 p| 2^-24 and 2^-20 for
 // the exponentials and the order of the sum: 3e-6 at most.
 template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 5) k_verify_rows(const Args a) {
     constexpr int VEC = Load<T>::VEC;
