@@ -197,7 +197,7 @@ __host__ __device__ constexpr size_t step_smem_bytes(int hs, int nr) {
     return (ring > parts ? ring : parts) + (size_t)step_rows(nr) * hs * 2;
 }
 __host__ __device__ constexpr int step_ctas(int hs, int nr) { // of an SM, as far as its shared memory and registers go
-    const int n = (int)(233472 / (step_smem_bytes(hs, nr) + 3072)), most = hs <= 64 && nr >= 3 ? 4 : 8;
+    const int n = (int)(233472 / (step_smem_bytes(hs, nr) + 3 * 1024)), most = hs <= 64 && nr >= 3 ? 4 : 8;
     return n < 1 ? 1 : n > most ? most : n;
 }
 

@@ -9,7 +9,7 @@
 // draws the token: that is a whole number which one more bit would change where u falls near a border, and a vocabulary has 10^5 of them, so the drawn row's weights and their sums are in
 // 64 bits; and where FP32's error could turn a decision, its row's sum is taken once more in 64 bits.
 // Where the token comes from max(p - q, 0), one pass takes both rows' sums and, on either side of which p / sum_p > q / sum_q by FP32's sums, those of the entries that weigh more in p: their difference is the
-// weight, whatever the sums come out as (a pass for the sums and one for the weights took 70 us in place of 37).
+// weight, whatever the sums come out as (entries that weigh the same to 2^-40 weigh nothing; a pass for the sums and one for the weights took 70 us in place of 37).
 // Bytes are the floor: 32 sequences of 5 drafts and 128256 FP32 logits of two models are 181 MB, 28 us; the call takes 53 (51 in a graph): the rows 23 (less is read where drafts are missing), the tokens 27-37, of
 // which a pass over two rows in 64 bits is 18: two exponentials an entry, 64-bit units at 23 % on average, their chains and the loads in between on the clusters that have one.  One sequence: 16.5, latency.
 // Nothing depends on an order of arrival.
@@ -187,6 +187,7 @@ template <typename T> __device__ __forceinline__ float4 load4(const T *x) {
 }
 // exp((x - top) / T) for x <= top, within 4e-15 of itself: 2^(k / 32) from a table, the rest, at most ln(2) / 64, by its series (P. T. P. Tang's table-driven exponential, 1989); below -690 it is 0.
 constexpr int EXP_TABLE = 32;
+constexpr double EVEN = 1.0 + 0x1p-40; // weights that agree to 2^-40 are the same: the sums' last bits are not drawn from
 struct Weight {
     const unsigned (*table)[EXP_TABLE]; // low, high words of 2^(i / 32): 32 banks each, no conflicts
     double scale;                       // 32 log2(e) / T
@@ -198,7 +199,7 @@ struct Weight {
         const double p = fma(fma(fma(fma(fma(A * A * A * A * A / 120.0, r, A * A * A * A / 24.0), r, A * A * A / 6.0), r, A * A / 2.0), r, A), r, 1.0) *
                          __hiloint2double((int)table[1][k & (EXP_TABLE - 1)], (int)table[0][k & (EXP_TABLE - 1)]);
         const bool some = x >= top - reach;
-        return __hiloint2double(some ? __double2hiint(p) + (k >> 5 << 20) : 0, some ? __double2loint(p) : 0);
+        return __hiloint2double(some ? __double2hiint(p) + (k >> 5) * (1 << 20) : 0, some ? __double2loint(p) : 0);
     }
 };
 
@@ -305,7 +306,7 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
                 const auto also = [&](double p, float yi) {
                     const double q = weight(yi, top_q);
                     part[1] += q;
-                    const bool more = p * by_p > q * by_q;
+                    const bool more = p * by_p > q * by_q * EVEN;
                     part[2] += more ? p : 0.0;
                     part[3] += more ? q : 0.0;
                 };
@@ -376,18 +377,20 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
     const float top_p = rows[n].top, top_q = differ ? of_draft(n).top : 0.0f;
     const auto one = [&](int j) -> double {
         const double p = j == without ? 0.0 : weight(Load<T>::one(x + j), top_p);
-        return differ ? fmax(p * by_p - weight(Load<T>::one(y + j), top_q) * by_q, 0.0) : p;
+        if (!differ) return p;
+        const double v = p * by_p, w = weight(Load<T>::one(y + j), top_q) * by_q;
+        return v > w * EVEN ? v - w : 0.0;
     };
     double total = 0.0;
     for (int r = 0; r < CLUSTER; r++) total += cta_weight(r);
-    const double border = (double)u[a.drafts] * total;
+    const double border = (double)u[a.drafts] * total, least = differ ? total * 1e-13 : 0.0; // (what rounding leaves of a share where both weigh the same)
     double before = 0.0, sum = 0.0;
     int chosen = -1;
     for (int r = 0; r < CLUSTER; r++) {
         const double w = cta_weight(r);
-        if (w > 0.0) { chosen = r; before = sum; }
+        if (w > least) { chosen = r; before = sum; }
         sum += w;
-        if (w > 0.0 && sum > border) break;
+        if (w > least && sum > border) break;
     }
     if (chosen != rank) return; // (the others are done: nothing of theirs is read any more)
     int w_chosen = 0;
@@ -395,9 +398,9 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
     sum = before;
     for (int w = 0; w < TOKEN_WARPS; w++) {
         const double v = warp_weight(w);
-        if (v > 0.0) { w_chosen = w; at = sum; }
+        if (v > least / TOKEN_WARPS) { w_chosen = w; at = sum; }
         sum += v;
-        if (v > 0.0 && sum > border) break;
+        if (v > least / TOKEN_WARPS && sum > border) break;
     }
     const int begin = begin_of(rank * TOKEN_WARPS + w_chosen), end = begin_of(rank * TOKEN_WARPS + w_chosen + 1);
     int last = -1; // this thread's last entry that weighs anything
@@ -432,6 +435,20 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
         __syncthreads();
         atomicMax(&found, last);
         __syncthreads();
+        if (found < 0) { // (a share of nothing but rounding: the last entry of the row that weighs anything, or its largest)
+            for (int j = tid; j < a.vocab; j += TOKEN_THREADS)
+                if (one(j) > 0.0) last = j;
+            __syncthreads();
+            atomicMax(&found, last);
+            __syncthreads();
+            if (found < 0) {
+                for (int j = tid; j < a.vocab; j += TOKEN_THREADS)
+                    if (Load<T>::one(x + j) == top_p) last = j;
+                __syncthreads();
+                atomicMax(&found, last);
+                __syncthreads();
+            }
+        }
     }
     if (tid == 0) a.out_tokens[(long long)s * (a.drafts + 1) + n] = found;
 }

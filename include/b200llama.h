@@ -653,7 +653,8 @@ int b200_test_paged_give_up(const b200_paged_cache *cache, const b200_paged_atte
  * behind them, then -1.  The token is the first index whose running sum of weights passes uniforms[drafts] times their sum; weights: p_n where no draft was left, else
  * max(p_n - q_n, 0) (without draft_logits p_n without the draft; p_n where that is all 0).  So the tokens are distributed as the target's own samples.  temperature 0 (else 1e-4 to 1e4): a draft is
  * accepted where it is its row's largest logit (the first of equal ones), the token is that of its row; uniforms and draft_logits are not read.  A row reached that has no distribution
- * (a NaN, an infinite logit or none above -inf) ends its sequence: its draft is not accepted, the token is -1.  Running sums of the drawn row, and decisions that FP32 cannot make, are in 64 bits.
+ * (a NaN, an infinite logit or none above -inf) ends its sequence: its draft is not accepted, the token is -1.  Running sums of the drawn row, and decisions that FP32 cannot make, are in 64 bits;
+ * a weight below e^-690 of its row's largest is 0, and so is a difference of weights that agree to 2^-40.
  * The workspace: b200_verify_drafts_workspace(args) bytes, 16-byte aligned, content does not matter, of no other call under way.  At most 64 drafts, 2^24 logits, 2^16 sequences. */
 typedef struct b200_verify_drafts_args {
     const void *logits, *draft_logits;

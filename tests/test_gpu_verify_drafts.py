@@ -112,6 +112,20 @@ def test_draft_that_its_model_cannot_have_made(pkg):
     assert accepted.tolist() == [1, 0] and tokens[1, 0] != 5
 
 
+@pytest.mark.parametrize("u", [0.0, 0.3, 1 - 2.0 ** -24])
+@pytest.mark.parametrize("V", [300, 40000])
+def test_entries_that_weigh_the_same_are_not_drawn(pkg, V, u):
+    """Two logits exchanged: the same sums, and all that is left over lies on one token, wherever the border falls."""
+    g = gen(V)
+    for low, high in ((V - 1, 0), (0, V - 1), (V // 2, V // 3), (5, 6)):
+        x = torch.randn(1, 2, V, device="cuda", generator=g)
+        x[0, 0, low], x[0, 0, high] = 1.0, 6.0
+        y = x[:, :1].clone()
+        y[0, 0, low], y[0, 0, high] = 6.0, 1.0
+        tokens, accepted = pkg.verify_drafts(x, torch.tensor([[low]], device="cuda", dtype=torch.int32), torch.tensor([[0.9, u]], device="cuda"), draft_logits=y)
+        assert accepted.item() == 0 and tokens.tolist() == [[high, -1]]
+
+
 @pytest.mark.parametrize("bad", ["nan", "inf", "empty"])
 @pytest.mark.parametrize("temperature", [1.0, 0.0])
 def test_rows_without_a_distribution(pkg, bad, temperature):
