@@ -189,15 +189,18 @@ template <typename T> __device__ __forceinline__ float4 load4(const T *x) {
 constexpr int EXP_TABLE = 32;
 constexpr double EVEN = 1.0 + 0x1p-40; // weights that agree to 2^-40 are the same: the sums' last bits are not drawn from
 struct Weight {
-    const unsigned (*table)[EXP_TABLE]; // low, high words of 2^(i / 32): 32 banks each, no conflicts
-    double scale;                       // 32 log2(e) / T
-    float reach;                        // 690 T
+    uint32_t table; // in shared memory: low, then high words of 2^(i / 32): 32 banks each, no conflicts
+    float reach;    // 690 T
+    double scale;   // 32 log2(e) / T
     __device__ __forceinline__ double operator()(float x, float top) const {
         constexpr double MAGIC = 6755399441055744.0, A = 0.693147180559945309417232 / EXP_TABLE; // 1.5 * 2^52: its last bits are those of the whole number added
         const double u = ((double)x - (double)top) * scale, d = u + MAGIC, r = u - (d - MAGIC);
         const int k = __double2loint(d);
-        const double p = fma(fma(fma(fma(fma(A * A * A * A * A / 120.0, r, A * A * A * A / 24.0), r, A * A * A / 6.0), r, A * A / 2.0), r, A), r, 1.0) *
-                         __hiloint2double((int)table[1][k & (EXP_TABLE - 1)], (int)table[0][k & (EXP_TABLE - 1)]);
+        int lo, hi;
+        const uint32_t at = table + (k & (EXP_TABLE - 1)) * 4;
+        asm("ld.shared.b32 %0, [%1];" : "=r"(lo) : "r"(at));
+        asm("ld.shared.b32 %0, [%1 + 128];" : "=r"(hi) : "r"(at));
+        const double p = fma(fma(fma(fma(fma(A * A * A * A * A / 120.0, r, A * A * A * A / 24.0), r, A * A * A / 6.0), r, A * A / 2.0), r, A), r, 1.0) * __hiloint2double(hi, lo);
         const bool some = x >= top - reach;
         return __hiloint2double(some ? __double2hiint(p) + (k >> 5) * (1 << 20) : 0, some ? __double2loint(p) : 0);
     }
@@ -221,7 +224,7 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
     const int *d = a.tokens + (long long)s * a.drafts;
     const float *u = a.uniforms + (long long)s * (a.drafts + 1);
     const int both = a.both;
-    const Weight weight = {table, EXP_TABLE * 1.44269504088896340736 / (double)a.temperature, 690.0f * a.temperature};
+    const Weight weight = {(uint32_t)__cvta_generic_to_shared(table), 690.0f * a.temperature, EXP_TABLE * 1.44269504088896340736 / (double)a.temperature};
     const auto target = [&](int i) { return (const T *)a.logits + s * a.ld_s + i * a.ld_r; };
     const auto draft = [&](int i) { return (const T *)a.draft_logits + s * a.draft_ld_s + i * a.draft_ld_r; };
     cluster.sync(); // every CTA is there before another writes into its memory
@@ -270,7 +273,7 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
             sum_p = rows[n].sum;
             sum_q = two ? of_draft(n).sum : 1.0;
         }
-        const double by_p = 1.0 / sum_p, by_q = 1.0 / sum_q;
+        const double edge = sum_p / sum_q * EVEN; // p / sum_p > q / sum_q where p > q edge
         double part[SUMS] = {0.0, 0.0, 0.0, 0.0};
         const int begin = begin_of(rank * TOKEN_WARPS + warp), end = begin_of(rank * TOKEN_WARPS + warp + 1);
         const float nothing = -CUDART_INF_F;
@@ -306,7 +309,7 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
                 const auto also = [&](double p, float yi) {
                     const double q = weight(yi, top_q);
                     part[1] += q;
-                    const bool more = p * by_p > q * by_q * EVEN;
+                    const bool more = p > q * edge;
                     part[2] += more ? p : 0.0;
                     part[3] += more ? q : 0.0;
                 };
