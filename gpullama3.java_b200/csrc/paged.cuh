@@ -69,7 +69,7 @@ struct Append {
 
 // A CTA takes a row, or some of its heads.  Lanes of a head: 8 entries each; WIDTH lanes (a power of two) serve one head.  Mean of squares in 64 bits (FP32 squares leave FP32's range from 2^64 on).  Pairs of neighbours lie in a
 // lane; pairs half the rotated part apart lie in lanes a fixed distance apart where half of it is a multiple of 8, and are read once more from memory where it is not.
-// Bytes are its floor: 512 rows of (32 + 2 * 8) heads of 128 in BF16 read and write 12.8 MB, 2.0 us; in a captured graph it takes 7.3 (10.2 as a call), a step's row 2.4: latency, a chain of loads (position, then
+// Bytes are its floor: 512 rows of (32 + 2 * 8) heads of 128 in BF16 read and write 12.8 MB, 2.0 us; in a captured graph it takes 7.4 (8.2 as a call), a step's row 2.4: latency, a chain of loads (position, then
 // page and angles) and 64-bit sums; a warp's index by division of a flat one was 1.2 us more.
 template <int HS, typename T, typename C> __global__ void __launch_bounds__(256) k_paged_append(const Append a) {
     constexpr int L = HS / 8, WIDTH = L <= 4 ? 4 : L <= 8 ? 8 : L <= 16 ? 16 : 32, PER_WARP = 32 / WIDTH;
@@ -732,7 +732,12 @@ template <int HS, typename T, int NR, int PARTS, bool LONE> __global__ void __la
                     }
                 }
 #pragma unroll
-        for (int i = 0; i < HS / 16; i++)
+        for (int i = 0; i < HS / 16; i++) {
+            // The products cut what they add to their sums.  With FP32 results a tile's are made from zero and added as FP32 numbers are, so that a long row's sums do not drift.
+            float tile_o[NR][4];
+            if constexpr (PARTS > 1)
+#pragma unroll
+                for (int n = 0; n < NR; n++) tile_o[n][0] = tile_o[n][1] = tile_o[n][2] = tile_o[n][3] = 0.0f;
 #pragma unroll
             for (int b = 0; b < KB; b++) {
                 uint32_t va[4];
@@ -740,8 +745,14 @@ template <int HS, typename T, int NR, int PARTS, bool LONE> __global__ void __la
 #pragma unroll
                 for (int n = 0; n < NR; n++)
 #pragma unroll
-                    for (int c = 0; c < PARTS; c++) mma<T>(o[n][i], va, pp[c][n][b][0], pp[c][n][b][1]);
+                    for (int c = 0; c < PARTS; c++) mma<T>(PARTS > 1 ? tile_o[n] : o[n][i], va, pp[c][n][b][0], pp[c][n][b][1]);
             }
+            if constexpr (PARTS > 1)
+#pragma unroll
+                for (int n = 0; n < NR; n++)
+#pragma unroll
+                    for (int u = 0; u < 4; u++) o[n][i][u] += tile_o[n][u];
+        }
         if (++stage == S) stage = 0;
     }
     cp_wait<0>();

@@ -70,7 +70,7 @@ PagedCut paged_cut(const b200_paged_cache &c, const b200_paged_attention_args &a
     // 768: 10.3/11.4, 1024: 12.6/11.6, 2048: 21.6/12.7; 4 rows of a head of 256: 256: 11.4/11.1, 512: 17.7/11.4; 32 rows of 8 heads of 128 (256 units where 444 have room: no two CTAs for each) all of
     // one length: 1024: 27.5/34.7, 2048: 48.6/56.2; 24 rows of up to 4099: 74/49.
     const long long room = (long long)sms * paged::step_ctas(c.head_size, k.nr), units = (long long)k.units;
-    const long long worth = 65536 / c.head_size * (room + 4 * units) / room * (2 * units > room ? 2 : 1);
+    const long long worth = (k.nr > 2 ? 10 : 20) * KT * (room + 4 * units) / room * (2 * units > room ? 2 : 1); // (a tile is latency, whatever the head's size)
     if (len > worth && groups <= paged::STEP_GROUPS && a.n <= paged::STEP_SHARED_ROWS) {
         const long long most = ((len + KT - 1) / KT + 1) * units / paged::SHARE_LEAST + 1;
         k.ctas = (int)(most < room ? most : room);

@@ -10,8 +10,8 @@
 // 64 bits; and where FP32's error could turn a decision, its row's sum is taken once more in 64 bits.
 // Where the token comes from max(p - q, 0), one pass takes both rows' sums and, on either side of which p / sum_p > q / sum_q by FP32's sums, those of the entries that weigh more in p: their difference is the
 // weight, whatever the sums come out as (entries that weigh the same to 2^-40 weigh nothing; a pass for the sums and one for the weights took 70 us in place of 37).
-// Bytes are the floor: 32 sequences of 5 drafts and 128256 FP32 logits of two models are 181 MB, 28 us; the call takes 53 (51 in a graph): the rows 23 (less is read where drafts are missing), the tokens 27-37, of
-// which a pass over two rows in 64 bits is 18: two exponentials an entry, 64-bit units at 23 % on average, their chains and the loads in between on the clusters that have one.  One sequence: 16.5, latency.
+// Bytes are the floor: 32 sequences of 5 drafts and 128256 FP32 logits of two models are 181 MB, 28 us; the call takes 51 (48 in a graph): the rows 23 (less is read where drafts are missing), the tokens 24-34, of
+// which a pass over two rows in 64 bits is 18: two exponentials an entry, 64-bit units at 23 % on average, their chains and the loads in between on the clusters that have one.  One sequence: 15.5 in a graph, latency.
 // Nothing depends on an order of arrival.
 #pragma once
 #include "kv4.cuh"
