@@ -264,6 +264,13 @@ int b200_test_paged_give_up(const b200_paged_cache *c, const b200_paged_attentio
     return paged_attention(c, a, stream, err, err_len, true);
 }
 
+int b200_test_verify_weights(const float *x, int32_t n, float top, float temperature, double *weights) {
+    if (n < 0 || (n && (!x || !weights)) || !(temperature >= 1e-4f && temperature <= 1e4f)) return B200_ERR_BAD_ARG;
+    const double scale = verify::exp_scale(temperature);
+    for (int32_t i = 0; i < n; i++) weights[i] = verify::exp_of(x[i], top, scale, [](int k) { return exp2((double)k / verify::EXP_TABLE); });
+    return B200_OK;
+}
+
 size_t b200_verify_drafts_workspace(const b200_verify_drafts_args *a) {
     if (!a || a->sequences <= 0 || a->drafts < 0 || a->vocab <= 0) return 0;
     const size_t rows = (size_t)a->sequences * (a->drafts + 1) + (a->draft_logits && a->temperature != 0.0f ? (size_t)a->sequences * a->drafts : 0);

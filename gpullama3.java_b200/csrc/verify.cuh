@@ -17,6 +17,8 @@
 #include "kv4.cuh"
 #include "logprobs.cuh"
 
+#include <string.h>
+
 namespace verify {
 
 namespace cg = cooperative_groups;
@@ -185,24 +187,60 @@ template <typename T> __device__ __forceinline__ float4 load4(const T *x) {
     const float2 a = kv4::to_f32x2(w.x, x), b = kv4::to_f32x2(w.y, x);
     return make_float4(a.x, a.y, b.x, b.y);
 }
-// exp((x - top) / T) for x <= top, within 4e-15 of itself: 2^(k / 32) from a table, the rest, at most ln(2) / 64, by its series (P. T. P. Tang's table-driven exponential, 1989); below -690 it is 0.
+// exp((x - top) / T) for x <= top: 2^(k / 32) from a table, the rest, at most ln(2) / 64, by its series (P. T. P. Tang's table-driven exponential, 1989).  Below e^-690 it is 0, and whether it is is told by the
+// 64-bit argument: x and top may be as large against T as they like (top - 690 T in FP32 would round to the neighbour of top, and let arguments in whose exponents leave the double's field).
 constexpr int EXP_TABLE = 32;
-constexpr double EVEN = 1.0 + 0x1p-40; // weights that agree to 2^-40 are the same: the sums' last bits are not drawn from
+constexpr double LOG2E_64 = 1.44269504088896340736, EVEN = 1.0 + 0x1p-40; // weights that agree to 2^-40 are the same: the sums' last bits are not drawn from
+constexpr uint32_t REACH = 0x40df1badu;                                    // high word of 690 * 32 log2(e) = 31854.7
+__host__ __device__ __forceinline__ uint32_t high_word(double v) {
+#ifdef __CUDA_ARCH__
+    return (uint32_t)__double2hiint(v);
+#else
+    uint64_t b;
+    memcpy(&b, &v, 8);
+    return (uint32_t)(b >> 32);
+#endif
+}
+__host__ __device__ __forceinline__ uint32_t low_word(double v) {
+#ifdef __CUDA_ARCH__
+    return (uint32_t)__double2loint(v);
+#else
+    uint64_t b;
+    memcpy(&b, &v, 8);
+    return (uint32_t)b;
+#endif
+}
+__host__ __device__ __forceinline__ double of_words(uint32_t high, uint32_t low) {
+#ifdef __CUDA_ARCH__
+    return __hiloint2double((int)high, (int)low);
+#else
+    const uint64_t b = (uint64_t)high << 32 | low;
+    double v;
+    memcpy(&v, &b, 8);
+    return v;
+#endif
+}
+__host__ __device__ inline double exp_scale(float temperature) { return EXP_TABLE * LOG2E_64 / (double)temperature; }
+// table(i): 2^(i / 32); also on the host, where tests look at it
+template <typename F> __host__ __device__ __forceinline__ double exp_of(float x, float top, double scale, F table) {
+    constexpr double MAGIC = 6755399441055744.0, A = 0.693147180559945309417232 / EXP_TABLE; // 1.5 * 2^52: its last bits are those of the whole number added
+    const double u = ((double)x - (double)top) * scale, d = u + MAGIC, r = u - (d - MAGIC);
+    const uint32_t k = low_word(d);
+    const double p = fma(fma(fma(fma(fma(A * A * A * A * A / 120.0, r, A * A * A * A / 24.0), r, A * A * A / 6.0), r, A * A / 2.0), r, A), r, 1.0) * table((int)(k & (EXP_TABLE - 1)));
+    const bool some = (high_word(u) & 0x7fffffffu) <= REACH; // (not -inf)
+    return of_words(some ? high_word(p) + ((uint32_t)((int)k >> 5) << 20) : 0u, some ? low_word(p) : 0u);
+}
 struct Weight {
     uint32_t table; // in shared memory: low, then high words of 2^(i / 32): 32 banks each, no conflicts
-    float reach;    // 690 T
     double scale;   // 32 log2(e) / T
     __device__ __forceinline__ double operator()(float x, float top) const {
-        constexpr double MAGIC = 6755399441055744.0, A = 0.693147180559945309417232 / EXP_TABLE; // 1.5 * 2^52: its last bits are those of the whole number added
-        const double u = ((double)x - (double)top) * scale, d = u + MAGIC, r = u - (d - MAGIC);
-        const int k = __double2loint(d);
-        int lo, hi;
-        const uint32_t at = table + (k & (EXP_TABLE - 1)) * 4;
-        asm("ld.shared.b32 %0, [%1];" : "=r"(lo) : "r"(at));
-        asm("ld.shared.b32 %0, [%1 + 128];" : "=r"(hi) : "r"(at));
-        const double p = fma(fma(fma(fma(fma(A * A * A * A * A / 120.0, r, A * A * A * A / 24.0), r, A * A * A / 6.0), r, A * A / 2.0), r, A), r, 1.0) * __hiloint2double(hi, lo);
-        const bool some = x >= top - reach;
-        return __hiloint2double(some ? __double2hiint(p) + (k >> 5) * (1 << 20) : 0, some ? __double2loint(p) : 0);
+        return exp_of(x, top, scale, [&](int i) {
+            uint32_t lo, hi;
+            const uint32_t at = table + i * 4;
+            asm("ld.shared.b32 %0, [%1];" : "=r"(lo) : "r"(at));
+            asm("ld.shared.b32 %0, [%1 + 128];" : "=r"(hi) : "r"(at));
+            return of_words(hi, lo);
+        });
     }
 };
 
@@ -224,7 +262,7 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
     const int *d = a.tokens + (long long)s * a.drafts;
     const float *u = a.uniforms + (long long)s * (a.drafts + 1);
     const int both = a.both;
-    const Weight weight = {(uint32_t)__cvta_generic_to_shared(table), 690.0f * a.temperature, EXP_TABLE * 1.44269504088896340736 / (double)a.temperature};
+    const Weight weight = {(uint32_t)__cvta_generic_to_shared(table), exp_scale(a.temperature)};
     const auto target = [&](int i) { return (const T *)a.logits + s * a.ld_s + i * a.ld_r; };
     const auto draft = [&](int i) { return (const T *)a.draft_logits + s * a.draft_ld_s + i * a.draft_ld_r; };
     cluster.sync(); // every CTA is there before another writes into its memory

@@ -670,6 +670,9 @@ typedef struct b200_verify_drafts_args {
 size_t b200_verify_drafts_workspace(const b200_verify_drafts_args *args);
 int b200_verify_drafts(const b200_verify_drafts_args *args, void *stream, char *err, size_t err_len);
 
+/* Test hook, on the host: the 64-bit weights exp((x - top) / temperature) of n logits x <= top, as the verification has them. */
+int b200_test_verify_weights(const float *x, int32_t n, float top, float temperature, double *weights);
+
 /* Number of kernels one decode step launches (bench.py's gpu_launches). */
 int b200_launches_per_decode(b200_plan *plan);
 

@@ -1,0 +1,42 @@
+"""The arithmetic of the verification of drafted tokens that decides whether it is right and whether it ends, on the host."""
+import ctypes as C
+import math
+from decimal import Decimal, localcontext
+
+import numpy as np
+import pytest
+
+
+def weights(pkg, x, top, temperature):
+    x = np.asarray(x, dtype=np.float32)
+    out = np.empty(len(x))
+    rc = pkg.native.lib().b200_test_verify_weights(x.ctypes.data_as(C.POINTER(C.c_float)), len(x), C.c_float(top), C.c_float(temperature), out.ctypes.data_as(C.POINTER(C.c_double)))
+    assert rc == 0
+    return out
+
+
+def exact(x, top, temperature):
+    with localcontext() as c:
+        c.prec = 60
+        return ((Decimal(float(np.float32(x))) - Decimal(float(np.float32(top)))) / Decimal(float(np.float32(temperature)))).exp()
+
+
+@pytest.mark.parametrize("temperature", [1e-4, 1e-3, 0.7, 1.0, 1e4])
+@pytest.mark.parametrize("top", [0.0, 1.0, -3.5, 81920.0, 1048577.0, 1.5e6, 1e7, 6e9, 1e10, -1e10, 2.7e9, 1e20, -1e30, 3e38])
+def test_weights_of_neighbours_of_large_logits(pkg, top, temperature):
+    """A row's logits may be so far from 0 that neighbouring numbers are hundreds of temperatures apart: weights are e^-(distance), or 0 where that is below e^-690, never anything else.
+
+    690 is told to 2^-20 of itself (the high word of a 64-bit number), so e^-690 to 690 * 2^-20 < 7e-4 of itself."""
+    x = [np.float32(top)]
+    for _ in range(40):
+        x.append(np.nextafter(x[-1], np.float32(-np.inf)))
+    x += [np.float32(top - d * temperature) for d in (1, 50, 500, 689, 689.9, 690.1, 691, 700, 710, 1000, 1380, 2000, 1e5, 1e30)] + [np.float32(-np.inf), np.float32(-3.4e38)]
+    x = [v for v in x if v <= np.float32(top)]
+    got = weights(pkg, x, top, temperature)
+    assert got[0] == 1.0
+    for v, w in zip(x, got):
+        far = (float(np.float32(top)) - float(v)) / float(np.float32(temperature))
+        if far > 690.001:
+            assert w == 0.0, (float(v), w)
+        else:
+            assert far > 689.999 and w == 0.0 or abs(Decimal(float(w)) / exact(v, top, temperature) - 1) <= Decimal(1e-12), (float(v), w)
