@@ -271,6 +271,11 @@ int b200_test_verify_weights(const float *x, int32_t n, float top, float tempera
     return B200_OK;
 }
 
+int b200_test_verify_next(int32_t kind, const double *sums, double *rows) {
+    if (kind < verify::TARGET || kind > verify::WHOLE || !sums || !rows) return B200_ERR_BAD_ARG;
+    return verify::after_pass(kind, sums, rows[0], rows[1]);
+}
+
 size_t b200_verify_drafts_workspace(const b200_verify_drafts_args *a) {
     if (!a || a->sequences <= 0 || a->drafts < 0 || a->vocab <= 0) return 0;
     const size_t rows = (size_t)a->sequences * (a->drafts + 1) + (a->draft_logits && a->temperature != 0.0f ? (size_t)a->sequences * a->drafts : 0);

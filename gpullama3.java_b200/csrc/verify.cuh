@@ -244,6 +244,22 @@ struct Weight {
     }
 };
 
+// Passes over the rows of a draft or of the token: for a verdict; of weights p; of p - q; of p - q once more, by exact sums; of p whole.  Behind one for a verdict comes the next such or the
+// token's first; behind the token's one with a higher number, or none any more.  So a sequence of c drafts takes c + 3 at most, whatever the sums are.
+enum Pass { VERDICT = -1, TARGET = 0, MORE = 1, MORE_EXACT = 2, WHOLE = 3, DRAW = 4, NOTHING = 5 }; // DRAW: the token is drawn from this pass; NOTHING: there is nothing to draw from
+__host__ __device__ __forceinline__ int after_pass(int kind, const double *all, double &sum_p, double &sum_q) { // all: the pass's sums; sum_p, sum_q: of the rows, exact ones behind MORE
+    const bool some = all[0] > 0.0 && all[0] < 1e300;
+    if (kind == TARGET) return some ? DRAW : WHOLE; // nothing but the draft: p as it is
+    if (kind == WHOLE) return some ? DRAW : NOTHING;
+    sum_p = all[0];
+    sum_q = all[1];
+    const double left = all[2] / sum_p - all[3] / sum_q;
+    // Which entries weigh more was told by FP32's sums, off by 1e-6 at most: an entry on the wrong side adds no more than that of itself, and few are that near.  Where little is left over they
+    // might count.
+    if (kind == MORE && !(left > 0.05)) return MORE_EXACT;
+    return some && left > 0.0 && left < 2.0 ? DRAW : WHOLE; // (WHOLE: the same distributions)
+}
+
 template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_verify_token(const Args a) {
     __shared__ Row rows[2 * MAX_DRAFTS + 1];    // target rows, then draft rows
     __shared__ signed char verdict[MAX_DRAFTS]; // 1 accepted, 0 not, -1 too close, -2 no distribution
@@ -290,24 +306,23 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
     // One pass over target row i, without entry `without`, and draft row i (two), which the cluster's warps share in order: sums of p, of q, and of both where p / sum_p > q / sum_q.
     const int share = share_of(a.vocab);
     const auto begin_of = [&](int w) { return (int)min((long long)w * share, (long long)a.vocab); };
-    int n = 0, kind = -1, without = -1; // kind: of the pass.  -1: for a verdict; 0: weights p; 1: p - q; 2: p - q once more, by exact sums; 3: p whole
-    double sum_p = 1.0, sum_q = 1.0;    // of the rows that the pass is for
-    bool fails = false;
-    for (;;) {
-        if (kind < 0) { // the next draft whose verdict takes a pass, or the token
+    int n = 0, kind = VERDICT, without = -1;
+    double sum_p = 1.0, sum_q = 1.0; // of the rows that the pass is for
+    bool fails = true; // (until a pass is there to draw from)
+    for (int pass = 0; pass < c + 3; pass++) {
+        if (kind == VERDICT) { // the next draft whose verdict takes a pass, or the token
             int v = 1;
             while (n < c && (v = verdict[n]) == 1) n++;
-            fails = n < c ? v == -2 : !(rows[c].sum > 0.0);
-            if (fails) break;
+            if (n < c ? v == -2 : !(rows[c].sum > 0.0)) break;
             if (n == c || v == 0) {
-                kind = n < c && both ? 1 : 0;
+                kind = n < c && both ? MORE : TARGET;
                 without = n < c && !both ? d[n] : -1; // a looked-up draft that did not stand
             }
         }
         const bool two = both && n < c;
         const T *x = target(n), *y = two ? draft(n) : nullptr;
         const float top_p = rows[n].top, top_q = two ? of_draft(n).top : 0.0f;
-        if (kind != 2) {
+        if (kind != MORE_EXACT) {
             sum_p = rows[n].sum;
             sum_q = two ? of_draft(n).sum : 1.0;
         }
@@ -379,23 +394,15 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
 #pragma unroll
             for (int k = 0; k < SUMS; k++) all[k] += sums.cta[k][r];
         // (all CTAs of the cluster come to the same)
-        if (kind < 0) {
+        if (kind == VERDICT) {
             if (tid == 0) verdict[n] = (signed char)(decide(n, all[0], all[1]) & 1);
             __syncthreads();
-        } else if (kind == 0 || kind == 3) {
-            if (all[0] > 0.0) break;
-            kind = 3; // nothing but the draft: p as it is
-            without = -1;
         } else {
-            sum_p = all[0];
-            sum_q = all[1];
-            const double left = all[2] / sum_p - all[3] / sum_q;
-            // Which entries weigh more was told by FP32's sums, off by 1e-6 at most: an entry on the wrong side adds no more than that of itself, and few are that near.  Where little is left over they
-            // might count.
-            if (kind == 2 || left > 0.05) {
-                if (left > 0.0) break;
-                kind = 3; // the same distributions
-            } else kind = 2;
+            const int next = after_pass(kind, all, sum_p, sum_q);
+            fails = next != DRAW;
+            if (next >= DRAW) break;
+            kind = next;
+            if (kind == WHOLE) without = -1;
         }
     }
     if (rank == 0) {
@@ -409,7 +416,7 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
     if (fails) return; // (the same in every CTA of the cluster)
 
     // ---- the token: which CTA, which warp's share, which entry: the first whose running sum passes the border, or the last that weighs anything ----
-    const bool differ = kind == 1 || kind == 2;
+    const bool differ = kind == MORE || kind == MORE_EXACT;
     const double by_p = 1.0 / sum_p, by_q = 1.0 / sum_q;
     const auto weight_of = [&](const double *p, const double *more_p, const double *more_q, int i) { return differ ? more_p[i] * by_p - more_q[i] * by_q : p[i]; };
     const auto cta_weight = [&](int r) { return weight_of(sums.cta[0], sums.cta[2], sums.cta[3], r); };
@@ -426,7 +433,7 @@ template <typename T> __global__ void __launch_bounds__(TOKEN_THREADS, 2) k_veri
     for (int r = 0; r < CLUSTER; r++) total += cta_weight(r);
     const double border = (double)u[a.drafts] * total, least = differ ? total * 1e-13 : 0.0; // (what rounding leaves of a share where both weigh the same)
     double before = 0.0, sum = 0.0;
-    int chosen = -1;
+    int chosen = 0; // (some CTA writes the token in any case)
     for (int r = 0; r < CLUSTER; r++) {
         const double w = cta_weight(r);
         if (w > least) { chosen = r; before = sum; }

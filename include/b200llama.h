@@ -672,6 +672,8 @@ int b200_verify_drafts(const b200_verify_drafts_args *args, void *stream, char *
 
 /* Test hook, on the host: the 64-bit weights exp((x - top) / temperature) of n logits x <= top, as the verification has them. */
 int b200_test_verify_weights(const float *x, int32_t n, float top, float temperature, double *weights);
+/* Test hook, on the host: what follows pass `kind` over a drawn row (0 to 3) with these four sums: the next pass's number, 4 (the token is drawn) or 5 (nothing to draw from); the rows' two sums. */
+int b200_test_verify_next(int32_t kind, const double *sums, double *rows);
 
 /* Number of kernels one decode step launches (bench.py's gpu_launches). */
 int b200_launches_per_decode(b200_plan *plan);

@@ -40,3 +40,32 @@ def test_weights_of_neighbours_of_large_logits(pkg, top, temperature):
             assert w == 0.0, (float(v), w)
         else:
             assert far > 689.999 and w == 0.0 or abs(Decimal(float(w)) / exact(v, top, temperature) - 1) <= Decimal(1e-12), (float(v), w)
+
+
+def test_passes_over_a_drawn_row_end(pkg):
+    """Whatever a pass's sums are, the next pass has a higher number or there is none: at most three passes, and 4 or 5 behind them."""
+    import itertools
+
+    values = [0.0, 1.0, 0.5, 1e-300, 1e-13, -1.0, -6e171, 1e308, math.inf, -math.inf, math.nan]
+    for kind in range(4):
+        for sums in itertools.product(values, repeat=4):
+            rows = (C.c_double * 2)(1.0, 1.0)
+            then = pkg.native.lib().b200_test_verify_next(kind, (C.c_double * 4)(*sums), rows)
+            assert kind < then <= 5, (kind, sums, then)
+            if then == 4:  # there is something to draw from
+                assert sums[0] > 0
+            if kind == 3:
+                assert then == (4 if 0 < sums[0] < 1e300 else 5)
+    for bad in (-1, 4, 5):
+        assert pkg.native.lib().b200_test_verify_next(bad, (C.c_double * 4)(), (C.c_double * 2)()) == -1
+
+
+def test_what_follows_a_pass(pkg):
+    def then(kind, *sums):
+        rows = (C.c_double * 2)(7.0, 7.0)
+        return pkg.native.lib().b200_test_verify_next(kind, (C.c_double * 4)(*sums), rows), tuple(rows)
+
+    assert then(0, 3.0, 0, 0, 0)[0] == 4 and then(0, 0.0, 0, 0, 0)[0] == 3  # nothing but the draft: p as it is
+    assert then(1, 2.0, 4.0, 1.0, 1.0) == (4, (2.0, 4.0))  # 1/2 - 1/4 is left over
+    assert then(1, 2.0, 4.0, 1.0, 1.95) == (2, (2.0, 4.0))  # little: once more by exact sums
+    assert then(2, 2.0, 4.0, 1.0, 1.95)[0] == 4 and then(2, 2.0, 4.0, 1.0, 2.0)[0] == 3  # the same distributions: p
