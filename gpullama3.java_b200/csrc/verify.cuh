@@ -187,10 +187,13 @@ template <typename T> __device__ __forceinline__ float4 load4(const T *x) {
     const float2 a = kv4::to_f32x2(w.x, x), b = kv4::to_f32x2(w.y, x);
     return make_float4(a.x, a.y, b.x, b.y);
 }
-// exp((x - top) / T) for x <= top: 2^(k / 32) from a table, the rest, at most ln(2) / 64, by its series (P. T. P. Tang's table-driven exponential, 1989).  Below e^-690 it is 0, and whether it is is told by the
+// exp((x - top) / T) for x <= top: 2^(k / 32) from a table, the rest, at most ln(2) / 64, by its series (P. T. P. Tang's table-driven exponential, 1989).  Off by 4.5e-16 |x - top| / T (the argument: the difference,
+// log2(e), the division by T and the product each round by 2^-53 of it) and 3e-15 of itself (the series leaves ln(2)^6 / 64^6 / 720 = 2.2e-15 out; table, series and product round): 3.2e-13 at the far end.  Below e^-690 it is 0, and whether it is is told by the
 // 64-bit argument: x and top may be as large against T as they like (top - 690 T in FP32 would round to the neighbour of top, and let arguments in whose exponents leave the double's field).
 constexpr int EXP_TABLE = 32;
-constexpr double LOG2E_64 = 1.44269504088896340736, EVEN = 1.0 + 0x1p-40; // weights that agree to 2^-40 are the same: the sums' last bits are not drawn from
+// Weights of p and q that agree to 2^-40 are the same, so that what rounding leaves is not drawn from: 9.1e-13 is more than two far weights and the rows' sums (one after the other in a lane at most 2^10 numbers of
+// the largest vocabulary: 1.2e-13 each) can be off, 8.8e-13.
+constexpr double LOG2E_64 = 1.44269504088896340736, EVEN = 1.0 + 0x1p-40;
 constexpr uint32_t REACH = 0x40df1badu;                                    // high word of 690 * 32 log2(e) = 31854.7
 __host__ __device__ __forceinline__ uint32_t high_word(double v) {
 #ifdef __CUDA_ARCH__

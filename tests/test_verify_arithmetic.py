@@ -69,3 +69,17 @@ def test_what_follows_a_pass(pkg):
     assert then(1, 2.0, 4.0, 1.0, 1.0) == (4, (2.0, 4.0))  # 1/2 - 1/4 is left over
     assert then(1, 2.0, 4.0, 1.0, 1.95) == (2, (2.0, 4.0))  # little: once more by exact sums
     assert then(2, 2.0, 4.0, 1.0, 1.95)[0] == 4 and then(2, 2.0, 4.0, 1.0, 2.0)[0] == 3  # the same distributions: p
+
+
+@pytest.mark.parametrize("temperature", [1e-4, 0.1, 0.6, 0.7, 1.0, 1.3, 17.0, 1e4])
+def test_weights_are_as_near_as_their_bound_says(pkg, temperature):
+    """4.5e-16 |x - top| / T and 3e-15 of the weight over the whole range: four roundings of 2^-53 in the argument, 4.44e-16 of it; the series' first missing term, (ln(2) / 64)^6 / 720 = 2.25e-15, the table's
+    2^-52 at most, and roundings of 2^-53 for the last step of the series and the product, and less than that in front of it, 0.45e-15.  Two of them and two sums (1.2e-13) stay below the margin of 2^-40."""
+    rng = np.random.default_rng(7)
+    for top in (0.0, 3.25, -11.0):
+        x = np.unique(np.float32(top) - np.float32(temperature) * np.concatenate([rng.uniform(0, 689, 1500), rng.uniform(0, 1, 300), 10.0 ** rng.uniform(-9, 2, 200)]).astype(np.float32)).astype(np.float32)
+        x = x[(x <= np.float32(top)) & (x >= np.float32(top) - np.float32(689.5 * temperature))]
+        for v, w in zip(x, weights(pkg, x, top, temperature)):
+            far = (float(np.float32(top)) - float(v)) / float(np.float32(temperature))
+            assert abs(Decimal(float(w)) / exact(v, top, temperature) - 1) <= Decimal(4.5e-16 * far + 3e-15), far
+    assert 2 * (4.5e-16 * 690 + 3e-15) + 2 * 1.2e-13 < 2.0 ** -40
