@@ -580,7 +580,7 @@ template <int HS, typename T, int NR, int PARTS, bool LONE> __global__ void __la
     for (int i = tid; i < ROWS * PIECES; i += STEP_WARPS * 32) { // queries
         const int r = i / PIECES, c = i % PIECES, token = token_of(r);
         uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows && a.scale != 0.0f) {
+        if (r < rows && a.scale != 0.0f && (LONE ? only.sequence : segment_of[token]) >= 0) { // (zeros for a row that sees nothing: padding may hold anything, and a NaN would reach the sums of the whole block)
             const uint16_t *q = (const uint16_t *)a.q + (long long)(token0 + token) * a.ldq + (size_t)(kvh * mul + row0 + r - token * mul) * HS + c * 8;
             if (a.vec) w = *reinterpret_cast<const uint4 *>(q);
             else w = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
