@@ -375,7 +375,7 @@ template <int KT, bool LONE, int THREADS> __device__ __forceinline__ void share_
 // ref follows the largest score seen so far only when that passes it by more than 2^8 (the first does), so that few tiles have anything to rescale; with FP16 it lies 2^7 below, so that
 // p reaches down to 2^-24 of 2^-15: a long tail of small ones still counts.
 // A value that is infinite or NaN would reach every row of the block as 0 * NaN, also those that do not see it, and sums of large BF16 values may leave FP32's range before they are divided: a
-// warp whose sums are not finite computes its share once more at the end, a row after the other in FP32, from what each sees, 2^-40 below its maximum (slow_rows).
+// warp whose sums are not finite computes its share once more at the end, a row after the other in FP32, from what each sees, with BF16 2^-40 below its maximum (slow_rows).
 // Bytes are its floor.  One row of 8 key/value heads of 128 over 131071 positions, 537 MB: 84-85 us (6.3 TB/s; floor 83), with the join 88 in a graph; 48 rows of up to 4099 positions of 8 heads of 64, 206 MB: 45
 // (floor 32), with the join 47; 16 sequences of 5 drafted tokens, 20 rows, over up to 8191 positions, 285 MB: 62 (floor 44), with the join 67, where the chains of products of six warps an SM (tensor pipes 22 %)
 // keep the copies from running ahead.  What a CTA holds was measured on these three: two warps with two tiles of 32 positions each; tiles of 16 with three places: 91, 47, 61-66; four warps: 90, 53-56, 62; products with
@@ -383,6 +383,7 @@ template <int KT, bool LONE, int THREADS> __device__ __forceinline__ void share_
 template <int HS, typename T> __device__ __noinline__ void slow_rows(const Step &a, const unsigned char *sQ, int rows, int row0, int token0, int kvh, int first, int last, int warp, const Segment *segments, const int *segment_of,
                                                                      const int *pos_of, float factor, float *parts, float *wref, float *wsum) {
     constexpr int KT = step_keys(HS), E = HS / 32; // entries of a lane
+    constexpr float DOWN = std::is_same<T, __half>::value ? 0.0f : 40.0f; // (sums of FP16 values stay in FP32's range as they are)
     const int lane = threadIdx.x & 31;
     for (int r = 0; r < rows; r++) {
         const int token = (row0 + r) / a.mul, own = segment_of[token];
@@ -412,7 +413,7 @@ template <int HS, typename T> __device__ __noinline__ void slow_rows(const Step 
             }
             const float grown = fmaxf(top, warp_max_f(s)), base = grown == -CUDART_INF_F ? 0.0f : grown, alpha = top == grown ? 1.0f : ex2((top - base) * factor);
             top = grown;
-            const float p = at != NO_ROW ? ex2(fmaf(s - base, factor, -40.0f)) : 0.0f;
+            const float p = at != NO_ROW ? ex2(fmaf(s - base, factor, -DOWN)) : 0.0f;
             l = l * alpha + p;
 #pragma unroll
             for (int e = 0; e < E; e++) o[e] *= alpha;
@@ -430,7 +431,7 @@ template <int HS, typename T> __device__ __noinline__ void slow_rows(const Step 
 #pragma unroll
         for (int e = 0; e < E; e++) parts[r * part_stride(HS) + e * 32 + lane] = o[e];
         if (lane == 0) {
-            wref[r] = top * factor + 40.0f;
+            wref[r] = top * factor + DOWN;
             wsum[r] = l;
         }
     }
@@ -636,6 +637,7 @@ template <int HS, typename T, int NR, int PARTS, bool LONE> __global__ void __la
     }
     Segment sg = only;
     int seg = 0, stage = 0;
+    bool huge = false; // a reference so large that it rounds by more than 2^-4 (the whole warp)
     for (int tile = first + warp; tile < last; tile += STEP_WARPS) {
         cp_wait<S - 2>();
         __syncwarp(); // and every lane has read the tile before, whose place the next copies take
@@ -710,8 +712,19 @@ template <int HS, typename T, int NR, int PARTS, bool LONE> __global__ void __la
 #pragma unroll
                         for (int i = 0; i < HS / 16; i++) { o[n][i][h] *= f; o[n][i][2 + h] *= f; }
                     }
+                    huge |= fabsf(ref[n][h]) > 1048576.0f;
                 }
+            huge = __any_sync(0xffffffffu, huge);
         }
+        // An exponent is the scaled score, not yet rounded, minus a reference that is: where that rounds by hundreds every probability of the row would be 0, or infinite.  There scores are rounded like it first.
+        if (huge)
+#pragma unroll
+            for (int n = 0; n < NR; n++)
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[n][b][i] *= factor;
+        const float by = huge ? 1.0f : factor;
         uint32_t pp[PARTS][NR][KB][2]; // of 8 positions each: of positions 2 t, 2 t + 1 and row g
 #pragma unroll
         for (int n = 0; n < NR; n++)
@@ -719,7 +732,7 @@ template <int HS, typename T, int NR, int PARTS, bool LONE> __global__ void __la
             for (int b = 0; b < KB; b++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const float p0 = ex2(fmaf(s[n][b][2 * i], factor, -ref[n][0])), p1 = ex2(fmaf(s[n][b][2 * i + 1], factor, -ref[n][1]));
+                    const float p0 = ex2(fmaf(s[n][b][2 * i], by, -ref[n][0])), p1 = ex2(fmaf(s[n][b][2 * i + 1], by, -ref[n][1]));
                     l[n][0] += p0;
                     l[n][1] += p1;
                     float2 left = make_float2(p0, p1);

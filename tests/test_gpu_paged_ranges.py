@@ -28,3 +28,39 @@ def test_what_padding_holds_does_not_matter(pkg, dtype, out, H, hs, slots, used,
     q[~live] = bad
     got = cache.attention(q, pos, tables, sequences=seq, dtype=out, chunk=slots)
     assert torch.equal(got[live], want[live]) and (got[~live & (kind == 2)] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,out", [(BF16, F32), (F16, F32), (BF16, BF16), (F16, F16)])
+@pytest.mark.parametrize("size", [1e5, 1.5e6, 9e6, 3e7, 7e7, 2e8, 9e8, 1.1e9, 7e9, 1.3e11, 2.9e13, 1e20, 1e30])
+@pytest.mark.parametrize("chunk,hs", [(1, 64), (1, 256), (4, 64), (4, 128), (40, 64)])
+def test_huge_scores(pkg, dtype, out, size, chunk, hs):
+    """Scores (times log2(e)) of up to 1e30, whose rounding alone is many powers of two.  Equal ones share a row out evenly, and one that is larger by 2^-7 of itself, 2^-7 size > 780 powers of two,
+    takes it alone.  The probabilities of equal scores are equal, so a mean's error is that of sums (m products of 16 an instruction, (m / 8 + 32) 2^-22), 2^-17 for the parts of a probability, its half
+    step with 16-bit results, all of the mean of |v|, and the result's half step."""
+    g, n = gen(hs + chunk), 500
+    cache, tables = paged(pkg, g, [n], 16, 1, hs, dtype)
+    at = torch.arange(n, device="cuda")
+    where = tables[0].long()[at // 16], 0, at % 16
+    pos = torch.arange(n - 40, n, device="cuda", dtype=torch.int32)
+    q = torch.full((40, 4, hs), 8.0, device="cuda", dtype=dtype)
+    scale = size * 0.6931471805599453 / (hs * 64.0)
+    values = cache.values[where].double().cpu()
+    off = (n / 8 + 32) * 2.0 ** -22 + 2.0 ** -17 + probability(cache, out)
+    for factor in (1.0, 0.83, 0.71):  # references that round up and down
+        cache.keys[where] = torch.full((n, hs), 8.0, device="cuda", dtype=dtype)
+        got = cache.attention(q, pos, tables, scale=scale * factor, chunk=chunk, dtype=out).double().cpu()
+        for i in range(40):
+            v = values[:n - 39 + i]
+            bound = P.rounding(v.mean(0), off * v.abs().mean(0), out)
+            assert ((got[i] - v.mean(0)).abs() <= bound).all()
+        best = int(torch.randint(0, n - 40, (), device="cuda", generator=g))
+        cache.keys[tables[0, best // 16], 0, best % 16] = 8.0625
+        got = cache.attention(q, pos, tables, scale=scale * factor, chunk=chunk, dtype=out).double().cpu()
+        assert ((got - values[best]).abs() <= P.rounding(values[best], off * values[best].abs(), out)).all()
+        grown = 8.0 + 0.0625 * (torch.arange(n, device="cuda") // 50)  # a maximum that grows every 50 positions, the last row's on 50 or fewer
+        cache.keys[where] = grown[:, None].expand(n, hs).to(dtype)
+        got = cache.attention(q, pos, tables, scale=scale * factor, chunk=chunk, dtype=out).double().cpu()
+        for i in range(40):
+            v = values[450:n - 39 + i]
+            bound = P.rounding(v.mean(0), off * v.abs().mean(0), out)
+            assert ((got[i] - v.mean(0)).abs() <= bound).all()
