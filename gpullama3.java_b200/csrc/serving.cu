@@ -4,6 +4,8 @@
 #include "paged_chunk.cuh"
 #include "verify.cuh"
 
+#include <math.h>
+
 namespace {
 
 struct Fail { // the caller's message buffer
@@ -247,6 +249,7 @@ static int paged_attention(const b200_paged_cache *c, const b200_paged_attention
     if (a->heads <= 0 || a->heads % c->kv_heads) return fail(B200_ERR_BAD_ARG, "%d query heads over %d key/value heads", a->heads, c->kv_heads);
     if (!known_type(a->out_type)) return fail(B200_ERR_UNSUPPORTED, "results of type %d (FP32, FP16 and BF16 are known)", a->out_type);
     if (a->window < 0 || a->max_len < 0 || a->chunk < 0) return fail(B200_ERR_BAD_ARG, "a negative window, length or chunk");
+    if (!(fabsf(a->scale) < INFINITY)) return fail(B200_ERR_BAD_ARG, "a scale of %g", (double)a->scale);
     if (reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(B200_ERR_BAD_ARG, "the workspace is not aligned");
     if (a->n == 0) return B200_OK;
     if (!a->q || !a->out) return fail(B200_ERR_BAD_ARG, "null rows");
