@@ -45,6 +45,21 @@ int check_rows(const b200_paged_cache *c, int n, const int32_t *positions, const
     return B200_OK;
 }
 
+struct Extent { // n rows of `width` bytes, `stride` bytes apart
+    const void *at;
+    __int128 stride, width;
+    int n;
+};
+Extent pool_of(const b200_paged_cache *c, const void *at) { return {at, 0, (__int128)c->pages * c->kv_heads * c->page_size * c->head_size * 2, 1}; }
+// Whether two such share a byte.  Rows of one stride may lie side by side, as parts of wider rows; others count as sharing where their extents do.
+bool overlap(const Extent &x, const Extent &y) {
+    const __int128 a = reinterpret_cast<uintptr_t>(x.at), b = reinterpret_cast<uintptr_t>(y.at);
+    if (a + (x.n - 1) * x.stride + x.width <= b || b + (y.n - 1) * y.stride + y.width <= a) return false;
+    if (x.n == 1 || y.n == 1 || x.stride != y.stride) return true;
+    const __int128 d = ((b - a) % x.stride + x.stride) % x.stride; // where y's rows begin within x's
+    return d < x.width || d + y.width > x.stride;
+}
+
 // How the attention of n rows is cut.
 struct PagedCut {
     int nr, tokens, blocks, ctas; // blocks of 8 nr rows; tokens of a group; blocks of a group and key/value head; CTAs that units are shared out over (0: a CTA a unit)
@@ -202,6 +217,13 @@ int b200_paged_append(const b200_paged_cache *c, const b200_paged_append_args *a
     const int64_t kv_width = (int64_t)c->kv_heads * c->head_size, q_width = (int64_t)a->heads * c->head_size;
     if (a->n > 1 && (a->k_stride < kv_width || a->v_stride < kv_width || (a->heads && (a->q_stride < q_width || a->q_out_stride < q_width)))) return fail(B200_ERR_BAD_ARG, "rows overlap: a stride is smaller than its row");
     if (a->heads + 2LL * c->kv_heads > (1LL << 18)) return fail(B200_ERR_UNSUPPORTED, "too many heads"); // (the grid's second dimension)
+    if (a->heads) { // warps write q_out while others still read
+        const int b = type_bytes(a->type);
+        const Extent out = {a->q_out, (__int128)a->q_out_stride * 2, (__int128)q_width * 2, a->n}, q = {a->q, (__int128)a->q_stride * b, (__int128)q_width * b, a->n},
+                     keys = {a->k, (__int128)a->k_stride * b, (__int128)kv_width * b, a->n}, values = {a->v, (__int128)a->v_stride * b, (__int128)kv_width * b, a->n};
+        if (overlap(out, q) || overlap(out, keys) || overlap(out, values) || overlap(out, pool_of(c, c->keys)) || overlap(out, pool_of(c, c->values)))
+            return fail(B200_ERR_BAD_ARG, "q_out may not overlap the rows or the cache");
+    }
     paged::Append k;
     k.pool = {c->keys, c->values, c->pages, c->kv_heads, shift_of(c->page_size)};
     k.rows = {a->positions, a->sequences, a->tables, a->table_stride, a->n, a->n_sequences, a->table_width * c->page_size};
@@ -256,6 +278,10 @@ static int paged_attention(const b200_paged_cache *c, const b200_paged_attention
     const int64_t width = (int64_t)a->heads * c->head_size;
     if (a->n > 1 && (a->q_stride < width || a->out_stride < width)) return fail(B200_ERR_BAD_ARG, "rows overlap: a stride is smaller than its row");
     if ((long long)a->n * a->heads > (1LL << 27)) return fail(B200_ERR_UNSUPPORTED, "too many rows in one call");
+    const int b = type_bytes(a->out_type);
+    const Extent out = {a->out, (__int128)a->out_stride * b, (__int128)width * b, a->n}, q = {a->q, (__int128)a->q_stride * 2, (__int128)width * 2, a->n};
+    const bool same = a->out == a->q && b == 2 && (a->n == 1 || a->out_stride == a->q_stride); // (a CTA reads the rows that it writes before it does)
+    if ((!same && overlap(out, q)) || overlap(out, pool_of(c, c->keys)) || overlap(out, pool_of(c, c->values))) return fail(B200_ERR_BAD_ARG, "results may be the queries, but not overlap them or the cache otherwise");
     OnDevice on(c->device);
     cudaError_t e = on.error;
     if (e == cudaSuccess) e = paged_attention_launch(*c, *a, (cudaStream_t)stream, give_up);

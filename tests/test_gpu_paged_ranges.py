@@ -64,3 +64,27 @@ def test_huge_scores(pkg, dtype, out, size, chunk, hs):
             v = values[450:n - 39 + i]
             bound = P.rounding(v.mean(0), off * v.abs().mean(0), out)
             assert ((got[i] - v.mean(0)).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("chunk,hs", [(1, 64), (3, 64), (40, 64), (40, 128), (40, 32)])
+def test_results_in_the_place_of_queries_or_beside_them(pkg, chunk, hs):
+    """``out`` may be the queries themselves, or another part of the same wider rows; what overlaps otherwise is refused."""
+    g = gen(chunk)
+    cache, tables = paged(pkg, g, [90, 3000], 16, 2, hs, BF16)
+    pos = torch.cat([torch.arange(50, 90, device="cuda"), torch.arange(2960, 3000, device="cuda")]).int()
+    seq = torch.arange(2, device="cuda", dtype=torch.int32).repeat_interleave(40)
+    wide = rand(g, 80, 3 * 8 * hs, dtype=BF16)
+    q, beside, across = (wide[:, i:i + 8 * hs].view(80, 8, hs) for i in (8 * hs, 16 * hs, 12 * hs))
+    want = cache.attention(q, pos, tables, sequences=seq, chunk=chunk)
+    cache.attention(q, pos, tables, sequences=seq, chunk=chunk, out=beside)
+    assert torch.equal(beside, want)
+    with pytest.raises(pkg.native.B200Error, match="overlap"):
+        cache.attention(q, pos, tables, sequences=seq, chunk=chunk, out=across)
+    cache.attention(q, pos, tables, sequences=seq, chunk=chunk, out=q)
+    assert torch.equal(q, want)
+    k, v = wide[:, :2 * hs].view(80, 2, hs), wide[:, 2 * hs:4 * hs].view(80, 2, hs)
+    turned = cache.append(k, v, pos, tables, sequences=seq, q=q, q_out=beside)
+    assert turned.data_ptr() == beside.data_ptr() and torch.equal(beside, q)
+    for bad in (across, wide[:, :8 * hs].view(80, 8, hs), cache.keys.view(-1)[:80 * 8 * hs].view(80, 8, hs)):
+        with pytest.raises(pkg.native.B200Error, match="overlap"):
+            cache.append(k, v, pos, tables, sequences=seq, q=q, q_out=bad)
