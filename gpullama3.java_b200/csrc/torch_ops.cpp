@@ -408,6 +408,7 @@ std::pair<Tensor, Tensor> verify_drafts(const Tensor &logits, const Tensor &draf
     a.drafts = (int32_t)K;
     a.vocab = (int32_t)V;
     a.temperature = (float)temperature;
+    if (a.temperature == 0.0f && temperature != 0.0) refused(B200_ERR_BAD_ARG, c10::str("a temperature of ", temperature, " (0, or 1e-4 to 1e4)").c_str()); // (FP32 would make it 0)
     a.logits = logits.data_ptr();
     a.row_stride = K > 0 ? logits.stride(1) : V;
     a.sequence_stride = S > 1 ? logits.stride(0) : 0;

@@ -29,3 +29,11 @@ def test_neighbours_of_large_logits(pkg, temperature, top, with_draft):
     only[:, :, 7] = top
     only[:, :, 8] = torch.nextafter(only[:, :, 7], below)
     check(pkg, only, drafts[:2, :0], torch.tensor([[0.2], [0.999]], device="cuda"), None, temperature)
+
+
+@pytest.mark.parametrize("temperature", [1e-50, -1e-50, 1e-46, 5e-324, 1e-45, 9e-5, 1.1e4, 1e300])
+def test_temperatures_that_are_refused(pkg, temperature):
+    """Also those that FP32 rounds to 0: they are not 0, and most likely tokens are not what was asked for."""
+    x, u = torch.zeros(1, 2, 8, device="cuda"), torch.zeros(1, 2, device="cuda")
+    with pytest.raises(pkg.native.B200Error, match="temperature"):
+        pkg.verify_drafts(x, torch.zeros(1, 1, device="cuda", dtype=torch.int32), u, temperature=temperature)
