@@ -3,6 +3,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -41,8 +42,9 @@ int type_of(at::ScalarType t, const char *what) {
     return -1;
 }
 
-// There are no backward passes: a graph that led through a call would end there without a word.
+// There are no derivatives: a graph that led through a call, or a tangent carried into it, would end there without a word.
 void outside_graph(const Tensor &t, const char *name) {
+    NEED(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !t._fw_grad(0).defined(), name, " carries a forward-mode tangent, and the operators have none: detach it");
     NEED(!t.requires_grad() || !at::GradMode::is_enabled(), name, " requires a gradient, and the operators have none: detach it, or call under torch.no_grad()");
 }
 

@@ -3,8 +3,8 @@ drafted ones (``b200_kv4_*``, ``b200_paged_*``, ``b200_log_probs``, ``b200_verif
 
 Every call runs on the current stream of its tensors' device, returns without waiting and can be captured into a CUDA graph.  Tensors are
 checked first: a wrong type, shape, device or layout raises ``ValueError`` (or ``TypeError``: no tensor at all) before anything is launched;
-what the library refuses raises ``native.B200Error``.  There are no backward passes: a tensor that requires a gradient is refused unless gradients are off
-(``torch.no_grad()``, ``torch.inference_mode()``).
+what the library refuses raises ``native.B200Error``.  There are no derivatives: a tensor that requires a gradient is refused unless gradients are off
+(``torch.no_grad()``, ``torch.inference_mode()``), one that carries a forward-mode tangent is refused until it is detached.
 """
 from __future__ import annotations
 
