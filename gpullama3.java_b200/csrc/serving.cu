@@ -325,6 +325,9 @@ int b200_verify_drafts(const b200_verify_drafts_args *a, void *stream, char *err
     const bool both = a->draft_logits && a->temperature != 0.0f && a->drafts > 0;
     const size_t need = b200_verify_drafts_workspace(a);
     if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16) return fail(B200_ERR_BAD_ARG, "a workspace of %zu bytes on a 16-byte boundary is needed", need);
+    const __int128 S = a->sequences;
+    const Extent drafts = {a->tokens, 0, S * a->drafts * 4, 1}, out = {a->out_tokens, 0, S * (a->drafts + 1) * 4, 1}, counts = {a->accepted, 0, S * 4, 1};
+    if ((a->drafts && (overlap(out, drafts) || overlap(counts, drafts))) || overlap(out, counts)) return fail(B200_ERR_BAD_ARG, "results may not overlap the drafts or one another"); // (other sequences still read them)
     verify::Args k;
     k.logits = a->logits; k.draft_logits = both ? a->draft_logits : nullptr;
     k.ld_s = a->sequence_stride; k.ld_r = a->row_stride; k.draft_ld_s = a->draft_sequence_stride; k.draft_ld_r = a->draft_row_stride;

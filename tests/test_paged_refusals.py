@@ -53,3 +53,13 @@ def test_attention_refuses_results_over_its_inputs(pkg, kw):
     cache = cache_of(pkg, keys=1 << 24, values=1 << 25)
     a = attention_of(pkg, **dict(dict(q=BASE, out_type=1), **kw))
     assert L.b200_paged_attention(C.byref(cache), C.byref(a), None, err, 256) == -1 and b"overlap" in err.value
+
+
+@pytest.mark.parametrize("kw", [dict(out_tokens=BASE), dict(out_tokens=BASE - 20), dict(out_tokens=BASE + 12), dict(accepted=BASE + 4), dict(accepted=2 * BASE + 20), dict(accepted=2 * BASE - 4)])
+def test_verification_refuses_results_over_its_drafts(pkg, kw):
+    """Two sequences of two drafts: 16 bytes of drafts, 24 of tokens, 8 of counts."""
+    L, err, a = pkg.native.lib(), C.create_string_buffer(256), pkg.native.VerifyDrafts()
+    for k, v in dict(dict(logits=256, sequence_stride=24, row_stride=8, sequences=2, drafts=2, vocab=8, temperature=1.0, tokens=BASE, uniforms=256, out_tokens=2 * BASE, accepted=3 * BASE, workspace=4 * BASE,
+                          workspace_bytes=1 << 16), **kw).items():
+        setattr(a, k, v)
+    assert L.b200_verify_drafts(C.byref(a), None, err, 256) == -1 and b"overlap" in err.value
