@@ -85,7 +85,10 @@ PagedCut paged_cut(const b200_paged_cache &c, const b200_paged_attention_args &a
     // Shared out where the rows are long enough to pay for it (about 6 us: every CTA looks at all rows' positions, the parts are joined by a kernel of their own) and the units leave room.  us of a
     // captured call, a CTA a unit / shared out, by positions: one row of 8 heads of 128: 384: 8.3/10.1, 512: 9.7/10.8, 768: 12.8/11.0, 2048: 28.4/11.4; 8 rows of 8 heads of 64 (of room for 888 units):
     // 768: 10.3/11.4, 1024: 12.6/11.6, 2048: 21.6/12.7; 4 rows of a head of 256: 256: 11.4/11.1, 512: 17.7/11.4; 32 rows of 8 heads of 128 (256 units where 444 have room: no two CTAs for each) all of
-    // one length: 1024: 27.5/34.7, 2048: 48.6/56.2; 24 rows of up to 4099: 74/49.
+    // one length: 1024: 27.5/34.7, 2048: 48.6/56.2; 24 rows of up to 4099: 74/49.  Three and four blocks of 8 rows, 8 heads, 16-bit results: 24 rows of 128: 320: 14.8/15.7, 384: 15.9/16.0, 512: 18.1/17.1, 1024: 27.2/17.3; 24 of
+    // 64: 384: 11.9/13.7, 512: 13.4/14.4, 640: 15.1/14.7; 32 of 128: 256: 17.9/21.4, 320: 19.6/19.2, 512: 24.6/21.1; 32 of 64: 384: 13.9/15.4, 512: 15.8/16.3, 640: 17.7/16.4; 30 of 96: 384: 18.9/19.1, 448: 20.3/20.4, 512: 21.6/20.5; FP32
+    // results, 24 of 128: 320: 17.4/17.4, 512: 22.5/19.3; 16 sequences (128 units for 444), 24 of 128: 768: 22.9/24.1, 1024: 28.5/27.9; 32 of 128: 640: 28.7/29.9, 768: 33.0/31.0; 32 of 64: 768: 19.7/21.5, 1024: 23.3/22.4.  Two of 128: 512:
+    // 14.7/14.7, 640: 16.8/14.7.  (Half the positions of one or two blocks; between 340 and 600 heads of 64 lose up to 2 us.)
     const long long room = (long long)sms * paged::step_ctas(c.head_size, k.nr), units = (long long)k.units;
     const long long worth = (k.nr > 2 ? 10 : 20) * KT * (room + 4 * units) / room * (2 * units > room ? 2 : 1); // (a tile is latency, whatever the head's size)
     if (len > worth && groups <= paged::STEP_GROUPS && a.n <= paged::STEP_SHARED_ROWS) {

@@ -247,7 +247,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> log_probs(const Tensor &logits, const
     return {lp, entropy, ids, values};
 }
 
-// Checks that calls on a pool of pages and on the 4-bit cache share.
+// Checks of the calls on a pool of pages and of the verification (the 4-bit cache has its own, with its messages).
 const int32_t *int_tensor(const Tensor &t, const char *name, int device, at::IntArrayRef sizes) {
     NEED(t.defined() && t.scalar_type() == at::kInt && t.sizes() == sizes, name, ": ", sizes, " of int32 is wanted, got ", shape(t));
     NEED(t.is_cuda() && t.get_device() == device, name, " is on ", t.device(), ", the call on cuda:", device);

@@ -9,8 +9,9 @@
 // draws the token: that is a whole number which one more bit would change where u falls near a border, and a vocabulary has 10^5 of them, so the drawn row's weights and their sums are in
 // 64 bits; and where FP32's error could turn a decision, its row's sum is taken once more in 64 bits.
 // Where the token comes from max(p - q, 0), one pass takes both rows' sums and, on either side of which p / sum_p > q / sum_q by FP32's sums, those of the entries that weigh more in p: their difference is the
-// weight, whatever the sums come out as (entries that weigh the same to 2^-40 weigh nothing; a pass for the sums and one for the weights took 70 us in place of 37).
-// Bytes are the floor: 32 sequences of 5 drafts and 128256 FP32 logits of two models are 181 MB, 28 us; the call takes 51 (48 in a graph): the rows 23 (less is read where drafts are missing), the tokens 24-34, of
+// weight (entries that weigh the same to 2^-40 weigh nothing; a pass for the sums and one for the weights took 70 us in place of 37).  An entry whose weights agree to FP32's error, 8e-6, may be counted on the wrong
+// side, by a difference of no more than that of itself: a border moves by 8e-6 of such entries' p.
+// Bytes are the floor: 32 sequences of 0 to 5 drafts, 84 in all, and 128256 FP32 logits of two models: 200 rows that count, 103 MB, 15.9 us; the call takes 51 (48 in a graph): the rows 23, the tokens 24-34, of
 // which a pass over two rows in 64 bits is 18: two exponentials an entry, 64-bit units at 23 % on average, their chains and the loads in between on the clusters that have one.  One sequence: 15.5 in a graph, latency.
 // Nothing depends on an order of arrival.
 #pragma once
@@ -59,8 +60,8 @@ __device__ __forceinline__ int given(const Args &a, int s, int most) {
     return most;
 }
 
-// A stretch is read whole into registers, so that all of its loads are under way at once: largest entry, then the sum.  FP32: an exponential's argument is off by at most 2^-24 of itself, so a row's sum by sum p |log2 p| 2^-24 and 2^-20 for
-// the exponentials and the order of the sum: 3e-6 at most.
+// A stretch is read whole into registers, so that all of its loads are under way at once: largest entry, then the sum.  FP32: an exponential's argument, distance times log2(e) / T, is off by at most 4 of 2^-24 of itself, so a row's sum by 4 ln(2) 2^-24 of
+// their mean, which a vocabulary of 2^24 keeps below 20, and 2^-20 for the exponentials and the order of the sum: 4e-6 at most.
 template <typename T> __global__ void __launch_bounds__(ROW_THREADS, 5) k_verify_rows(const Args a) {
     constexpr int VEC = Load<T>::VEC;
     __shared__ float warp_top[ROW_THREADS / 32], warp_sum[ROW_THREADS / 32];
@@ -257,7 +258,7 @@ __host__ __device__ __forceinline__ int after_pass(int kind, const double *all, 
     sum_p = all[0];
     sum_q = all[1];
     const double left = all[2] / sum_p - all[3] / sum_q;
-    // Which entries weigh more was told by FP32's sums, off by 1e-6 at most: an entry on the wrong side adds no more than that of itself, and few are that near.  Where little is left over they
+    // Which entries weigh more was told by FP32's sums, each off by 4e-6 at most: an entry on the wrong side adds no more than twice that of itself, and few are that near.  Where little is left over they
     // might count.
     if (kind == MORE && !(left > 0.05)) return MORE_EXACT;
     return some && left > 0.0 && left < 2.0 ? DRAW : WHOLE; // (WHOLE: the same distributions)

@@ -83,19 +83,21 @@ class PagedKVCache(_ops.Paged):
     [pages, kv_heads, page_size, head_size] are the memory itself, torch's; zeros at first.
 
     ``positions`` (and ``sequences``) of a call are int32 tensors on the cache's device with an entry per row; ``sequences=None`` is the first table's.  A row whose sequence has no table or whose
-    position lies behind its table is padding: nothing is read, stored or written for it.  A table entry outside the pool is no page: nothing is stored there, nobody sees its positions.  At
+    position lies behind its table is padding: nothing is stored or written for it, and what lies in its rows does not matter.  A table entry outside the pool is no page: nothing is stored there, nobody sees its positions.  At
     most 2^29 positions a table.  Calls that store and read the same positions belong on one stream, or are ordered by events.
 
     append(k, v, positions, tables, sequences=None, q=None, q_norm=None, k_norm=None, eps=1e-6, cos=None, sin=None, layout="half", q_out=None)
         Stores rows ``k``, ``v`` [n, kv_heads, head_size] (FP32, FP16 or BF16; parts of a wider row are fine), rounded once.  ``q`` [n, heads, head_size] of the same type comes back in the
         cache's type.  On the way the heads of q and k are RMS-normed (``q_norm`` / ``k_norm`` [head_size]) and their first 2 r entries rotated (``cos`` / ``sin`` [positions, r]; r is
         head_size / 2 for whole heads; scaled or stretched positions are a matter of these tables; pairs by ``layout``: "half": i and i + r, or "interleaved": 2 i and 2 i + 1).  A position
-        behind these tables is padding.  Two rows of a call must not name the same place; ``q_out``, which may not overlap ``q``, is left as it was where a row is padding or has a negative position.
+        behind these tables is padding.  Two rows of a call must not name the same place; ``q_out``, which may not overlap ``q``, ``k``, ``v`` or the cache (refused), is left as it was where a row is padding or has a negative position.
 
     attention(q, positions, tables, sequences=None, scale=None, window=0, max_len=0, chunk=1, dtype=None, out=None)
         Causal attention of rows ``q`` [n, heads, head_size] of the cache's type: the row at position p sees the positions up to p of its sequence, the last ``window`` of them (0: all);
         ``scale`` is head_size ** -0.5 unless given.  Results are of the cache's type unless ``dtype`` says FP32, FP16 or BF16.  ``chunk`` (neighbouring rows that are successive tokens of one
-        sequence: drafted tokens, a prompt's chunk) and ``max_len`` (largest position + 1, 0: unknown) only choose how the work is split.  ``dtype`` chooses the precision too: 16-bit results come
+        sequence: drafted tokens, a prompt's chunk) and ``max_len`` (largest position + 1, 0: unknown) only choose how the work is split, but tell them: rows of a prompt without ``chunk`` read all pages once each, where a chunk's
+        read them once for 32 rows or 128, tens of times as fast; and a call of more than 256 single rows (or of 256 groups) gives each its own CTAs, however long it is.  ``out`` may be ``q`` itself, but not overlap it or the cache
+        otherwise (refused).  ``dtype`` chooses the precision too: 16-bit results come
         from probabilities of the cache's type, half a step off each, FP32 results from several such numbers (24 bits BF16, 22 FP16).  A row that sees nothing is zeros; a value that is
         infinite or NaN reaches the rows that see it, and only those."""
 

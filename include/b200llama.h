@@ -600,13 +600,13 @@ typedef struct b200_paged_cache {
 } b200_paged_cache;
 
 /* The rows of a call on a paged cache: row r stands at positions[r] of sequence `sequences ? sequences[r] : 0`, whose table is the table_width entries from tables + sequence * table_stride
- * on (device arrays).  A row whose sequence lies outside [0, n_sequences) or whose position lies behind its table is padding: nothing is read, stored or written for it.  A negative
- * position is a row without keys.  At most 2^29 positions a table. */
+ * on (device arrays).  A row whose sequence lies outside [0, n_sequences) or whose position lies behind its table is padding: nothing is stored or written for it, and what lies in its
+ * rows does not matter (their memory has to be there).  A negative position is a row without keys.  At most 2^29 positions a table. */
 
 /* Rows of a QKV product -> pages, as b200_kv4_append: head norms (the mean of squares in 64 bits) and rotation in FP32, rounded once to the cache's type.  The rotation turns the first
  * rope_dims entries of a head (an even number): cos / sin are FP32 [rope_rows][rope_dims / 2], pairs by rope_layout within that part; a position behind rope_rows is padding.  q_out receives
- * the queries in the cache's type (it may not overlap q).  A row of a negative position is not stored and its q_out not written, one whose page is none is not stored.  Two rows of a call
- * must not name the same place. */
+ * the queries in the cache's type (it may not overlap q, k, v or the cache: refused; parts of the same wider rows side by side are fine).  A row of a negative position is not stored and its
+ * q_out not written, one whose page is none is not stored.  Two rows of a call must not name the same place. */
 typedef struct b200_paged_append_args {
     int32_t n, heads, type, rope_layout, rope_dims, rope_rows; /* type: of the rows, F32, F16 or BF16 */
     const void *q, *k, *v;
@@ -621,9 +621,10 @@ typedef struct b200_paged_append_args {
 int b200_paged_append(const b200_paged_cache *cache, const b200_paged_append_args *args, void *stream, char *err, size_t err_len);
 
 /* Causal attention of n query rows of the cache's type over the pages of their sequences: the row at position p sees the positions j <= p that have a page, the last `window` of them
- * where window > 0; query head h reads key/value head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type (F32, F16, BF16).  Queries and keys are multiplied as they are,
- * sums are FP32, and a probability is a number of the cache's type (8 bits BF16, 11 FP16: with results of 16 bits, which round as much) or several of them (24 bits, 22: with FP32 results).  A row
- * that sees nothing, or only scores of -inf, is zeros.  A value that is infinite or NaN makes its entry not finite in the rows that see it, and only in those.  chunk (0 or 1: single
+ * where window > 0; scale is a finite number; query head h reads key/value head h / (heads / kv_heads); out = softmax(scale * <q, k>) v in out_type (F32, F16, BF16).  Queries and keys are
+ * multiplied as they are, sums are FP32, and a probability is a number of the cache's type (8 bits BF16, 11 FP16: with results of 16 bits, which round as much) or several of them (24 bits, 22: with FP32 results).  out
+ * may be q itself (same stride, 16-bit results), but not overlap it or the cache otherwise: refused.  A row that sees nothing, or only scores of -inf, is zeros.  A value that is infinite or NaN
+ * makes its entry not finite in the rows that see it, and only in those.  chunk (0 or 1: single
  * steps; how many neighbouring rows are successive tokens of one sequence) and max_len (0: unknown; the largest position + 1) only choose how the work is split.  Chunks of 64 rows (tokens x query
  * heads of a key/value head) and more with 16-bit results and heads of 64, 96 or 128 run on the tensor cores' own memory; waits inside that kernel end after half a second, and should one ever run
  * out, its rows are NaN.  So does a workspace: few rows over many positions fill the GPU where the call gets b200_paged_attention_workspace(cache, args) bytes (0: it needs
@@ -653,8 +654,10 @@ int b200_test_paged_give_up(const b200_paged_cache *cache, const b200_paged_atte
  * behind them, then -1.  The token is the first index whose running sum of weights passes uniforms[drafts] times their sum; weights: p_n where no draft was left, else
  * max(p_n - q_n, 0) (without draft_logits p_n without the draft; p_n where that is all 0).  So the tokens are distributed as the target's own samples.  temperature 0 (else 1e-4 to 1e4): a draft is
  * accepted where it is its row's largest logit (the first of equal ones), the token is that of its row; uniforms and draft_logits are not read.  A row reached that has no distribution
- * (a NaN, an infinite logit or none above -inf) ends its sequence: its draft is not accepted, the token is -1.  Running sums of the drawn row, and decisions that FP32 cannot make, are in 64 bits;
- * a weight below e^-690 of its row's largest is 0, and so is a difference of weights that agree to 2^-40.
+ * (a NaN, an infinite logit or none above -inf) ends its sequence: its draft is not accepted, the token is -1.  The drawn row's weights and running sums, and decisions that FP32 cannot make, are in 64 bits;
+ * a weight below e^-690 of its row's largest is 0, and so is a difference of weights that agree to 2^-40.  Where more than 0.05 of max(p - q, 0) is left, which entries weigh more in p is told by FP32's sums: an
+ * entry whose p and q agree to 8e-6 may count by its difference, or not, in the running sum in front of others, which moves a border by 8e-6 of such entries' p.
+ * out_tokens and accepted may not overlap the tokens or one another: refused.
  * The workspace: b200_verify_drafts_workspace(args) bytes, 16-byte aligned, content does not matter, of no other call under way.  At most 64 drafts, 2^24 logits, 2^16 sequences. */
 typedef struct b200_verify_drafts_args {
     const void *logits, *draft_logits;
