@@ -279,6 +279,20 @@ struct Paged {
         if (rc != B200_OK) refused(rc, err);
     }
     at::ScalarType dtype() const { return keys.scalar_type(); }
+    // The memory as it is now: the tensors are the caller's too, who may free or move what they lie in (storage().resize_) between calls.
+    const void *place(const Tensor &t, const char *name) const {
+        outside_graph(t, name);
+        NEED(t.sizes() == at::IntArrayRef({pages, kv_heads, page_size, head_size}) && t.is_contiguous() && t.scalar_type() == (cache.type == B200_GGML_F16 ? at::kHalf : at::kBFloat16) && t.get_device() == device, name,
+             " are no longer the tensor of the cache's shape, type and device: ", shape(t));
+        NEED(t.storage().nbytes() >= (size_t)(t.storage_offset() + t.numel()) * 2, name, ": their memory has been taken away");
+        return t.data_ptr();
+    }
+    b200_paged_cache now() const {
+        b200_paged_cache c = cache;
+        c.keys = const_cast<void *>(place(keys, "keys"));
+        c.values = const_cast<void *>(place(values, "values"));
+        return c;
+    }
     void *stream() const { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream(); }
 
     // rows [n, heads, head_size] whose heads lie one behind the other: entries between rows
@@ -356,7 +370,8 @@ struct Paged {
         }
         if (n) {
             char err[256] = "";
-            const int rc = b200_paged_append(&cache, &a, stream(), err, sizeof err);
+            const b200_paged_cache here = now();
+            const int rc = b200_paged_append(&here, &a, stream(), err, sizeof err);
             if (rc != B200_OK) refused(rc, err);
         }
         return out;
@@ -386,12 +401,13 @@ struct Paged {
         a.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)head_size));
         if (n == 0) return out;
         Tensor work; // from the stream's own pool: calls on other streams, and captured graphs, have theirs
-        if ((a.workspace_bytes = b200_paged_attention_workspace(&cache, &a)) > 0) {
+        const b200_paged_cache here = now();
+        if ((a.workspace_bytes = b200_paged_attention_workspace(&here, &a)) > 0) {
             work = fresh({(int64_t)(a.workspace_bytes / 4)}, at::kFloat, device);
             a.workspace = work.data_ptr();
         }
         char err[256] = "";
-        const int rc = b200_paged_attention(&cache, &a, stream(), err, sizeof err);
+        const int rc = b200_paged_attention(&here, &a, stream(), err, sizeof err);
         if (rc != B200_OK) refused(rc, err);
         return out;
     }

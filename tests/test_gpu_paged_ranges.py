@@ -88,3 +88,35 @@ def test_results_in_the_place_of_queries_or_beside_them(pkg, chunk, hs):
     for bad in (across, wide[:, :8 * hs].view(80, 8, hs), cache.keys.view(-1)[:80 * 8 * hs].view(80, 8, hs)):
         with pytest.raises(pkg.native.B200Error, match="overlap"):
             cache.append(k, v, pos, tables, sequences=seq, q=q, q_out=bad)
+
+
+def test_memory_that_is_taken_away_or_moves(pkg):
+    """``keys`` and ``values`` are the caller's too: a call without their memory is refused, and one after they have moved uses them where they are."""
+    g = gen(2)
+    cache, tables = paged(pkg, g, [70], 16, 2, 64, BF16)
+    q, pos, k = rand(g, 3, 8, 64, dtype=BF16), ints(67, 68, 69), rand(g, 3, 2, 64, dtype=BF16)
+    cache.append(k, k, pos, tables)
+    want, keys = cache.attention(q, pos, tables), cache.keys.clone()
+    bytes_ = cache.keys.untyped_storage().nbytes()
+    torch.cuda.synchronize()
+    for t in (cache.keys, cache.values):
+        kept = t.clone()
+        t.untyped_storage().resize_(0)
+        with pytest.raises(ValueError, match="taken away"):
+            cache.attention(q, pos, tables)
+        with pytest.raises(ValueError, match="taken away"):
+            cache.append(k, k, pos, tables)
+        filler = torch.empty(bytes_ // 2, device="cuda", dtype=BF16)  # another tenant of what was freed
+        t.untyped_storage().resize_(bytes_)
+        t.copy_(kept)
+        del filler
+    assert torch.equal(cache.attention(q, pos, tables), want) and torch.equal(cache.keys.view(torch.int16), keys.view(torch.int16))
+    cache.keys.requires_grad_()
+    with pytest.raises(ValueError, match="gradient"):
+        cache.append(k, k, pos, tables)
+    cache.keys.requires_grad_(False)
+    cache.keys.transpose_(1, 2)
+    with pytest.raises(ValueError, match="shape"):
+        cache.attention(q, pos, tables)
+    cache.keys.transpose_(1, 2)
+    assert torch.equal(cache.attention(q, pos, tables), want)
