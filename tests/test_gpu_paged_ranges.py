@@ -120,3 +120,27 @@ def test_memory_that_is_taken_away_or_moves(pkg):
         cache.attention(q, pos, tables)
     cache.keys.transpose_(1, 2)
     assert torch.equal(cache.attention(q, pos, tables), want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("out", [F32, None])
+@pytest.mark.parametrize("size", [3e6, 7e7, 1.1e9, 1.3e11, 1e25])
+@pytest.mark.parametrize("chunk,hs", [(1, 64), (5, 128), (33, 64)])
+def test_huge_scores_of_rows_that_are_shared(pkg, dtype, out, size, chunk, hs):
+    """As above over 9000 positions, whose parts are joined: equal scores, a single larger one, and a maximum that grows every 1000 positions.  Sums: (m / 8 + 32) 2^-22 and the parts' join."""
+    g, n, out = gen(hs + chunk), 9000, out or dtype
+    cache, tables = paged(pkg, g, [n], 16, 1, hs, dtype)
+    at = torch.arange(n, device="cuda")
+    where = tables[0].long()[at // 16], 0, at % 16
+    pos = torch.arange(n - chunk, n, device="cuda", dtype=torch.int32)
+    q = torch.full((chunk, 4, hs), 8.0, device="cuda", dtype=dtype)
+    values = cache.values[where].double().cpu()
+    off = (n / 8 + 32) * 2.0 ** -22 + 2.0 ** -17 + probability(cache, out)
+    for factor in (1.0, 0.83, 0.71):
+        scale = factor * size * 0.6931471805599453 / (hs * 64.0)
+        for keys, first in ((torch.full((n,), 8.0, device="cuda"), 0), (8.0 + 0.0625 * (at // 1000), 8000), (torch.where(at == 4321, 8.0625, 8.0), None)):
+            cache.keys[where] = keys[:, None].expand(n, hs).to(dtype)
+            got = cache.attention(q, pos, tables, scale=scale, chunk=chunk, dtype=out).double().cpu()
+            for i in range(chunk):
+                v = values[4321:4322] if first is None else values[first:n - chunk + 1 + i]
+                assert ((got[i] - v.mean(0)).abs() <= P.rounding(v.mean(0), off * v.abs().mean(0), out)).all()
