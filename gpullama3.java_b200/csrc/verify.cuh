@@ -11,8 +11,8 @@
 // Where the token comes from max(p - q, 0), one pass takes both rows' sums and, on either side of which p / sum_p > q / sum_q by FP32's sums, those of the entries that weigh more in p: their difference is the
 // weight (entries that weigh the same to 2^-40 weigh nothing; a pass for the sums and one for the weights took 70 us in place of 37).  An entry whose weights agree to FP32's error, 8e-6, may be counted on the wrong
 // side, by a difference of no more than that of itself: a border moves by 8e-6 of such entries' p.
-// Bytes are the floor: 32 sequences of 0 to 5 drafts, 84 in all, and 128256 FP32 logits of two models: 200 rows that count, 103 MB, 15.9 us; the call takes 51 (48 in a graph): the rows 23, the tokens 24-34, of
-// which a pass over two rows in 64 bits is 18: two exponentials an entry, 64-bit units at 23 % on average, their chains and the loads in between on the clusters that have one.  One sequence: 15.5 in a graph, latency.
+// Bytes are the floor: 32 sequences of 0 to 5 drafts, 84 in all, and 128256 FP32 logits of two models: 200 rows that count, 103 MB, 15.9 us; the call takes 53-55 (48 in a graph): the rows 23, the tokens 24-34, of
+// which a pass over two rows in 64 bits is 18: two exponentials an entry, 64-bit units at 23 % on average, their chains and the loads in between on the clusters that have one.  One sequence: 15.7 in a graph, latency.
 // Nothing depends on an order of arrival.
 #pragma once
 #include "kv4.cuh"
